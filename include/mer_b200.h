@@ -65,6 +65,8 @@ typedef enum mer_status {
 #define MER_DEVSTAT_TIMEOUT 0x4u          /* bounded wait expired */
 #define MER_DEVSTAT_SHORT_SELECTION 0x8u  /* fewer than top_k finite scores */
 
+#define MER_DEVSTAT_BAD_CACHE 0x10u       /* a batch named a page, a length or rows that are not there (attention) */
+
 #define MER_EXPERT_NONE 0xFFFFFFFFu /* id written for an unfilled top-k slot / "no shared expert" */
 
 /* Scoring function of the router (ScoringFunc, gating.rs:94-97). */
@@ -403,6 +405,72 @@ int mer_moe_layer_forward(mer_backend *b, uint32_t layer, const float *x, size_t
  * must not overlap. */
 int mer_moe_layer_forward_device(mer_backend *b, uint32_t layer, const float *d_x, size_t n_tokens,
                                  float *d_out, uint32_t *d_ids, float *d_weights, void *stream);
+
+/* ---- attention over a paged cache, per layer: what lies between two MoE layers beside the projections (the reference's
+ * engine runs it on the host: RmsNorm per head, RoPE and the KV cache of transformer.rs, paged by block_pool.rs).
+ * mer_attention_install once per layer (any layer number, with or without a router), then per step on device rows:
+ *   mer_kv_append_device         q, k and v of the batch's rows: RMSNorm of every query and key head, position rotation,
+ *                                queries out in the cache's type, keys and values into the pages;
+ *   mer_attention_forward_device those queries over all that their sequences have in the cache, causal.
+ * A batch is n_seqs sequences of any lengths.  Sequence s brings the rows row_start[s] .. row_start[s + 1] (its newest tokens: one
+ * in decode, a prompt or a chunk of one, or none) and has kv_len[s] tokens with them; row i of its n rows stands at position
+ * kv_len[s] - n + i.  Token p of it lies in page page_table[s * table_stride + p / page_tokens], at p % page_tokens.  The tables are
+ * device memory and are read by the kernels alone: a captured call follows them from replay to replay, n_seqs and n_rows being
+ * upper bounds (sequences without rows, and rows behind the last sequence, which are left as they were).
+ * Both calls are asynchronous on `stream` and allocate nothing; max_tokens does not bound n_rows.  The attention kernels share a
+ * workspace of the backend: calls on different streams must not overlap.  Pointers are memory of the backend's device.
+ *
+ * Rows see nothing behind their own position, before their window, in pages that the table does not name or of other sequences, and
+ * what no row of a tile sees is not read: it may hold anything.  A key or value that is not finite makes the rows that see it not finite
+ * and may do so with other rows of its sequence in the same call.  A page number that is not below n_pages, a position beyond table_stride pages
+ * or a sequence with more rows than tokens is latched as MER_DEVSTAT_BAD_CACHE and reported once, by mer_stream_check
+ * (MER_ERR_VALIDATION_DISPATCH): a row without a place in its sequence is not appended and attends to nothing (zeros), a
+ * token without a page is not appended and counts as zeros where it is seen.  No memory outside the given buffers is touched. ---- */
+#define MER_VALUE_F32 0
+#define MER_VALUE_F16 1
+#define MER_VALUE_BF16 2
+#define MER_ATTENTION_MAX_HEAD_DIM 256
+#define MER_ATTENTION_ROPE_PAIRS 0x1u /* neighbours (2j, 2j + 1) rotate into one another, not halves (j, j + rope_dims / 2) */
+typedef struct mer_attention_cfg {
+  uint32_t q_heads, kv_heads;  /* kv_heads divides q_heads: query head h reads key head h / (q_heads / kv_heads) */
+  uint32_t head_dim;           /* a multiple of 8 up to MER_ATTENTION_MAX_HEAD_DIM */
+  uint32_t page_tokens;        /* any number */
+  int32_t cache_type;          /* MER_VALUE_F16 or MER_VALUE_BF16: keys, values, queries and outputs */
+  uint32_t window;             /* a row sees itself and window - 1 tokens before; 0 = all */
+  uint32_t rope_dims;          /* leading values of a head that are rotated; 0 = none */
+  uint32_t flags;              /* MER_ATTENTION_* */
+  float scale;                 /* of the scores; 0 = 1 / sqrt(head_dim) */
+  float norm_eps;
+  float rope_scale;            /* times cosine and sine (YaRN's attention factor); 0 = 1 */
+  uint32_t reserved;
+  const float *q_norm, *k_norm;  /* host [head_dim] RMSNorm weights of each head, or NULL = no norm */
+  const double *rope_freq;       /* host [rope_dims / 2] radians per position */
+  const float *sinks;            /* host [q_heads] a score without a value in each head's softmax, or NULL */
+} mer_attention_cfg;
+/* Copies the host arrays.  Installing a layer anew waits for the device; graphs captured with the old one must not be replayed. */
+int mer_attention_install(mer_backend *b, uint32_t layer, const mer_attention_cfg *cfg);
+
+typedef struct mer_kv_batch { /* device pointers; strides in values, multiples of 8; pages on 16 bytes */
+  void *k_pages, *v_pages;    /* value d of head h of token t of page p lies at p * page_stride + t * token_stride + h * head_stride + d */
+  uint64_t page_stride, token_stride, head_stride;
+  const uint32_t *page_table; /* [n_seqs x table_stride] */
+  const uint32_t *row_start;  /* [n_seqs + 1], not falling */
+  const uint32_t *kv_len;     /* [n_seqs] */
+  uint32_t n_pages, table_stride, n_seqs, n_rows;
+} mer_kv_batch;
+typedef struct mer_qkv_rows { /* device pointers; rows of heads side by side, e.g. three parts of one fused projection's rows */
+  const void *q, *k, *v;      /* [n_rows x q_heads * head_dim], [n_rows x kv_heads * head_dim]; q may be NULL */
+  void *q_out;                /* [n_rows x q_heads * head_dim] of the cache's type; may be q where type and stride are the same */
+  uint64_t q_stride, k_stride, v_stride, q_out_stride; /* values between rows; 0 = rows without gaps */
+  int32_t value_type;         /* MER_VALUE_* of q, k and v */
+  uint32_t reserved;
+} mer_qkv_rows;
+/* Norm and rotation in fp32 (angles in 64 bits), one rounding to the cache's type. */
+int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_qkv_rows *rows, void *stream);
+/* d_q and d_out: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8; 0 = no gaps).
+ * Scores, softmax and sums in fp32. */
+int mer_attention_forward_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const void *d_q, uint64_t q_stride,
+                                 void *d_out, uint64_t out_stride, void *stream);
 
 /* dequantize_q4_0_to_f32 / dequantize_q8_0_to_f32 (inference.rs:852-868, 963-979) on the
  * resident copy: projection 0 = gate, 1 = up, 2 = down; out is d_model*d_ff floats (host). */

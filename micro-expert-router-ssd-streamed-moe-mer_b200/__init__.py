@@ -8,7 +8,7 @@ read like the reference's own.  There is no CPU fallback: if the library is miss
 CUDA device is present, calls raise.
 """
 from .capi import (ABI_SYMBOLS, DTYPE_Q4_0, DTYPE_Q8_0, EXPERT_NONE, LIB_PATH, SCORE_SIGMOID, SCORE_SOFTMAX,
-                   MerCounters, MerErrorInfo, load_library)
+                   VALUE_BF16, VALUE_F16, VALUE_F32, KvBatch, MerCounters, MerErrorInfo, QkvRows, load_library)
 from .backend import (Backend, GpuExpertBatchDispatchOutcome, GpuExpertDispatchError, GpuExpertDispatchErrorKind,
                       expert_bytes, expert_forward_noalloc, expert_forward_noalloc_bounded, expert_noalloc_check,
                       routed_expert_gpu_compatibility)
@@ -19,8 +19,8 @@ from .gating import LinearGate, RoutingDecision, ScoringFunc
 __all__ = [
     "ABI_SYMBOLS", "Backend", "DTYPE_Q4_0", "DTYPE_Q8_0", "EXPERT_NONE", "GpuExpertBatchDispatchOutcome",
     "GpuAdmission", "GpuDemandAdmissionError", "GpuDemandAdmissionPreflight", "GpuExpertCache",
-    "GpuExpertDispatchError", "GpuExpertDispatchErrorKind", "GpuHotPromotionOutcome", "GpuLookup", "LIB_PATH", "LinearGate", "MerCounters", "MerErrorInfo",
-    "RoutingDecision", "SCORE_SIGMOID", "SCORE_SOFTMAX", "ScoringFunc", "expert_bytes", "expert_forward_noalloc",
+    "GpuExpertDispatchError", "GpuExpertDispatchErrorKind", "GpuHotPromotionOutcome", "GpuLookup", "KvBatch", "LIB_PATH", "LinearGate", "MerCounters",
+    "MerErrorInfo", "QkvRows", "RoutingDecision", "SCORE_SIGMOID", "SCORE_SOFTMAX", "ScoringFunc", "VALUE_BF16", "VALUE_F16", "VALUE_F32", "expert_bytes", "expert_forward_noalloc",
     "expert_forward_noalloc_bounded", "expert_noalloc_check",
     "load_library",
     "routed_expert_gpu_compatibility",

@@ -267,6 +267,34 @@ class Backend:
         self._check(self.lib.mer_moe_layer_forward_device(self.h, layer, C.c_void_p(d_x), n_tokens, C.c_void_p(d_out),
                                                           C.c_void_p(d_ids), C.c_void_p(d_weights), C.c_void_p(stream)))
 
+    # -- attention over a paged cache ---------------------------------------------------------
+    def install_attention(self, layer, q_heads, kv_heads, head_dim, cache_type, page_tokens, window=0, scale=0.0, q_norm=None, k_norm=None,
+                          norm_eps=1e-6, rope_freq=None, rope_pairs=False, rope_scale=1.0, sinks=None):
+        """The attention side of `layer`: heads, cache (VALUE_F16 or VALUE_BF16, tokens of a page), window, per-head RMSNorm weights
+        [head_dim], rotation frequencies in radians per position (two values of a head each), sinks [q_heads]."""
+        keep = [None if v is None else np.ascontiguousarray(v, dtype=t) for v, t in
+                ((q_norm, np.float32), (k_norm, np.float32), (rope_freq, np.float64), (sinks, np.float32))]
+        for v, name, n in zip(keep, ("q_norm", "k_norm", "rope_freq", "sinks"), (head_dim, head_dim, None, q_heads)):
+            if v is not None and (v.ndim != 1 or (n is not None and v.size != n)):
+                raise ValueError(f"{name} must have length {n}" if n is not None else f"{name} must have one axis")
+        cfg = capi.MerAttentionCfg(q_heads, kv_heads, head_dim, page_tokens, cache_type, window, 0 if keep[2] is None else 2 * keep[2].size,
+                                   capi.ATTENTION_ROPE_PAIRS if rope_pairs else 0, scale, norm_eps, rope_scale, 0,
+                                   *(None if v is None else v.ctypes.data for v in keep))
+        self._check(self.lib.mer_attention_install(self.h, layer, C.byref(cfg)))
+
+    def kv_append_device(self, layer, batch, rows, stream=0):
+        """Rows of q|k|v (QkvRows) of a batch (KvBatch): norms, rotation, queries out, keys and values into the pages; asynchronous on
+        `stream` (a cudaStream_t as int)."""
+        rc = self.lib.mer_kv_append_device(self.h, layer, batch, rows, stream)
+        if rc != 0:
+            self._check(rc)
+
+    def attention_forward_device(self, layer, batch, d_q, d_out, stream=0, q_stride=0, out_stride=0):
+        """Query rows over what their sequences have in the cache; device pointers (ints), asynchronous on `stream`."""
+        rc = self.lib.mer_attention_forward_device(self.h, layer, batch, d_q, q_stride, d_out, out_stride, stream)
+        if rc != 0:
+            self._check(rc)
+
     def stream_check(self, layer, stream=0):
         """Synchronises `stream` and raises the typed error the device status word holds, if any (for _device calls)."""
         self._check(self.lib.mer_stream_check(self.h, layer, C.c_void_p(stream)))

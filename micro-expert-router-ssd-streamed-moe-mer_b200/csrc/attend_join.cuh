@@ -1,0 +1,160 @@
+// The way of a CTA through its run of blocks, and the end of a tile: its rows stored, or the parts of several CTAs joined.
+#pragma once
+
+#include "attention.cuh"
+#include "ptx.cuh"
+
+namespace {
+
+// First block of a CTA's run.
+__device__ __forceinline__ uint64_t run_first(const RunStart &r, uint32_t cta) { return r.total * cta / r.parts; }
+// The CTA whose run holds block x.
+__device__ __forceinline__ uint32_t run_of(const RunStart &r, uint64_t x) {
+  uint32_t c = (uint32_t)(x * r.parts / r.total);
+  while (run_first(r, c) > x) c--;
+  while (run_first(r, c + 1) <= x) c++;
+  return c;
+}
+
+template <uint32_t KB>
+struct RunWalk {
+  const KvBatchDev &kv;
+  const TileShape &ts;
+  uint32_t window, min_n, max_n;
+  uint64_t left, at, skip;   // blocks of the run that are left, the next one's number, and how far in its sequence it lies (first tile only)
+  SeqWork w;
+  uint32_t seq, v_head, tile;
+  bool fresh = true;
+
+  __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, uint32_t lo, uint32_t hi, const RunStart &r)
+      : kv(kv_), ts(ts_), window(window_), min_n(lo), max_n(hi), skip(r.offset), seq(r.seq), v_head(0), tile(0) {
+    at = run_first(r, blockIdx.x);
+    left = run_first(r, blockIdx.x + 1) - at;
+  }
+  // The next tile of the run, or a part of one; a whole warp (every warp of the CTA for itself).
+  __device__ bool next(TileWork *t) {
+    if (left == 0) return false;
+    uint32_t from = 0;  // blocks of the tile that are not this run's
+    if (fresh) {
+      fresh = false;
+      w = seq_work(kv, seq, ts.tokens, min_n, max_n);
+      const uint64_t per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window);
+      v_head = (uint32_t)(skip / per_head);
+      const uint64_t x = skip - v_head * per_head;
+      uint64_t before;
+      tile = find_tile<KB>(w, ts.tokens, window, x, &before);
+      from = (uint32_t)(x - before);
+    } else if (++tile >= w.tiles) {
+      tile = 0;
+      if (++v_head >= ts.v_heads) {
+        v_head = 0;
+        do {
+          seq++;
+          if (seq >= kv.n_seqs) return false;
+          w = seq_work(kv, seq, ts.tokens, min_n, max_n);
+        } while (w.tiles == 0);
+      }
+    }
+    w.tile_blocks<KB>(tile, ts.tokens, window, &t->tile_lo, &t->tile_hi);
+    t->at = at - from;
+    t->lo = t->tile_lo + from;
+    t->hi = (uint32_t)min((uint64_t)t->tile_hi, t->lo + left);
+    left -= t->hi - t->lo;
+    at += t->hi - t->lo;
+    t->seq = seq, t->row0 = w.row0, t->past = w.past;
+    t->token0 = tile * ts.tokens;
+    t->tokens = min(ts.tokens, w.n - t->token0);
+    t->kv_head = v_head / ts.chunks;
+    const uint32_t chunk = v_head - t->kv_head * ts.chunks;
+    t->head0 = t->kv_head * ts.group + chunk * ts.heads;
+    t->heads = min(ts.heads, ts.group - chunk * ts.heads);
+    return true;
+  }
+};
+
+// Rows that have no place in their sequence (it brings more rows than it has tokens) see nothing: zero.
+template <typename T, uint32_t THREADS>
+__device__ void clear_rows_without_place(const AttnLayer &a, const KvBatchDev &kv, uint32_t min_n, uint32_t max_n, T *out, uint64_t out_stride, uint32_t *status) {
+  for (uint32_t s0 = 0; s0 < kv.n_seqs; s0 += THREADS) {
+    const uint32_t s = s0 + threadIdx.x;
+    uint32_t row = 0, n = 0, len = 0;
+    if (s < kv.n_seqs) seq_rows(kv, s, &row, &n, &len);
+    const bool some = n > len && n >= min_n && n <= max_n;
+    if (some) atomicOr(status, MER_DEVSTAT_BAD_CACHE);
+    if (!__syncthreads_or(some)) continue;
+    for (uint32_t i = s0; i < min(kv.n_seqs, s0 + THREADS); i++) {
+      seq_rows(kv, i, &row, &n, &len);
+      if (n <= len || n < min_n || n > max_n) continue;
+      const uint32_t width = a.q_heads * a.head_dim;
+      for (uint64_t e = threadIdx.x; e < (uint64_t)(n - len) * width; e += THREADS) out[(row + e / width) * out_stride + e % width] = Num<T>::one(0.0f);
+    }
+  }
+}
+
+// Floats of a part: maximum and sum of R rows, and their outputs.
+__host__ __device__ constexpr uint32_t part_floats(uint32_t R, uint32_t DP) { return R * (DP + 2); }
+// Where a CTA leaves its part of a tile: a run has parts of two tiles at most, its first and its last.
+__device__ __forceinline__ uint32_t part_slot(const RunStart &r, const TileWork &t, uint32_t cta) { return 2 * cta + (run_first(r, cta) >= t.at ? 0 : 1); }
+
+// Four values from column c on of row r of a tile.
+template <typename T>
+__device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t, uint32_t r, uint32_t c, float top, float sum, const float4 &acc, T *out, uint64_t out_stride) {
+  if (c >= a.head_dim) return;
+  const uint32_t tok = r / t.heads, head = t.head0 + r - tok * t.heads;
+  if (a.sinks) sum += exp2_approx(__ldg(a.sinks + head) * LOG2E - top + P_SHIFT);
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint2 v = make_uint2(Num<T>::pack(acc.x * f, acc.y * f), Num<T>::pack(acc.z * f, acc.w * f));
+  *reinterpret_cast<uint2 *>(out + (uint64_t)(t.row0 + t.token0 + tok) * out_stride + (uint64_t)head * a.head_dim + c) = v;
+}
+
+// After the CTA's threads have stored its part of the tile.  The CTA that arrives last joins the parts in the order of the runs and leaves the
+// count at zero; `work`: shared memory for R * (parts + 1) + 2 floats.
+template <typename T, int R, int DP, uint32_t THREADS>
+__device__ void join_parts(const AttnLayer &a, const TileWork &t, const RunStart &run, uint32_t rows, const AttnWorkspace &ws, T *out, uint64_t out_stride, float *work) {
+  const uint32_t tid = threadIdx.x;
+  const uint32_t c0 = run_of(run, t.at), c1 = run_of(run, t.at + (t.tile_hi - t.tile_lo) - 1), n = c1 - c0 + 1;
+  uint32_t *flag = reinterpret_cast<uint32_t *>(work);
+  __syncthreads();
+  if (tid == 0) {
+    const bool is_last = arrive_acq_rel(ws.counts + c0) + 1 == n;
+    if (is_last) ws.counts[c0] = 0;
+    *flag = is_last;
+  }
+  __syncthreads();
+  const bool is_last = *flag;
+  __syncthreads();
+  if (!is_last) return;
+  const float *first = ws.parts + (size_t)part_slot(run, t, c0) * part_floats(R, DP), *others = ws.parts + (size_t)2 * (c0 + 1) * part_floats(R, DP);
+  auto part = [&](uint32_t i) { return i == 0 ? first : others + (size_t)2 * (i - 1) * part_floats(R, DP); };
+  float *w = work, *total = work + R * n, *tops = total + R;  // [row][part] maxima, then factors
+  for (uint32_t i = tid; i < rows * n; i += THREADS) w[i] = __ldcg(part(i % n) + i / n);
+  __syncthreads();
+  for (uint32_t r = tid; r < rows; r += THREADS) {
+    float top = -INFINITY;
+    for (uint32_t i = 0; i < n; i++) top = fmaxf(top, w[r * n + i]);
+    tops[r] = top;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < rows * n; i += THREADS) w[i] = w[i] == -INFINITY ? 0.0f : exp2_approx(w[i] - tops[i / n]);
+  __syncthreads();
+  for (uint32_t r = tid; r < rows; r += THREADS) {
+    float sum = 0.0f;
+    for (uint32_t i = 0; i < n; i++) sum = fmaf(w[r * n + i], __ldcg(part(i) + R + r), sum);
+    total[r] = sum;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < rows * (DP / 4); i += THREADS) {
+    const uint32_t r = i / (DP / 4), c = i % (DP / 4) * 4;
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+    for (uint32_t k = 0; k < n; k++) {
+      const float f = w[r * n + k];
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(k) + 2 * R + (size_t)r * DP + c));
+      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    }
+    store_row<T>(a, t, r, c, tops[r], total[r], acc, out, out_stride);
+  }
+  __syncthreads();
+}
+
+}  // namespace

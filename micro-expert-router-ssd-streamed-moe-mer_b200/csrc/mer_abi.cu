@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "../../include/mer_b200.h"
+#include "attention.h"
 #include "copy_pool.h"
 #include "kernels.h"
 #include "replay_table.h"
@@ -100,6 +101,11 @@ struct mer_backend {
 
   std::unordered_map<uint32_t, RouterEntry> routers;
   int kernel_path = 0;
+
+  // attention side (mer_attention_install); workspace and pinned status word from the first installation on
+  std::unordered_map<uint32_t, AttnLayer> attn_layers;
+  AttnWorkspace attn_ws{};
+  uint32_t *h_attn_status = nullptr;
 
   // pipelined host entry (mer_moe_layer_forward_submit / _wait): per slot its own device x / out and status copy
   struct AsyncSlot {
@@ -412,9 +418,11 @@ int require_resident(mer_backend *b, uint32_t layer, uint32_t id) {
 }
 
 void a2a_free(mer_backend *b);  // mer_abi_ep_nccl.inc
+void attention_free(mer_backend *b);  // mer_abi_attention.inc
 
 void free_all(mer_backend *b) {
   a2a_free(b);
+  attention_free(b);
   auto F = [](auto *&p) {
     if (p) cudaFree((void *)p);
     p = nullptr;
@@ -2173,8 +2181,18 @@ MER_EXPORT int mer_stream_check(mer_backend *b, uint32_t layer, void *stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   CU(MER_ERR_READBACK_MAP, "cudaMemcpyAsync(status)",
      cudaMemcpyAsync(b->h_u32 + b->max_pairs, b->d_status, 4, cudaMemcpyDeviceToHost, s));
+  uint32_t attn = 0;
+  if (b->h_attn_status)
+    CU(MER_ERR_READBACK_MAP, "cudaMemcpyAsync(attention status)", cudaMemcpyAsync(b->h_attn_status, b->attn_ws.status, 4, cudaMemcpyDeviceToHost, s));
   CU(MER_ERR_READBACK_MAP, "cudaStreamSynchronize", cudaStreamSynchronize(s));
-  return check_device_status(b, b->h_u32[b->max_pairs], layer, expert);
+  if (b->h_attn_status && (attn = *b->h_attn_status) != 0) {  // kept until it is read here
+    CU(MER_ERR_READBACK_MAP, "cudaMemsetAsync(attention status)", cudaMemsetAsync(b->attn_ws.status, 0, 4, s));
+    CU(MER_ERR_READBACK_MAP, "cudaStreamSynchronize", cudaStreamSynchronize(s));
+  }
+  const int rc = check_device_status(b, b->h_u32[b->max_pairs] | attn, layer, expert);
+  if (rc == MER_OK && (attn & MER_DEVSTAT_BAD_CACHE))
+    return fail(b, MER_ERR_VALIDATION_DISPATCH, layer, expert, "a page number, a length or a row range of a batch lies outside its cache (device status 0x%x)", attn);
+  return rc;
 }
 
 MER_EXPORT int mer_dequant_projection_f32(mer_backend *b, uint32_t expert_id, int projection, float *out) {
@@ -2282,4 +2300,5 @@ MER_EXPORT int mer_set_kernel_path(mer_backend *b, int path) {
   return MER_OK;
 }
 
+#include "mer_abi_attention.inc"
 #include "mer_abi_ep_nccl.inc"
