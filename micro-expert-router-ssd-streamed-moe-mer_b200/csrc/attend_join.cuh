@@ -107,54 +107,38 @@ __device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t,
   *reinterpret_cast<uint2 *>(out + (uint64_t)(t.row0 + t.token0 + tok) * out_stride + (uint64_t)head * a.head_dim + c) = v;
 }
 
-// After the CTA's threads have stored its part of the tile.  The CTA that arrives last joins the parts in the order of the runs and leaves the
-// count at zero; `work`: shared memory for R * (parts + 1) + 2 floats.
-template <typename T, int R, int DP, uint32_t THREADS>
-__device__ void join_parts(const AttnLayer &a, const TileWork &t, const RunStart &run, uint32_t rows, const AttnWorkspace &ws, T *out, uint64_t out_stride, float *work) {
+// After `threads` threads have stored their CTA's part of the tile.  The CTA that arrives last joins the parts in the order of the runs and
+// leaves the count at zero.  `sync` holds all of those threads together; `flag`: a word of shared memory.
+template <typename T, int R, int DP, uint32_t THREADS, typename Sync>
+__device__ void join_parts(const AttnLayer &a, const TileWork &t, const RunStart &run, uint32_t rows, const AttnWorkspace &ws, T *out, uint64_t out_stride,
+                           volatile uint32_t *flag, Sync sync) {
   const uint32_t tid = threadIdx.x;
   const uint32_t c0 = run_of(run, t.at), c1 = run_of(run, t.at + (t.tile_hi - t.tile_lo) - 1), n = c1 - c0 + 1;
-  uint32_t *flag = reinterpret_cast<uint32_t *>(work);
-  __syncthreads();
+  sync();
   if (tid == 0) {
     const bool is_last = arrive_acq_rel(ws.counts + c0) + 1 == n;
     if (is_last) ws.counts[c0] = 0;
     *flag = is_last;
   }
-  __syncthreads();
-  const bool is_last = *flag;
-  __syncthreads();
-  if (!is_last) return;
+  sync();
+  if (!*flag) return;
   const float *first = ws.parts + (size_t)part_slot(run, t, c0) * part_floats(R, DP), *others = ws.parts + (size_t)2 * (c0 + 1) * part_floats(R, DP);
-  auto part = [&](uint32_t i) { return i == 0 ? first : others + (size_t)2 * (i - 1) * part_floats(R, DP); };
-  float *w = work, *total = work + R * n, *tops = total + R;  // [row][part] maxima, then factors
-  for (uint32_t i = tid; i < rows * n; i += THREADS) w[i] = __ldcg(part(i % n) + i / n);
-  __syncthreads();
-  for (uint32_t r = tid; r < rows; r += THREADS) {
-    float top = -INFINITY;
-    for (uint32_t i = 0; i < n; i++) top = fmaxf(top, w[r * n + i]);
-    tops[r] = top;
-  }
-  __syncthreads();
-  for (uint32_t i = tid; i < rows * n; i += THREADS) w[i] = w[i] == -INFINITY ? 0.0f : exp2_approx(w[i] - tops[i / n]);
-  __syncthreads();
-  for (uint32_t r = tid; r < rows; r += THREADS) {
-    float sum = 0.0f;
-    for (uint32_t i = 0; i < n; i++) sum = fmaf(w[r * n + i], __ldcg(part(i) + R + r), sum);
-    total[r] = sum;
-  }
-  __syncthreads();
   for (uint32_t i = tid; i < rows * (DP / 4); i += THREADS) {
     const uint32_t r = i / (DP / 4), c = i % (DP / 4) * 4;
     float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 8
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
     for (uint32_t k = 0; k < n; k++) {
-      const float f = w[r * n + k];
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(k) + 2 * R + (size_t)r * DP + c));
-      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+      const float *part = k == 0 ? first : others + (size_t)2 * (k - 1) * part_floats(R, DP);
+      const float m = __ldcg(part + r), l = __ldcg(part + R + r);
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + 2 * R + (size_t)r * DP + c));
+      const float now = fmaxf(top, m), old = top == -INFINITY ? 0.0f : exp2_approx(top - now), f = m == -INFINITY ? 0.0f : exp2_approx(m - now);
+      top = now;
+      sum = fmaf(f, l, sum * old);
+      acc.x = fmaf(f, v.x, acc.x * old), acc.y = fmaf(f, v.y, acc.y * old), acc.z = fmaf(f, v.z, acc.z * old), acc.w = fmaf(f, v.w, acc.w * old);
     }
-    store_row<T>(a, t, r, c, tops[r], total[r], acc, out, out_stride);
+    store_row<T>(a, t, r, c, top, sum, acc, out, out_stride);
   }
-  __syncthreads();
 }
 
 }  // namespace

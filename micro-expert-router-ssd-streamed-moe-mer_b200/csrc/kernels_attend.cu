@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   constexpr uint32_t KB = S::KB, THREADS = S::THREADS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_work[THREADS / 32 + 4];
+  __shared__ uint32_t s_flag;
   uint8_t *s_q = smem;                               // [R][DP], swizzled
   uint8_t *s_ring = smem + R * DP * 2;               // [NW][ST][k, v][16][DP]
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -286,7 +287,10 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
       }
     }
     __syncthreads();
-    if (!whole) join_parts<T, R, DP, THREADS>(p.a, t, run, rows, p.ws, (T *)p.out, p.out_stride, reinterpret_cast<float *>(s_ring));
+    if (!whole) {
+      join_parts<T, R, DP, THREADS>(p.a, t, run, rows, p.ws, (T *)p.out, p.out_stride, &s_flag, [] { __syncthreads(); });
+      __syncthreads();
+    }
   }
 }
 
@@ -308,15 +312,18 @@ cudaError_t launch_stream(const AttendParams &p, bool two, int sm_count, cudaStr
 
 }  // namespace
 
-size_t attend_part_floats(int sm_count) { return (size_t)2 * sm_count * part_floats(32, 256); }
+size_t attend_part_floats(int sm_count) {
+  return std::max({(size_t)2 * sm_count * part_floats(32, 128), (size_t)2 * sm_count * part_floats(16, 256), attend_tc_part_floats(sm_count)});
+}
 size_t attend_counts(int sm_count) { return (size_t)sm_count; }
 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
-  AttendParams p{a, kv, q, out, q_stride, out_stride, ws, 0xFFFFFFFFu};
-  // 16 rows of a tile hold the heads of one token, or as many tokens as the batch has per sequence on average; else 32
-  const uint32_t group = a.q_heads / a.kv_heads;
-  const bool two = (uint64_t)group * ((kv.n_rows + kv.n_seqs - 1) / kv.n_seqs) > 16;
+  // Rows of a sequence's tile on average.  16 and 32 are the tiles of the streaming kernel; beyond those it would read the cache once
+  // per 32 rows, and multiply them at the legacy rate.
+  const uint64_t rows = (uint64_t)(a.q_heads / a.kv_heads) * ((kv.n_rows + kv.n_seqs - 1) / kv.n_seqs);
   *launches += 1;
-  return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, two, sm_count, s) : launch_stream<__nv_bfloat16>(p, two, sm_count, s);
+  if (rows > 32 && a.head_dim <= 128) return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+  AttendParams p{a, kv, q, out, q_stride, out_stride, ws, 0xFFFFFFFFu};
+  return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, rows > 16, sm_count, s) : launch_stream<__nv_bfloat16>(p, rows > 16, sm_count, s);
 }
