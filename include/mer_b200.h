@@ -450,7 +450,7 @@ typedef struct mer_attention_cfg {
 /* Copies the host arrays.  Installing a layer anew waits for the device; graphs captured with the old one must not be replayed. */
 int mer_attention_install(mer_backend *b, uint32_t layer, const mer_attention_cfg *cfg);
 
-typedef struct mer_kv_batch { /* device pointers; strides in values, multiples of 8; pages on 16 bytes */
+typedef struct mer_kv_batch { /* device pointers; strides in values, multiples of 8; pages on 16 bytes, keys and values within 64 GB each */
   void *k_pages, *v_pages;    /* value d of head h of token t of page p lies at p * page_stride + t * token_stride + h * head_stride + d */
   uint64_t page_stride, token_stride, head_stride;
   const uint32_t *page_table; /* [n_seqs x table_stride] */
@@ -467,7 +467,7 @@ typedef struct mer_qkv_rows { /* device pointers; rows of heads side by side, e.
 } mer_qkv_rows;
 /* Norm and rotation in fp32 (angles in 64 bits), one rounding to the cache's type. */
 int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_qkv_rows *rows, void *stream);
-/* d_q and d_out: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8; 0 = no gaps).
+/* d_q and d_out: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8 below 2^26; 0 = no gaps).
  * Scores, softmax and sums in fp32. */
 int mer_attention_forward_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const void *d_q, uint64_t q_stride,
                                  void *d_out, uint64_t out_stride, void *stream);

@@ -6,53 +6,38 @@
 
 namespace {
 
-// First block of a CTA's run.
-__device__ __forceinline__ uint64_t run_first(const RunStart &r, uint32_t cta) { return r.total * cta / r.parts; }
-// The CTA whose run holds block x.
-__device__ __forceinline__ uint32_t run_of(const RunStart &r, uint64_t x) {
-  uint32_t c = (uint32_t)(x * r.parts / r.total);
-  while (run_first(r, c) > x) c--;
-  while (run_first(r, c + 1) <= x) c++;
-  return c;
-}
-
 template <uint32_t KB>
 struct RunWalk {
   const KvBatchDev &kv;
   const TileShape &ts;
   uint32_t window, min_n, max_n;
-  uint64_t left, at, skip;   // blocks of the run that are left, the next one's number, and how far in its sequence it lies (first tile only)
+  uint64_t left, at;  // blocks of the run that are left, and the next one's number
   SeqWork w;
-  uint32_t seq, v_head, tile;
+  uint32_t seq, v_head, tile, from;  // from: blocks of the tile that are not this run's (its first tile alone)
   bool fresh = true;
 
   __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, uint32_t lo, uint32_t hi, const RunStart &r)
-      : kv(kv_), ts(ts_), window(window_), min_n(lo), max_n(hi), skip(r.offset), seq(r.seq), v_head(0), tile(0) {
+      : kv(kv_), ts(ts_), window(window_), min_n(lo), max_n(hi), w(r.w), seq(r.seq), v_head(r.v_head), tile(r.tile), from(r.from) {
     at = run_first(r, blockIdx.x);
-    left = run_first(r, blockIdx.x + 1) - at;
+    left = r.total == 0 ? 0 : run_first(r, blockIdx.x + 1) - at;
   }
-  // The next tile of the run, or a part of one; a whole warp (every warp of the CTA for itself).
+  // The next tile of the run, or a part of one.
   __device__ bool next(TileWork *t) {
     if (left == 0) return false;
-    uint32_t from = 0;  // blocks of the tile that are not this run's
     if (fresh) {
       fresh = false;
-      w = seq_work(kv, seq, ts.tokens, min_n, max_n);
-      const uint64_t per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window);
-      v_head = (uint32_t)(skip / per_head);
-      const uint64_t x = skip - v_head * per_head;
-      uint64_t before;
-      tile = find_tile<KB>(w, ts.tokens, window, x, &before);
-      from = (uint32_t)(x - before);
-    } else if (++tile >= w.tiles) {
-      tile = 0;
-      if (++v_head >= ts.v_heads) {
-        v_head = 0;
-        do {
-          seq++;
-          if (seq >= kv.n_seqs) return false;
-          w = seq_work(kv, seq, ts.tokens, min_n, max_n);
-        } while (w.tiles == 0);
+    } else {
+      from = 0;
+      if (++tile >= w.tiles) {
+        tile = 0;
+        if (++v_head >= ts.v_heads) {
+          v_head = 0;
+          do {
+            seq++;
+            if (seq >= kv.n_seqs) return false;
+            w = seq_work(kv, seq, ts.tokens, min_n, max_n);
+          } while (w.tiles == 0);
+        }
       }
     }
     w.tile_blocks<KB>(tile, ts.tokens, window, &t->tile_lo, &t->tile_hi);
@@ -64,7 +49,7 @@ struct RunWalk {
     t->seq = seq, t->row0 = w.row0, t->past = w.past;
     t->token0 = tile * ts.tokens;
     t->tokens = min(ts.tokens, w.n - t->token0);
-    t->kv_head = v_head / ts.chunks;
+    t->kv_head = ts.chunks == 1 ? v_head : v_head / ts.chunks;
     const uint32_t chunk = v_head - t->kv_head * ts.chunks;
     t->head0 = t->kv_head * ts.group + chunk * ts.heads;
     t->heads = min(ts.heads, ts.group - chunk * ts.heads);
@@ -107,38 +92,26 @@ __device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t,
   *reinterpret_cast<uint2 *>(out + (uint64_t)(t.row0 + t.token0 + tok) * out_stride + (uint64_t)head * a.head_dim + c) = v;
 }
 
-// After `threads` threads have stored their CTA's part of the tile.  The CTA that arrives last joins the parts in the order of the runs and
-// leaves the count at zero.  `sync` holds all of those threads together; `flag`: a word of shared memory.
-template <typename T, int R, int DP, uint32_t THREADS, typename Sync>
-__device__ void join_parts(const AttnLayer &a, const TileWork &t, const RunStart &run, uint32_t rows, const AttnWorkspace &ws, T *out, uint64_t out_stride,
-                           volatile uint32_t *flag, Sync sync) {
-  const uint32_t tid = threadIdx.x;
-  const uint32_t c0 = run_of(run, t.at), c1 = run_of(run, t.at + (t.tile_hi - t.tile_lo) - 1), n = c1 - c0 + 1;
-  sync();
-  if (tid == 0) {
-    const bool is_last = arrive_acq_rel(ws.counts + c0) + 1 == n;
-    if (is_last) ws.counts[c0] = 0;
-    *flag = is_last;
-  }
-  sync();
-  if (!*flag) return;
-  const float *first = ws.parts + (size_t)part_slot(run, t, c0) * part_floats(R, DP), *others = ws.parts + (size_t)2 * (c0 + 1) * part_floats(R, DP);
-  for (uint32_t i = tid; i < rows * (DP / 4); i += THREADS) {
-    const uint32_t r = i / (DP / 4), c = i % (DP / 4) * 4;
-    float4 acc = make_float4(0, 0, 0, 0);
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-    for (uint32_t k = 0; k < n; k++) {
-      const float *part = k == 0 ? first : others + (size_t)2 * (k - 1) * part_floats(R, DP);
-      const float m = __ldcg(part + r), l = __ldcg(part + R + r);
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + 2 * R + (size_t)r * DP + c));
-      const float now = fmaxf(top, m), old = top == -INFINITY ? 0.0f : exp2_approx(top - now), f = m == -INFINITY ? 0.0f : exp2_approx(m - now);
-      top = now;
-      sum = fmaf(f, l, sum * old);
-      acc.x = fmaf(f, v.x, acc.x * old), acc.y = fmaf(f, v.y, acc.y * old), acc.z = fmaf(f, v.z, acc.z * old), acc.w = fmaf(f, v.w, acc.w * old);
-    }
-    store_row<T>(a, t, r, c, top, sum, acc, out, out_stride);
-  }
+// The runs that have a part of a tile: c0, and n - 1 after it.
+__device__ __forceinline__ void runs_of_tile(const RunStart &run, const TileWork &t, uint32_t *c0, uint32_t *n) {
+  *c0 = run_of(run, t.at);
+  *n = run_of(run, t.at + (t.tile_hi - t.tile_lo) - 1) - *c0 + 1;
 }
+// Part k of a tile in the workspace.
+__device__ __forceinline__ const float *part_of_tile(const RunStart &run, const TileWork &t, const float *parts, uint32_t c0, uint32_t k, uint32_t floats) {
+  return parts + (size_t)(k == 0 ? part_slot(run, t, c0) : 2 * (c0 + k)) * floats;
+}
+
+// Running maximum, sum and four values of a row, part by part.
+struct Joined {
+  float top = -INFINITY, sum = 0.0f;
+  float4 acc = make_float4(0, 0, 0, 0);
+  __device__ __forceinline__ void add(float m, float l, const float4 &v) {
+    const float now = fmaxf(top, m), old = top == -INFINITY ? 0.0f : exp2_approx(top - now), f = m == -INFINITY ? 0.0f : exp2_approx(m - now);
+    top = now;
+    sum = fmaf(f, l, sum * old);
+    acc.x = fmaf(f, v.x, acc.x * old), acc.y = fmaf(f, v.y, acc.y * old), acc.z = fmaf(f, v.z, acc.z * old), acc.w = fmaf(f, v.w, acc.w * old);
+  }
+};
 
 }  // namespace

@@ -13,19 +13,24 @@
 
 #include "attention.h"
 #include "../../include/mer_b200.h"
+#include "page_map.h"
 
 namespace {
 
-// sum over 0 <= i < n of floor((a i + b) / m), a, b >= 0: the lattice points under a line, by Euclid's steps on (a, m).
-__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint32_t divided(uint32_t n, const FastDiv &f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+// 64-bit division is 70 instructions; nearly always 32 bits will do.
+__device__ __forceinline__ uint64_t divided(uint64_t a, uint64_t b) { return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b; }
+
+// sum over 0 <= i < n of floor((a i + b) / m): the lattice points under a line, by Euclid's steps on (a, m).  a n + b below 2^32.
+__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   uint64_t sum = 0;
   while (n) {
-    if (a >= m) sum += (n - 1) * n / 2 * (a / m), a %= m;
-    if (b >= m) sum += n * (b / m), b %= m;
-    const uint64_t y = a * n + b;
+    if (a >= m) sum += (uint64_t)(n - 1) * n / 2 * (a / m), a %= m;
+    if (b >= m) sum += (uint64_t)n * (b / m), b %= m;
+    const uint32_t y = a * n + b;
     if (y < m) break;
     n = y / m, b = y % m;
-    const uint64_t t = m;
+    const uint32_t t = m;
     m = a, a = t;
   }
   return sum;
@@ -41,26 +46,31 @@ struct SeqWork {
   template <uint32_t KB>
   __device__ __forceinline__ uint64_t blocks_before(uint32_t j, uint32_t tokens, uint32_t window) const {
     if (j == 0) return 0;
+    if (tiles == 1) {
+      uint32_t lo, hi;
+      tile_blocks<KB>(0, tokens, window, &lo, &hi);
+      return hi - lo;
+    }
     const uint32_t full = j == tiles ? j - 1 : j;  // the last tile may be a short one
-    uint64_t hi = full == 0 ? 0 : floor_sum(full, KB, tokens, (uint64_t)past + tokens + KB - 1);
-    if (full != j) hi += ((uint64_t)past + n + KB - 1) / KB;
+    uint64_t hi = full == 0 ? 0 : floor_sum(full, KB, tokens, past + tokens + KB - 1);
+    if (full != j) hi += (past + n + KB - 1) / KB;
     if (window == 0) return hi;
     // a tile's first row sees nothing before past + j * tokens - window + 1
     const uint32_t from = past + 1 >= window ? 0 : (window - 1 - past + tokens - 1) / tokens;
-    return from >= j ? hi : hi - floor_sum(j - from, KB, tokens, (uint64_t)past + (uint64_t)from * tokens + 1 - window);
+    return from >= j ? hi : hi - floor_sum(j - from, KB, tokens, past + from * tokens + 1 - window);
   }
   template <uint32_t KB>
   __device__ __forceinline__ void tile_blocks(uint32_t j, uint32_t tokens, uint32_t window, uint32_t *lo, uint32_t *hi) const {
-    const uint64_t first = (uint64_t)j * tokens, last = min((uint64_t)n, first + tokens);
-    *hi = (uint32_t)((past + last + KB - 1) / KB);
-    *lo = window && past + first + 1 > window ? (uint32_t)((past + first + 1 - window) / KB) : 0u;
+    const uint32_t first = j * tokens, last = min(n, first + tokens);
+    *hi = (past + last + KB - 1) / KB;
+    *lo = window && past + first + 1 > window ? (past + first + 1 - window) / KB : 0u;
   }
 };
 
 // How heads and rows of a layer lie in tiles of R rows: heads of a group are taken `heads` at a time.
 struct TileShape {
   uint32_t group, chunks, heads, tokens, v_heads;
-  __host__ __device__ TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R) {
+  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R) {
     group = q_heads / kv_heads;
     chunks = (group + R - 1) / R;
     heads = (group + chunks - 1) / chunks;
@@ -90,78 +100,145 @@ __device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, ui
   return w;
 }
 
-// Where a CTA's run of blocks starts.
+// The cut of a batch's blocks into runs, and where this CTA's starts.
 struct RunStart {
-  uint64_t total;   // blocks of the batch
-  uint64_t offset;  // of the run's first block in its sequence
-  uint32_t seq;
-  uint32_t parts;   // CTAs that share the work
+  uint64_t total, each;  // blocks of the batch, blocks of a run: `more` runs have one more
+  uint32_t parts, more;  // CTAs that share the work
+  uint32_t seq;          // the sequence of the run's first block
+  uint32_t v_head, tile, from;  // its head, its tile, and the tile's blocks before it
+  SeqWork w;
+};
+// First block of a CTA's run.
+__device__ __forceinline__ uint64_t run_first(const RunStart &r, uint32_t cta) { return r.each * cta + min(cta, r.more); }
+// The CTA whose run holds block x.
+__device__ __forceinline__ uint32_t run_of(const RunStart &r, uint64_t x) {
+  const uint64_t wide = (r.each + 1) * r.more;
+  return x < wide ? (uint32_t)divided(x, r.each + 1) : r.more + (uint32_t)divided(x - wide, r.each);
+}
+
+struct RunFound {
+  uint64_t sums[16], more_sums[16];
+  uint64_t offset, per_head;
+  SeqWork w;
+  uint32_t seq, tile, from;
 };
 
-// All threads of the CTA; `work`: 2 * THREADS / 32 + 4 words of 64 bits in shared memory.  Threads take consecutive sequences each.
-template <uint32_t KB, uint32_t THREADS>
-__device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t window, uint32_t min_n, uint32_t max_n, uint32_t cta, uint32_t ctas,
-                             uint32_t min_blocks, uint64_t *work) {
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (kv.n_seqs + THREADS - 1) / THREADS;
-  const uint32_t s0 = min(kv.n_seqs, tid * each), s1 = min(kv.n_seqs, s0 + each);
-  uint64_t mine = 0;
-  for (uint32_t s = s0; s < s1; s++) {
-    const SeqWork w = seq_work(kv, s, ts.tokens, min_n, max_n);
-    mine += w.blocks_before<KB>(w.tiles, ts.tokens, window) * ts.v_heads;
-  }
+// Sum of `mine` over the threads before this one, and over all; `sums`: a word for each warp.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint64_t scan_threads(uint64_t mine, uint64_t *sums, uint64_t *total) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const uint64_t o = __shfl_up_sync(0xFFFFFFFFu, incl, d);
     if (lane >= (uint32_t)d) incl += o;
   }
-  if (lane == 31) work[warp] = incl;
+  if (lane == 31) sums[warp] = incl;
   __syncthreads();
-  uint64_t before = 0, total = 0;
+  uint64_t before = 0, all = 0;
+#pragma unroll
   for (uint32_t i = 0; i < THREADS / 32; i++) {
-    const uint64_t v = work[i];
+    const uint64_t v = sums[i];
     before += i < warp ? v : 0;
-    total += v;
+    all += v;
   }
-  const uint64_t first = before + incl - mine;
+  *total = all;
+  return before + incl - mine;
+}
+
+// All threads of the CTA (16 warps at most), which take consecutive sequences each; `found` in shared memory.
+template <uint32_t KB, uint32_t THREADS>
+__device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t window, uint32_t min_n, uint32_t max_n, uint32_t cta, uint32_t ctas,
+                             uint32_t min_blocks, RunFound &found) {
+  const uint32_t tid = threadIdx.x, each = (kv.n_seqs + THREADS - 1) / THREADS;
+  const uint32_t s0 = min(kv.n_seqs, tid * each), s1 = min(kv.n_seqs, s0 + each);
+  uint64_t mine = 0, per_head = 0, total;
+  SeqWork w{};
+  for (uint32_t s = s0; s < s1; s++) {
+    w = seq_work(kv, s, ts.tokens, min_n, max_n);
+    per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window);
+    mine += per_head * ts.v_heads;
+  }
+  const uint64_t first = scan_threads<THREADS>(mine, found.sums, &total);
   RunStart r;
   r.total = total;
-  r.parts = (uint32_t)max((uint64_t)1, min((uint64_t)ctas, total / min_blocks));
-  const uint64_t x0 = cta < r.parts ? total * cta / r.parts : total;
-  uint64_t *found = work + THREADS / 32;
-  if (tid == 0) found[0] = kv.n_seqs, found[1] = 0;
-  __syncthreads();
+  r.parts = (uint32_t)max((uint64_t)1, min((uint64_t)ctas, min_blocks == 1 ? total : divided(total, min_blocks)));
+  r.each = divided(total, r.parts);
+  r.more = (uint32_t)(total - r.each * r.parts);
+  const uint64_t x0 = run_first(r, min(cta, r.parts));
   if (x0 >= first && x0 < first + mine) {
     uint64_t at = first;
-    for (uint32_t s = s0; s < s1; s++) {
-      const SeqWork w = seq_work(kv, s, ts.tokens, min_n, max_n);
-      const uint64_t u = w.blocks_before<KB>(w.tiles, ts.tokens, window) * ts.v_heads;
-      if (x0 < at + u) {
-        found[0] = s, found[1] = x0 - at;
-        break;
+    uint32_t s = s0;
+    if (s1 - s0 > 1) {
+      for (;; s++) {
+        w = seq_work(kv, s, ts.tokens, min_n, max_n);
+        per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window);
+        if (x0 < at + per_head * ts.v_heads) break;
+        at += per_head * ts.v_heads;
       }
-      at += u;
     }
+    found.seq = s, found.offset = x0 - at, found.per_head = per_head, found.w = w;
   }
+  if (tid == 0) found.tile = 0;
   __syncthreads();
-  r.seq = (uint32_t)found[0];
-  r.offset = found[1];
+  if (cta >= r.parts || total == 0) return r;  // no run
+  r.seq = found.seq, r.w = found.w;
+  r.v_head = (uint32_t)divided(found.offset, found.per_head);
+  const uint64_t x = found.offset - r.v_head * found.per_head;
+  if (r.w.tiles > 1) {  // threads take consecutive tiles each
+    const uint32_t some = (r.w.tiles + THREADS - 1) / THREADS, j0 = min(r.w.tiles, tid * some), j1 = min(r.w.tiles, j0 + some);
+    uint32_t lo, hi;
+    mine = 0;
+    for (uint32_t j = j0; j < j1; j++) r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi), mine += hi - lo;
+    uint64_t at = scan_threads<THREADS>(mine, found.more_sums, &total);
+    if (x >= at && x < at + mine) {
+      for (uint32_t j = j0;; j++) {
+        r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi);
+        if (x < at + (hi - lo)) {
+          found.tile = j, found.from = (uint32_t)(x - at);
+          break;
+        }
+        at += hi - lo;
+      }
+    }
+    __syncthreads();
+    r.tile = found.tile, r.from = found.from;
+  } else {
+    r.tile = 0, r.from = (uint32_t)x;
+  }
   return r;
 }
 
-// The tile of a head that holds block `x` of the head's, and how many blocks the tiles before it have.  A whole warp; every lane tries a tile.
-template <uint32_t KB>
-__device__ __forceinline__ uint32_t find_tile(const SeqWork &w, uint32_t tokens, uint32_t window, uint64_t x, uint64_t *before) {
-  uint32_t lo = 0, hi = w.tiles;  // blocks_before(lo) <= x < blocks_before(hi)
-  while (hi - lo > 1) {
-    const uint32_t step = (hi - lo + 31) / 32, j = min(hi, lo + step * ((threadIdx.x & 31) + 1));
-    const uint32_t below = __ballot_sync(0xFFFFFFFFu, j < hi && w.blocks_before<KB>(j, tokens, window) <= x);
-    const uint32_t k = __popc(below);
-    hi = min(hi, lo + step * (k + 1));
-    lo += step * k;
+// Where the tokens of a sequence lie, for one key head.
+struct PagePlaces {
+  const uint32_t *pages;
+  uint32_t widest, n_pages, page_tokens, page, token, head;  // the strides in pieces of 16 bytes
+  FastDiv div;
+
+  __device__ __forceinline__ PagePlaces(const KvBatchDev &kv, uint32_t page_tokens_, uint32_t seq, uint32_t kv_head)
+      : pages(kv.page_table + (uint64_t)seq * kv.table_stride), widest(kv.table_stride), n_pages(kv.n_pages), page_tokens(page_tokens_),
+        page((uint32_t)(kv.page_stride / 8)), token((uint32_t)(kv.token_stride / 8)), head(kv_head * (uint32_t)(kv.head_stride / 8)), div(kv.page_tokens) {}
+  // The entry of the table for a token: to be asked for well before the place.
+  __device__ __forceinline__ uint32_t entry(uint32_t key) const {
+    const uint32_t slot = divided(key, div);
+    return slot < widest ? __ldg(pages + slot) : 0xFFFFFFFFu;
   }
-  *before = w.blocks_before<KB>(lo, tokens, window);
-  return lo;
+  __device__ __forceinline__ uint32_t in_page(uint32_t key) const { return key - divided(key, div) * page_tokens; }
+  // The token's place in pieces of 16 bytes; ~0 and `bad` where the page is not there.
+  __device__ __forceinline__ uint32_t place(uint32_t key, uint32_t number, uint32_t *bad) const {
+    if (number >= n_pages) {
+      *bad = 1;
+      return 0xFFFFFFFFu;
+    }
+    return number * page + in_page(key) * token + head;
+  }
+};
+
+// 64 values of a run of tokens of a page, swizzled; zeros where the page number is not one of the map's.
+__device__ __forceinline__ void page_g2s(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t token, uint32_t head, uint32_t page, bool head_first, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x),
+               "r"(head_first ? head : token), "r"(head_first ? token : head), "r"(page), "r"(bar)
+               : "memory");
 }
 
 // Which tile a CTA works on: its place in the batch and in the run.

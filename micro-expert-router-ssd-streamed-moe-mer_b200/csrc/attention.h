@@ -4,6 +4,17 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+// Division of numbers below 2^31 by a constant of a launch.
+struct FastDiv {
+  uint32_t mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f{0, 0};
+  while ((1ull << f.shift) < d) f.shift++;
+  f.mul = (uint32_t)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+  return f;
+}
+
 // One installed layer (mer_attention_install); the pointers are device memory.
 struct AttnLayer {
   uint32_t q_heads, kv_heads, head_dim, page_tokens;
@@ -18,10 +29,14 @@ struct AttnLayer {
   const float *sinks;             // [q_heads] or null
 };
 
+// A token's place in the pages as a 32-bit number of 16-byte pieces.
+#define KV_MAX_SPAN (((1ull << 32) - 1) * 8)
+
 // mer_kv_batch as the kernels take it.
 struct KvBatchDev {
   void *k_pages, *v_pages;
-  uint64_t page_stride, token_stride, head_stride;  // in values
+  uint64_t page_stride, token_stride, head_stride;  // in values; all places lie below KV_MAX_SPAN
+  FastDiv page_tokens;
   const uint32_t *page_table, *row_start, *kv_len;
   uint32_t n_pages, table_stride, n_seqs, n_rows;
 };

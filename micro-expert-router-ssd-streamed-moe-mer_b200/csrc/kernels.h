@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #define MER_BLOCK_ELEMS 32
 #define MER_Q4_BLOCK_BYTES 18
 #define MER_Q8_BLOCK_BYTES 34
@@ -170,6 +172,20 @@ inline cudaError_t launch_overlapped(void (*kern)(P...), dim3 grid, unsigned blo
   cfg.gridDim = grid, cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = smem, cfg.stream = s;
   cfg.attrs = at, cfg.numAttrs = cooperative ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
+// Lets kernel `Kern` have `bytes` of dynamic shared memory on the current device; the runtime is asked once (0.4 us).
+template <auto Kern>
+inline cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // Pinned host memory <-> device inside a call's own sequence, a few KB (launch_host_out: `rows` rows of `words` words, `stride` apart,

@@ -3,8 +3,8 @@
 //   o = sum_j 2^(s_j - m) v_j / (sum_j 2^(s_j - m) [+ 2^(sink - m)]),  s_j = q . k_j * scale * log2 e,  m = max_j s_j
 //
 // in one pass over the keys with the running maximum and sum of every row.  What bounds it is reading the cache: per 16 tokens 16 * 2 *
-// head_dim values for at most 32 rows of work.  So a warp is a stream of its own: it copies the next chunks of 16 tokens (rows of the pages,
-// 16 bytes a lane, swizzled) into a ring that no other warp sees, multiplies the one that has landed (mma.sync on 16 x 16 tiles; at this rate of
+// head_dim values for at most 32 rows of work.  So a warp is a stream of its own: it copies the next chunks of 16 tokens (tiled copies of 8 or 16
+// tokens of a page; row by row, 16 bytes a lane, where a sequence's end or a window cuts a chunk or pages have no such runs) into a ring that no other warp sees, multiplies the one that has landed (mma.sync on 16 x 16 tiles; at this rate of
 // operations the legacy tensor path is idle most of the time) and keeps maximum, sum and output of its own tokens in registers: no barrier
 // in the loop.  The warps' results are joined in shared memory at the end of a tile, those of several CTAs through the workspace (attention.cuh).
 // The weights go to the second product in the cache's type, 2^-9 (bf16) or 2^-12 (f16) of each at most, like the values they multiply; sums are fp32.
@@ -26,7 +26,9 @@ struct AttendParams {
   void *out;
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
-  uint32_t max_rows;  // sequences with more rows are another kernel's
+  TileShape ts;
+  uint32_t box;  // tokens of a tiled copy (8 or 16), 0: none
+  bool head_first;
 };
 
 // Rows of a tile are MT * 16, warps NW, chunks in flight per warp ST.
@@ -38,11 +40,6 @@ struct StreamShape {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -62,32 +59,37 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Byte offset of 16-byte piece `c` of row `r`; eight rows of one column of pieces lie in eight different bank groups.
-template <int DP>
+// Byte offset of 16-byte piece `c` of row `r` of ROWS: 64 values of every row, then the next 64, in the 128-byte swizzle; eight rows of one
+// column of pieces lie in eight different bank groups.
+template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t piece(uint32_t r, uint32_t c) {
-  return r * (DP * 2) + ((c ^ (r & 7)) << 4);
+  return (c >> 3) * (ROWS * 128) + r * 128 + (((c ^ r) & 7) << 4);
 }
 
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(const AttendParams p) {
+__global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(const AttendParams p, const __grid_constant__ PageMaps maps) {
   using S = StreamShape<DP>;
   constexpr int NW = S::NW, ST = S::ST, R = MT * 16;
   constexpr uint32_t KB = S::KB, THREADS = S::THREADS;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_work[THREADS / 32 + 4];
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ uint64_t s_full[NW * ST];  // a chunk has landed: every lane of its warp arrives
+  __shared__ RunFound s_found;
   __shared__ uint32_t s_flag;
-  uint8_t *s_q = smem;                               // [R][DP], swizzled
-  uint8_t *s_ring = smem + R * DP * 2;               // [NW][ST][k, v][16][DP]
+  uint8_t *s_ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // [NW][ST][k, v][DP / 64][16][64]
+  uint8_t *s_q = s_ring + NW * ST * S::CHUNK;                                  // [DP / 64][R][64]
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t D = p.a.head_dim, page_tokens = p.a.page_tokens, window = p.a.window;
-  const TileShape ts(p.a.q_heads, p.a.kv_heads, R);
+  const TileShape &ts = p.ts;
+  for (uint32_t i = tid; i < NW * ST; i += THREADS) mbar_init(&s_full[i], 32);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, 0, p.max_rows, blockIdx.x, gridDim.x, 1, s_work);
-  if (blockIdx.x == 0) clear_rows_without_place<T, THREADS>(p.a, p.kv, 0, p.max_rows, (T *)p.out, p.out_stride, p.ws.status);
+  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, 1, s_found);
+  if (blockIdx.x == 0) clear_rows_without_place<T, THREADS>(p.a, p.kv, 0, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run.parts) return;
-  RunWalk<KB> walk(p.kv, ts, window, 0, p.max_rows, run);
+  RunWalk<KB> walk(p.kv, ts, window, 0, 0xFFFFFFFFu, run);
   const float to_log2 = p.a.scale * LOG2E;
+  uint32_t fill = 0, stage = 0, stage_phase = 0, timed_out = 0;  // of the warp's ring: what is asked for next, what is taken next
   const uint32_t ring = smem_u32(s_ring) + warp * (ST * S::CHUNK), q_addr = smem_u32(s_q);
 
   TileWork t;
@@ -95,47 +97,59 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
     const uint32_t rows = t.tokens * t.heads;
     const uint32_t end = t.past + t.token0 + t.tokens;  // behind the last token that a row of the tile sees
     const uint32_t start = window && t.past + t.token0 + 1 > window ? t.past + t.token0 + 1 - window : 0;
-    const uint32_t *pages = p.kv.page_table + (uint64_t)t.seq * p.kv.table_stride;
-    // ---- the ring: lanes 0 .. 15 know where the chunk's tokens lie, one chunk ahead
+    // ---- the ring.  A lane knows where its part of a chunk lies, ST chunks ahead: lanes 0 .. 15 a row of one that is copied row by row; of others, the first
+    // lanes a tiled copy of the keys each, the next ones of the values.
+    const PagePlaces pages(p.kv, page_tokens, t.seq, t.kv_head);
+    constexpr uint32_t SUBS = DP / 64;
+    const uint32_t copies = p.box ? 16 / p.box * SUBS : 0, copy = lane < copies ? lane : lane - copies, copy_row = copy / SUBS * p.box;
     uint32_t bad = 0;
-    auto look_up = [&](uint32_t blk) -> uint64_t {  // the lane's token in the pages, in values; ~0: not to be read
-      const uint32_t key = blk * KB + warp * 16 + (lane & 15);
-      if (blk >= t.hi || key < start || key >= end) return ~0ull;
-      const uint32_t slot = key / page_tokens;
-      const uint32_t page = slot < p.kv.table_stride ? __ldg(pages + slot) : 0xFFFFFFFFu;
-      if (page >= p.kv.n_pages) {
-        bad = 1;
-        return ~0ull;
+    auto wanted = [&](uint32_t blk) { return blk < t.hi && blk * KB + warp * 16 < end && blk * KB + warp * 16 + 16 > start; };
+    auto tiled = [&](uint32_t blk) { return p.box && blk * KB + warp * 16 >= start && blk * KB + warp * 16 + 16 <= end; };
+    auto key_of = [&](uint32_t blk) { return blk * KB + warp * 16 + (tiled(blk) ? copy_row : lane & 15); };
+    auto to_read = [&](uint32_t blk) { return wanted(blk) && (tiled(blk) ? lane < 2 * copies : key_of(blk) >= start && key_of(blk) < end); };
+    auto entry = [&](uint32_t blk) { return to_read(blk) ? pages.entry(key_of(blk)) : 0u; };
+    auto issue = [&](uint32_t blk, uint32_t number) {
+      if (!wanted(blk)) return;
+      const uint32_t dst = ring + fill * S::CHUNK, bar = smem_u32(&s_full[warp * ST + fill]);
+      fill = fill + 1 == ST ? 0 : fill + 1;
+      if (tiled(blk)) {
+        if (start) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage may have been filled row by row
+        if (lane < 2 * copies) {
+          if (number >= p.kv.n_pages) bad = 1;
+          const bool v = lane >= copies;
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(p.box * 128) : "memory");
+          page_g2s(dst + (v ? 16 * DP * 2 : 0) + (copy % SUBS) * 2048 + copy_row * 128, v ? &maps.v : &maps.k, (copy % SUBS) * 64, pages.in_page(key_of(blk)), t.kv_head,
+                   min(number, p.kv.n_pages), p.head_first, bar);
+        } else {
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+        }
+        return;
       }
-      return page * p.kv.page_stride + (uint64_t)(key - slot * page_tokens) * p.kv.token_stride + t.kv_head * p.kv.head_stride;
-    };
-    auto issue = [&](uint64_t place, uint32_t stage) {
-      const uint32_t dst = ring + stage * S::CHUNK;
+      const uint32_t place = to_read(blk) ? pages.place(key_of(blk), number, &bad) : 0xFFFFFFFFu;
 #pragma unroll
       for (int i = 0; i < DP / 16; i++) {
         const uint32_t idx = i * 32 + lane, r = idx / (DP / 8), c = idx % (DP / 8);
-        const uint64_t at = __shfl_sync(0xFFFFFFFFu, place, r);
-        const bool in = at != ~0ull && c * 8 < D;
-        const uint64_t off = in ? at + c * 8 : 0;
-        cp_async16(dst + piece<DP>(r, c), (const T *)p.kv.k_pages + off, in ? 16 : 0);
-        cp_async16(dst + 16 * DP * 2 + piece<DP>(r, c), (const T *)p.kv.v_pages + off, in ? 16 : 0);
+        const uint32_t at = __shfl_sync(0xFFFFFFFFu, place, r);
+        const bool in = at != 0xFFFFFFFFu && c * 8 < D;
+        const uint64_t off = in ? ((uint64_t)at + c) * 16 : 0;
+        cp_async16(dst + piece<16>(r, c), (const char *)p.kv.k_pages + off, in ? 16 : 0);
+        cp_async16(dst + 16 * DP * 2 + piece<16>(r, c), (const char *)p.kv.v_pages + off, in ? 16 : 0);
       }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     };
-    uint64_t ahead = look_up(t.lo);
+    uint32_t ahead[ST];
 #pragma unroll
-    for (int i = 0; i < ST - 1; i++) {
-      const uint64_t place = ahead;
-      ahead = look_up(t.lo + i + 1);
-      if (t.lo + i < t.hi) issue(place, i);
-      cp_async_commit();
-    }
+    for (int i = 0; i < ST; i++) ahead[i] = entry(t.lo + i);
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) issue(t.lo + i, ahead[i]);
+    uint32_t next_entry = ahead[ST - 1];
     // ---- queries, while the first chunks are on their way
     for (uint32_t i = tid; i < R * (DP / 8); i += THREADS) {
       const uint32_t r = i / (DP / 8), c = i % (DP / 8), tok = r / t.heads, h = r - tok * t.heads;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < rows && c * 8 < D)
         v = __ldg(reinterpret_cast<const uint4 *>((const T *)p.q + (uint64_t)(t.row0 + t.token0 + tok) * p.q_stride + (uint64_t)(t.head0 + h) * D + c * 8));
-      *reinterpret_cast<uint4 *>(s_q + piece<DP>(r, c)) = v;
+      *reinterpret_cast<uint4 *>(s_q + piece<R>(r, c)) = v;
     }
     __syncthreads();
     // tokens that the lane's rows see: (first, last] of each
@@ -154,20 +168,17 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
       m[mt][0] = m[mt][1] = -INFINITY;
       l[mt][0] = l[mt][1] = 0.0f;
     }
-    uint32_t stage = 0, fill = ST - 1;
     for (uint32_t blk = t.lo; blk < t.hi; blk++) {
       {
-        const uint64_t place = ahead;
-        ahead = look_up(blk + ST);
-        if (blk + ST - 1 < t.hi) issue(place, fill);
-        cp_async_commit();
-        fill = fill + 1 == ST ? 0 : fill + 1;
+        const uint32_t number = next_entry;
+        next_entry = entry(blk + ST);
+        __syncwarp();  // the chunk that lay in this stage has been read
+        issue(blk + ST - 1, number);
       }
-      cp_async_wait<ST - 1>();
-      __syncwarp();
+      if (!wanted(blk)) continue;
       const uint32_t key0 = blk * KB + warp * 16, base = ring + stage * S::CHUNK;
-      stage = stage + 1 == ST ? 0 : stage + 1;
-      if (key0 >= end || key0 + 16 <= start) continue;
+      timed_out |= !mbar_wait(&s_full[warp * ST + stage], stage_phase);
+      stage = stage + 1 == ST ? 0 : stage + 1, stage_phase ^= stage == 0;
       float s[MT][2][4];
 #pragma unroll
       for (int mt = 0; mt < MT; mt++)
@@ -178,11 +189,11 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
 #pragma unroll
       for (int kk = 0; kk < DP / 16; kk++) {
         uint32_t kf[4];
-        ldm4(kf, base + piece<DP>((lane / 16) * 8 + (lane & 7), kk * 2 + ((lane >> 3) & 1)));
+        ldm4(kf, base + piece<16>((lane / 16) * 8 + (lane & 7), kk * 2 + ((lane >> 3) & 1)));
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
           uint32_t qf[4];
-          ldm4(qf, q_addr + piece<DP>(mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4)));
+          ldm4(qf, q_addr + piece<R>(mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4)));
           mma16816<T>(s[mt][0], qf, kf[0], kf[1]);
           mma16816<T>(s[mt][1], qf, kf[2], kf[3]);
         }
@@ -237,7 +248,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
 #pragma unroll
       for (int dn = 0; dn < DP / 16; dn++) {
         uint32_t vf[4];
-        ldm4_trans(vf, vbase + piece<DP>(((lane >> 3) & 1) * 8 + (lane & 7), dn * 2 + (lane >> 4)));
+        ldm4_trans(vf, vbase + piece<16>(((lane >> 3) & 1) * 8 + (lane & 7), dn * 2 + (lane >> 4)));
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
           mma16816<T>(o[mt][2 * dn], pf[mt], vf[0], vf[1]);
@@ -245,9 +256,9 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         }
       }
     }
-    cp_async_wait<0>();
     if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
     // ---- the warps' results: [warp][row] maximum and sum, [warp][row][DP] output, where the rings were
+    constexpr int OP = DP + 8;  // floats of a row of it: the rows of a fragment lie in different banks
     float *s_m = reinterpret_cast<float *>(s_ring), *s_l = s_m + NW * R, *s_o = s_l + NW * R;
     __syncthreads();
 #pragma unroll
@@ -258,10 +269,11 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
         const uint32_t r = mt * 16 + e * 8 + lane / 4;
+        if (r >= rows) continue;
         if ((lane & 3) == 0) s_m[warp * R + r] = m[mt][e], s_l[warp * R + r] = sum;
 #pragma unroll
         for (int i = 0; i < DP / 8; i++)
-          *reinterpret_cast<float2 *>(s_o + ((size_t)warp * R + r) * DP + i * 8 + (lane & 3) * 2) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+          *reinterpret_cast<float2 *>(s_o + ((size_t)warp * R + r) * OP + i * 8 + (lane & 3) * 2) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
       }
     __syncthreads();
     const bool whole = t.lo == t.tile_lo && t.hi == t.tile_hi;
@@ -275,7 +287,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
 #pragma unroll
       for (int w = 0; w < NW; w++) {
         const float mw = s_m[w * R + r], f = mw == -INFINITY ? 0.0f : exp2_approx(mw - top);
-        const float4 v = *reinterpret_cast<const float4 *>(s_o + ((size_t)w * R + r) * DP + c);
+        const float4 v = *reinterpret_cast<const float4 *>(s_o + ((size_t)w * R + r) * OP + c);
         sum = fmaf(f, s_l[w * R + r], sum);
         acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
       }
@@ -286,28 +298,86 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         *reinterpret_cast<float4 *>(part + 2 * R + (size_t)r * DP + c) = acc;
       }
     }
-    __syncthreads();
     if (!whole) {
-      join_parts<T, R, DP, THREADS>(p.a, t, run, rows, p.ws, (T *)p.out, p.out_stride, &s_flag, [] { __syncthreads(); });
       __syncthreads();
+      // The CTA that arrives last joins the parts in the order of the runs and leaves the count at zero: a warp a row, its lanes first over the parts (their
+      // factors), then over the row's values.
+      uint32_t c0, n;
+      runs_of_tile(run, t, &c0, &n);
+      if (tid == 0) {
+        const bool is_last = arrive_acq_rel(p.ws.counts + c0) + 1 == n;
+        if (is_last) p.ws.counts[c0] = 0;
+        s_flag = is_last;
+      }
+      __syncthreads();
+      if (s_flag) {
+        constexpr int V = DP / 32;  // values of a lane
+        const float *first = part_of_tile(run, t, p.ws.parts, c0, 0, part_floats(R, DP)), *others = part_of_tile(run, t, p.ws.parts, c0, 1, part_floats(R, DP));
+        auto part_of = [&](uint32_t k) { return k == 0 ? first : others + (size_t)(k - 1) * (2 * part_floats(R, DP)); };
+        for (uint32_t r = warp; r < rows; r += NW) {
+          float top = -INFINITY, total = 0.0f, acc[V];
+          for (uint32_t k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(part_of(k) + r));
+#pragma unroll
+          for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+#pragma unroll
+          for (int i = 0; i < V; i++) acc[i] = 0.0f;
+          for (uint32_t k0 = 0; k0 < n; k0 += 32) {
+            float f = 0.0f;
+            if (k0 + lane < n) {
+              const float *from = part_of(k0 + lane);
+              const float mk = __ldcg(from + r);
+              f = mk == -INFINITY ? 0.0f : exp2_approx(mk - top);
+              total = fmaf(f, __ldcg(from + R + r), total);
+            }
+            const float *row = part_of(k0) + 2 * R + (size_t)r * DP + lane * V;
+            const uint32_t some = min(32u, n - k0);
+#pragma unroll 8
+            for (uint32_t k = 0; k < some; k++) {
+              const float fk = __shfl_sync(0xFFFFFFFFu, f, k);
+              float v[V];
+              if constexpr (V == 2)
+                *reinterpret_cast<float2 *>(v) = __ldcg(reinterpret_cast<const float2 *>(row));
+              else
+#pragma unroll
+                for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(v + i) = __ldcg(reinterpret_cast<const float4 *>(row + i));
+#pragma unroll
+              for (int i = 0; i < V; i++) acc[i] = fmaf(fk, v[i], acc[i]);
+              row = k0 + k == 0 ? others + 2 * R + (size_t)r * DP + lane * V : row + 2 * part_floats(R, DP);
+            }
+          }
+#pragma unroll
+          for (int d = 16; d; d /= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+          const uint32_t tok = r / t.heads, head = t.head0 + r - tok * t.heads;
+          if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
+          const float f = total == 0.0f ? 0.0f : 1.0f / total;
+          T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D + lane * V;
+#pragma unroll
+          for (int i = 0; i < V; i += 2)
+            if (lane * V + i < D) reinterpret_cast<uint32_t *>(out)[i / 2] = Num<T>::pack(acc[i] * f, acc[i + 1] * f);
+        }
+      }
     }
+    // the rings are tiled copies' again
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
   }
+  if (timed_out) atomicOr(p.ws.status, MER_DEVSTAT_TIMEOUT);
 }
 
 template <typename T, int DP, int MT>
-cudaError_t launch_stream(const AttendParams &p, int sm_count, cudaStream_t s) {
+cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
   using S = StreamShape<DP>;
-  constexpr size_t SMEM = (size_t)MT * 16 * DP * 2 + (size_t)S::NW * S::ST * S::CHUNK;
-  static_assert((size_t)S::NW * MT * 16 * (DP + 2) * 4 <= (size_t)S::NW * S::ST * S::CHUNK, "the warps' results lie in the rings");
-  const cudaError_t e = cudaFuncSetAttribute(k_attend_stream<T, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+  constexpr size_t SMEM = 1024 + (size_t)MT * 16 * DP * 2 + (size_t)S::NW * S::ST * S::CHUNK;
+  static_assert((size_t)S::NW * MT * 16 * (DP + 10) * 4 <= (size_t)S::NW * S::ST * S::CHUNK, "the warps' results lie in the rings");
+  const cudaError_t e = allow_smem<k_attend_stream<T, DP, MT>>(SMEM);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(k_attend_stream<T, DP, MT>, dim3(sm_count), S::THREADS, SMEM, s, false, p);
+  return launch_overlapped(k_attend_stream<T, DP, MT>, dim3(sm_count), S::THREADS, SMEM, s, false, p, maps);
 }
 template <typename T>
-cudaError_t launch_stream(const AttendParams &p, bool two, int sm_count, cudaStream_t s) {
-  if (p.a.head_dim <= 64) return two ? launch_stream<T, 64, 2>(p, sm_count, s) : launch_stream<T, 64, 1>(p, sm_count, s);
-  if (p.a.head_dim <= 128) return two ? launch_stream<T, 128, 2>(p, sm_count, s) : launch_stream<T, 128, 1>(p, sm_count, s);
-  return launch_stream<T, 256, 1>(p, sm_count, s);
+cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, bool two, int sm_count, cudaStream_t s) {
+  if (p.a.head_dim <= 64) return two ? launch_stream<T, 64, 2>(p, maps, sm_count, s) : launch_stream<T, 64, 1>(p, maps, sm_count, s);
+  if (p.a.head_dim <= 128) return two ? launch_stream<T, 128, 2>(p, maps, sm_count, s) : launch_stream<T, 128, 1>(p, maps, sm_count, s);
+  return launch_stream<T, 256, 1>(p, maps, sm_count, s);
 }
 
 }  // namespace
@@ -324,6 +394,9 @@ cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *
   const uint64_t rows = (uint64_t)(a.q_heads / a.kv_heads) * ((kv.n_rows + kv.n_seqs - 1) / kv.n_seqs);
   *launches += 1;
   if (rows > 32 && a.head_dim <= 128) return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
-  AttendParams p{a, kv, q, out, q_stride, out_stride, ws, 0xFFFFFFFFu};
-  return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, rows > 16, sm_count, s) : launch_stream<__nv_bfloat16>(p, rows > 16, sm_count, s);
+  const PageMapShape m(a, kv, 16);
+  PageMaps maps{};
+  const bool mapped = encode_page_maps(&maps, m, a, kv);
+  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, rows > 16 && a.head_dim <= 128 ? 32 : 16), mapped ? m.rows : 0, m.head_first};
+  return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, rows > 16, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, rows > 16, sm_count, s);
 }

@@ -6,13 +6,14 @@
 //   P = 2^(S * scale - m + shift)               a thread owns a row: its maximum and sum need no other thread
 //   O[128 x d] += P[128 x 128] V[128 x d]       P from tensor memory, where it takes the place of S; V's rows run along N
 //
-//   * Warps 0..3 and 4..7 are the softmax of one group of rows each, warp 8 issues the MMAs, warps 9 and 10 copy.  While one group's
+//   * Warps 0..3 and 4..7 are the softmax of one group of rows each, warps 8..11 copy, warp 12 issues the MMAs (13..15 fill its group).  While one group's
 //     softmax runs the tensor core multiplies for the other: [P V of block j, Q K of block j + 1] of one, then of the other.
 //   * The reference maximum of a row follows its maximum only when that has grown by more than 2^LAG; then alone the output in tensor memory is rescaled, by
 //     the softmax warps themselves.  Until then weights are larger than 1 by up to that factor, which f16 and fp32 hold.  What makes that safe without a
 //     barrier: the MMAs complete in order, so the S of block j being there says that the P V of block j - 1 has been added.
-//   * Keys and values come as rows of the pages, 16 bytes a lane (cp.async), whatever the page size is, and are written in the
-//     swizzle that the MMA reads; a copying warp makes its rows visible to the tensor core (proxy fence) and arrives.
+//   * Keys and values come by tiled copies of runs of tokens of a page, 64 values wide; blocks that a sequence's end or a window cuts, and pages that
+//     have no such runs (of 1 or 5 tokens, say), row by row, 16 bytes a lane (cp.async), zeros where nothing is to be read.  Row by row alone a
+//     block took 4000 cycles.
 //   * Rows of P that see nothing of a block hold zeros, and what no row sees is filled with zeros instead of being read.
 // What bounds it: exponentials and MMAs, 2048 cycles each for a block of both groups at 16 and 8192 a cycle.
 // Every wait is bounded; on expiry the CTA latches MER_DEVSTAT_TIMEOUT, stops issuing work, waits (bounded) for what is in flight,
@@ -35,10 +36,16 @@ struct TcParams {
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
   uint32_t min_blocks;
+  TileShape ts;
+  uint32_t box;  // tokens of a tiled copy, 0: none
+  bool head_first;
 };
 
-constexpr uint32_t TC_R = 256, TC_KB = 128, TC_WARPS = 11, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
-constexpr uint32_t TC_MMA = 8, TC_LOAD = 9, TC_LOADERS = 2;
+constexpr uint32_t TC_R = 256, TC_KB = 128, TC_WARPS = 16, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
+constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12;
+// Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
+constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
+static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
 constexpr float LAG = 3.0f;  // with P_SHIFT the largest weight is 2^15
 constexpr uint32_t TC_CONTROL = 1024;  // barriers and words in front of the operands
 
@@ -54,8 +61,8 @@ struct TcShape {
 struct TcControl {
   uint64_t full[10], empty[10];  // stages of the ring
   uint64_t q_full, q_empty, s_full[2], p_ready[2], o_full[2], soft, drain;
-  uint64_t work[TC_THREADS / 32 + 4];
-  uint32_t tmem, flag;
+  RunFound found;
+  uint32_t tmem, flag[2];  // flags take turns: a sync lies between two uses of one
   volatile uint32_t abort;
 };
 static_assert(sizeof(TcControl) <= TC_CONTROL, "control block");
@@ -70,7 +77,7 @@ __device__ __forceinline__ void copies_left() {
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
+__global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, const __grid_constant__ PageMaps maps) {
   using S = TcShape<DP>;
   extern __shared__ __align__(16) uint8_t smem[];
   TcControl &ctl = *reinterpret_cast<TcControl *>(smem);
@@ -78,10 +85,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
   const uint32_t s_q = operands, s_ring = operands + 2 * S::QTILE;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t D = p.a.head_dim, window = p.a.window;
-  const TileShape ts(p.a.q_heads, p.a.kv_heads, TC_R);
+  const TileShape &ts = p.ts;
   if (tid == 0) {
-    for (uint32_t i = 0; i < S::STAGES; i++) mbar_init(&ctl.full[i], TC_LOADERS), mbar_init(&ctl.empty[i], 1);
-    mbar_init(&ctl.q_full, TC_LOADERS), mbar_init(&ctl.q_empty, 1);
+    for (uint32_t i = 0; i < S::STAGES; i++) mbar_init(&ctl.full[i], TC_LOADERS * 32), mbar_init(&ctl.empty[i], 1);
+    mbar_init(&ctl.q_full, TC_LOADERS * 32), mbar_init(&ctl.q_empty, 1);
     for (int x = 0; x < 2; x++) mbar_init(&ctl.s_full[x], 1), mbar_init(&ctl.p_ready[x], 4), mbar_init(&ctl.o_full[x], 1);
     mbar_init(&ctl.soft, SOFT_THREADS / 32), mbar_init(&ctl.drain, 1);
     ctl.abort = 0;
@@ -89,7 +96,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
   }
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.work);
+  const RunStart run = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
   if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, 0, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run.parts) return;
   if (warp == TC_MMA) {
@@ -115,11 +122,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
   auto aborted = [&] { return __any_sync(0xFFFFFFFFu, ctl.abort) != 0; };
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
     // ---------------------------------------------------------------- softmax: a thread has row x * 128 + (tid & 127) of the tile
     const uint32_t x = warp >> 2, row = tid;
     const uint32_t tm_lane = tm + ((warp & 3) << 21), s_at = tm_lane + x * 128, o_at = tm_lane + 256 + x * DP;
     const float to_log2 = p.a.scale * LOG2E;
-    uint32_t blocks = 0, tiles = 0, syncs = 0;  // phases of s_full, o_full, soft
+    uint32_t blocks = 0, tiles = 0, syncs = 0, flags = 0;  // phases of s_full, o_full, soft; uses of the flags
     auto sync = [&] {
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.soft);
@@ -138,18 +146,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
         for (uint32_t blk = t.lo; blk < t.hi; blk++, blocks++) {
           if (!wait(&ctl.s_full[x], blocks & 1)) break;
           tm_fence_after();
-          float s[128];
-          tm_load(s_at, s);
+          float s[4][32];
+#pragma unroll
+          for (int h = 0; h < 4; h++) tm_load_begin(s_at + h * 32, s[h]);
+          tm_wait_load();
+#pragma unroll
+          for (int h = 0; h < 4; h++) tm_loaded(s[h]);
           const uint32_t key0 = blk * TC_KB;
           if (key0 + TC_KB - 1 > see0 || key0 < least1) {
 #pragma unroll
-            for (int i = 0; i < 128; i++) s[i] = key0 + i <= see && key0 + i >= least ? s[i] : -INFINITY;
+            for (int i = 0; i < 128; i++) s[i / 32][i % 32] = key0 + i <= see && key0 + i >= least ? s[i / 32][i % 32] : -INFINITY;
           }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int i = 0; i < 128; i += 4)
 #pragma unroll
-            for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[i + e]);
+            for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[i / 32][i % 32 + e]);
           const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2;
           const bool grow = now > m + LAG || (m == -INFINITY && now > m);
           if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -175,7 +187,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
             uint32_t v[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-              const float a = exp2_approx(fmaf(s[h * 64 + 2 * i], to_log2, -less)), b = exp2_approx(fmaf(s[h * 64 + 2 * i + 1], to_log2, -less));
+              const float a = exp2_approx(fmaf(s[2 * h + i / 16][2 * i % 32], to_log2, -less)),
+                          b = exp2_approx(fmaf(s[2 * h + i / 16][2 * i % 32 + 1], to_log2, -less));
               sum[i & 3] += a + b;
               v[i] = Num<T>::pack(a, b);
             }
@@ -189,41 +202,94 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
         }
       }
       const bool whole = t.lo == t.tile_lo && t.hi == t.tile_hi;
-      float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(TC_R, DP);
       if (active) {
         if (!wait(&ctl.o_full[x], tiles++ & 1)) break;
         tm_fence_after();
-        const uint32_t tok = row / t.heads, head = t.head0 + row - tok * t.heads;
-        float f = 1.0f;
-        if (whole && row < rows) {
-          const float total = p.a.sinks ? l + exp2_approx(__ldg(p.a.sinks + head) * LOG2E - m + P_SHIFT) : l;
-          f = total == 0.0f ? 0.0f : 1.0f / total;
+      }
+      // The rows of a tile that other runs have parts of.  Its first run comes to it last, at its own end: mostly the others have left their parts by then,
+      // and it adds them to what it has.  Where they have not, it leaves its own like them, and whoever arrives last joins them, in the same order.
+      uint32_t c0 = 0, n = 1, mine = 0;  // `mine`: this CTA has part 0 and all others are there
+      bool joins = whole;
+      if (!whole) {
+        runs_of_tile(run, t, &c0, &n);
+        if (blockIdx.x == c0) {
+          if (tid == 0) ctl.flag[flags & 1] = load_acquire(p.ws.counts + c0) == n - 1;
+          sync();
+          joins = mine = ctl.flag[flags++ & 1];
         }
+      }
+      // Parts lie as [piece of four values][row]: the rows of a warp side by side.
+      float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(TC_R, DP);
+      if (!joins) {
+        if (active) {
+          if (row < rows) part[row] = m, part[TC_R + row] = l;
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            __syncwarp();
+            tm_load(o_at + c, o);
+            if (row < rows) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) reinterpret_cast<float4 *>(part + 2 * TC_R)[(c + i) / 4 * TC_R + row] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+        }
+        sync();
+        if (tid == 0) ctl.flag[flags & 1] = arrive_acq_rel(p.ws.counts + c0) + 1 == n;
+        sync();
+        joins = ctl.flag[flags++ & 1];
+      }
+      if (!whole && joins && tid == 0) p.ws.counts[c0] = 0;
+      if (joins && active) {
+        const bool own = whole || mine;  // part 0 is in tensor memory
+        const uint32_t tok = row / t.heads, head = t.head0 + row - tok * t.heads;
+        // the row's reference and sum over all parts
+        float top = own ? m : -INFINITY, total = own ? l : 0.0f;
+        for (uint32_t k = own ? 1 : 0; k < n; k++) {
+          const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP));
+          Joined j;
+          j.top = top, j.sum = total;
+          j.add(__ldcg(from + row), __ldcg(from + TC_R + row), make_float4(0, 0, 0, 0));
+          top = j.top, total = j.sum;
+        }
+        if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
         T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D;
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           float o[32];
           __syncwarp();
           tm_load(o_at + c, o);
-          if (row >= rows) continue;
-          if (whole) {
+          float mo = own ? m : -INFINITY;
+          for (uint32_t k = own ? 1 : 0; k < n; k++) {
+            const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP));
+            const float mk = __ldcg(from + row), now = fmaxf(mo, mk);
+            const float old = mo == -INFINITY ? 0.0f : exp2_approx(mo - now), g = mk == -INFINITY ? 0.0f : exp2_approx(mk - now);
+            mo = now;
+            float4 v[8];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              const uint4 v = make_uint4(Num<T>::pack(o[i] * f, o[i + 1] * f), Num<T>::pack(o[i + 2] * f, o[i + 3] * f), Num<T>::pack(o[i + 4] * f, o[i + 5] * f),
-                                         Num<T>::pack(o[i + 6] * f, o[i + 7] * f));
-              if (c + i < (int)D) *reinterpret_cast<uint4 *>(out + c + i) = v;
+            for (int i = 0; i < 8; i++) v[i] = __ldcg(reinterpret_cast<const float4 *>(from + 2 * TC_R) + (c / 4 + i) * TC_R + row);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const bool start = k == 0;
+              o[4 * i] = start ? v[i].x : fmaf(g, v[i].x, o[4 * i] * old), o[4 * i + 1] = start ? v[i].y : fmaf(g, v[i].y, o[4 * i + 1] * old);
+              o[4 * i + 2] = start ? v[i].z : fmaf(g, v[i].z, o[4 * i + 2] * old), o[4 * i + 3] = start ? v[i].w : fmaf(g, v[i].w, o[4 * i + 3] * old);
             }
-          } else {
+          }
+          if (row >= rows) continue;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(part + 2 * TC_R + (size_t)row * DP + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 32; i += 8) {
+            const uint4 v = make_uint4(Num<T>::pack(o[i] * f, o[i + 1] * f), Num<T>::pack(o[i + 2] * f, o[i + 3] * f), Num<T>::pack(o[i + 4] * f, o[i + 5] * f),
+                                       Num<T>::pack(o[i + 6] * f, o[i + 7] * f));
+            if (c + i < (int)D) *reinterpret_cast<uint4 *>(out + c + i) = v;
           }
         }
-        if (!whole && row < rows) part[row] = m, part[TC_R + row] = l;
-        tm_fence_before();
       }
-      if (!whole && !aborted()) join_parts<T, TC_R, DP, SOFT_THREADS>(p.a, t, run, rows, p.ws, (T *)p.out, p.out_stride, &ctl.flag, sync);
+      tm_fence_before();
     }
-  } else if (warp == TC_MMA) {
+  } else if (warp >= TC_MMA) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == TC_MMA) {
     // ---------------------------------------------------------------- MMA issue
     const uint32_t leader = tm_elect();
     constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : 1u;
@@ -243,6 +309,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
       const uint32_t groups = t.tokens * t.heads > 128 ? 2 : 1;
       if (!wait(&ctl.q_full, tiles & 1)) break;
       if (!wait(&ctl.full[stage], phase)) break;
+      proxy_fence();
       tm_fence_after();
       for (uint32_t x = 0; x < groups; x++) qk(x, stage);
       tm_commit(leader, &ctl.empty[stage]);
@@ -255,6 +322,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
         next_stage();
         if (!(ok = wait(&ctl.full[v_stage], v_phase))) break;
         if (more && !(ok = wait(&ctl.full[stage], phase))) break;
+        proxy_fence();
         for (uint32_t x = 0; x < groups; x++) {
           if (!(ok = wait(&ctl.p_ready[x], (x ? blocks1 : blocks) & 1))) break;
           tm_fence_after();
@@ -283,87 +351,91 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
       tm_commit(leader, &ctl.drain);
       mbar_drain(&ctl.drain, 0, 1000000000ull);
     }
+    }
   } else {
-    // ---------------------------------------------------------------- copies: warp w has the rows w * 64 .. of a block, and half of the queries
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    // ---------------------------------------------------------------- copies: warp w has the rows w * 32 .. of a block, and a quarter of the queries
     const uint32_t w = warp - TC_LOAD;
     uint32_t stage = 0, phase = 0, tiles = 0, bad = 0;
-    uint64_t *pending[3] = {nullptr, nullptr, nullptr};  // barriers of the copies in flight, the newest first
-    auto landed = [&](uint64_t *bar) {
-      proxy_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    auto settle = [&] {  // everything in flight has landed
-      copies_left<0>();
+    // The barrier counts a lane's copies when they have landed; the MMA warp makes them visible to the tensor core.  (A proxy fence
+    // here would wait for the copies behind them as well: 4900 cycles a block, 2 stages in flight instead of 5.)
+    auto submit = [&](uint64_t *bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
+    // 32 rows from shared-memory address `dst` on; a lane has the place of one of them in pieces of 16 bytes, ~0: zeros.  Lane i copies piece
+    // i % PIECES of every row that it has a part in, whose place in the swizzle repeats after 8 rows.
+    constexpr uint32_t PIECES = DP / 8, AT_ONCE = 32 / PIECES;  // pieces of a row, rows of one instruction
+    const uint32_t c = lane % PIECES, r0 = lane / PIECES;
+    const uint32_t sub = (c / 8) * 16384, col = c & 7;
+    const bool in_head = c * 8 < D;
+    auto copy_rows = [&](uint32_t dst, const void *base, uint32_t place) {
+      const char *from = (const char *)base + c * 16;
+      dst += sub + r0 * 128;
 #pragma unroll
-      for (int i = 2; i >= 0; i--) {
-        if (pending[i]) landed(pending[i]);
-        pending[i] = nullptr;
+      for (uint32_t i = 0; i < 32 / AT_ONCE; i++) {
+        const uint32_t r = i * AT_ONCE + r0, at = __shfl_sync(0xFFFFFFFFu, place, r);
+        const bool in = at != 0xFFFFFFFFu && in_head;
+        copy16(dst + i * (AT_ONCE * 128) + ((col ^ (r & 7)) << 4), in ? from + (uint64_t)at * 16 : (const char *)base, in ? 16 : 0);
       }
     };
-    auto submit = [&](uint64_t *bar) {
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      copies_left<3>();
-      if (pending[2]) landed(pending[2]);
-      pending[2] = pending[1], pending[1] = pending[0], pending[0] = bar;
-    };
-    auto claim = [&](uint64_t *bar, uint32_t parity) {  // nothing is held back while this warp waits
-      if (__all_sync(0xFFFFFFFFu, mbar_test(bar, parity))) return true;
-      settle();
-      return wait(bar, parity);
-    };
-    constexpr uint32_t PIECES = DP / 8;  // of a row
     while (!aborted() && walk.next(&t)) {
       const uint32_t rows = t.tokens * t.heads;
-      if (!claim(&ctl.q_empty, (tiles & 1) ^ 1)) break;
-      for (uint32_t i = lane; i < 128 * PIECES; i += 32) {
-        const uint32_t r = w * 128 + i / PIECES, c = i % PIECES, tok = r / t.heads, h = r - tok * t.heads;
-        const bool in = r < rows && c * 8 < D;
-        const T *src = (const T *)p.q;
-        if (in) src += (uint64_t)(t.row0 + t.token0 + tok) * p.q_stride + (uint64_t)(t.head0 + h) * D + c * 8;
-        copy16(s_q + w * S::QTILE + (c / 8) * 16384 + (i / PIECES) * 128 + (((c ^ r) & 7) << 4), src, in ? 16 : 0);
+      if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
+#pragma unroll 1
+      for (uint32_t i = 0; i < 2; i++) {
+        const uint32_t r = w * 64 + i * 32 + lane, tok = r / t.heads;
+        // the tile's rows lie within 2^32 pieces of its first one
+        const uint32_t place = r < rows ? tok * (uint32_t)(p.q_stride / 8) + (r - tok * t.heads) * (D / 8) : 0xFFFFFFFFu;
+        copy_rows(s_q + (w / 2) * S::QTILE + ((w & 1) * 64 + i * 32) * 128, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
       }
       submit(&ctl.q_full);
       tiles++;
       const uint32_t end = t.past + t.token0 + t.tokens;
       const uint32_t start = window && t.past + t.token0 + 1 > window ? t.past + t.token0 + 1 - window : 0;
-      const uint32_t *pages = p.kv.page_table + (uint64_t)t.seq * p.kv.table_stride;
-      // a lane knows where the tokens w * 64 + lane and + 32 of the block lie, a block ahead
-      auto look_up = [&](uint32_t blk, uint32_t half) -> uint64_t {
-        const uint32_t key = blk * TC_KB + w * 64 + half * 32 + lane;
-        if (blk >= t.hi || key < start || key >= end) return ~0ull;
-        const uint32_t slot = key / p.a.page_tokens;
-        const uint32_t page = slot < p.kv.table_stride ? __ldg(pages + slot) : 0xFFFFFFFFu;
-        if (page >= p.kv.n_pages) {
-          bad = 1;
-          return ~0ull;
-        }
-        return page * p.kv.page_stride + (uint64_t)(key - slot * p.a.page_tokens) * p.kv.token_stride + t.kv_head * p.kv.head_stride;
+      const PagePlaces pages(p.kv, p.a.page_tokens, t.seq, t.kv_head);
+      // a lane's token of a block: the first of its tiled copy, or a row
+      constexpr uint32_t SUBS = S::SUBS;
+      const uint32_t copy = lane * TC_LOADERS + w, copy_row = copy / SUBS * p.box, copies = p.box ? TC_KB / p.box * SUBS : 0;
+      auto tiled = [&](uint32_t blk) { return p.box && blk * TC_KB >= start && blk * TC_KB + TC_KB <= end; };
+      auto entry = [&](uint32_t blk) {
+        const bool whole = tiled(blk);
+        const uint32_t key = blk * TC_KB + (whole ? copy_row : w * 32 + lane);
+        return blk < t.hi && (whole ? copy < copies : key >= start && key < end) ? pages.entry(key) : 0u;
       };
-      uint64_t ahead[2] = {look_up(t.lo, 0), look_up(t.lo, 1)};
+      uint32_t ahead[2] = {entry(t.lo), entry(t.lo + 1)};
       bool ok = true;
       for (uint32_t blk = t.lo; blk < t.hi && ok; blk++) {
-        const uint64_t place[2] = {ahead[0], ahead[1]};
-        ahead[0] = look_up(blk + 1, 0), ahead[1] = look_up(blk + 1, 1);
+        const uint32_t number = ahead[0];
+        ahead[0] = ahead[1];
+        ahead[1] = entry(blk + 2);
+        if (tiled(blk)) {
+          const uint32_t token = pages.in_page(blk * TC_KB + copy_row);
+          if (copy < copies && number >= p.kv.n_pages) bad = 1;
 #pragma unroll 1
-        for (int kv = 0; kv < 2; kv++) {
-          const T *base = (const T *)(kv ? p.kv.v_pages : p.kv.k_pages);
-          if (!(ok = claim(&ctl.empty[stage], phase ^ 1))) break;
-          const uint32_t dst = s_ring + stage * S::STAGE;
-#pragma unroll
-          for (int i = 0; i < (int)(64 * PIECES / 32); i++) {
-            const uint32_t idx = i * 32 + lane, r = idx / PIECES, c = idx % PIECES;
-            const uint64_t at = __shfl_sync(0xFFFFFFFFu, place[i / (PIECES)], r & 31);
-            const bool in = at != ~0ull && c * 8 < D;
-            copy16(dst + (c / 8) * (TC_KB * 128) + (w * 64 + r) * 128 + (((c ^ r) & 7) << 4), base + (in ? at + c * 8 : 0), in ? 16 : 0);
+          for (int kv = 0; kv < 2; kv++) {
+            if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
+            if (copy < copies) {
+              mbar_expect_tx(&ctl.full[stage], p.box * 128);
+              page_g2s(s_ring + stage * S::STAGE + (copy % SUBS) * (TC_KB * 128) + copy_row * 128, kv ? &maps.v : &maps.k, (copy % SUBS) * 64, token, t.kv_head,
+                       min(number, p.kv.n_pages), p.head_first, smem_u32(&ctl.full[stage]));
+            } else {
+              mbar_arrive(&ctl.full[stage]);
+            }
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
           }
-          submit(&ctl.full[stage]);
-          stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
+        } else {
+          const uint32_t key = blk * TC_KB + w * 32 + lane;
+          const uint32_t place = key >= start && key < end ? pages.place(key, number, &bad) : 0xFFFFFFFFu;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; kv++) {
+            if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
+            copy_rows(s_ring + stage * S::STAGE + w * (32 * 128), kv ? p.kv.v_pages : p.kv.k_pages, place);
+            submit(&ctl.full[stage]);
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
+          }
         }
       }
       if (!ok) break;
     }
-    settle();
+    copies_left<0>();
     if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
   }
   tm_fence_before();
@@ -372,14 +444,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p) {
 }
 
 template <typename T, int DP>
-cudaError_t launch_tc(const TcParams &p, int sm_count, cudaStream_t s) {
-  const cudaError_t e = cudaFuncSetAttribute(k_attend_tc<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcShape<DP>::SMEM);
+cudaError_t launch_tc(const TcParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
+  const cudaError_t e = allow_smem<k_attend_tc<T, DP>>(TcShape<DP>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(k_attend_tc<T, DP>, dim3(sm_count), TC_THREADS, TcShape<DP>::SMEM, s, false, p);
+  return launch_overlapped(k_attend_tc<T, DP>, dim3(sm_count), TC_THREADS, TcShape<DP>::SMEM, s, false, p, maps);
 }
 template <typename T>
-cudaError_t launch_tc(const TcParams &p, int sm_count, cudaStream_t s) {
-  return p.a.head_dim <= 64 ? launch_tc<T, 64>(p, sm_count, s) : launch_tc<T, 128>(p, sm_count, s);
+cudaError_t launch_tc(const TcParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
+  return p.a.head_dim <= 64 ? launch_tc<T, 64>(p, maps, sm_count, s) : launch_tc<T, 128>(p, maps, sm_count, s);
 }
 
 }  // namespace
@@ -388,6 +460,9 @@ size_t attend_tc_part_floats(int sm_count) { return (size_t)2 * sm_count * part_
 
 cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                              int sm_count, cudaStream_t s) {
-  const TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2};
-  return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, sm_count, s) : launch_tc<__nv_bfloat16>(p, sm_count, s);
+  const PageMapShape m(a, kv, TC_KB);
+  PageMaps maps{};
+  const bool mapped = encode_page_maps(&maps, m, a, kv);
+  const TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, TileShape(a.q_heads, a.kv_heads, TC_R), mapped ? m.rows : 0, m.head_first};
+  return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);
 }
