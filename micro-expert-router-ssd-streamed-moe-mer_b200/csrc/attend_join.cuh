@@ -13,7 +13,7 @@ struct RunWalk {
   uint32_t window, min_n, max_n;
   uint64_t left, at;  // blocks of the run that are left, and the next one's number
   SeqWork w;
-  uint32_t seq, v_head, tile, from;  // from: blocks of the tile that are not this run's (its first tile alone)
+  uint32_t seq, v_head, tile, from;  // from: what of the tile is not this run's (its first tile alone)
   bool fresh = true;
 
   __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, uint32_t lo, uint32_t hi, const RunStart &r)
@@ -41,11 +41,13 @@ struct RunWalk {
       }
     }
     w.tile_blocks<KB>(tile, ts.tokens, window, &t->tile_lo, &t->tile_hi);
-    t->at = at - from;
-    t->lo = t->tile_lo + from;
-    t->hi = (uint32_t)min((uint64_t)t->tile_hi, t->lo + left);
-    left -= t->hi - t->lo;
-    at += t->hi - t->lo;
+    const uint32_t to = (uint32_t)min((uint64_t)(ts.start + t->tile_hi - t->tile_lo), from + left);
+    t->at = at - from + ts.start;
+    t->lo = t->tile_lo + (from > ts.start ? from - ts.start : 0);
+    left -= to - from;
+    at += to - from;
+    if (to <= ts.start) return false;  // the run ends in front of the tile's first block: the next one begins it
+    t->hi = t->tile_lo + to - ts.start;
     t->seq = seq, t->row0 = w.row0, t->past = w.past;
     t->token0 = tile * ts.tokens;
     t->tokens = min(ts.tokens, w.n - t->token0);

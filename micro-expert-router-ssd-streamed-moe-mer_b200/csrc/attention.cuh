@@ -3,7 +3,8 @@
 // A tile is up to R rows (tokens x the query heads of one key head) of one sequence; its work is counted in blocks of KB tokens
 // of the cache, of which it has only those that one of its rows sees.  The blocks of all tiles in order
 // (sequence, key head, tile) are cut into one equal run per CTA, so a long sequence is split over many CTAs and many short ones
-// share one, whatever the lengths are; nothing of this needs the lengths on the host.  A tile that lies in the runs of several CTAs is
+// share one, whatever the lengths are; nothing of this needs the lengths on the host.  A tile counts for `start` blocks more than it has, in front of its
+// own: what beginning and ending one costs.  A tile that lies in the runs of several CTAs is
 // joined by the one that arrives last, in the order of the runs: results do not depend on who that is.
 #pragma once
 
@@ -69,8 +70,8 @@ struct SeqWork {
 
 // How heads and rows of a layer lie in tiles of R rows: heads of a group are taken `heads` at a time.
 struct TileShape {
-  uint32_t group, chunks, heads, tokens, v_heads;
-  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R) {
+  uint32_t group, chunks, heads, tokens, v_heads, start;
+  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R, uint32_t start_) : start(start_) {
     group = q_heads / kv_heads;
     chunks = (group + R - 1) / R;
     heads = (group + chunks - 1) / chunks;
@@ -105,7 +106,7 @@ struct RunStart {
   uint64_t total, each;  // blocks of the batch, blocks of a run: `more` runs have one more
   uint32_t parts, more;  // CTAs that share the work
   uint32_t seq;          // the sequence of the run's first block
-  uint32_t v_head, tile, from;  // its head, its tile, and the tile's blocks before it
+  uint32_t v_head, tile, from;  // its head, its tile, and what of the tile lies before it
   SeqWork w;
 };
 // First block of a CTA's run.
@@ -156,7 +157,7 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
   SeqWork w{};
   for (uint32_t s = s0; s < s1; s++) {
     w = seq_work(kv, s, ts.tokens, min_n, max_n);
-    per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window);
+    per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) + w.tiles * ts.start;
     mine += per_head * ts.v_heads;
   }
   const uint64_t first = scan_threads<THREADS>(mine, found.sums, &total);
@@ -172,7 +173,7 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
     if (s1 - s0 > 1) {
       for (;; s++) {
         w = seq_work(kv, s, ts.tokens, min_n, max_n);
-        per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window);
+        per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) + w.tiles * ts.start;
         if (x0 < at + per_head * ts.v_heads) break;
         at += per_head * ts.v_heads;
       }
@@ -189,16 +190,16 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
     const uint32_t some = (r.w.tiles + THREADS - 1) / THREADS, j0 = min(r.w.tiles, tid * some), j1 = min(r.w.tiles, j0 + some);
     uint32_t lo, hi;
     mine = 0;
-    for (uint32_t j = j0; j < j1; j++) r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi), mine += hi - lo;
+    for (uint32_t j = j0; j < j1; j++) r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi), mine += hi - lo + ts.start;
     uint64_t at = scan_threads<THREADS>(mine, found.more_sums, &total);
     if (x >= at && x < at + mine) {
       for (uint32_t j = j0;; j++) {
         r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi);
-        if (x < at + (hi - lo)) {
+        if (x < at + (hi - lo + ts.start)) {
           found.tile = j, found.from = (uint32_t)(x - at);
           break;
         }
-        at += hi - lo;
+        at += hi - lo + ts.start;
       }
     }
     __syncthreads();

@@ -19,6 +19,8 @@
 
 namespace {
 
+constexpr uint32_t START_BLOCKS = 2;  // what a tile costs beside its blocks, in blocks
+
 struct AttendParams {
   AttnLayer a;
   KvBatchDev kv;
@@ -397,6 +399,6 @@ cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *
   const PageMapShape m(a, kv, 16);
   PageMaps maps{};
   const bool mapped = encode_page_maps(&maps, m, a, kv);
-  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, rows > 16 && a.head_dim <= 128 ? 32 : 16), mapped ? m.rows : 0, m.head_first};
+  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, rows > 16 && a.head_dim <= 128 ? 32 : 16, START_BLOCKS), mapped ? m.rows : 0, m.head_first};
   return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, rows > 16, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, rows > 16, sm_count, s);
 }

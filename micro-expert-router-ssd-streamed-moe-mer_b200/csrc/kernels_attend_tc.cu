@@ -39,6 +39,12 @@ struct TcParams {
   TileShape ts;
   uint32_t box;  // tokens of a tiled copy, 0: none
   bool head_first;
+  bool q_mapped;  // queries by tiled copies
+  bool out32;     // output rows are whole pieces of 32 bytes
+};
+struct TcMaps {
+  PageMaps pages;
+  CUtensorMap q;  // [row][head][value]
 };
 
 constexpr uint32_t TC_R = 256, TC_KB = 128, TC_WARPS = 16, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
@@ -46,6 +52,7 @@ constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12;
 // Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
 constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
+constexpr uint32_t TC_START = 3;  // what a tile costs beside its blocks, in blocks
 constexpr float LAG = 3.0f;  // with P_SHIFT the largest weight is 2^15
 constexpr uint32_t TC_CONTROL = 1024;  // barriers and words in front of the operands
 
@@ -54,13 +61,13 @@ struct TcShape {
   static constexpr uint32_t SUBS = DP / 64;                // pieces of 64 values of a row
   static constexpr uint32_t STAGE = SUBS * TC_KB * 128;    // keys or values of a block
   static constexpr uint32_t STAGES = DP == 128 ? 5 : 10;
-  static constexpr uint32_t QTILE = SUBS * 128 * 128;
-  static constexpr size_t SMEM = TC_CONTROL + 1024 + 2 * QTILE + STAGES * STAGE;  // 1024: the operands lie on whole atoms
+  static constexpr uint32_t QSUB = TC_R * 128;             // 64 values of all queries of a tile
+  static constexpr size_t SMEM = TC_CONTROL + 1024 + SUBS * QSUB + STAGES * STAGE;  // 1024: the operands lie on whole atoms
 };
 
 struct TcControl {
   uint64_t full[10], empty[10];  // stages of the ring
-  uint64_t q_full, q_empty, s_full[2], p_ready[2], o_full[2], soft, drain;
+  uint64_t q_full, q_empty, s_full[2], p_half[2], p_ready[2], o_full[2], soft, drain;
   RunFound found;
   uint32_t tmem, flag[2];  // flags take turns: a sync lies between two uses of one
   volatile uint32_t abort;
@@ -76,20 +83,43 @@ __device__ __forceinline__ void copies_left() {
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Two fp32 values in one register pair.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+// 32 bytes to an address on 32 bytes.
+__device__ __forceinline__ void store32(void *p, const uint4 &a, const uint4 &b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, const __grid_constant__ PageMaps maps) {
+__global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, const __grid_constant__ TcMaps maps) {
   using S = TcShape<DP>;
   extern __shared__ __align__(16) uint8_t smem[];
   TcControl &ctl = *reinterpret_cast<TcControl *>(smem);
   const uint32_t operands = (smem_u32(smem) + TC_CONTROL + 1023u) & ~1023u;
-  const uint32_t s_q = operands, s_ring = operands + 2 * S::QTILE;
+  const uint32_t s_q = operands, s_ring = operands + S::SUBS * S::QSUB;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t D = p.a.head_dim, window = p.a.window;
   const TileShape &ts = p.ts;
   if (tid == 0) {
     for (uint32_t i = 0; i < S::STAGES; i++) mbar_init(&ctl.full[i], TC_LOADERS * 32), mbar_init(&ctl.empty[i], 1);
     mbar_init(&ctl.q_full, TC_LOADERS * 32), mbar_init(&ctl.q_empty, 1);
-    for (int x = 0; x < 2; x++) mbar_init(&ctl.s_full[x], 1), mbar_init(&ctl.p_ready[x], 4), mbar_init(&ctl.o_full[x], 1);
+    for (int x = 0; x < 2; x++) mbar_init(&ctl.s_full[x], 1), mbar_init(&ctl.p_half[x], 4), mbar_init(&ctl.p_ready[x], 4), mbar_init(&ctl.o_full[x], 1);
     mbar_init(&ctl.soft, SOFT_THREADS / 32), mbar_init(&ctl.drain, 1);
     ctl.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -153,9 +183,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
 #pragma unroll
           for (int h = 0; h < 4; h++) tm_loaded(s[h]);
           const uint32_t key0 = blk * TC_KB;
-          if (key0 + TC_KB - 1 > see0 || key0 < least1) {
+          if (key0 + TC_KB - 1 > see0) {  // the row sees the first `seen` tokens of the block
+            const int seen = (int)(see + 1) - (int)key0;
 #pragma unroll
-            for (int i = 0; i < 128; i++) s[i / 32][i % 32] = key0 + i <= see && key0 + i >= least ? s[i / 32][i % 32] : -INFINITY;
+            for (int i = 0; i < 128; i++) s[i / 32][i % 32] = i < seen ? s[i / 32][i % 32] : -INFINITY;
+          }
+          if (key0 < least1) {  // and not the first `old` ones
+            const int old = (int)least - (int)key0;
+#pragma unroll
+            for (int i = 0; i < 128; i++) s[i / 32][i % 32] = i >= old ? s[i / 32][i % 32] : -INFINITY;
           }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -181,24 +217,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             }
           }
           const float less = m == -INFINITY ? 0.0f : m - P_SHIFT;
-          float sum[4] = {0, 0, 0, 0};
+          uint64_t sum[2] = {0, 0};
+          const uint64_t scale2 = pack2(to_log2, to_log2), less2 = pack2(-less, -less);
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             uint32_t v[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-              const float a = exp2_approx(fmaf(s[2 * h + i / 16][2 * i % 32], to_log2, -less)),
-                          b = exp2_approx(fmaf(s[2 * h + i / 16][2 * i % 32 + 1], to_log2, -less));
-              sum[i & 3] += a + b;
+              float a, b;
+              unpack2(fma2(pack2(s[2 * h + i / 16][2 * i % 32], s[2 * h + i / 16][2 * i % 32 + 1]), scale2, less2), a, b);
+              a = exp2_approx(a), b = exp2_approx(b);
+              sum[i & 1] = add2(sum[i & 1], pack2(a, b));
               v[i] = Num<T>::pack(a, b);
             }
             tm_store(s_at + h * 32, v);
+            tm_wait_store();
+            tm_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h ? &ctl.p_ready[x] : &ctl.p_half[x]);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tm_wait_store();
-          tm_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.p_ready[x]);
+          {
+            float a, b;
+            unpack2(add2(sum[0], sum[1]), a, b);
+            l += a + b;
+          }
         }
       }
       const bool whole = t.lo == t.tile_lo && t.hi == t.tile_hi;
@@ -277,11 +319,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             }
           }
           if (row >= rows) continue;
+          uint4 v[4];
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            const uint4 v = make_uint4(Num<T>::pack(o[i] * f, o[i + 1] * f), Num<T>::pack(o[i + 2] * f, o[i + 3] * f), Num<T>::pack(o[i + 4] * f, o[i + 5] * f),
-                                       Num<T>::pack(o[i + 6] * f, o[i + 7] * f));
-            if (c + i < (int)D) *reinterpret_cast<uint4 *>(out + c + i) = v;
+          for (int i = 0; i < 4; i++)
+            v[i] = make_uint4(Num<T>::pack(o[8 * i] * f, o[8 * i + 1] * f), Num<T>::pack(o[8 * i + 2] * f, o[8 * i + 3] * f), Num<T>::pack(o[8 * i + 4] * f, o[8 * i + 5] * f),
+                              Num<T>::pack(o[8 * i + 6] * f, o[8 * i + 7] * f));
+          if (p.out32) {  // a lane's rows lie apart: the wider its stores, the fewer lines they touch
+            if (c < (int)D) store32(out + c, v[0], v[1]);
+            if (c + 16 < (int)D) store32(out + c + 16, v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (c + 8 * i < (int)D) *reinterpret_cast<uint4 *>(out + c + 8 * i) = v[i];
           }
         }
       }
@@ -301,7 +350,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     auto qk = [&](uint32_t x, uint32_t st) {
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
-        tm_mma_ss(leader, tm + x * 128, tm_desc(s_q + x * S::QTILE + (k / 4) * 16384 + (k & 3) * 32, 16),
+        tm_mma_ss(leader, tm + x * 128, tm_desc(s_q + (k / 4) * S::QSUB + x * 16384 + (k & 3) * 32, 16),
                   tm_desc(s_ring + st * S::STAGE + (k / 4) * (TC_KB * 128) + (k & 3) * 32, 16), QK, k != 0);
       tm_commit(leader, &ctl.s_full[x]);
     };
@@ -324,11 +373,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         if (more && !(ok = wait(&ctl.full[stage], phase))) break;
         proxy_fence();
         for (uint32_t x = 0; x < groups; x++) {
-          if (!(ok = wait(&ctl.p_ready[x], (x ? blocks1 : blocks) & 1))) break;
-          tm_fence_after();
 #pragma unroll
-          for (int k = 0; k < (int)TC_KB / 16; k++)
-            tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, tm_desc(s_ring + v_stage * S::STAGE + k * 2048, TC_KB * 128), PV, k != 0 || blk != t.lo);
+          for (int h = 0; h < 2; h++) {
+            if (!(ok = wait(h ? &ctl.p_ready[x] : &ctl.p_half[x], (x ? blocks1 : blocks) & 1))) break;
+            tm_fence_after();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; k++)
+              tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, tm_desc(s_ring + v_stage * S::STAGE + k * 2048, TC_KB * 128), PV, k != 0 || blk != t.lo);
+          }
+          if (!ok) break;
           if (more)
             qk(x, stage);
           else
@@ -364,11 +417,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     // i % PIECES of every row that it has a part in, whose place in the swizzle repeats after 8 rows.
     constexpr uint32_t PIECES = DP / 8, AT_ONCE = 32 / PIECES;  // pieces of a row, rows of one instruction
     const uint32_t c = lane % PIECES, r0 = lane / PIECES;
-    const uint32_t sub = (c / 8) * 16384, col = c & 7;
+    const uint32_t col = c & 7;
     const bool in_head = c * 8 < D;
-    auto copy_rows = [&](uint32_t dst, const void *base, uint32_t place) {
+    auto copy_rows = [&](uint32_t dst, uint32_t sub, const void *base, uint32_t place) {
       const char *from = (const char *)base + c * 16;
-      dst += sub + r0 * 128;
+      dst += (c / 8) * sub + r0 * 128;
 #pragma unroll
       for (uint32_t i = 0; i < 32 / AT_ONCE; i++) {
         const uint32_t r = i * AT_ONCE + r0, at = __shfl_sync(0xFFFFFFFFu, place, r);
@@ -379,14 +432,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     while (!aborted() && walk.next(&t)) {
       const uint32_t rows = t.tokens * t.heads;
       if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
+      if (p.q_mapped) {
+        // 64 values of ts.heads heads of ts.tokens rows; those behind the sequence's end are other rows or zeros, which nobody stores
+        if (lane == 0 && w < S::SUBS) {
+          const uint32_t bar = smem_u32(&ctl.q_full);
+          mbar_expect_tx(&ctl.q_full, ts.tokens * ts.heads * 128);
+          asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(s_q + w * S::QSUB),
+                       "l"(&maps.q), "r"(w * 64), "r"(t.head0), "r"(t.row0 + t.token0), "r"(bar)
+                       : "memory");
+        } else {
+          mbar_arrive(&ctl.q_full);
+        }
+      } else {
 #pragma unroll 1
-      for (uint32_t i = 0; i < 2; i++) {
-        const uint32_t r = w * 64 + i * 32 + lane, tok = r / t.heads;
-        // the tile's rows lie within 2^32 pieces of its first one
-        const uint32_t place = r < rows ? tok * (uint32_t)(p.q_stride / 8) + (r - tok * t.heads) * (D / 8) : 0xFFFFFFFFu;
-        copy_rows(s_q + (w / 2) * S::QTILE + ((w & 1) * 64 + i * 32) * 128, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
+        for (uint32_t i = 0; i < 2; i++) {
+          const uint32_t r = w * 64 + i * 32 + lane, tok = r / t.heads;
+          // the tile's rows lie within 2^32 pieces of its first one
+          const uint32_t place = r < rows ? tok * (uint32_t)(p.q_stride / 8) + (r - tok * t.heads) * (D / 8) : 0xFFFFFFFFu;
+          copy_rows(s_q + (w * 64 + i * 32) * 128, S::QSUB, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
+        }
+        submit(&ctl.q_full);
       }
-      submit(&ctl.q_full);
       tiles++;
       const uint32_t end = t.past + t.token0 + t.tokens;
       const uint32_t start = window && t.past + t.token0 + 1 > window ? t.past + t.token0 + 1 - window : 0;
@@ -414,7 +480,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
             if (copy < copies) {
               mbar_expect_tx(&ctl.full[stage], p.box * 128);
-              page_g2s(s_ring + stage * S::STAGE + (copy % SUBS) * (TC_KB * 128) + copy_row * 128, kv ? &maps.v : &maps.k, (copy % SUBS) * 64, token, t.kv_head,
+              page_g2s(s_ring + stage * S::STAGE + (copy % SUBS) * (TC_KB * 128) + copy_row * 128, kv ? &maps.pages.v : &maps.pages.k, (copy % SUBS) * 64, token, t.kv_head,
                        min(number, p.kv.n_pages), p.head_first, smem_u32(&ctl.full[stage]));
             } else {
               mbar_arrive(&ctl.full[stage]);
@@ -427,7 +493,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
 #pragma unroll 1
           for (int kv = 0; kv < 2; kv++) {
             if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
-            copy_rows(s_ring + stage * S::STAGE + w * (32 * 128), kv ? p.kv.v_pages : p.kv.k_pages, place);
+            copy_rows(s_ring + stage * S::STAGE + w * (32 * 128), TC_KB * 128, kv ? p.kv.v_pages : p.kv.k_pages, place);
             submit(&ctl.full[stage]);
             stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
           }
@@ -444,13 +510,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
 }
 
 template <typename T, int DP>
-cudaError_t launch_tc(const TcParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
+cudaError_t launch_tc(const TcParams &p, const TcMaps &maps, int sm_count, cudaStream_t s) {
   const cudaError_t e = allow_smem<k_attend_tc<T, DP>>(TcShape<DP>::SMEM);
   if (e != cudaSuccess) return e;
   return launch_overlapped(k_attend_tc<T, DP>, dim3(sm_count), TC_THREADS, TcShape<DP>::SMEM, s, false, p, maps);
 }
 template <typename T>
-cudaError_t launch_tc(const TcParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
+cudaError_t launch_tc(const TcParams &p, const TcMaps &maps, int sm_count, cudaStream_t s) {
   return p.a.head_dim <= 64 ? launch_tc<T, 64>(p, maps, sm_count, s) : launch_tc<T, 128>(p, maps, sm_count, s);
 }
 
@@ -461,8 +527,10 @@ size_t attend_tc_part_floats(int sm_count) { return (size_t)2 * sm_count * part_
 cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                              int sm_count, cudaStream_t s) {
   const PageMapShape m(a, kv, TC_KB);
-  PageMaps maps{};
-  const bool mapped = encode_page_maps(&maps, m, a, kv);
-  const TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, TileShape(a.q_heads, a.kv_heads, TC_R), mapped ? m.rows : 0, m.head_first};
+  TcMaps maps{};
+  const bool mapped = encode_page_maps(&maps.pages, m, a, kv);
+  TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START), mapped ? m.rows : 0, m.head_first, false, false};
+  p.q_mapped = p.ts.chunks == 1 && encode_row_map(&maps.q, q, a, kv.n_rows, q_stride, p.ts.heads, p.ts.tokens);
+  p.out32 = a.head_dim % 16 == 0 && ((uintptr_t)out | out_stride * 2) % 32 == 0;
   return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);
 }

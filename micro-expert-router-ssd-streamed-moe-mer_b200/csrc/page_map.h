@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/mer_b200.h"
 #include "attention.h"
 
 // A page as the encoder sees it: [page][token][head][value], or tokens and heads the other way round, whichever makes the strides rise.
@@ -44,22 +45,33 @@ struct PageMaps {
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                    const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// False where these pages have no map: then rows are copied one by one.
-inline bool encode_page_maps(PageMaps *maps, const PageMapShape &m, const AttnLayer &a, const KvBatchDev &kv) {
+// The driver's encoder, looked up once; null when the driver has none.
+inline EncodeTiledFn page_map_encoder() {
   static const EncodeTiledFn fn = [] {
     void *p = nullptr;
     cudaDriverEntryPointQueryResult q;
     const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
     return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
   }();
-  if (!fn || m.rows == 0) return false;
+  return fn;
+}
+inline bool encode_map(CUtensorMap *map, const AttnLayer &a, const void *base, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+  const EncodeTiledFn fn = page_map_encoder();
   const cuuint32_t step[4] = {1, 1, 1, 1};
+  return fn && fn(map, a.cache_type == MER_VALUE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(base), dims, strides, box,
+                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// False where these pages have no map: then rows are copied one by one.
+inline bool encode_page_maps(PageMaps *maps, const PageMapShape &m, const AttnLayer &a, const KvBatchDev &kv) {
+  if (m.rows == 0) return false;
   const cuuint64_t dims[4] = {m.dims[0], m.dims[1], m.dims[2], m.dims[3]}, strides[3] = {m.strides[0], m.strides[1], m.strides[2]};
   const cuuint32_t box[4] = {m.box[0], m.box[1], m.box[2], m.box[3]};
-  const CUtensorMapDataType type = a.cache_type == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  for (int i = 0; i < 2; i++)
-    if (fn(i ? &maps->v : &maps->k, type, 4, i ? kv.v_pages : kv.k_pages, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return false;
-  return true;
+  return encode_map(&maps->k, a, kv.k_pages, 4, dims, strides, box) && encode_map(&maps->v, a, kv.v_pages, 4, dims, strides, box);
+}
+// Rows of heads, `heads` of `rows` rows at a time.
+inline bool encode_row_map(CUtensorMap *map, const void *base, const AttnLayer &a, uint32_t n_rows, uint64_t stride, uint32_t heads, uint32_t rows) {
+  if (stride % a.head_dim) return false;
+  const cuuint64_t dims[3] = {a.head_dim, a.q_heads, n_rows}, strides[2] = {a.head_dim * 2ull, stride * 2};
+  const cuuint32_t box[3] = {64, heads, rows};
+  return encode_map(map, a, base, 3, dims, strides, box);
 }
