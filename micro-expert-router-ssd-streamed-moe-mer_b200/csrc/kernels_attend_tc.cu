@@ -6,7 +6,8 @@
 //   P = 2^(S * scale - m + shift)               a thread owns a row: its maximum and sum need no other thread
 //   O[128 x d] += P[128 x 128] V[128 x d]       P from tensor memory, where it takes the place of S; V's rows run along N
 //
-//   * Warps 0..3 and 4..7 are the softmax of one group of rows each, warps 8..11 copy, warp 12 issues the MMAs (13..15 fill its group).  While one group's
+//   * Warps 0..3 and 4..7 are the softmax of one group of rows each, warps 8..11 copy, warp 12 issues the MMAs, warp 13 goes ahead through the run and leaves
+//     the next tile's place in shared memory (14 and 15 fill the group).  While one group's
 //     softmax runs the tensor core multiplies for the other: [P V of block j, Q K of block j + 1] of one, then of the other.
 //   * The reference maximum of a row follows its maximum only when that has grown by more than 2^LAG; then alone the output in tensor memory is rescaled, by
 //     the softmax warps themselves.  Until then weights are larger than 1 by up to that factor, which f16 and fp32 hold.  What makes that safe without a
@@ -48,12 +49,13 @@ struct TcMaps {
 };
 
 constexpr uint32_t TC_R = 256, TC_KB = 128, TC_WARPS = 16, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
-constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12;
+constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12, TC_WALK = 13, TILE_USERS = 13;  // the warps that work on a tile
 // Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
 constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
 constexpr uint32_t TC_START = 3;  // what a tile costs beside its blocks, in blocks
 constexpr float LAG = 3.0f;  // with P_SHIFT the largest weight is 2^15
+constexpr int POLY_EVERY = 4;  // pairs of weights per pair that the polynomial makes
 constexpr uint32_t TC_CONTROL = 1024;  // barriers and words in front of the operands
 
 template <int DP>
@@ -68,6 +70,9 @@ struct TcShape {
 struct TcControl {
   uint64_t full[10], empty[10];  // stages of the ring
   uint64_t q_full, q_empty, s_full[2], p_half[2], p_ready[2], o_full[2], soft, drain;
+  uint64_t tile_full[2], tile_empty[2];
+  TileWork tile[2];  // tokens == 0: there is none left
+  RunStart run;
   RunFound found;
   uint32_t tmem, flag[2];  // flags take turns: a sync lies between two uses of one
   volatile uint32_t abort;
@@ -100,6 +105,24 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
+// 2^x of two values by Cody and Waite's reduction x = i + f, |f| <= 1/2, and a polynomial of degree 4 for 2^f (Remez, relative error 2.7e-6: 2^-18.5), on the
+// fp32 units instead of the special function unit.  Below 2^-126 it stays there.
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float &a, float &b) {
+  constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+  unpack2(x, a, b);
+  x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const uint64_t t = add2(x, pack2(ROUND, ROUND));
+  const uint64_t f = fma2(add2(t, pack2(-ROUND, -ROUND)), pack2(-1.0f, -1.0f), x);
+  uint64_t r = fma2(f, pack2(9.570101911e-03f, 9.570101911e-03f), pack2(5.591786032e-02f, 5.591786032e-02f));
+  r = fma2(r, f, pack2(2.402474483e-01f, 2.402474483e-01f));
+  r = fma2(r, f, pack2(6.931218147e-01f, 6.931218147e-01f));
+  r = fma2(r, f, pack2(9.999992614e-01f, 9.999992614e-01f));
+  float ta, tb, ra, rb;
+  unpack2(t, ta, tb);
+  unpack2(r, ra, rb);
+  a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
+}
 // 32 bytes to an address on 32 bytes.
 __device__ __forceinline__ void store32(void *p, const uint4 &a, const uint4 &b) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
@@ -121,14 +144,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     mbar_init(&ctl.q_full, TC_LOADERS * 32), mbar_init(&ctl.q_empty, 1);
     for (int x = 0; x < 2; x++) mbar_init(&ctl.s_full[x], 1), mbar_init(&ctl.p_half[x], 4), mbar_init(&ctl.p_ready[x], 4), mbar_init(&ctl.o_full[x], 1);
     mbar_init(&ctl.soft, SOFT_THREADS / 32), mbar_init(&ctl.drain, 1);
+    for (int i = 0; i < 2; i++) mbar_init(&ctl.tile_full[i], 1), mbar_init(&ctl.tile_empty[i], TILE_USERS);
     ctl.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
+  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
   if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, 0, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
-  if (blockIdx.x >= run.parts) return;
+  if (blockIdx.x >= run_here.parts) return;
+  if (tid == 0) ctl.run = run_here;
   if (warp == TC_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -138,8 +163,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   tm_fence_after();
   const uint32_t tm = ctl.tmem;
   // columns: S (and P) of the two groups at 0 and 128, their O at 256 and 256 + DP
-  RunWalk<TC_KB> walk(p.kv, ts, window, 0, 0xFFFFFFFFu, run);
-  TileWork t;
   // For whole warps, which stay together whatever comes of it.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     const bool ok = mbar_wait(bar, parity, &ctl.abort);
@@ -150,6 +173,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     return __all_sync(0xFFFFFFFFu, ok) != 0;
   };
   auto aborted = [&] { return __any_sync(0xFFFFFFFFu, ctl.abort) != 0; };
+  // The run's tiles, one after the other; done_with() when the warp no longer looks at one.
+  uint32_t turn = 0;
+  const RunStart &run = ctl.run;
+  auto next_tile = [&] { return wait(&ctl.tile_full[turn & 1], (turn >> 1) & 1) && !aborted() && ctl.tile[turn & 1].tokens != 0; };
+  auto done_with = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.tile_empty[turn & 1]);
+    turn++;
+  };
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
@@ -163,7 +195,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (lane == 0) mbar_arrive(&ctl.soft);
       wait(&ctl.soft, syncs++ & 1);
     };
-    while (!aborted() && walk.next(&t)) {
+    while (next_tile()) {
+      const TileWork &t = ctl.tile[turn & 1];
       const uint32_t rows = t.tokens * t.heads;
       const bool active = rows > x * 128;
       const uint32_t first = t.past + t.token0, see = first + min(row, rows - 1) / t.heads;
@@ -173,7 +206,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         // blocks that every row of the group sees whole need no mask
         const uint32_t see0 = first + x * 128 / t.heads, see1 = first + min(x * 128 + 127, rows - 1) / t.heads;
         const uint32_t least1 = window && see1 + 1 > window ? see1 + 1 - window : 0;
-        for (uint32_t blk = t.lo; blk < t.hi; blk++, blocks++) {
+        const uint32_t lo = t.lo, hi = t.hi;
+        for (uint32_t blk = lo; blk < hi; blk++, blocks++) {
           if (!wait(&ctl.s_full[x], blocks & 1)) break;
           tm_fence_after();
           float s[4][32];
@@ -204,7 +238,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             const float f = grow ? (m == -INFINITY ? 0.0f : exp2_approx(m - now)) : 1.0f;
             if (grow) m = now;
             l *= f;
-            if (blk != t.lo) {
+            if (blk != lo) {
               float o[32];
 #pragma unroll 1
               for (int c = 0; c < DP; c += 32) {
@@ -224,9 +258,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             uint32_t v[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) {
+              const uint64_t at = fma2(pack2(s[2 * h + i / 16][2 * i % 32], s[2 * h + i / 16][2 * i % 32 + 1]), scale2, less2);
               float a, b;
-              unpack2(fma2(pack2(s[2 * h + i / 16][2 * i % 32], s[2 * h + i / 16][2 * i % 32 + 1]), scale2, less2), a, b);
-              a = exp2_approx(a), b = exp2_approx(b);
+              if (i % POLY_EVERY == POLY_EVERY - 1) {
+                exp2_poly2(at, a, b);
+              } else {
+                unpack2(at, a, b);
+                a = exp2_approx(a), b = exp2_approx(b);
+              }
               sum[i & 1] = add2(sum[i & 1], pack2(a, b));
               v[i] = Num<T>::pack(a, b);
             }
@@ -335,6 +374,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
       }
       tm_fence_before();
+      done_with();
     }
   } else if (warp >= TC_MMA) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
@@ -347,15 +387,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     uint32_t stage = 0, phase = 0, tiles = 0, blocks = 0;  // blocks: phases of p_ready[0]; of p_ready[1] the same while its group is active
     uint32_t blocks1 = 0;
     auto next_stage = [&] { stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0; };
+    // the low words of the descriptors; those of the pieces of an operand lie constants apart
+    constexpr uint64_t ALONG_K = (64ull << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16), ALONG_N = (64ull << 32) | (1ull << 46) | (2ull << 61) | ((uint64_t)(TC_KB * 128 >> 4) << 16);
+    const uint32_t q_at = s_q >> 4, ring_at = s_ring >> 4;
     auto qk = [&](uint32_t x, uint32_t st) {
+      const uint32_t a = q_at + x * (16384 >> 4), b = ring_at + st * (S::STAGE >> 4);
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
-        tm_mma_ss(leader, tm + x * 128, tm_desc(s_q + (k / 4) * S::QSUB + x * 16384 + (k & 3) * 32, 16),
-                  tm_desc(s_ring + st * S::STAGE + (k / 4) * (TC_KB * 128) + (k & 3) * 32, 16), QK, k != 0);
+        tm_mma_ss(leader, tm + x * 128, ALONG_K | (a + (k / 4) * (S::QSUB >> 4) + (k & 3) * 2), ALONG_K | (b + (k / 4) * (TC_KB * 128 >> 4) + (k & 3) * 2), QK, k != 0);
       tm_commit(leader, &ctl.s_full[x]);
     };
-    while (!aborted() && walk.next(&t)) {
-      const uint32_t groups = t.tokens * t.heads > 128 ? 2 : 1;
+    while (next_tile()) {
+      const uint32_t groups = ctl.tile[turn & 1].tokens * ctl.tile[turn & 1].heads > 128 ? 2 : 1, lo = ctl.tile[turn & 1].lo, hi = ctl.tile[turn & 1].hi;
+      done_with();
       if (!wait(&ctl.q_full, tiles & 1)) break;
       if (!wait(&ctl.full[stage], phase)) break;
       proxy_fence();
@@ -363,11 +407,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       for (uint32_t x = 0; x < groups; x++) qk(x, stage);
       tm_commit(leader, &ctl.empty[stage]);
       next_stage();
-      if (t.lo + 1 == t.hi) tm_commit(leader, &ctl.q_empty);
+      if (lo + 1 == hi) tm_commit(leader, &ctl.q_empty);
       bool ok = true;
-      for (uint32_t blk = t.lo; blk < t.hi && ok; blk++) {
+      for (uint32_t blk = lo; blk < hi && ok; blk++) {
         const uint32_t v_stage = stage, v_phase = phase;
-        const bool more = blk + 1 < t.hi;
+        const bool more = blk + 1 < hi;
         next_stage();
         if (!(ok = wait(&ctl.full[v_stage], v_phase))) break;
         if (more && !(ok = wait(&ctl.full[stage], phase))) break;
@@ -379,7 +423,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             tm_fence_after();
 #pragma unroll
             for (int k = 4 * h; k < 4 * h + 4; k++)
-              tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, tm_desc(s_ring + v_stage * S::STAGE + k * 2048, TC_KB * 128), PV, k != 0 || blk != t.lo);
+              tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, ALONG_N | (ring_at + v_stage * (S::STAGE >> 4) + k * 128), PV, k != 0 || blk != lo);
           }
           if (!ok) break;
           if (more)
@@ -394,7 +438,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         if (more) {
           tm_commit(leader, &ctl.empty[stage]);
           next_stage();
-          if (blk + 2 == t.hi) tm_commit(leader, &ctl.q_empty);
+          if (blk + 2 == hi) tm_commit(leader, &ctl.q_empty);
         }
       }
       if (!ok) break;
@@ -404,6 +448,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       tm_commit(leader, &ctl.drain);
       mbar_drain(&ctl.drain, 0, 1000000000ull);
     }
+    } else if (warp == TC_WALK) {
+      // -------------------------------------------------------------- the way through the run
+      RunWalk<TC_KB> walk(p.kv, ts, window, 0, 0xFFFFFFFFu, ctl.run);
+      TileWork t;
+      for (uint32_t i = 0;; i++) {
+        const bool more = walk.next(&t);
+        if (!more) t.tokens = 0;
+        if (!wait(&ctl.tile_empty[i & 1], ((i >> 1) & 1) ^ 1)) break;
+        if (lane == 0) {
+          ctl.tile[i & 1] = t;
+          mbar_arrive(&ctl.tile_full[i & 1]);
+        }
+        if (!more) break;
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
@@ -429,7 +487,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         copy16(dst + i * (AT_ONCE * 128) + ((col ^ (r & 7)) << 4), in ? from + (uint64_t)at * 16 : (const char *)base, in ? 16 : 0);
       }
     };
-    while (!aborted() && walk.next(&t)) {
+    while (next_tile()) {
+      const TileWork t = ctl.tile[turn & 1];
+      done_with();
       const uint32_t rows = t.tokens * t.heads;
       if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
       if (p.q_mapped) {
