@@ -252,6 +252,12 @@ struct TileWork {
   uint64_t at;               // the tile's first block among all
 };
 
+// The first token that a row of the tile sees.
+__device__ __forceinline__ uint32_t first_seen(const TileWork &t, uint32_t window) {
+  const uint32_t behind = t.past + t.token0 + 1;
+  return window && behind > window ? behind - window : 0;
+}
+
 template <typename T>
 struct Num;
 template <>
@@ -284,9 +290,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// Weights of the softmax are made as 2^(s - max + P_SHIFT): an f16 then holds weights down to 2^-36 of a row's largest, so that what a
+// Weights of the softmax are made as 2^(s - max + P_SHIFT): an f16 then holds weights down to 2^-32 of a row's largest, so that what a
 // long row's many small ones sum to is not lost.  The shift is in the sums as well and cancels.
-constexpr float P_SHIFT = 12.0f;
+constexpr float P_SHIFT = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 }  // namespace

@@ -29,6 +29,7 @@ struct AttendParams {
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
   TileShape ts;
+  uint32_t max_rows;  // sequences with more rows are the other kernel's
   uint32_t box;  // tokens of a tiled copy (8 or 16), 0: none
   bool head_first;
 };
@@ -86,10 +87,10 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, 1, s_found);
-  if (blockIdx.x == 0) clear_rows_without_place<T, THREADS>(p.a, p.kv, 0, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
+  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, 0, p.max_rows, blockIdx.x, gridDim.x, 1, s_found);
+  if (blockIdx.x == 0) clear_rows_without_place<T, THREADS>(p.a, p.kv, 0, p.max_rows, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run.parts) return;
-  RunWalk<KB> walk(p.kv, ts, window, 0, 0xFFFFFFFFu, run);
+  RunWalk<KB> walk(p.kv, ts, window, 0, p.max_rows, run);
   const float to_log2 = p.a.scale * LOG2E;
   uint32_t fill = 0, stage = 0, stage_phase = 0, timed_out = 0;  // of the warp's ring: what is asked for next, what is taken next
   const uint32_t ring = smem_u32(s_ring) + warp * (ST * S::CHUNK), q_addr = smem_u32(s_q);
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   while (walk.next(&t)) {
     const uint32_t rows = t.tokens * t.heads;
     const uint32_t end = t.past + t.token0 + t.tokens;  // behind the last token that a row of the tile sees
-    const uint32_t start = window && t.past + t.token0 + 1 > window ? t.past + t.token0 + 1 - window : 0;
+    const uint32_t start = first_seen(t, window);
     // ---- the ring.  A lane knows where its part of a chunk lies, ST chunks ahead: lanes 0 .. 15 a row of one that is copied row by row; of others, the first
     // lanes a tiled copy of the keys each, the next ones of the values.
     const PagePlaces pages(p.kv, page_tokens, t.seq, t.kv_head);
@@ -182,23 +183,30 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
       timed_out |= !mbar_wait(&s_full[warp * ST + stage], stage_phase);
       stage = stage + 1 == ST ? 0 : stage + 1, stage_phase ^= stage == 0;
       float s[MT][2][4];
+      {
+        // One tile of rows: the products of even and odd pieces of a head apart, so that half as many wait for one another.
+        constexpr int CHAINS = MT == 1 ? 2 : 1;
+        float c[CHAINS][MT][2][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; mt++)
+        for (int i = 0; i < CHAINS * MT * 8; i++) (&c[0][0][0][0])[i] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int kk = 0; kk < DP / 16; kk++) {
+          uint32_t kf[4];
+          ldm4(kf, base + piece<16>((lane / 16) * 8 + (lane & 7), kk * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[mt][n][e] = 0.0f;
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; kk++) {
-        uint32_t kf[4];
-        ldm4(kf, base + piece<16>((lane / 16) * 8 + (lane & 7), kk * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-          uint32_t qf[4];
-          ldm4(qf, q_addr + piece<R>(mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4)));
-          mma16816<T>(s[mt][0], qf, kf[0], kf[1]);
-          mma16816<T>(s[mt][1], qf, kf[2], kf[3]);
+          for (int mt = 0; mt < MT; mt++) {
+            uint32_t qf[4];
+            ldm4(qf, q_addr + piece<R>(mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4)));
+            mma16816<T>(c[kk % CHAINS][mt][0], qf, kf[0], kf[1]);
+            mma16816<T>(c[kk % CHAINS][mt][1], qf, kf[2], kf[3]);
+          }
         }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[mt][n][e] = CHAINS == 2 ? c[0][mt][n][e] + c[CHAINS - 1][mt][n][e] : c[0][mt][n][e];
       }
       uint32_t pf[MT][4];
 #pragma unroll
@@ -317,45 +325,56 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         const float *first = part_of_tile(run, t, p.ws.parts, c0, 0, part_floats(R, DP)), *others = part_of_tile(run, t, p.ws.parts, c0, 1, part_floats(R, DP));
         auto part_of = [&](uint32_t k) { return k == 0 ? first : others + (size_t)(k - 1) * (2 * part_floats(R, DP)); };
         for (uint32_t r = warp; r < rows; r += NW) {
-          float top = -INFINITY, total = 0.0f, acc[V];
+          // a lane's values of AT_ONCE parts are asked for before the parts' maxima are known
+          constexpr uint32_t AT_ONCE = V == 8 || MT == 2 ? 8 : 16;
+          float top = -INFINITY, total = 0.0f, acc[V], v[AT_ONCE][V];
+          auto ask = [&](uint32_t k0) {
+#pragma unroll
+            for (uint32_t k = 0; k < AT_ONCE; k++) {
+              if (k0 + k >= n) continue;
+              const float *row = part_of(k0 + k) + 2 * R + (size_t)r * DP + lane * V;
+              if constexpr (V == 2)
+                *reinterpret_cast<float2 *>(v[k]) = __ldcg(reinterpret_cast<const float2 *>(row));
+              else
+#pragma unroll
+                for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(v[k] + i) = __ldcg(reinterpret_cast<const float4 *>(row + i));
+            }
+          };
+          ask(0);
           for (uint32_t k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(part_of(k) + r));
 #pragma unroll
           for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
 #pragma unroll
           for (int i = 0; i < V; i++) acc[i] = 0.0f;
-          for (uint32_t k0 = 0; k0 < n; k0 += 32) {
-            float f = 0.0f;
-            if (k0 + lane < n) {
-              const float *from = part_of(k0 + lane);
-              const float mk = __ldcg(from + r);
-              f = mk == -INFINITY ? 0.0f : exp2_approx(mk - top);
-              total = fmaf(f, __ldcg(from + R + r), total);
+          float f = 0.0f;  // of part (k0 rounded down to 32) + lane
+          for (uint32_t k0 = 0; k0 < n; k0 += AT_ONCE) {
+            if (k0 % 32 == 0) {
+              f = 0.0f;
+              if (k0 + lane < n) {
+                const float *from = part_of(k0 + lane);
+                const float mk = __ldcg(from + r);
+                f = mk == -INFINITY ? 0.0f : exp2_approx(mk - top);
+                total = fmaf(f, __ldcg(from + R + r), total);
+              }
             }
-            const float *row = part_of(k0) + 2 * R + (size_t)r * DP + lane * V;
-            const uint32_t some = min(32u, n - k0);
-#pragma unroll 8
-            for (uint32_t k = 0; k < some; k++) {
-              const float fk = __shfl_sync(0xFFFFFFFFu, f, k);
-              float v[V];
-              if constexpr (V == 2)
-                *reinterpret_cast<float2 *>(v) = __ldcg(reinterpret_cast<const float2 *>(row));
-              else
+            if (k0) ask(k0);
 #pragma unroll
-                for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(v + i) = __ldcg(reinterpret_cast<const float4 *>(row + i));
+            for (uint32_t k = 0; k < AT_ONCE; k++) {
+              const float fk = __shfl_sync(0xFFFFFFFFu, f, (k0 + k) & 31);
 #pragma unroll
-              for (int i = 0; i < V; i++) acc[i] = fmaf(fk, v[i], acc[i]);
-              row = k0 + k == 0 ? others + 2 * R + (size_t)r * DP + lane * V : row + 2 * part_floats(R, DP);
+              for (int i = 0; i < V; i++)
+                if (k0 + k < n) acc[i] = fmaf(fk, v[k][i], acc[i]);
             }
           }
 #pragma unroll
           for (int d = 16; d; d /= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
           const uint32_t tok = r / t.heads, head = t.head0 + r - tok * t.heads;
           if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
-          const float f = total == 0.0f ? 0.0f : 1.0f / total;
+          const float unit = total == 0.0f ? 0.0f : 1.0f / total;
           T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D + lane * V;
 #pragma unroll
           for (int i = 0; i < V; i += 2)
-            if (lane * V + i < D) reinterpret_cast<uint32_t *>(out)[i / 2] = Num<T>::pack(acc[i] * f, acc[i + 1] * f);
+            if (lane * V + i < D) reinterpret_cast<uint32_t *>(out)[i / 2] = Num<T>::pack(acc[i] * unit, acc[i + 1] * unit);
         }
       }
     }
@@ -391,14 +410,26 @@ size_t attend_counts(int sm_count) { return (size_t)sm_count; }
 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
-  // Rows of a sequence's tile on average.  16 and 32 are the tiles of the streaming kernel; beyond those it would read the cache once
-  // per 32 rows, and multiply them at the legacy rate.
-  const uint64_t rows = (uint64_t)(a.q_heads / a.kv_heads) * ((kv.n_rows + kv.n_seqs - 1) / kv.n_seqs);
+  // Rows x heads of a key head that a sequence has on average.  Up to 32, the streaming kernel's largest tile, it takes the batch alone.  Beyond,
+  // sequences that fit its 16 rows (32 where a token has more heads than that) stay with it, the others are the tensor-core kernel's: that one
+  // multiplies 128 rows whatever a sequence has, and reads a single token's cache at half the rate.  It takes the batch alone where there is one sequence, or
+  // 256 rows a sequence on average, whose own work outweighs single tokens among them (the other kernel's look at the batch is 4 us).
+  const uint32_t group = a.q_heads / a.kv_heads;
+  const uint64_t rows = (uint64_t)group * ((kv.n_rows + kv.n_seqs - 1) / kv.n_seqs);
+  const bool many = rows > 32 && a.head_dim <= 128;
+  const bool two = a.head_dim <= 128 && (many ? group > 16 : rows > 16);
+  const uint32_t max_rows = many ? (two ? 32 : 16) / group : 0xFFFFFFFFu;
+  const bool alone = many && (kv.n_seqs == 1 || kv.n_rows / kv.n_seqs >= 256);
+  if (max_rows > 0 && !alone) {
+    const PageMapShape m(a, kv, 16);
+    PageMaps maps{};
+    const bool mapped = encode_page_maps(&maps, m, a, kv);
+    const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, two ? 32 : 16, START_BLOCKS), max_rows, mapped ? m.rows : 0, m.head_first};
+    const cudaError_t e = a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, two, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, two, sm_count, s);
+    if (e != cudaSuccess) return e;
+    *launches += 1;
+  }
+  if (!many) return cudaSuccess;
   *launches += 1;
-  if (rows > 32 && a.head_dim <= 128) return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
-  const PageMapShape m(a, kv, 16);
-  PageMaps maps{};
-  const bool mapped = encode_page_maps(&maps, m, a, kv);
-  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, rows > 16 && a.head_dim <= 128 ? 32 : 16, START_BLOCKS), mapped ? m.rows : 0, m.head_first};
-  return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, rows > 16, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, rows > 16, sm_count, s);
+  return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, alone ? 0 : max_rows + 1, sm_count, s);
 }

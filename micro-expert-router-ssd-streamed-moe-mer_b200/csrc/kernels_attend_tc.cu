@@ -36,7 +36,7 @@ struct TcParams {
   void *out;
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
-  uint32_t min_blocks;
+  uint32_t min_blocks, min_rows;  // sequences with fewer rows are the streaming kernel's
   TileShape ts;
   uint32_t box;  // tokens of a tiled copy, 0: none
   bool head_first;
@@ -53,9 +53,8 @@ constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12, TC_WALK = 13, TILE_
 // Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
 constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
-constexpr uint32_t TC_START = 3;  // what a tile costs beside its blocks, in blocks
-constexpr float LAG = 3.0f;  // with P_SHIFT the largest weight is 2^15
-constexpr int POLY_EVERY = 4;  // pairs of weights per pair that the polynomial makes
+constexpr uint32_t TC_START = 1;  // what a tile costs beside its blocks, in blocks
+constexpr float LAG = 7.0f;        // with P_SHIFT the largest weight is 2^15 (scores of a standard deviation of 2: 157 us at 3, 146 so)
 constexpr uint32_t TC_CONTROL = 1024;  // barriers and words in front of the operands
 
 template <int DP>
@@ -105,24 +104,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
-// 2^x of two values by Cody and Waite's reduction x = i + f, |f| <= 1/2, and a polynomial of degree 4 for 2^f (Remez, relative error 2.7e-6: 2^-18.5), on the
-// fp32 units instead of the special function unit.  Below 2^-126 it stays there.
-__device__ __forceinline__ void exp2_poly2(uint64_t x, float &a, float &b) {
-  constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
-  unpack2(x, a, b);
-  x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const uint64_t t = add2(x, pack2(ROUND, ROUND));
-  const uint64_t f = fma2(add2(t, pack2(-ROUND, -ROUND)), pack2(-1.0f, -1.0f), x);
-  uint64_t r = fma2(f, pack2(9.570101911e-03f, 9.570101911e-03f), pack2(5.591786032e-02f, 5.591786032e-02f));
-  r = fma2(r, f, pack2(2.402474483e-01f, 2.402474483e-01f));
-  r = fma2(r, f, pack2(6.931218147e-01f, 6.931218147e-01f));
-  r = fma2(r, f, pack2(9.999992614e-01f, 9.999992614e-01f));
-  float ta, tb, ra, rb;
-  unpack2(t, ta, tb);
-  unpack2(r, ra, rb);
-  a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
-}
 // 32 bytes to an address on 32 bytes.
 __device__ __forceinline__ void store32(void *p, const uint4 &a, const uint4 &b) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
@@ -150,8 +131,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   }
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, 0, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
-  if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, 0, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
+  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, p.min_rows, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
+  if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, p.min_rows, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run_here.parts) return;
   if (tid == 0) ctl.run = run_here;
   if (warp == TC_MMA) {
@@ -229,9 +210,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
           }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 128; i += 4)
+          for (int i = 0; i < 128; i += 8)
 #pragma unroll
-            for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[i / 32][i % 32 + e]);
+            for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(s[i / 32][i % 32 + 2 * e], s[i / 32][i % 32 + 2 * e + 1]), top[e]);
           const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * to_log2;
           const bool grow = now > m + LAG || (m == -INFINITY && now > m);
           if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -260,12 +241,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             for (int i = 0; i < 32; i++) {
               const uint64_t at = fma2(pack2(s[2 * h + i / 16][2 * i % 32], s[2 * h + i / 16][2 * i % 32 + 1]), scale2, less2);
               float a, b;
-              if (i % POLY_EVERY == POLY_EVERY - 1) {
-                exp2_poly2(at, a, b);
-              } else {
-                unpack2(at, a, b);
-                a = exp2_approx(a), b = exp2_approx(b);
-              }
+              unpack2(at, a, b);
+              a = exp2_approx(a), b = exp2_approx(b);
               sum[i & 1] = add2(sum[i & 1], pack2(a, b));
               v[i] = Num<T>::pack(a, b);
             }
@@ -398,11 +375,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       tm_commit(leader, &ctl.s_full[x]);
     };
     while (next_tile()) {
-      const uint32_t groups = ctl.tile[turn & 1].tokens * ctl.tile[turn & 1].heads > 128 ? 2 : 1, lo = ctl.tile[turn & 1].lo, hi = ctl.tile[turn & 1].hi;
+      const TileWork &t = ctl.tile[turn & 1];
+      const uint32_t groups = t.tokens * t.heads > 128 ? 2 : 1, lo = t.lo, hi = t.hi;
+      // Blocks below `by_rows` and from `by_rows_again` on are filled row by row: not by the proxy that the tensor core reads through.
+      const uint32_t by_rows = p.box ? min(hi, (first_seen(t, window) + TC_KB - 1) / TC_KB) : hi, by_rows_again = (t.past + t.token0 + t.tokens) / TC_KB;
+      auto visible = [&](uint32_t blk) {
+        if (blk < by_rows || blk >= by_rows_again) proxy_fence();
+      };
       done_with();
       if (!wait(&ctl.q_full, tiles & 1)) break;
       if (!wait(&ctl.full[stage], phase)) break;
-      proxy_fence();
+      if (!p.q_mapped) proxy_fence();
+      visible(lo);
       tm_fence_after();
       for (uint32_t x = 0; x < groups; x++) qk(x, stage);
       tm_commit(leader, &ctl.empty[stage]);
@@ -415,7 +399,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         next_stage();
         if (!(ok = wait(&ctl.full[v_stage], v_phase))) break;
         if (more && !(ok = wait(&ctl.full[stage], phase))) break;
-        proxy_fence();
+        visible(blk);
+        if (more) visible(blk + 1);
         for (uint32_t x = 0; x < groups; x++) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
@@ -450,7 +435,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     }
     } else if (warp == TC_WALK) {
       // -------------------------------------------------------------- the way through the run
-      RunWalk<TC_KB> walk(p.kv, ts, window, 0, 0xFFFFFFFFu, ctl.run);
+      RunWalk<TC_KB> walk(p.kv, ts, window, p.min_rows, 0xFFFFFFFFu, ctl.run);
       TileWork t;
       for (uint32_t i = 0;; i++) {
         const bool more = walk.next(&t);
@@ -515,7 +500,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       }
       tiles++;
       const uint32_t end = t.past + t.token0 + t.tokens;
-      const uint32_t start = window && t.past + t.token0 + 1 > window ? t.past + t.token0 + 1 - window : 0;
+      const uint32_t start = first_seen(t, window);
       const PagePlaces pages(p.kv, p.a.page_tokens, t.seq, t.kv_head);
       // a lane's token of a block: the first of its tiled copy, or a row
       constexpr uint32_t SUBS = S::SUBS;
@@ -585,11 +570,11 @@ cudaError_t launch_tc(const TcParams &p, const TcMaps &maps, int sm_count, cudaS
 size_t attend_tc_part_floats(int sm_count) { return (size_t)2 * sm_count * part_floats(TC_R, 128); }
 
 cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
-                             int sm_count, cudaStream_t s) {
+                             uint32_t min_rows, int sm_count, cudaStream_t s) {
   const PageMapShape m(a, kv, TC_KB);
   TcMaps maps{};
   const bool mapped = encode_page_maps(&maps.pages, m, a, kv);
-  TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START), mapped ? m.rows : 0, m.head_first, false, false};
+  TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, min_rows, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START), mapped ? m.rows : 0, m.head_first, false, false};
   p.q_mapped = p.ts.chunks == 1 && encode_row_map(&maps.q, q, a, kv.n_rows, q_stride, p.ts.heads, p.ts.tokens);
   p.out32 = a.head_dim % 16 == 0 && ((uintptr_t)out | out_stride * 2) % 32 == 0;
   return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);

@@ -18,25 +18,32 @@ namespace {
 constexpr uint32_t KV_THREADS = 256;
 constexpr uint32_t KV_ROWS = 4;  // rows of a CTA at most
 
+// V values as they lie in memory.
 template <typename T, int V>
-struct Vec {
-  T v[V];
+struct Raw {
+  static constexpr int BYTES = sizeof(T) * V;
+  __align__(16) T t[V];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; i++) reinterpret_cast<uint4 *>(t)[i] = *(reinterpret_cast<const uint4 *>(p) + i);
+    } else if constexpr (BYTES == 8) {
+      reinterpret_cast<uint2 *>(t)[0] = *reinterpret_cast<const uint2 *>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++) t[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; i++) x[i] = Num<T>::f(t[i]);
+  }
 };
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T *p, float (&x)[V]) {
-  constexpr int BYTES = sizeof(T) * V;
-  __align__(16) T t[V];
-  if constexpr (BYTES % 16 == 0) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; i++) reinterpret_cast<uint4 *>(t)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-  } else if constexpr (BYTES == 8) {
-    reinterpret_cast<uint2 *>(t)[0] = __ldg(reinterpret_cast<const uint2 *>(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) t[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < V; i++) x[i] = Num<T>::f(t[i]);
+  Raw<T, V> r;
+  r.load(p);
+  r.get(x);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T *p, const float (&x)[V]) {
@@ -73,8 +80,36 @@ __global__ void __launch_bounds__(KV_THREADS) k_kv_append(const KvParams p) {
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t row0 = blockIdx.x * p.rows, n_rows = min(p.rows, p.kv.n_rows - row0);
   const uint32_t heads = a.q_heads + 2 * a.kv_heads, h0 = blockIdx.y * p.head_step, h1 = min(heads, h0 + p.head_step);
+  // The thread's part of the unit'th (row, head) of the CTA: pair m of the head's vectors.  Behind the rotated values neighbours pair up, of which
+  // the last may have no second.
+  const uint32_t sub = tid & (p.group - 1), unit0 = tid / p.group, units = KV_THREADS / p.group;
+  const uint32_t n_heads = h1 - h0, D = a.head_dim, half = a.rope_dims / 2;
+  constexpr int STEPS = V == 1 ? 4 : 1;  // V == 1: 32 lanes take up to 4 pairs each
+  uint32_t at[STEPS][2];
+#pragma unroll
+  for (int k = 0; k < STEPS; k++) {
+    const uint32_t m = sub + k * p.group, rot = a.rope_dims / (2 * V);
+    at[k][0] = m < rot && !a.rope_pairs ? m * V : 2 * m * V;
+    at[k][1] = at[k][0] + (m < rot && !a.rope_pairs ? half : V);
+  }
+  Raw<IN, V> next[STEPS][2];
+  auto ask = [&](uint32_t u) {
+    if (u >= n_rows * n_heads) return;
+    const uint32_t r = n_rows == 1 ? 0 : u / n_heads, h = h0 + u - r * n_heads;
+    const uint64_t row = row0 + r;
+    const IN *src = h < a.q_heads ? (const IN *)p.r.q + row * p.r.q_stride + (uint64_t)h * D
+                    : h < a.q_heads + a.kv_heads ? (const IN *)p.r.k + row * p.r.k_stride + (uint64_t)(h - a.q_heads) * D
+                                                 : (const IN *)p.r.v + row * p.r.v_stride + (uint64_t)(h - a.q_heads - a.kv_heads) * D;
+    if (h < a.q_heads && !p.r.q) return;
+#pragma unroll
+    for (int k = 0; k < STEPS; k++)
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        if (at[k][e] < D) next[k][e].load(src + at[k][e]);
+  };
   grid_dep_wait();
   grid_dep_launch();
+  ask(unit0);  // while positions and places are looked up
   if (warp < n_rows) {  // a warp finds a row's sequence: the last one that starts at the row or before it
     const uint32_t row = row0 + warp;
     uint32_t starts = 0;
@@ -100,7 +135,6 @@ __global__ void __launch_bounds__(KV_THREADS) k_kv_append(const KvParams p) {
     if (lane == 0) s_pos[warp] = pos, s_place[warp] = place;
   }
   __syncthreads();
-  const uint32_t half = a.rope_dims / 2;
   for (uint32_t i = tid; i < n_rows * half; i += KV_THREADS) {
     const uint32_t r = i / half, j = i - r * half;
     if (s_pos[r] < 0) continue;
@@ -111,43 +145,32 @@ __global__ void __launch_bounds__(KV_THREADS) k_kv_append(const KvParams p) {
   }
   __syncthreads();
 
-  const uint32_t sub = tid & (p.group - 1), unit0 = tid / p.group, units = KV_THREADS / p.group;
-  const uint32_t n_heads = h1 - h0, D = a.head_dim;
   // every group of lanes makes the same number of steps, so that the shuffles of a warp meet
   for (uint32_t u0 = 0; u0 < n_rows * n_heads; u0 += units) {
-    const uint32_t u = u0 + unit0, r = u / n_heads, h = h0 + u - r * n_heads;
+    const uint32_t u = u0 + unit0, r = n_rows == 1 ? 0 : u / n_heads, h = h0 + u - r * n_heads;
     const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
     const bool on = u < n_rows * n_heads && s_pos[r] >= 0 && (!is_q || p.r.q);
     const uint32_t head = is_q ? h : is_k ? h - a.q_heads : h - a.q_heads - a.kv_heads;
     const uint64_t row = row0 + r;
-    const IN *src = nullptr;
     OUT *dst = nullptr;
-    if (on) {
-      src = is_q ? (const IN *)p.r.q + row * p.r.q_stride : is_k ? (const IN *)p.r.k + row * p.r.k_stride : (const IN *)p.r.v + row * p.r.v_stride;
-      src += (uint64_t)head * D;
+    if (on)
       dst = is_q ? (OUT *)p.r.q_out + row * p.r.q_out_stride + (uint64_t)head * D
                  : (OUT *)(is_k ? p.kv.k_pages : p.kv.v_pages) + s_place[r] + head * p.kv.head_stride;
-    }
-    // The thread's vectors: pair m of the head.  Behind the rotated values neighbours pair up, of which the last may have no second.
-    constexpr int STEPS = V == 1 ? 4 : 1;  // V == 1: 32 lanes take up to 4 pairs each
     float x[STEPS][2][V];
-    uint32_t at[STEPS][2];
     float sq = 0.0f;
 #pragma unroll
-    for (int k = 0; k < STEPS; k++) {
-      const uint32_t m = sub + k * p.group, rot = a.rope_dims / (2 * V);
-      at[k][0] = m < rot && !a.rope_pairs ? m * V : 2 * m * V;
-      at[k][1] = at[k][0] + (m < rot && !a.rope_pairs ? half : V);
+    for (int k = 0; k < STEPS; k++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const bool in = on && at[k][e] < D;
+        if (on && at[k][e] < D)
+          next[k][e].get(x[k][e]);
+        else
 #pragma unroll
-        for (int i = 0; i < V; i++) x[k][e][i] = 0.0f;
-        if (in) load_vec<IN, V>(src + at[k][e], x[k][e]);
+          for (int i = 0; i < V; i++) x[k][e][i] = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; i++) sq = fmaf(x[k][e][i], x[k][e][i], sq);
       }
-    }
+    ask(u + units);
     const float *w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
     for (uint32_t d = 1; d < p.group; d *= 2) sq += __shfl_xor_sync(0xFFFFFFFFu, sq, d);
     const float unit = w ? rsqrtf(sq / (float)D + a.norm_eps) : 1.0f;
@@ -187,7 +210,7 @@ __global__ void __launch_bounds__(KV_THREADS) k_kv_append(const KvParams p) {
         }
       }
     }
-    // q may be rotated in place: all of a head's values are in registers before its first store
+    // q may be rotated in place: all of a head's values are in registers before its first store, and no other thread asks for them
     __syncwarp();
     if (on) {
 #pragma unroll
