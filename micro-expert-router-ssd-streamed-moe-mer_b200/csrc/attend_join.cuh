@@ -10,14 +10,14 @@ template <uint32_t KB>
 struct RunWalk {
   const KvBatchDev &kv;
   const TileShape &ts;
-  uint32_t window, min_n, max_n;
+  uint32_t window;
   uint64_t left, at;  // blocks of the run that are left, and the next one's number
   SeqWork w;
   uint32_t seq, v_head, tile, from;  // from: what of the tile is not this run's (its first tile alone)
   bool fresh = true;
 
-  __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, uint32_t lo, uint32_t hi, const RunStart &r)
-      : kv(kv_), ts(ts_), window(window_), min_n(lo), max_n(hi), w(r.w), seq(r.seq), v_head(r.v_head), tile(r.tile), from(r.from) {
+  __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, const RunStart &r)
+      : kv(kv_), ts(ts_), window(window_), w(r.w), seq(r.seq), v_head(r.v_head), tile(r.tile), from(r.from) {
     at = run_first(r, blockIdx.x);
     left = r.total == 0 ? 0 : run_first(r, blockIdx.x + 1) - at;
   }
@@ -35,7 +35,7 @@ struct RunWalk {
           do {
             seq++;
             if (seq >= kv.n_seqs) return false;
-            w = seq_work(kv, seq, ts.tokens, min_n, max_n);
+            w = seq_work(kv, seq, ts.tokens);
           } while (w.tiles == 0);
         }
       }
@@ -61,17 +61,17 @@ struct RunWalk {
 
 // Rows that have no place in their sequence (it brings more rows than it has tokens) see nothing: zero.
 template <typename T, uint32_t THREADS>
-__device__ void clear_rows_without_place(const AttnLayer &a, const KvBatchDev &kv, uint32_t min_n, uint32_t max_n, T *out, uint64_t out_stride, uint32_t *status) {
+__device__ void clear_rows_without_place(const AttnLayer &a, const KvBatchDev &kv, T *out, uint64_t out_stride, uint32_t *status) {
   for (uint32_t s0 = 0; s0 < kv.n_seqs; s0 += THREADS) {
     const uint32_t s = s0 + threadIdx.x;
     uint32_t row = 0, n = 0, len = 0;
     if (s < kv.n_seqs) seq_rows(kv, s, &row, &n, &len);
-    const bool some = n > len && n >= min_n && n <= max_n;
+    const bool some = n > len;
     if (some) atomicOr(status, MER_DEVSTAT_BAD_CACHE);
     if (!__syncthreads_or(some)) continue;
     for (uint32_t i = s0; i < min(kv.n_seqs, s0 + THREADS); i++) {
       seq_rows(kv, i, &row, &n, &len);
-      if (n <= len || n < min_n || n > max_n) continue;
+      if (n <= len) continue;
       const uint32_t width = a.q_heads * a.head_dim;
       for (uint64_t e = threadIdx.x; e < (uint64_t)(n - len) * width; e += THREADS) out[(row + e / width) * out_stride + e % width] = Num<T>::one(0.0f);
     }

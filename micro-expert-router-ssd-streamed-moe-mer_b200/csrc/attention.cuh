@@ -89,10 +89,9 @@ __device__ __forceinline__ void seq_rows(const KvBatchDev &kv, uint32_t s, uint3
   *len = min(__ldg(kv.kv_len + s), 0x7FFFFFFFu);
 }
 // Rows that have no place (more rows than tokens) see nothing.
-__device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, uint32_t tokens, uint32_t min_n, uint32_t max_n) {
+__device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, uint32_t tokens) {
   uint32_t row, n, len;
   seq_rows(kv, s, &row, &n, &len);
-  if (n < min_n || n > max_n) n = 0;
   const uint32_t skip = n > len ? n - len : 0;
   SeqWork w;
   w.row0 = row + skip, w.n = n - skip, w.past = len - w.n;
@@ -149,14 +148,14 @@ __device__ __forceinline__ uint64_t scan_threads(uint64_t mine, uint64_t *sums, 
 
 // All threads of the CTA (16 warps at most), which take consecutive sequences each; `found` in shared memory.
 template <uint32_t KB, uint32_t THREADS>
-__device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t window, uint32_t min_n, uint32_t max_n, uint32_t cta, uint32_t ctas,
+__device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t window, uint32_t cta, uint32_t ctas,
                              uint32_t min_blocks, RunFound &found) {
   const uint32_t tid = threadIdx.x, each = (kv.n_seqs + THREADS - 1) / THREADS;
   const uint32_t s0 = min(kv.n_seqs, tid * each), s1 = min(kv.n_seqs, s0 + each);
   uint64_t mine = 0, per_head = 0, total;
   SeqWork w{};
   for (uint32_t s = s0; s < s1; s++) {
-    w = seq_work(kv, s, ts.tokens, min_n, max_n);
+    w = seq_work(kv, s, ts.tokens);
     per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) + w.tiles * ts.start;
     mine += per_head * ts.v_heads;
   }
@@ -172,7 +171,7 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
     uint32_t s = s0;
     if (s1 - s0 > 1) {
       for (;; s++) {
-        w = seq_work(kv, s, ts.tokens, min_n, max_n);
+        w = seq_work(kv, s, ts.tokens);
         per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) + w.tiles * ts.start;
         if (x0 < at + per_head * ts.v_heads) break;
         at += per_head * ts.v_heads;

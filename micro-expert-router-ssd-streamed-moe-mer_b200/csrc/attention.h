@@ -60,7 +60,7 @@ size_t attend_part_floats(int sm_count);
 // kernels_attend_tc.cu
 size_t attend_tc_part_floats(int sm_count);
 cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
-                             uint32_t min_rows, int sm_count, cudaStream_t s);
+                             int sm_count, cudaStream_t s);
 // kernels_attend.cu
 size_t attend_counts(int sm_count);
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,

@@ -29,7 +29,6 @@ struct AttendParams {
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
   TileShape ts;
-  uint32_t max_rows;  // sequences with more rows are the other kernel's
   uint32_t box;  // tokens of a tiled copy (8 or 16), 0: none
   bool head_first;
 };
@@ -87,10 +86,10 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, 0, p.max_rows, blockIdx.x, gridDim.x, 1, s_found);
-  if (blockIdx.x == 0) clear_rows_without_place<T, THREADS>(p.a, p.kv, 0, p.max_rows, (T *)p.out, p.out_stride, p.ws.status);
+  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, 1, s_found);
+  if (blockIdx.x == 0) clear_rows_without_place<T, THREADS>(p.a, p.kv, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run.parts) return;
-  RunWalk<KB> walk(p.kv, ts, window, 0, p.max_rows, run);
+  RunWalk<KB> walk(p.kv, ts, window, run);
   const float to_log2 = p.a.scale * LOG2E;
   uint32_t fill = 0, stage = 0, stage_phase = 0, timed_out = 0;  // of the warp's ring: what is asked for next, what is taken next
   const uint32_t ring = smem_u32(s_ring) + warp * (ST * S::CHUNK), q_addr = smem_u32(s_q);
@@ -395,41 +394,30 @@ cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_co
   return launch_overlapped(k_attend_stream<T, DP, MT>, dim3(sm_count), S::THREADS, SMEM, s, false, p, maps);
 }
 template <typename T>
-cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, bool two, int sm_count, cudaStream_t s) {
-  if (p.a.head_dim <= 64) return two ? launch_stream<T, 64, 2>(p, maps, sm_count, s) : launch_stream<T, 64, 1>(p, maps, sm_count, s);
-  if (p.a.head_dim <= 128) return two ? launch_stream<T, 128, 2>(p, maps, sm_count, s) : launch_stream<T, 128, 1>(p, maps, sm_count, s);
-  return launch_stream<T, 256, 1>(p, maps, sm_count, s);
+cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
+  if (p.a.head_dim <= 64) return launch_stream<T, 64, 1>(p, maps, sm_count, s);
+  return p.a.head_dim <= 128 ? launch_stream<T, 128, 1>(p, maps, sm_count, s) : launch_stream<T, 256, 1>(p, maps, sm_count, s);
 }
 
 }  // namespace
 
 size_t attend_part_floats(int sm_count) {
-  return std::max({(size_t)2 * sm_count * part_floats(32, 128), (size_t)2 * sm_count * part_floats(16, 256), attend_tc_part_floats(sm_count)});
+  return std::max((size_t)2 * sm_count * part_floats(16, 256), attend_tc_part_floats(sm_count));
 }
 size_t attend_counts(int sm_count) { return (size_t)sm_count; }
 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
-  // Rows x heads of a key head that a sequence has on average.  Up to 32, the streaming kernel's largest tile, it takes the batch alone.  Beyond,
-  // sequences that fit its 16 rows (32 where a token has more heads than that) stay with it, the others are the tensor-core kernel's: that one
-  // multiplies 128 rows whatever a sequence has, and reads a single token's cache at half the rate.  It takes the batch alone where there is one sequence, or
-  // 256 rows a sequence on average, whose own work outweighs single tokens among them (the other kernel's look at the batch is 4 us).
-  const uint32_t group = a.q_heads / a.kv_heads;
-  const uint64_t rows = (uint64_t)group * ((kv.n_rows + kv.n_seqs - 1) / kv.n_seqs);
-  const bool many = rows > 32 && a.head_dim <= 128;
-  const bool two = a.head_dim <= 128 && (many ? group > 16 : rows > 16);
-  const uint32_t max_rows = many ? (two ? 32 : 16) / group : 0xFFFFFFFFu;
-  const bool alone = many && (kv.n_seqs == 1 || kv.n_rows / kv.n_seqs >= 256);
-  if (max_rows > 0 && !alone) {
-    const PageMapShape m(a, kv, 16);
-    PageMaps maps{};
-    const bool mapped = encode_page_maps(&maps, m, a, kv);
-    const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, two ? 32 : 16, START_BLOCKS), max_rows, mapped ? m.rows : 0, m.head_first};
-    const cudaError_t e = a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, two, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, two, sm_count, s);
-    if (e != cudaSuccess) return e;
+  // One row a sequence and no more heads of a key head than a tile has rows: the streaming kernel.  Any more rows: the tensor-core kernel, whose 128 rows a group cost
+  // the same whatever they hold.
+  if (a.head_dim <= 128 && (kv.n_rows > kv.n_seqs || a.q_heads / a.kv_heads > 16)) {
     *launches += 1;
+    return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
   }
-  if (!many) return cudaSuccess;
+  const PageMapShape m(a, kv, 16);
+  PageMaps maps{};
+  const bool mapped = encode_page_maps(&maps, m, a, kv);
+  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, 16, START_BLOCKS), mapped ? m.rows : 0, m.head_first};
   *launches += 1;
-  return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, alone ? 0 : max_rows + 1, sm_count, s);
+  return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, sm_count, s);
 }

@@ -9,6 +9,8 @@
 //   * Warps 0..3 and 4..7 are the softmax of one group of rows each, warps 8..11 copy, warp 12 issues the MMAs, warp 13 goes ahead through the run and leaves
 //     the next tile's place in shared memory (14 and 15 fill the group).  While one group's
 //     softmax runs the tensor core multiplies for the other: [P V of block j, Q K of block j + 1] of one, then of the other.
+//   * A tile of up to 128 rows (single tokens, drafts) has one group of rows; the two take its blocks in turn and their results are joined at its end, so that it is
+//     read as fast as two groups of rows would be multiplied.
 //   * The reference maximum of a row follows its maximum only when that has grown by more than 2^LAG; then alone the output in tensor memory is rescaled, by
 //     the softmax warps themselves.  Until then weights are larger than 1 by up to that factor, which f16 and fp32 hold.  What makes that safe without a
 //     barrier: the MMAs complete in order, so the S of block j being there says that the P V of block j - 1 has been added.
@@ -37,7 +39,7 @@ struct TcParams {
   void *out;
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
-  uint32_t min_blocks, min_rows;  // sequences with fewer rows are the streaming kernel's
+  uint32_t min_blocks;
   TileShape ts;
   uint32_t box;  // tokens of a tiled copy, 0: none
   bool head_first;
@@ -56,7 +58,7 @@ constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
 constexpr uint32_t TC_START = 1;  // what a tile costs beside its blocks, in blocks
 constexpr float LAG = 7.0f;        // with P_SHIFT the largest weight is 2^15 (scores of a standard deviation of 2: 157 us at 3, 146 so)
-constexpr uint32_t TC_CONTROL = 1024;  // barriers and words in front of the operands
+constexpr uint32_t TC_CONTROL = 2048;  // barriers and words in front of the operands
 
 template <int DP>
 struct TcShape {
@@ -74,6 +76,7 @@ struct TcControl {
   TileWork tile[2];  // tokens == 0: there is none left
   RunStart run;
   RunFound found;
+  float one_m[128], one_l[128];  // of the second group's rows where both have the same ones
   uint32_t tmem, flag[2];  // flags take turns: a sync lies between two uses of one
   volatile uint32_t abort;
 };
@@ -115,8 +118,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   }
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, p.min_rows, 0xFFFFFFFFu, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
-  if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, p.min_rows, 0xFFFFFFFFu, (T *)p.out, p.out_stride, p.ws.status);
+  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
+  if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run_here.parts) return;
   if (tid == 0) ctl.run = run_here;
   if (warp == TC_MMA) {
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
     // ---------------------------------------------------------------- softmax: a thread has row x * 128 + (tid & 127) of the tile
-    const uint32_t x = warp >> 2, row = tid;
+    const uint32_t x = warp >> 2;
     const uint32_t tm_lane = tm + ((warp & 3) << 21), s_at = tm_lane + x * 128, o_at = tm_lane + 256 + x * DP;
     const float to_log2 = p.a.scale * LOG2E;
     uint32_t blocks = 0, tiles = 0, syncs = 0, flags = 0;  // phases of s_full, o_full, soft; uses of the flags
@@ -163,16 +166,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     while (next_tile()) {
       const TileWork &t = ctl.tile[turn & 1];
       const uint32_t rows = t.tokens * t.heads;
-      const bool active = rows > x * 128;
+      const uint32_t lo = t.lo, hi = t.hi;
+      const bool one = rows <= 128, two_parts = one && hi - lo > 1;  // one group of rows, of which both warps' groups have blocks
+      const uint32_t row0 = one ? 0 : x * 128, row = row0 + (tid & 127);
+      const bool active = one ? lo + x < hi : rows > row0;
       const uint32_t first = t.past + t.token0, see = first + min(row, rows - 1) / t.heads;
       const uint32_t least = window && see + 1 > window ? see + 1 - window : 0;  // the row sees least .. see
       float m = -INFINITY, l = 0.0f;
       if (active) {
         // blocks that every row of the group sees whole need no mask
-        const uint32_t see0 = first + x * 128 / t.heads, see1 = first + min(x * 128 + 127, rows - 1) / t.heads;
+        const uint32_t see0 = first + row0 / t.heads, see1 = first + min(row0 + 127, rows - 1) / t.heads;
         const uint32_t least1 = window && see1 + 1 > window ? see1 + 1 - window : 0;
-        const uint32_t lo = t.lo, hi = t.hi;
-        for (uint32_t blk = lo; blk < hi; blk++, blocks++) {
+        const uint32_t blk0 = one ? lo + x : lo;
+        for (uint32_t blk = blk0; blk < hi; blk += one ? 2 : 1, blocks++) {
           if (!wait(&ctl.s_full[x], blocks & 1)) break;
           tm_fence_after();
           float s[4][32];
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             const float f = grow ? (m == -INFINITY ? 0.0f : exp2_approx(m - now)) : 1.0f;
             if (grow) m = now;
             l *= f;
-            if (blk != lo) {
+            if (blk != blk0) {
               float o[32];
 #pragma unroll 1
               for (int c = 0; c < DP; c += 32) {
@@ -243,11 +249,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
           }
         }
       }
-      const bool whole = t.lo == t.tile_lo && t.hi == t.tile_hi;
-      if (active) {
-        if (!wait(&ctl.o_full[x], tiles++ & 1)) break;
+      const bool whole = lo == t.tile_lo && hi == t.tile_hi;
+      const bool ends = one ? x == 0 : active;  // this thread has a row's end to see to
+      if (active && !wait(&ctl.o_full[x], tiles++ & 1)) break;
+      tm_fence_after();
+      // Of one row's two halves the first group's thread sees to both: it reaches the other's output in tensor memory.
+      float mine_f = 1.0f, other_f = 0.0f;
+      if (two_parts) {
+        if (x == 1) ctl.one_m[tid & 127] = m, ctl.one_l[tid & 127] = l;
+        tm_fence_before();
+        sync();
         tm_fence_after();
+        if (x == 0) {
+          const float m1 = ctl.one_m[row], l1 = ctl.one_l[row], top = fmaxf(m, m1);
+          mine_f = m == -INFINITY ? 0.0f : exp2_approx(m - top), other_f = m1 == -INFINITY ? 0.0f : exp2_approx(m1 - top);
+          m = top, l = l * mine_f + l1 * other_f;
+        }
       }
+      auto load_o = [&](int c, float(&o)[32]) {
+        __syncwarp();
+        tm_load(o_at + c, o);
+        if (two_parts) {
+          float o1[32];
+          tm_load(o_at + DP + c, o1);
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = o[i] * mine_f + o1[i] * other_f;
+        }
+      };
       // The rows of a tile that other runs have parts of.  Its first run comes to it last, at its own end: mostly the others have left their parts by then,
       // and it adds them to what it has.  Where they have not, it leaves its own like them, and whoever arrives last joins them, in the same order.
       uint32_t c0 = 0, n = 1, mine = 0;  // `mine`: this CTA has part 0 and all others are there
@@ -263,13 +291,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       // Parts lie as [piece of four values][row]: the rows of a warp side by side.
       float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(TC_R, DP);
       if (!joins) {
-        if (active) {
+        if (ends) {
           if (row < rows) part[row] = m, part[TC_R + row] = l;
 #pragma unroll 1
           for (int c = 0; c < DP; c += 32) {
             float o[32];
-            __syncwarp();
-            tm_load(o_at + c, o);
+            load_o(c, o);
             if (row < rows) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) reinterpret_cast<float4 *>(part + 2 * TC_R)[(c + i) / 4 * TC_R + row] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
@@ -282,7 +309,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         joins = ctl.flag[flags++ & 1];
       }
       if (!whole && joins && tid == 0) p.ws.counts[c0] = 0;
-      if (joins && active) {
+      if (joins && ends) {
         const bool own = whole || mine;  // part 0 is in tensor memory
         const uint32_t tok = row / t.heads, head = t.head0 + row - tok * t.heads;
         // the row's reference and sum over all parts
@@ -300,8 +327,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           float o[32];
-          __syncwarp();
-          tm_load(o_at + c, o);
+          load_o(c, o);
           float mo = own ? m : -INFINITY;
           for (uint32_t k = own ? 1 : 0; k < n; k++) {
             const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP));
@@ -335,6 +361,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
       }
       tm_fence_before();
+      if (two_parts) sync();  // the second group's output has been read
       done_with();
     }
   } else if (warp >= TC_MMA) {
@@ -345,73 +372,100 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t BASE = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((128u >> 4) << 24);
     constexpr uint32_t QK = BASE | ((TC_KB >> 3) << 17), PV = BASE | (1u << 16) | ((DP >> 3) << 17);
-    uint32_t stage = 0, phase = 0, tiles = 0, blocks = 0;  // blocks: phases of p_ready[0]; of p_ready[1] the same while its group is active
-    uint32_t blocks1 = 0;
-    auto next_stage = [&] { stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0; };
+    uint32_t tiles = 0, blocks0 = 0, blocks1 = 0, at = 0;  // phases of q_full and p_ready; places of the ring before the tile's: keys of its block j are at + 2 j, values the next
+    auto place = [&](uint64_t *bars, uint32_t q) { return &bars[q % S::STAGES]; };
+    auto landed = [&](uint32_t q) { return wait(place(ctl.full, q), (q / S::STAGES) & 1); };
     // the low words of the descriptors; those of the pieces of an operand lie constants apart
     constexpr uint64_t ALONG_K = (64ull << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16), ALONG_N = (64ull << 32) | (1ull << 46) | (2ull << 61) | ((uint64_t)(TC_KB * 128 >> 4) << 16);
     const uint32_t q_at = s_q >> 4, ring_at = s_ring >> 4;
-    auto qk = [&](uint32_t x, uint32_t st) {
-      const uint32_t a = q_at + x * (16384 >> 4), b = ring_at + st * (S::STAGE >> 4);
+    auto qk = [&](uint32_t x, uint32_t rows_of, uint32_t q) {  // the scores of a group for the keys at place q
+      const uint32_t a = q_at + rows_of * (16384 >> 4), b = ring_at + q % S::STAGES * (S::STAGE >> 4);
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
         tm_mma_ss(leader, tm + x * 128, ALONG_K | (a + (k / 4) * (S::QSUB >> 4) + (k & 3) * 2), ALONG_K | (b + (k / 4) * (TC_KB * 128 >> 4) + (k & 3) * 2), QK, k != 0);
       tm_commit(leader, &ctl.s_full[x]);
     };
+    auto pv = [&](uint32_t x, uint32_t q, bool first) {  // its weights times the values at place q
+      const uint32_t b = ring_at + q % S::STAGES * (S::STAGE >> 4);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (!wait(h ? &ctl.p_ready[x] : &ctl.p_half[x], (x ? blocks1 : blocks0) & 1)) return false;
+        tm_fence_after();
+#pragma unroll
+        for (int k = 4 * h; k < 4 * h + 4; k++) tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, ALONG_N | (b + k * 128), PV, k != 0 || !first);
+      }
+      blocks0 += x == 0, blocks1 += x == 1;
+      return true;
+    };
+    auto free_place = [&](uint32_t q) { tm_commit(leader, place(ctl.empty, q)); };
     while (next_tile()) {
       const TileWork &t = ctl.tile[turn & 1];
-      const uint32_t groups = t.tokens * t.heads > 128 ? 2 : 1, lo = t.lo, hi = t.hi;
+      const uint32_t rows = t.tokens * t.heads, lo = t.lo, n = t.hi - t.lo;
       // Blocks below `by_rows` and from `by_rows_again` on are filled row by row: not by the proxy that the tensor core reads through.
-      const uint32_t by_rows = p.box ? min(hi, (first_seen(t, window) + TC_KB - 1) / TC_KB) : hi, by_rows_again = (t.past + t.token0 + t.tokens) / TC_KB;
-      auto visible = [&](uint32_t blk) {
-        if (blk < by_rows || blk >= by_rows_again) proxy_fence();
+      const uint32_t by_rows = p.box ? (first_seen(t, window) + TC_KB - 1) / TC_KB : 0xFFFFFFFFu, by_rows_again = (t.past + t.token0 + t.tokens) / TC_KB;
+      auto visible = [&](uint32_t j) {
+        if (lo + j < by_rows || lo + j >= by_rows_again) proxy_fence();
       };
       done_with();
-      if (!wait(&ctl.q_full, tiles & 1)) break;
-      if (!wait(&ctl.full[stage], phase)) break;
+      if (!wait(&ctl.q_full, tiles++ & 1)) break;
       if (!p.q_mapped) proxy_fence();
-      visible(lo);
-      tm_fence_after();
-      for (uint32_t x = 0; x < groups; x++) qk(x, stage);
-      tm_commit(leader, &ctl.empty[stage]);
-      next_stage();
-      if (lo + 1 == hi) tm_commit(leader, &ctl.q_empty);
       bool ok = true;
-      for (uint32_t blk = lo; blk < hi && ok; blk++) {
-        const uint32_t v_stage = stage, v_phase = phase;
-        const bool more = blk + 1 < hi;
-        next_stage();
-        if (!(ok = wait(&ctl.full[v_stage], v_phase))) break;
-        if (more && !(ok = wait(&ctl.full[stage], phase))) break;
-        visible(blk);
-        if (more) visible(blk + 1);
-        for (uint32_t x = 0; x < groups; x++) {
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            if (!(ok = wait(h ? &ctl.p_ready[x] : &ctl.p_half[x], (x ? blocks1 : blocks) & 1))) break;
-            tm_fence_after();
-#pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; k++)
-              tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, ALONG_N | (ring_at + v_stage * (S::STAGE >> 4) + k * 128), PV, k != 0 || blk != lo);
+      if (rows <= 128) {  // the groups take the blocks in turn
+        for (uint32_t j = 0; j < 2 && j < n && ok; j++) {
+          if (!(ok = landed(at + 2 * j))) break;
+          visible(j);
+          tm_fence_after();
+          qk(j, 0, at + 2 * j);
+          free_place(at + 2 * j);
+          if (j + 1 == n) tm_commit(leader, &ctl.q_empty);
+        }
+        for (uint32_t j = 0; j < n && ok; j++) {
+          const uint32_t x = j & 1, v = at + 2 * j + 1, k = at + 2 * (j + 2);
+          if (!(ok = landed(v))) break;
+          visible(j);
+          if (!(ok = pv(x, v, j < 2))) break;
+          free_place(v);
+          if (j + 2 < n) {
+            if (!(ok = landed(k))) break;
+            visible(j + 2);
+            qk(x, 0, k);
+            free_place(k);
+            if (j + 3 == n) tm_commit(leader, &ctl.q_empty);
+          } else {
+            tm_commit(leader, &ctl.o_full[x]);
+          }
+        }
+      } else {
+        if (!landed(at)) break;
+        visible(0);
+        tm_fence_after();
+        for (uint32_t x = 0; x < 2; x++) qk(x, x, at);
+        free_place(at);
+        if (n == 1) tm_commit(leader, &ctl.q_empty);
+        for (uint32_t j = 0; j < n && ok; j++) {
+          const uint32_t v = at + 2 * j + 1, k = v + 1;
+          const bool more = j + 1 < n;
+          if (!(ok = landed(v))) break;
+          if (more && !(ok = landed(k))) break;
+          visible(j);
+          if (more) visible(j + 1);
+          for (uint32_t x = 0; x < 2; x++) {
+            if (!(ok = pv(x, v, j == 0))) break;
+            if (more)
+              qk(x, x, k);
+            else
+              tm_commit(leader, &ctl.o_full[x]);
           }
           if (!ok) break;
-          if (more)
-            qk(x, stage);
-          else
-            tm_commit(leader, &ctl.o_full[x]);
-        }
-        if (!ok) break;
-        blocks++;
-        if (groups == 2) blocks1++;
-        tm_commit(leader, &ctl.empty[v_stage]);
-        if (more) {
-          tm_commit(leader, &ctl.empty[stage]);
-          next_stage();
-          if (blk + 2 == hi) tm_commit(leader, &ctl.q_empty);
+          free_place(v);
+          if (more) {
+            free_place(k);
+            if (j + 2 == n) tm_commit(leader, &ctl.q_empty);
+          }
         }
       }
       if (!ok) break;
-      tiles++;
+      at += 2 * n;
     }
     if (aborted()) {
       tm_commit(leader, &ctl.drain);
@@ -419,7 +473,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     }
     } else if (warp == TC_WALK) {
       // -------------------------------------------------------------- the way through the run
-      RunWalk<TC_KB> walk(p.kv, ts, window, p.min_rows, 0xFFFFFFFFu, ctl.run);
+      RunWalk<TC_KB> walk(p.kv, ts, window, ctl.run);
       TileWork t;
       for (uint32_t i = 0;; i++) {
         const bool more = walk.next(&t);
@@ -554,11 +608,11 @@ cudaError_t launch_tc(const TcParams &p, const TcMaps &maps, int sm_count, cudaS
 size_t attend_tc_part_floats(int sm_count) { return (size_t)2 * sm_count * part_floats(TC_R, 128); }
 
 cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
-                             uint32_t min_rows, int sm_count, cudaStream_t s) {
+                             int sm_count, cudaStream_t s) {
   const PageMapShape m(a, kv, TC_KB);
   TcMaps maps{};
   const bool mapped = encode_page_maps(&maps.pages, m, a, kv);
-  TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, min_rows, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START), mapped ? m.rows : 0, m.head_first, false, false};
+  TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START), mapped ? m.rows : 0, m.head_first, false, false};
   p.q_mapped = p.ts.chunks == 1 && encode_row_map(&maps.q, q, a, kv.n_rows, q_stride, p.ts.heads, p.ts.tokens);
   p.out32 = a.head_dim % 16 == 0 && ((uintptr_t)out | out_stride * 2) % 32 == 0;
   return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);
