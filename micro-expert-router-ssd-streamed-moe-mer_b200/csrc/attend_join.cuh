@@ -1,4 +1,4 @@
-// The way of a CTA through its run of blocks, and the end of a tile: its rows stored, or the parts of several CTAs joined.
+// The way of a CTA through its run, and the end of a tile: its rows stored, or the parts of several CTAs joined.
 #pragma once
 
 #include "attention.cuh"
@@ -11,7 +11,7 @@ struct RunWalk {
   const KvBatchDev &kv;
   const TileShape &ts;
   uint32_t window;
-  uint64_t left, at;  // blocks of the run that are left, and the next one's number
+  uint64_t left, at;  // units of the run that are left, and the next one's number
   SeqWork w;
   uint32_t seq, v_head, tile, from;  // from: what of the tile is not this run's (its first tile alone)
   bool fresh = true;
@@ -21,33 +21,35 @@ struct RunWalk {
     at = run_first(r, blockIdx.x);
     left = r.total == 0 ? 0 : run_first(r, blockIdx.x + 1) - at;
   }
-  // The next tile of the run, or a part of one.
+  // The next tile of the run, or a part of one.  A block is the run's that its first unit lies in.
   __device__ bool next(TileWork *t) {
-    if (left == 0) return false;
-    if (fresh) {
-      fresh = false;
-    } else {
-      from = 0;
-      if (++tile >= w.tiles) {
-        tile = 0;
-        if (++v_head >= ts.v_heads) {
-          v_head = 0;
-          do {
-            seq++;
-            if (seq >= kv.n_seqs) return false;
-            w = seq_work(kv, seq, ts.tokens);
-          } while (w.tiles == 0);
+    do {
+      if (left == 0) return false;
+      if (fresh) {
+        fresh = false;
+      } else {
+        from = 0;
+        if (++tile >= w.tiles) {
+          tile = 0;
+          if (++v_head >= ts.v_heads) {
+            v_head = 0;
+            do {
+              seq++;
+              if (seq >= kv.n_seqs) return false;
+              w = seq_work(kv, seq, ts.tokens);
+            } while (w.tiles == 0);
+          }
         }
       }
-    }
-    w.tile_blocks<KB>(tile, ts.tokens, window, &t->tile_lo, &t->tile_hi);
-    const uint32_t to = (uint32_t)min((uint64_t)(ts.start + t->tile_hi - t->tile_lo), from + left);
-    t->at = at - from + ts.start;
-    t->lo = t->tile_lo + (from > ts.start ? from - ts.start : 0);
-    left -= to - from;
-    at += to - from;
-    if (to <= ts.start) return false;  // the run ends in front of the tile's first block: the next one begins it
-    t->hi = t->tile_lo + to - ts.start;
+      w.tile_blocks<KB>(tile, ts.tokens, window, &t->tile_lo, &t->tile_hi);
+      t->units = block_units(ts, w.n);
+      const uint32_t to = (uint32_t)min((uint64_t)(ts.start + (t->tile_hi - t->tile_lo) * t->units), from + left);
+      auto blocks_until = [&](uint32_t unit) { return unit <= ts.start ? 0u : t->units == 1 ? unit - ts.start : (unit - ts.start + t->units - 1) / t->units; };
+      t->at = at - from + ts.start;
+      t->lo = t->tile_lo + blocks_until(from), t->hi = t->tile_lo + blocks_until(to);
+      left -= to - from;
+      at += to - from;
+    } while (t->lo >= t->hi);  // no block of it
     t->seq = seq, t->row0 = w.row0, t->past = w.past;
     t->token0 = tile * ts.tokens;
     t->tokens = min(ts.tokens, w.n - t->token0);
@@ -97,23 +99,11 @@ __device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t,
 // The runs that have a part of a tile: c0, and n - 1 after it.
 __device__ __forceinline__ void runs_of_tile(const RunStart &run, const TileWork &t, uint32_t *c0, uint32_t *n) {
   *c0 = run_of(run, t.at);
-  *n = run_of(run, t.at + (t.tile_hi - t.tile_lo) - 1) - *c0 + 1;
+  *n = run_of(run, t.at + (uint64_t)(t.tile_hi - t.tile_lo - 1) * t.units) - *c0 + 1;
 }
 // Part k of a tile in the workspace.
 __device__ __forceinline__ const float *part_of_tile(const RunStart &run, const TileWork &t, const float *parts, uint32_t c0, uint32_t k, uint32_t floats) {
   return parts + (size_t)(k == 0 ? part_slot(run, t, c0) : 2 * (c0 + k)) * floats;
 }
-
-// Running maximum, sum and four values of a row, part by part.
-struct Joined {
-  float top = -INFINITY, sum = 0.0f;
-  float4 acc = make_float4(0, 0, 0, 0);
-  __device__ __forceinline__ void add(float m, float l, const float4 &v) {
-    const float now = fmaxf(top, m), old = top == -INFINITY ? 0.0f : exp2_approx(top - now), f = m == -INFINITY ? 0.0f : exp2_approx(m - now);
-    top = now;
-    sum = fmaf(f, l, sum * old);
-    acc.x = fmaf(f, v.x, acc.x * old), acc.y = fmaf(f, v.y, acc.y * old), acc.z = fmaf(f, v.z, acc.z * old), acc.w = fmaf(f, v.w, acc.w * old);
-  }
-};
 
 }  // namespace

@@ -3,8 +3,8 @@
 // A tile is up to R rows (tokens x the query heads of one key head) of one sequence; its work is counted in blocks of KB tokens
 // of the cache, of which it has only those that one of its rows sees.  The blocks of all tiles in order
 // (sequence, key head, tile) are cut into one equal run per CTA, so a long sequence is split over many CTAs and many short ones
-// share one, whatever the lengths are; nothing of this needs the lengths on the host.  A tile counts for `start` blocks more than it has, in front of its
-// own: what beginning and ending one costs.  A tile that lies in the runs of several CTAs is
+// share one, whatever the lengths are; nothing of this needs the lengths on the host.  The runs are equal in units: a block has one, or
+// `dense` of a sequence with so many rows that its blocks take longer, and a tile has `start` units in front of its blocks, for beginning and ending it.  A tile that lies in the runs of several CTAs is
 // joined by the one that arrives last, in the order of the runs: results do not depend on who that is.
 #pragma once
 
@@ -70,8 +70,8 @@ struct SeqWork {
 
 // How heads and rows of a layer lie in tiles of R rows: heads of a group are taken `heads` at a time.
 struct TileShape {
-  uint32_t group, chunks, heads, tokens, v_heads, start;
-  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R, uint32_t start_) : start(start_) {
+  uint32_t group, chunks, heads, tokens, v_heads, start, dense, sparse_rows;  // sparse_rows: a sequence with more has dense blocks
+  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R, uint32_t start_, uint32_t dense_, uint32_t sparse_rows_) : start(start_), dense(dense_), sparse_rows(sparse_rows_) {
     group = q_heads / kv_heads;
     chunks = (group + R - 1) / R;
     heads = (group + chunks - 1) / chunks;
@@ -80,6 +80,9 @@ struct TileShape {
     v_heads = kv_heads * chunks;
   }
 };
+
+// Units of a block of a sequence.
+__device__ __forceinline__ uint32_t block_units(const TileShape &ts, uint32_t n) { return n * ts.heads > ts.sparse_rows ? ts.dense : 1; }
 
 // Rows of sequence s in the batch, cut to the batch: wrong tables read nothing outside it.
 __device__ __forceinline__ void seq_rows(const KvBatchDev &kv, uint32_t s, uint32_t *row, uint32_t *n, uint32_t *len) {
@@ -102,15 +105,15 @@ __device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, ui
 
 // The cut of a batch's blocks into runs, and where this CTA's starts.
 struct RunStart {
-  uint64_t total, each;  // blocks of the batch, blocks of a run: `more` runs have one more
+  uint64_t total, each;  // units of the batch, units of a run: `more` runs have one more
   uint32_t parts, more;  // CTAs that share the work
-  uint32_t seq;          // the sequence of the run's first block
-  uint32_t v_head, tile, from;  // its head, its tile, and what of the tile lies before it
+  uint32_t seq;          // the sequence of the run's first unit
+  uint32_t v_head, tile, from;  // its head, its tile, and the tile's units before it
   SeqWork w;
 };
-// First block of a CTA's run.
+// First unit of a CTA's run.
 __device__ __forceinline__ uint64_t run_first(const RunStart &r, uint32_t cta) { return r.each * cta + min(cta, r.more); }
-// The CTA whose run holds block x.
+// The CTA whose run holds unit x.
 __device__ __forceinline__ uint32_t run_of(const RunStart &r, uint64_t x) {
   const uint64_t wide = (r.each + 1) * r.more;
   return x < wide ? (uint32_t)divided(x, r.each + 1) : r.more + (uint32_t)divided(x - wide, r.each);
@@ -149,20 +152,20 @@ __device__ __forceinline__ uint64_t scan_threads(uint64_t mine, uint64_t *sums, 
 // All threads of the CTA (16 warps at most), which take consecutive sequences each; `found` in shared memory.
 template <uint32_t KB, uint32_t THREADS>
 __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t window, uint32_t cta, uint32_t ctas,
-                             uint32_t min_blocks, RunFound &found) {
+                             uint32_t min_units, RunFound &found) {
   const uint32_t tid = threadIdx.x, each = (kv.n_seqs + THREADS - 1) / THREADS;
   const uint32_t s0 = min(kv.n_seqs, tid * each), s1 = min(kv.n_seqs, s0 + each);
   uint64_t mine = 0, per_head = 0, total;
   SeqWork w{};
   for (uint32_t s = s0; s < s1; s++) {
     w = seq_work(kv, s, ts.tokens);
-    per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) + w.tiles * ts.start;
+    per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) * block_units(ts, w.n) + w.tiles * ts.start;
     mine += per_head * ts.v_heads;
   }
   const uint64_t first = scan_threads<THREADS>(mine, found.sums, &total);
   RunStart r;
   r.total = total;
-  r.parts = (uint32_t)max((uint64_t)1, min((uint64_t)ctas, min_blocks == 1 ? total : divided(total, min_blocks)));
+  r.parts = (uint32_t)max((uint64_t)1, min((uint64_t)ctas, min_units == 1 ? total : divided(total, min_units)));
   r.each = divided(total, r.parts);
   r.more = (uint32_t)(total - r.each * r.parts);
   const uint64_t x0 = run_first(r, min(cta, r.parts));
@@ -172,7 +175,7 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
     if (s1 - s0 > 1) {
       for (;; s++) {
         w = seq_work(kv, s, ts.tokens);
-        per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) + w.tiles * ts.start;
+        per_head = w.blocks_before<KB>(w.tiles, ts.tokens, window) * block_units(ts, w.n) + w.tiles * ts.start;
         if (x0 < at + per_head * ts.v_heads) break;
         at += per_head * ts.v_heads;
       }
@@ -188,17 +191,18 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
   if (r.w.tiles > 1) {  // threads take consecutive tiles each
     const uint32_t some = (r.w.tiles + THREADS - 1) / THREADS, j0 = min(r.w.tiles, tid * some), j1 = min(r.w.tiles, j0 + some);
     uint32_t lo, hi;
+    const uint32_t units = block_units(ts, r.w.n);
     mine = 0;
-    for (uint32_t j = j0; j < j1; j++) r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi), mine += hi - lo + ts.start;
+    for (uint32_t j = j0; j < j1; j++) r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi), mine += (hi - lo) * units + ts.start;
     uint64_t at = scan_threads<THREADS>(mine, found.more_sums, &total);
     if (x >= at && x < at + mine) {
       for (uint32_t j = j0;; j++) {
         r.w.tile_blocks<KB>(j, ts.tokens, window, &lo, &hi);
-        if (x < at + (hi - lo + ts.start)) {
+        if (x < at + ((hi - lo) * units + ts.start)) {
           found.tile = j, found.from = (uint32_t)(x - at);
           break;
         }
-        at += hi - lo + ts.start;
+        at += (hi - lo) * units + ts.start;
       }
     }
     __syncthreads();
@@ -248,7 +252,8 @@ struct TileWork {
   uint32_t kv_head, head0, heads;  // query heads head0 .. head0 + heads
   uint32_t seq, lo, hi;      // blocks of this run
   uint32_t tile_lo, tile_hi; // blocks of the whole tile
-  uint64_t at;               // the tile's first block among all
+  uint64_t at;               // the unit of the tile's first block among all
+  uint32_t units;            // of a block
 };
 
 // The first token that a row of the tile sees.

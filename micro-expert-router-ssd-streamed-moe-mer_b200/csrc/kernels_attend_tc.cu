@@ -39,7 +39,7 @@ struct TcParams {
   void *out;
   uint64_t q_stride, out_stride;
   AttnWorkspace ws;
-  uint32_t min_blocks;
+  uint32_t min_units;
   TileShape ts;
   uint32_t box;  // tokens of a tiled copy, 0: none
   bool head_first;
@@ -56,9 +56,11 @@ constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12, TC_WALK = 13, TILE_
 // Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
 constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
-constexpr uint32_t TC_START = 1;  // what a tile costs beside its blocks, in blocks
+// What a tile costs beside its blocks, and a block of two groups of rows, in blocks of one: 8000, 3500 and 1900 cycles.
+constexpr uint32_t TC_START = 4, TC_DENSE = 2, TC_MIN_RUN = 4;
+static_assert(TC_MIN_RUN >= TC_DENSE, "every run inside a tile has a block of it");
 constexpr float LAG = 7.0f;        // with P_SHIFT the largest weight is 2^15 (scores of a standard deviation of 2: 157 us at 3, 146 so)
-constexpr uint32_t TC_CONTROL = 2048;  // barriers and words in front of the operands
+constexpr uint32_t TC_CONTROL = 3072;  // barriers and words in front of the operands, which lie on whole atoms of 1024 bytes
 
 template <int DP>
 struct TcShape {
@@ -66,7 +68,7 @@ struct TcShape {
   static constexpr uint32_t STAGE = SUBS * TC_KB * 128;    // keys or values of a block
   static constexpr uint32_t STAGES = DP == 128 ? 5 : 10;
   static constexpr uint32_t QSUB = TC_R * 128;             // 64 values of all queries of a tile
-  static constexpr size_t SMEM = TC_CONTROL + 1024 + SUBS * QSUB + STAGES * STAGE;  // 1024: the operands lie on whole atoms
+  static constexpr size_t SMEM = TC_CONTROL + SUBS * QSUB + STAGES * STAGE;
 };
 
 struct TcControl {
@@ -76,11 +78,11 @@ struct TcControl {
   TileWork tile[2];  // tokens == 0: there is none left
   RunStart run;
   RunFound found;
-  float one_m[128], one_l[128];  // of the second group's rows where both have the same ones
+  float one_m[2][128], one_l[2][128];  // what the groups say of rows that both have
   uint32_t tmem, flag[2];  // flags take turns: a sync lies between two uses of one
   volatile uint32_t abort;
 };
-static_assert(sizeof(TcControl) <= TC_CONTROL, "control block");
+static_assert(sizeof(TcControl) <= TC_CONTROL && TC_CONTROL % 1024 == 0, "control block");
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -100,9 +102,9 @@ __device__ __forceinline__ void store32(void *p, const uint4 &a, const uint4 &b)
 template <typename T, int DP>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, const __grid_constant__ TcMaps maps) {
   using S = TcShape<DP>;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   TcControl &ctl = *reinterpret_cast<TcControl *>(smem);
-  const uint32_t operands = (smem_u32(smem) + TC_CONTROL + 1023u) & ~1023u;
+  const uint32_t operands = smem_u32(smem) + TC_CONTROL;
   const uint32_t s_q = operands, s_ring = operands + S::SUBS * S::QSUB;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t D = p.a.head_dim, window = p.a.window;
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   }
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, p.min_blocks, ctl.found);
+  const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, p.min_units, ctl.found);
   if (blockIdx.x == 0) clear_rows_without_place<T, TC_THREADS>(p.a, p.kv, (T *)p.out, p.out_stride, p.ws.status);
   if (blockIdx.x >= run_here.parts) return;
   if (tid == 0) ctl.run = run_here;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
     // ---------------------------------------------------------------- softmax: a thread has row x * 128 + (tid & 127) of the tile
     const uint32_t x = warp >> 2;
-    const uint32_t tm_lane = tm + ((warp & 3) << 21), s_at = tm_lane + x * 128, o_at = tm_lane + 256 + x * DP;
+    const uint32_t tm_lane = tm + ((warp & 3) << 21), s_at = tm_lane + x * 128, own_o = tm_lane + 256 + x * DP;
     const float to_log2 = p.a.scale * LOG2E;
     uint32_t blocks = 0, tiles = 0, syncs = 0, flags = 0;  // phases of s_full, o_full, soft; uses of the flags
     auto sync = [&] {
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       const bool one = rows <= 128, two_parts = one && hi - lo > 1;  // one group of rows, of which both warps' groups have blocks
       const uint32_t row0 = one ? 0 : x * 128, row = row0 + (tid & 127);
       const bool active = one ? lo + x < hi : rows > row0;
-      const uint32_t first = t.past + t.token0, see = first + min(row, rows - 1) / t.heads;
+      const uint32_t tok = min(row, rows - 1) / t.heads, first = t.past + t.token0, see = first + tok;
       const uint32_t least = window && see + 1 > window ? see + 1 - window : 0;  // the row sees least .. see
       float m = -INFINITY, l = 0.0f;
       if (active) {
@@ -213,11 +215,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
               float o[32];
 #pragma unroll 1
               for (int c = 0; c < DP; c += 32) {
-                tm_load(o_at + c, o);
+                tm_load(own_o + c, o);
                 uint32_t v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __float_as_uint(o[i] * f);
-                tm_store(o_at + c, v);
+                tm_store(own_o + c, v);
               }
             }
           }
@@ -250,22 +252,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
       }
       const bool whole = lo == t.tile_lo && hi == t.tile_hi;
-      const bool ends = one ? x == 0 : active;  // this thread has a row's end to see to
       if (active && !wait(&ctl.o_full[x], tiles++ & 1)) break;
       tm_fence_after();
-      // Of one row's two halves the first group's thread sees to both: it reaches the other's output in tensor memory.
-      float mine_f = 1.0f, other_f = 0.0f;
-      if (two_parts) {
-        if (x == 1) ctl.one_m[tid & 127] = m, ctl.one_l[tid & 127] = l;
+      // Rows of one group: each group of warps sees to half of their values, of both outputs in tensor memory.
+      const bool ends = one || active;
+      float f0 = 1.0f, f1 = 0.0f;  // factors of the two outputs
+      if (one) {
+        ctl.one_m[x][row] = m, ctl.one_l[x][row] = l;
         tm_fence_before();
         sync();
         tm_fence_after();
-        if (x == 0) {
-          const float m1 = ctl.one_m[row], l1 = ctl.one_l[row], top = fmaxf(m, m1);
-          mine_f = m == -INFINITY ? 0.0f : exp2_approx(m - top), other_f = m1 == -INFINITY ? 0.0f : exp2_approx(m1 - top);
-          m = top, l = l * mine_f + l1 * other_f;
-        }
+        const float m0 = ctl.one_m[0][row], m1 = ctl.one_m[1][row];
+        m = fmaxf(m0, m1);
+        f0 = m0 == -INFINITY ? 0.0f : exp2_approx(m0 - m), f1 = m1 == -INFINITY ? 0.0f : exp2_approx(m1 - m);
+        l = ctl.one_l[0][row] * f0 + ctl.one_l[1][row] * f1;
       }
+      const int c_first = one && x == 1 ? DP / 2 : 0, c_end = one && x == 0 ? DP / 2 : DP;
+      const uint32_t o_at = tm_lane + 256 + (one ? 0 : x * DP);
       auto load_o = [&](int c, float(&o)[32]) {
         __syncwarp();
         tm_load(o_at + c, o);
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
           float o1[32];
           tm_load(o_at + DP + c, o1);
 #pragma unroll
-          for (int i = 0; i < 32; i++) o[i] = o[i] * mine_f + o1[i] * other_f;
+          for (int i = 0; i < 32; i++) o[i] = o[i] * f0 + o1[i] * f1;
         }
       };
       // The rows of a tile that other runs have parts of.  Its first run comes to it last, at its own end: mostly the others have left their parts by then,
@@ -289,12 +292,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
       }
       // Parts lie as [piece of four values][row]: the rows of a warp side by side.
-      float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(TC_R, DP);
       if (!joins) {
+        float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(TC_R, DP);
         if (ends) {
-          if (row < rows) part[row] = m, part[TC_R + row] = l;
+          if (row < rows && c_first == 0) part[row] = m, part[TC_R + row] = l;
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
+          for (int c = c_first; c < c_end; c += 32) {
             float o[32];
             load_o(c, o);
             if (row < rows) {
@@ -311,37 +314,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (!whole && joins && tid == 0) p.ws.counts[c0] = 0;
       if (joins && ends) {
         const bool own = whole || mine;  // part 0 is in tensor memory
-        const uint32_t tok = row / t.heads, head = t.head0 + row - tok * t.heads;
+        const uint32_t head = t.head0 + min(row, rows - 1) - tok * t.heads;
         // the row's reference and sum over all parts
-        float top = own ? m : -INFINITY, total = own ? l : 0.0f;
-        for (uint32_t k = own ? 1 : 0; k < n; k++) {
-          const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP));
-          Joined j;
-          j.top = top, j.sum = total;
-          j.add(__ldcg(from + row), __ldcg(from + TC_R + row), make_float4(0, 0, 0, 0));
-          top = j.top, total = j.sum;
+        const uint32_t k0 = own ? 1 : 0;
+        float top = own ? m : -INFINITY, total;
+        for (uint32_t k = k0; k < n; k++) top = fmaxf(top, __ldcg(part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP)) + row));
+        auto weight = [&](float m_of) { return m_of == -INFINITY ? 0.0f : exp2_approx(m_of - top); };
+        const float own_f = own ? weight(m) : 0.0f;
+        total = l * own_f;
+        for (uint32_t k = k0; k < n; k++) {
+          const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP)) + row;
+          total = k == 0 ? weight(__ldcg(from)) * __ldcg(from + TC_R) : fmaf(weight(__ldcg(from)), __ldcg(from + TC_R), total);
         }
         if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
         const float f = total == 0.0f ? 0.0f : 1.0f / total;
         T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D;
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = c_first; c < c_end; c += 32) {
           float o[32];
           load_o(c, o);
-          float mo = own ? m : -INFINITY;
-          for (uint32_t k = own ? 1 : 0; k < n; k++) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] *= own_f;
+          for (uint32_t k = k0; k < n; k++) {
             const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP));
-            const float mk = __ldcg(from + row), now = fmaxf(mo, mk);
-            const float old = mo == -INFINITY ? 0.0f : exp2_approx(mo - now), g = mk == -INFINITY ? 0.0f : exp2_approx(mk - now);
-            mo = now;
             float4 v[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = __ldcg(reinterpret_cast<const float4 *>(from + 2 * TC_R) + (c / 4 + i) * TC_R + row);
+            const float w = weight(__ldcg(from + row));
 #pragma unroll
             for (int i = 0; i < 8; i++) {
               const bool start = k == 0;
-              o[4 * i] = start ? v[i].x : fmaf(g, v[i].x, o[4 * i] * old), o[4 * i + 1] = start ? v[i].y : fmaf(g, v[i].y, o[4 * i + 1] * old);
-              o[4 * i + 2] = start ? v[i].z : fmaf(g, v[i].z, o[4 * i + 2] * old), o[4 * i + 3] = start ? v[i].w : fmaf(g, v[i].w, o[4 * i + 3] * old);
+              o[4 * i] = start ? w * v[i].x : fmaf(w, v[i].x, o[4 * i]), o[4 * i + 1] = start ? w * v[i].y : fmaf(w, v[i].y, o[4 * i + 1]);
+              o[4 * i + 2] = start ? w * v[i].z : fmaf(w, v[i].z, o[4 * i + 2]), o[4 * i + 3] = start ? w * v[i].w : fmaf(w, v[i].w, o[4 * i + 3]);
             }
           }
           if (row >= rows) continue;
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
       }
       tm_fence_before();
-      if (two_parts) sync();  // the second group's output has been read
+      if (one) sync();  // both outputs have been read
       done_with();
     }
   } else if (warp >= TC_MMA) {
@@ -612,7 +616,7 @@ cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const voi
   const PageMapShape m(a, kv, TC_KB);
   TcMaps maps{};
   const bool mapped = encode_page_maps(&maps.pages, m, a, kv);
-  TcParams p{a, kv, q, out, q_stride, out_stride, ws, 2, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START), mapped ? m.rows : 0, m.head_first, false, false};
+  TcParams p{a, kv, q, out, q_stride, out_stride, ws, TC_MIN_RUN, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START, TC_DENSE, 128), mapped ? m.rows : 0, m.head_first, false, false};
   p.q_mapped = p.ts.chunks == 1 && encode_row_map(&maps.q, q, a, kv.n_rows, q_stride, p.ts.heads, p.ts.tokens);
   p.out32 = a.head_dim % 16 == 0 && ((uintptr_t)out | out_stride * 2) % 32 == 0;
   return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);
