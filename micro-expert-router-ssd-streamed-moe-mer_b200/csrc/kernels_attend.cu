@@ -1,9 +1,9 @@
-// Attention of few new rows over a paged cache: single tokens, drafts.  Any head size up to 256 in steps of 8.
+// Attention of single new tokens over a paged cache, and of any rows with heads of more than 128 values.  Head sizes up to 256 in steps of 8.
 //
 //   o = sum_j 2^(s_j - m) v_j / (sum_j 2^(s_j - m) [+ 2^(sink - m)]),  s_j = q . k_j * scale * log2 e,  m = max_j s_j
 //
 // in one pass over the keys with the running maximum and sum of every row.  What bounds it is reading the cache: per 16 tokens 16 * 2 *
-// head_dim values for at most 32 rows of work.  So a warp is a stream of its own: it copies the next chunks of 16 tokens (tiled copies of 8 or 16
+// head_dim values for at most 16 rows of work.  So a warp is a stream of its own: it copies the next chunks of 16 tokens (tiled copies of 8 or 16
 // tokens of a page; row by row, 16 bytes a lane, where a sequence's end or a window cuts a chunk or pages have no such runs) into a ring that no other warp sees, multiplies the one that has landed (mma.sync on 16 x 16 tiles; at this rate of
 // operations the legacy tensor path is idle most of the time) and keeps maximum, sum and output of its own tokens in registers: no barrier
 // in the loop.  The warps' results are joined in shared memory at the end of a tile, those of several CTAs through the workspace (attention.cuh).
@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr uint32_t START_UNITS = 2;  // what a tile costs beside its blocks, in blocks
+constexpr uint32_t START_UNITS = 3;  // what a tile costs beside its blocks, in blocks
 
 struct AttendParams {
   AttnLayer a;
@@ -33,7 +33,7 @@ struct AttendParams {
   bool head_first;
 };
 
-// Rows of a tile are MT * 16, warps NW, chunks in flight per warp ST.
+// Warps NW, chunks in flight per warp ST.
 template <int DP>
 struct StreamShape {
   static constexpr int NW = DP == 256 ? 4 : 8, ST = DP == 64 ? 6 : 3;
@@ -48,6 +48,12 @@ __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
 }
 __device__ __forceinline__ void ldm4_trans(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+// A load that stays where it stands among the copies.
+__device__ __forceinline__ uint4 load_now(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
 }
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -68,22 +74,25 @@ __device__ __forceinline__ uint32_t piece(uint32_t r, uint32_t c) {
   return (c >> 3) * (ROWS * 128) + r * 128 + (((c ^ r) & 7) << 4);
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP>
 __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(const AttendParams p, const __grid_constant__ PageMaps maps) {
   using S = StreamShape<DP>;
-  constexpr int NW = S::NW, ST = S::ST, R = MT * 16;
+  constexpr int NW = S::NW, ST = S::ST, R = 16;
   constexpr uint32_t KB = S::KB, THREADS = S::THREADS;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ uint64_t s_full[NW * ST];  // a chunk has landed: every lane of its warp arrives
   __shared__ RunFound s_found;
   __shared__ uint32_t s_flag;
+  __shared__ uint64_t s_join;
   uint8_t *s_ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // [NW][ST][k, v][DP / 64][16][64]
   uint8_t *s_q = s_ring + NW * ST * S::CHUNK;                                  // [DP / 64][R][64]
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t D = p.a.head_dim, page_tokens = p.a.page_tokens, window = p.a.window;
   const TileShape &ts = p.ts;
   for (uint32_t i = tid; i < NW * ST; i += THREADS) mbar_init(&s_full[i], 32);
+  if (tid == 0) mbar_init(&s_join, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (tid == 0 && p.box) prefetch_map(&maps.k), prefetch_map(&maps.v);
   grid_dep_wait();
   grid_dep_launch();
   const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, 1, s_found);
@@ -91,7 +100,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   if (blockIdx.x >= run.parts) return;
   RunWalk<KB> walk(p.kv, ts, window, run);
   const float to_log2 = p.a.scale * LOG2E;
-  uint32_t fill = 0, stage = 0, stage_phase = 0, timed_out = 0;  // of the warp's ring: what is asked for next, what is taken next
+  uint32_t fill = 0, stage = 0, stage_phase = 0, join_phase = 0, timed_out = 0;  // of the warp's ring: what is asked for next, what is taken next
   const uint32_t ring = smem_u32(s_ring) + warp * (ST * S::CHUNK), q_addr = smem_u32(s_q);
 
   TileWork t;
@@ -139,37 +148,35 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     };
+    // Queries are asked for ahead of the keys: behind these they would wait for a full ring of every SM.
+    constexpr uint32_t Q_PIECES = (R * (DP / 8) + THREADS - 1) / THREADS;  // of a thread
     uint32_t ahead[ST];
 #pragma unroll
     for (int i = 0; i < ST; i++) ahead[i] = entry(t.lo + i);
+    uint4 q[Q_PIECES];
+#pragma unroll
+    for (uint32_t u = 0; u < Q_PIECES; u++) {
+      const uint32_t i = tid + u * THREADS, r = i / (DP / 8), c = i % (DP / 8), tok = r / t.heads, h = r - tok * t.heads;
+      q[u] = make_uint4(0, 0, 0, 0);
+      if (r < rows && c * 8 < D)  // rows <= R: also the threads that have none
+        q[u] = load_now((const T *)p.q + (uint64_t)(t.row0 + t.token0 + tok) * p.q_stride + (uint64_t)(t.head0 + h) * D + c * 8);
+    }
 #pragma unroll
     for (int i = 0; i < ST - 1; i++) issue(t.lo + i, ahead[i]);
     uint32_t next_entry = ahead[ST - 1];
-    // ---- queries, while the first chunks are on their way
-    for (uint32_t i = tid; i < R * (DP / 8); i += THREADS) {
-      const uint32_t r = i / (DP / 8), c = i % (DP / 8), tok = r / t.heads, h = r - tok * t.heads;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows && c * 8 < D)
-        v = __ldg(reinterpret_cast<const uint4 *>((const T *)p.q + (uint64_t)(t.row0 + t.token0 + tok) * p.q_stride + (uint64_t)(t.head0 + h) * D + c * 8));
-      *reinterpret_cast<uint4 *>(s_q + piece<R>(r, c)) = v;
+#pragma unroll
+    for (uint32_t u = 0; u < Q_PIECES; u++) {
+      const uint32_t i = tid + u * THREADS;
+      if (i < R * (DP / 8)) *reinterpret_cast<uint4 *>(s_q + piece<R>(i / (DP / 8), i % (DP / 8))) = q[u];
     }
     __syncthreads();
-    // tokens that the lane's rows see: (first, last] of each
-    uint32_t last[MT][2];
+    // the last tokens that the lane's two rows see
+    const uint32_t last[2] = {t.past + t.token0 + min(lane / 4, rows - 1) / t.heads, t.past + t.token0 + min(8 + lane / 4, rows - 1) / t.heads};
+    float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int i = 0; i < DP / 8; i++)
 #pragma unroll
-      for (int e = 0; e < 2; e++) last[mt][e] = t.past + t.token0 + min(mt * 16 + e * 8 + lane / 4, rows - 1) / t.heads;
-    float o[MT][DP / 8][4], m[MT][2], l[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-      for (int i = 0; i < DP / 8; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[mt][i][e] = 0.0f;
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.0f;
-    }
+      for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
     for (uint32_t blk = t.lo; blk < t.hi; blk++) {
       {
         const uint32_t number = next_entry;
@@ -181,88 +188,65 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
       const uint32_t key0 = blk * KB + warp * 16, base = ring + stage * S::CHUNK;
       timed_out |= !mbar_wait(&s_full[warp * ST + stage], stage_phase);
       stage = stage + 1 == ST ? 0 : stage + 1, stage_phase ^= stage == 0;
-      float s[MT][2][4];
+      float s[2][4];
       {
-        // One tile of rows: the products of even and odd pieces of a head apart, so that half as many wait for one another.
-        constexpr int CHAINS = MT == 1 ? 2 : 1;
-        float c[CHAINS][MT][2][4];
-#pragma unroll
-        for (int i = 0; i < CHAINS * MT * 8; i++) (&c[0][0][0][0])[i] = 0.0f;
+        // the products of even and odd pieces of a head apart, so that half as many wait for one another
+        float c[2][2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < DP / 16; kk++) {
-          uint32_t kf[4];
+          uint32_t kf[4], qf[4];
           ldm4(kf, base + piece<16>((lane / 16) * 8 + (lane & 7), kk * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-          for (int mt = 0; mt < MT; mt++) {
-            uint32_t qf[4];
-            ldm4(qf, q_addr + piece<R>(mt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4)));
-            mma16816<T>(c[kk % CHAINS][mt][0], qf, kf[0], kf[1]);
-            mma16816<T>(c[kk % CHAINS][mt][1], qf, kf[2], kf[3]);
-          }
+          ldm4(qf, q_addr + piece<R>(((lane >> 3) & 1) * 8 + (lane & 7), kk * 2 + (lane >> 4)));
+          mma16816<T>(c[kk & 1][0], qf, kf[0], kf[1]);
+          mma16816<T>(c[kk & 1][1], qf, kf[2], kf[3]);
         }
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-          for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[mt][n][e] = CHAINS == 2 ? c[0][mt][n][e] + c[CHAINS - 1][mt][n][e] : c[0][mt][n][e];
-      }
-      uint32_t pf[MT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) {
-        float top[2] = {-INFINITY, -INFINITY};
-        const uint32_t key = key0 + (lane & 3) * 2;
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const uint32_t at = key + n * 8 + (e & 1), see = last[mt][e >> 1];
-            const bool seen = at <= see && (window == 0 || at + window > see);
-            s[mt][n][e] = seen ? s[mt][n][e] * to_log2 : -INFINITY;
-            top[e >> 1] = fmaxf(top[e >> 1], s[mt][n][e]);
-          }
+          for (int e = 0; e < 4; e++) s[n][e] = c[0][n][e] + c[1][n][e];
+      }
+      float top[2] = {-INFINITY, -INFINITY}, less[2];
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t at = key0 + (lane & 3) * 2 + n * 8 + (e & 1), see = last[e >> 1];
+          const bool seen = at <= see && (window == 0 || at + window > see);
+          s[n][e] = seen ? s[n][e] * to_log2 : -INFINITY;
+          top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], 1));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], 2));
+        top[e] = fmaxf(top[e], m[e]);
+        less[e] = top[e] == -INFINITY ? 0.0f : top[e] - P_SHIFT;
+      }
+      if (__any_sync(0xFFFFFFFFu, top[0] != m[0] || top[1] != m[1])) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          top[e] = fmaxf(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], 1));
-          top[e] = fmaxf(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], 2));
-          top[e] = fmaxf(top[e], m[mt][e]);
+          const float f = m[e] == -INFINITY ? 0.0f : exp2_approx(m[e] - top[e]);
+          l[e] *= f;
+          m[e] = top[e];
+#pragma unroll
+          for (int i = 0; i < DP / 8; i++) o[i][2 * e] *= f, o[i][2 * e + 1] *= f;
         }
-        const bool moved = top[0] != m[mt][0] || top[1] != m[mt][1];
-        float less[2];
-#pragma unroll
-        for (int e = 0; e < 2; e++) less[e] = top[e] == -INFINITY ? 0.0f : top[e] - P_SHIFT;
-        if (__any_sync(0xFFFFFFFFu, moved)) {
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float f = m[mt][e] == -INFINITY ? 0.0f : exp2_approx(m[mt][e] - top[e]);
-            l[mt][e] *= f;
-            m[mt][e] = top[e];
-#pragma unroll
-            for (int i = 0; i < DP / 8; i++) o[mt][i][2 * e] *= f, o[mt][i][2 * e + 1] *= f;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            s[mt][n][e] = exp2_approx(s[mt][n][e] - less[e >> 1]);
-            l[mt][e >> 1] += s[mt][n][e];
-          }
-        pf[mt][0] = Num<T>::pack(s[mt][0][0], s[mt][0][1]);
-        pf[mt][1] = Num<T>::pack(s[mt][0][2], s[mt][0][3]);
-        pf[mt][2] = Num<T>::pack(s[mt][1][0], s[mt][1][1]);
-        pf[mt][3] = Num<T>::pack(s[mt][1][2], s[mt][1][3]);
       }
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s[n][e] = exp2_approx(s[n][e] - less[e >> 1]);
+          l[e >> 1] += s[n][e];
+        }
+      const uint32_t pf[4] = {Num<T>::pack(s[0][0], s[0][1]), Num<T>::pack(s[0][2], s[0][3]), Num<T>::pack(s[1][0], s[1][1]), Num<T>::pack(s[1][2], s[1][3])};
       const uint32_t vbase = base + 16 * DP * 2;
 #pragma unroll
       for (int dn = 0; dn < DP / 16; dn++) {
         uint32_t vf[4];
         ldm4_trans(vf, vbase + piece<16>(((lane >> 3) & 1) * 8 + (lane & 7), dn * 2 + (lane >> 4)));
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-          mma16816<T>(o[mt][2 * dn], pf[mt], vf[0], vf[1]);
-          mma16816<T>(o[mt][2 * dn + 1], pf[mt], vf[2], vf[3]);
-        }
+        mma16816<T>(o[2 * dn], pf, vf[0], vf[1]);
+        mma16816<T>(o[2 * dn + 1], pf, vf[2], vf[3]);
       }
     }
     if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
@@ -271,19 +255,16 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
     float *s_m = reinterpret_cast<float *>(s_ring), *s_l = s_m + NW * R, *s_o = s_l + NW * R;
     __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int e = 0; e < 2; e++) {
+      float sum = l[e];
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      const uint32_t r = e * 8 + lane / 4;
+      if (r >= rows) continue;
+      if ((lane & 3) == 0) s_m[warp * R + r] = m[e], s_l[warp * R + r] = sum;
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        float sum = l[mt][e];
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-        const uint32_t r = mt * 16 + e * 8 + lane / 4;
-        if (r >= rows) continue;
-        if ((lane & 3) == 0) s_m[warp * R + r] = m[mt][e], s_l[warp * R + r] = sum;
-#pragma unroll
-        for (int i = 0; i < DP / 8; i++)
-          *reinterpret_cast<float2 *>(s_o + ((size_t)warp * R + r) * OP + i * 8 + (lane & 3) * 2) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
-      }
+      for (int i = 0; i < DP / 8; i++) *reinterpret_cast<float2 *>(s_o + ((size_t)warp * R + r) * OP + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+    }
     __syncthreads();
     const bool whole = t.lo == t.tile_lo && t.hi == t.tile_hi;
     float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(R, DP);
@@ -309,8 +290,8 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
     }
     if (!whole) {
       __syncthreads();
-      // The CTA that arrives last joins the parts in the order of the runs and leaves the count at zero: a warp a row, its lanes first over the parts (their
-      // factors), then over the row's values.
+      // The CTA that arrives last joins the parts in the order of the runs and leaves the count at zero.  A part's maxima, sums and rows lie one behind the
+      // other: each is one bulk copy into the rings, all in flight at once (a round trip for what other SMs have just written is 1500 to 3000 cycles).
       uint32_t c0, n;
       runs_of_tile(run, t, &c0, &n);
       if (tid == 0) {
@@ -318,62 +299,63 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         if (is_last) p.ws.counts[c0] = 0;
         s_flag = is_last;
       }
+      asm volatile("fence.proxy.async;" ::: "memory");  // what this CTA has in the rings, and what the others have left in memory
       __syncthreads();
       if (s_flag) {
-        constexpr int V = DP / 32;  // values of a lane
-        const float *first = part_of_tile(run, t, p.ws.parts, c0, 0, part_floats(R, DP)), *others = part_of_tile(run, t, p.ws.parts, c0, 1, part_floats(R, DP));
-        auto part_of = [&](uint32_t k) { return k == 0 ? first : others + (size_t)(k - 1) * (2 * part_floats(R, DP)); };
-        for (uint32_t r = warp; r < rows; r += NW) {
-          // a lane's values of AT_ONCE parts are asked for before the parts' maxima are known
-          constexpr uint32_t AT_ONCE = V == 8 || MT == 2 ? 8 : 16;
-          float top = -INFINITY, total = 0.0f, acc[V], v[AT_ONCE][V];
-          auto ask = [&](uint32_t k0) {
+        constexpr int V = DP / 32, TURNS = R / NW;  // values of a lane, rows of a warp
+        const uint32_t each = 2 * R + rows * DP, at_once = NW * ST * S::CHUNK / 4 / each;
+        const float *s_parts = reinterpret_cast<const float *>(s_ring);
+        float acc[TURNS][V], top[TURNS], total[TURNS];
 #pragma unroll
-            for (uint32_t k = 0; k < AT_ONCE; k++) {
-              if (k0 + k >= n) continue;
-              const float *row = part_of(k0 + k) + 2 * R + (size_t)r * DP + lane * V;
-              if constexpr (V == 2)
-                *reinterpret_cast<float2 *>(v[k]) = __ldcg(reinterpret_cast<const float2 *>(row));
-              else
+        for (int u = 0; u < TURNS; u++) {
+          top[u] = -INFINITY, total[u] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(v[k] + i) = __ldcg(reinterpret_cast<const float4 *>(row + i));
-            }
-          };
-          ask(0);
-          for (uint32_t k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(part_of(k) + r));
+          for (int i = 0; i < V; i++) acc[u][i] = 0.0f;
+        }
+        for (uint32_t k0 = 0; k0 < n; k0 += at_once) {
+          const uint32_t some = min(at_once, n - k0);
+          asm volatile("fence.proxy.async;" ::: "memory");
+          __syncthreads();
+          if (tid == 0) mbar_expect_tx(&s_join, some * each * 4);
+          for (uint32_t k = tid; k < some; k += THREADS)
+            bulk_g2s(s_ring + (size_t)k * each * 4, part_of_tile(run, t, p.ws.parts, c0, k0 + k, part_floats(R, DP)), each * 4, &s_join);
+          timed_out |= !mbar_wait(&s_join, join_phase);
+          join_phase ^= 1;
 #pragma unroll
-          for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+          for (int u = 0; u < TURNS; u++) {
+            const uint32_t r = warp + u * NW;
+            if (r >= rows) continue;
+            float now = top[u];
+            for (uint32_t k = lane; k < some; k += 32) now = fmaxf(now, s_parts[k * each + r]);
 #pragma unroll
-          for (int i = 0; i < V; i++) acc[i] = 0.0f;
-          float f = 0.0f;  // of part (k0 rounded down to 32) + lane
-          for (uint32_t k0 = 0; k0 < n; k0 += AT_ONCE) {
-            if (k0 % 32 == 0) {
-              f = 0.0f;
-              if (k0 + lane < n) {
-                const float *from = part_of(k0 + lane);
-                const float mk = __ldcg(from + r);
-                f = mk == -INFINITY ? 0.0f : exp2_approx(mk - top);
-                total = fmaf(f, __ldcg(from + R + r), total);
-              }
-            }
-            if (k0) ask(k0);
+            for (int d = 16; d; d /= 2) now = fmaxf(now, __shfl_xor_sync(0xFFFFFFFFu, now, d));
+            const float old = top[u] == -INFINITY ? 0.0f : exp2_approx(top[u] - now);
+            top[u] = now;
+            total[u] *= old;
 #pragma unroll
-            for (uint32_t k = 0; k < AT_ONCE; k++) {
-              const float fk = __shfl_sync(0xFFFFFFFFu, f, (k0 + k) & 31);
+            for (int i = 0; i < V; i++) acc[u][i] *= old;
+#pragma unroll 4
+            for (uint32_t k = 0; k < some; k++) {
+              const float *part = s_parts + k * each;
+              const float m = part[r], f = m == -INFINITY ? 0.0f : exp2_approx(m - now);
+              total[u] = fmaf(f, part[R + r], total[u]);
 #pragma unroll
-              for (int i = 0; i < V; i++)
-                if (k0 + k < n) acc[i] = fmaf(fk, v[k][i], acc[i]);
+              for (int i = 0; i < V; i++) acc[u][i] = fmaf(f, part[2 * R + r * DP + lane * V + i], acc[u][i]);
             }
           }
+        }
 #pragma unroll
-          for (int d = 16; d; d /= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+        for (int u = 0; u < TURNS; u++) {
+          const uint32_t r = warp + u * NW;
+          if (r >= rows) continue;
           const uint32_t tok = r / t.heads, head = t.head0 + r - tok * t.heads;
-          if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
-          const float unit = total == 0.0f ? 0.0f : 1.0f / total;
+          float sum = total[u];
+          if (p.a.sinks) sum += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top[u] + P_SHIFT);
+          const float unit = sum == 0.0f ? 0.0f : 1.0f / sum;
           T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D + lane * V;
 #pragma unroll
           for (int i = 0; i < V; i += 2)
-            if (lane * V + i < D) reinterpret_cast<uint32_t *>(out)[i / 2] = Num<T>::pack(acc[i] * unit, acc[i + 1] * unit);
+            if (lane * V + i < D) reinterpret_cast<uint32_t *>(out)[i / 2] = Num<T>::pack(acc[u][i] * unit, acc[u][i + 1] * unit);
         }
       }
     }
@@ -384,19 +366,19 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   if (timed_out) atomicOr(p.ws.status, MER_DEVSTAT_TIMEOUT);
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP>
 cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
   using S = StreamShape<DP>;
-  constexpr size_t SMEM = 1024 + (size_t)MT * 16 * DP * 2 + (size_t)S::NW * S::ST * S::CHUNK;
-  static_assert((size_t)S::NW * MT * 16 * (DP + 10) * 4 <= (size_t)S::NW * S::ST * S::CHUNK, "the warps' results lie in the rings");
-  const cudaError_t e = allow_smem<k_attend_stream<T, DP, MT>>(SMEM);
+  constexpr size_t SMEM = 1024 + (size_t)16 * DP * 2 + (size_t)S::NW * S::ST * S::CHUNK;
+  static_assert((size_t)S::NW * 16 * (DP + 10) * 4 <= (size_t)S::NW * S::ST * S::CHUNK, "the warps' results lie in the rings");
+  const cudaError_t e = allow_smem<k_attend_stream<T, DP>>(SMEM);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(k_attend_stream<T, DP, MT>, dim3(sm_count), S::THREADS, SMEM, s, false, p, maps);
+  return launch_overlapped(k_attend_stream<T, DP>, dim3(sm_count), S::THREADS, SMEM, s, false, p, maps);
 }
 template <typename T>
 cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_count, cudaStream_t s) {
-  if (p.a.head_dim <= 64) return launch_stream<T, 64, 1>(p, maps, sm_count, s);
-  return p.a.head_dim <= 128 ? launch_stream<T, 128, 1>(p, maps, sm_count, s) : launch_stream<T, 256, 1>(p, maps, sm_count, s);
+  if (p.a.head_dim <= 64) return launch_stream<T, 64>(p, maps, sm_count, s);
+  return p.a.head_dim <= 128 ? launch_stream<T, 128>(p, maps, sm_count, s) : launch_stream<T, 256>(p, maps, sm_count, s);
 }
 
 }  // namespace

@@ -118,6 +118,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     ctl.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == TC_LOAD * 32 && p.box) prefetch_map(&maps.pages.k), prefetch_map(&maps.pages.v);
+  if (tid == TC_LOAD * 32 && p.q_mapped) prefetch_map(&maps.q);
   grid_dep_wait();
   grid_dep_launch();
   const RunStart run_here = find_run<TC_KB, TC_THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, p.min_units, ctl.found);
