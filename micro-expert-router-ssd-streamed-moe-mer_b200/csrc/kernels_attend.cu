@@ -1,4 +1,4 @@
-// Attention of single new tokens over a paged cache, and of any rows with heads of more than 128 values.  Head sizes up to 256 in steps of 8.
+// Attention of single new tokens over a paged cache.  Head sizes up to 256 in steps of 8.
 //
 //   o = sum_j 2^(s_j - m) v_j / (sum_j 2^(s_j - m) [+ 2^(sink - m)]),  s_j = q . k_j * scale * log2 e,  m = max_j s_j
 //
@@ -392,7 +392,7 @@ cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *
                           int sm_count, cudaStream_t s, int *launches) {
   // One row a sequence and no more heads of a key head than a tile has rows: the streaming kernel.  Any more rows: the tensor-core kernel, whose 128 rows a group cost
   // the same whatever they hold.
-  if (a.head_dim <= 128 && (kv.n_rows > kv.n_seqs || a.q_heads / a.kv_heads > 16)) {
+  if (kv.n_rows > kv.n_seqs || a.q_heads / a.kv_heads > 16) {
     *launches += 1;
     return launch_attend_tc(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
   }

@@ -1,4 +1,4 @@
-// Attention of many new rows over a paged cache: prompts, chunks of prompts, steps that mix them with single tokens.  Heads of up to 128 values.
+// Attention of many new rows over a paged cache: prompts, chunks of prompts, steps that mix them with single tokens.
 //
 // The same one pass as kernels_attend.cu, on tcgen05: a tile is two groups of 128 rows (tokens x heads of a key head), a block 128 tokens.
 //
@@ -11,9 +11,11 @@
 //     softmax runs the tensor core multiplies for the other: [P V of block j, Q K of block j + 1] of one, then of the other.
 //   * A tile of up to 128 rows (single tokens, drafts) has one group of rows; the two take its blocks in turn and their results are joined at its end, so that it is
 //     read as fast as two groups of rows would be multiplied.
+//   * Heads of more than 128 values: a tile has one group of rows, and the two places for scores take its blocks in turn, so that Q K of block j + 1 runs
+//     while the first group of warps makes the weights of block j.
 //   * The reference maximum of a row follows its maximum only when that has grown by more than 2^LAG; then alone the output in tensor memory is rescaled, by
 //     the softmax warps themselves.  Until then weights are larger than 1 by up to that factor, which f16 and fp32 hold.  What makes that safe without a
-//     barrier: the MMAs complete in order, so the S of block j being there says that the P V of block j - 1 has been added.
+//     barrier: the MMAs complete in order, so the S of block j being there says that the P V of block j - 1 has been added (with wide heads a barrier says so).
 //   * Keys and values come by tiled copies of runs of tokens of a page, 64 values wide; blocks that a sequence's end or a window cuts, and pages that
 //     have no such runs (of 1 or 5 tokens, say), row by row, 16 bytes a lane (cp.async), zeros where nothing is to be read.  Row by row alone a
 //     block took 4000 cycles.
@@ -22,6 +24,8 @@
 // Every wait is bounded; on expiry the CTA latches MER_DEVSTAT_TIMEOUT, stops issuing work, waits (bounded) for what is in flight,
 // frees its tensor memory and returns.
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "attend_join.cuh"
 #include "attention.cuh"
@@ -51,12 +55,13 @@ struct TcMaps {
   CUtensorMap q;  // [row][head][value]
 };
 
-constexpr uint32_t TC_R = 256, TC_KB = 128, TC_WARPS = 16, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
+constexpr uint32_t TC_KB = 128, TC_WARPS = 16, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
 constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12, TC_WALK = 13, TILE_USERS = 13;  // the warps that work on a tile
 // Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
 constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
-// What a tile costs beside its blocks, and a block of two groups of rows, in blocks of one: 8000, 3500 and 1900 cycles.
+// What a tile costs beside its blocks, and a block of two groups of rows, in blocks of one: 8000, 3500 and 1900 cycles (heads of 128; wide heads have tiles of
+// one group alone).
 constexpr uint32_t TC_START = 4, TC_DENSE = 2, TC_MIN_RUN = 4;
 static_assert(TC_MIN_RUN >= TC_DENSE, "every run inside a tile has a block of it");
 constexpr float LAG = 7.0f;        // with P_SHIFT the largest weight is 2^15 (scores of a standard deviation of 2: 157 us at 3, 146 so)
@@ -66,14 +71,16 @@ template <int DP>
 struct TcShape {
   static constexpr uint32_t SUBS = DP / 64;                // pieces of 64 values of a row
   static constexpr uint32_t STAGE = SUBS * TC_KB * 128;    // keys or values of a block
-  static constexpr uint32_t STAGES = DP == 128 ? 5 : 10;
-  static constexpr uint32_t QSUB = TC_R * 128;             // 64 values of all queries of a tile
+  static constexpr bool WIDE = DP == 256;                  // one group of rows, whose outputs take as much tensor memory as two groups' of 128 values
+  static constexpr uint32_t R = WIDE ? 128 : 256;          // rows of a tile
+  static constexpr uint32_t STAGES = DP == 256 ? 2 : DP == 128 ? 5 : 10;
+  static constexpr uint32_t QSUB = R * 128;              // 64 values of all queries of a tile
   static constexpr size_t SMEM = TC_CONTROL + SUBS * QSUB + STAGES * STAGE;
 };
 
 struct TcControl {
   uint64_t full[10], empty[10];  // stages of the ring
-  uint64_t q_full, q_empty, s_full[2], p_half[2], p_ready[2], o_full[2], soft, drain;
+  uint64_t q_full, q_empty, s_full[2], p_half[2], p_ready[2], o_full[2], added, soft, drain;
   uint64_t tile_full[2], tile_empty[2];
   TileWork tile[2];  // tokens == 0: there is none left
   RunStart run;
@@ -113,7 +120,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     for (uint32_t i = 0; i < S::STAGES; i++) mbar_init(&ctl.full[i], TC_LOADERS * 32), mbar_init(&ctl.empty[i], 1);
     mbar_init(&ctl.q_full, TC_LOADERS * 32), mbar_init(&ctl.q_empty, 1);
     for (int x = 0; x < 2; x++) mbar_init(&ctl.s_full[x], 1), mbar_init(&ctl.p_half[x], 4), mbar_init(&ctl.p_ready[x], 4), mbar_init(&ctl.o_full[x], 1);
-    mbar_init(&ctl.soft, SOFT_THREADS / 32), mbar_init(&ctl.drain, 1);
+    mbar_init(&ctl.added, 1), mbar_init(&ctl.soft, SOFT_THREADS / 32), mbar_init(&ctl.drain, 1);
     for (int i = 0; i < 2; i++) mbar_init(&ctl.tile_full[i], 1), mbar_init(&ctl.tile_empty[i], TILE_USERS);
     ctl.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
     // ---------------------------------------------------------------- softmax: a thread has row x * 128 + (tid & 127) of the tile
     const uint32_t x = warp >> 2;
-    const uint32_t tm_lane = tm + ((warp & 3) << 21), s_at = tm_lane + x * 128, own_o = tm_lane + 256 + x * DP;
+    const uint32_t tm_lane = tm + ((warp & 3) << 21), own_o = tm_lane + 256 + (S::WIDE ? 0 : x * DP);
     const float to_log2 = p.a.scale * LOG2E;
     uint32_t blocks = 0, tiles = 0, syncs = 0, flags = 0;  // phases of s_full, o_full, soft; uses of the flags
     auto sync = [&] {
@@ -171,9 +178,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       const TileWork &t = ctl.tile[turn & 1];
       const uint32_t rows = t.tokens * t.heads;
       const uint32_t lo = t.lo, hi = t.hi;
-      const bool one = rows <= 128, two_parts = one && hi - lo > 1;  // one group of rows, of which both warps' groups have blocks
+      const bool one = S::WIDE || rows <= 128, two_parts = one && !S::WIDE && hi - lo > 1;  // one group of rows, of which both warps' groups have blocks
       const uint32_t row0 = one ? 0 : x * 128, row = row0 + (tid & 127);
-      const bool active = one ? lo + x < hi : rows > row0;
+      const bool active = S::WIDE ? x == 0 : one ? lo + x < hi : rows > row0;
       const uint32_t tok = min(row, rows - 1) / t.heads, first = t.past + t.token0, see = first + tok;
       const uint32_t least = window && see + 1 > window ? see + 1 - window : 0;  // the row sees least .. see
       float m = -INFINITY, l = 0.0f;
@@ -182,8 +189,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         const uint32_t see0 = first + row0 / t.heads, see1 = first + min(row0 + 127, rows - 1) / t.heads;
         const uint32_t least1 = window && see1 + 1 > window ? see1 + 1 - window : 0;
         const uint32_t blk0 = one ? lo + x : lo;
-        for (uint32_t blk = blk0; blk < hi; blk += one ? 2 : 1, blocks++) {
-          if (!wait(&ctl.s_full[x], blocks & 1)) break;
+        for (uint32_t blk = blk0; blk < hi; blk += one && !S::WIDE ? 2 : 1, blocks++) {
+          // where the block's scores are, and the phase of that place
+          const uint32_t at = S::WIDE ? blocks & 1 : x, phase = S::WIDE ? blocks >> 1 & 1 : blocks & 1, s_at = tm_lane + at * 128;
+          if (!wait(&ctl.s_full[at], phase)) break;
           tm_fence_after();
           float s[4][32];
 #pragma unroll
@@ -213,7 +222,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             const float f = grow ? (m == -INFINITY ? 0.0f : exp2_approx(m - now)) : 1.0f;
             if (grow) m = now;
             l *= f;
+            if (S::WIDE && blk != blk0 && !wait(&ctl.added, (blocks - 1) & 1)) break;
             if (blk != blk0) {
+              if (S::WIDE) tm_fence_after();
               float o[32];
 #pragma unroll 1
               for (int c = 0; c < DP; c += 32) {
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
             tm_wait_store();
             tm_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(h ? &ctl.p_ready[x] : &ctl.p_half[x]);
+            if (lane == 0) mbar_arrive(h ? &ctl.p_ready[at] : &ctl.p_half[at]);
           }
           {
             float a, b;
@@ -270,7 +281,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         l = ctl.one_l[0][row] * f0 + ctl.one_l[1][row] * f1;
       }
       const int c_first = one && x == 1 ? DP / 2 : 0, c_end = one && x == 0 ? DP / 2 : DP;
-      const uint32_t o_at = tm_lane + 256 + (one ? 0 : x * DP);
+      const uint32_t o_at = one ? tm_lane + 256 : own_o;
       auto load_o = [&](int c, float(&o)[32]) {
         __syncwarp();
         tm_load(o_at + c, o);
@@ -295,16 +306,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       }
       // Parts lie as [piece of four values][row]: the rows of a warp side by side.
       if (!joins) {
-        float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(TC_R, DP);
+        float *part = p.ws.parts + (size_t)part_slot(run, t, blockIdx.x) * part_floats(S::R, DP);
         if (ends) {
-          if (row < rows && c_first == 0) part[row] = m, part[TC_R + row] = l;
+          if (row < rows && c_first == 0) part[row] = m, part[S::R + row] = l;
 #pragma unroll 1
           for (int c = c_first; c < c_end; c += 32) {
             float o[32];
             load_o(c, o);
             if (row < rows) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) reinterpret_cast<float4 *>(part + 2 * TC_R)[(c + i) / 4 * TC_R + row] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32; i += 4) reinterpret_cast<float4 *>(part + 2 * S::R)[(c + i) / 4 * S::R + row] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
           }
         }
@@ -320,13 +331,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         // the row's reference and sum over all parts
         const uint32_t k0 = own ? 1 : 0;
         float top = own ? m : -INFINITY, total;
-        for (uint32_t k = k0; k < n; k++) top = fmaxf(top, __ldcg(part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP)) + row));
+        for (uint32_t k = k0; k < n; k++) top = fmaxf(top, __ldcg(part_of_tile(run, t, p.ws.parts, c0, k, part_floats(S::R, DP)) + row));
         auto weight = [&](float m_of) { return m_of == -INFINITY ? 0.0f : exp2_approx(m_of - top); };
         const float own_f = own ? weight(m) : 0.0f;
         total = l * own_f;
         for (uint32_t k = k0; k < n; k++) {
-          const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP)) + row;
-          total = k == 0 ? weight(__ldcg(from)) * __ldcg(from + TC_R) : fmaf(weight(__ldcg(from)), __ldcg(from + TC_R), total);
+          const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(S::R, DP)) + row;
+          total = k == 0 ? weight(__ldcg(from)) * __ldcg(from + S::R) : fmaf(weight(__ldcg(from)), __ldcg(from + S::R), total);
         }
         if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
         const float f = total == 0.0f ? 0.0f : 1.0f / total;
@@ -338,10 +349,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
 #pragma unroll
           for (int i = 0; i < 32; i++) o[i] *= own_f;
           for (uint32_t k = k0; k < n; k++) {
-            const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(TC_R, DP));
+            const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(S::R, DP));
             float4 v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = __ldcg(reinterpret_cast<const float4 *>(from + 2 * TC_R) + (c / 4 + i) * TC_R + row);
+            for (int i = 0; i < 8; i++) v[i] = __ldcg(reinterpret_cast<const float4 *>(from + 2 * S::R) + (c / 4 + i) * S::R + row);
             const float w = weight(__ldcg(from + row));
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -378,7 +389,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr uint32_t BASE = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((128u >> 4) << 24);
     constexpr uint32_t QK = BASE | ((TC_KB >> 3) << 17), PV = BASE | (1u << 16) | ((DP >> 3) << 17);
-    uint32_t tiles = 0, blocks0 = 0, blocks1 = 0, at = 0;  // phases of q_full and p_ready; places of the ring before the tile's: keys of its block j are at + 2 j, values the next
+    uint32_t tiles = 0, blocks0 = 0, blocks1 = 0, at = 0, turns = 0;  // phases of q_full and p_ready; places of the ring before the tile's: keys of its block j are at + 2 j, values the next
     auto place = [&](uint64_t *bars, uint32_t q) { return &bars[q % S::STAGES]; };
     auto landed = [&](uint32_t q) { return wait(place(ctl.full, q), (q / S::STAGES) & 1); };
     // the low words of the descriptors; those of the pieces of an operand lie constants apart
@@ -391,14 +402,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         tm_mma_ss(leader, tm + x * 128, ALONG_K | (a + (k / 4) * (S::QSUB >> 4) + (k & 3) * 2), ALONG_K | (b + (k / 4) * (TC_KB * 128 >> 4) + (k & 3) * 2), QK, k != 0);
       tm_commit(leader, &ctl.s_full[x]);
     };
-    auto pv = [&](uint32_t x, uint32_t q, bool first) {  // its weights times the values at place q
+    auto pv = [&](uint32_t x, uint32_t q, bool first) {  // its weights (of place x) times the values at place q
       const uint32_t b = ring_at + q % S::STAGES * (S::STAGE >> 4);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         if (!wait(h ? &ctl.p_ready[x] : &ctl.p_half[x], (x ? blocks1 : blocks0) & 1)) return false;
         tm_fence_after();
 #pragma unroll
-        for (int k = 4 * h; k < 4 * h + 4; k++) tm_mma_ts(leader, tm + 256 + x * DP, tm + x * 128 + k * 8, ALONG_N | (b + k * 128), PV, k != 0 || !first);
+        for (int k = 4 * h; k < 4 * h + 4; k++) tm_mma_ts(leader, tm + 256 + (S::WIDE ? 0 : x * DP), tm + x * 128 + k * 8, ALONG_N | (b + k * 128), PV, k != 0 || !first);
       }
       blocks0 += x == 0, blocks1 += x == 1;
       return true;
@@ -416,7 +427,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (!wait(&ctl.q_full, tiles++ & 1)) break;
       if (!p.q_mapped) proxy_fence();
       bool ok = true;
-      if (rows <= 128) {  // the groups take the blocks in turn
+      if (S::WIDE) {  // the places for scores take the blocks in turn
+        for (uint32_t j = 0; j <= n && ok; j++) {
+          if (j < n) {
+            if (!(ok = landed(at + 2 * j))) break;
+            visible(j);
+            tm_fence_after();
+            qk((turns + j) & 1, 0, at + 2 * j);
+            free_place(at + 2 * j);
+            if (j + 1 == n) tm_commit(leader, &ctl.q_empty);
+          }
+          if (j == 0) continue;
+          const uint32_t v = at + 2 * j - 1;
+          if (!(ok = landed(v))) break;
+          visible(j - 1);
+          if (!(ok = pv((turns + j - 1) & 1, v, j == 1))) break;
+          free_place(v);
+          tm_commit(leader, &ctl.added);
+          if (j == n) tm_commit(leader, &ctl.o_full[0]);
+        }
+        turns += n;
+      } else if (rows <= 128) {  // the groups take the blocks in turn
         for (uint32_t j = 0; j < 2 && j < n && ok; j++) {
           if (!(ok = landed(at + 2 * j))) break;
           visible(j);
@@ -534,11 +565,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
       } else {
 #pragma unroll 1
-        for (uint32_t i = 0; i < 2; i++) {
-          const uint32_t r = w * 64 + i * 32 + lane, tok = r / t.heads;
+        for (uint32_t i = 0; i < S::R / (TC_LOADERS * 32); i++) {
+          const uint32_t r = w * (S::R / TC_LOADERS) + i * 32 + lane, tok = r / t.heads;
           // the tile's rows lie within 2^32 pieces of its first one
           const uint32_t place = r < rows ? tok * (uint32_t)(p.q_stride / 8) + (r - tok * t.heads) * (D / 8) : 0xFFFFFFFFu;
-          copy_rows(s_q + (w * 64 + i * 32) * 128, S::QSUB, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
+          copy_rows(s_q + (w * (S::R / TC_LOADERS) + i * 32) * 128, S::QSUB, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
         }
         submit(&ctl.q_full);
       }
@@ -606,19 +637,20 @@ cudaError_t launch_tc(const TcParams &p, const TcMaps &maps, int sm_count, cudaS
 }
 template <typename T>
 cudaError_t launch_tc(const TcParams &p, const TcMaps &maps, int sm_count, cudaStream_t s) {
-  return p.a.head_dim <= 64 ? launch_tc<T, 64>(p, maps, sm_count, s) : launch_tc<T, 128>(p, maps, sm_count, s);
+  if (p.a.head_dim <= 64) return launch_tc<T, 64>(p, maps, sm_count, s);
+  return p.a.head_dim <= 128 ? launch_tc<T, 128>(p, maps, sm_count, s) : launch_tc<T, 256>(p, maps, sm_count, s);
 }
 
 }  // namespace
 
-size_t attend_tc_part_floats(int sm_count) { return (size_t)2 * sm_count * part_floats(TC_R, 128); }
+size_t attend_tc_part_floats(int sm_count) { return (size_t)2 * sm_count * std::max(part_floats(TcShape<128>::R, 128), part_floats(TcShape<256>::R, 256)); }
 
 cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                              int sm_count, cudaStream_t s) {
   const PageMapShape m(a, kv, TC_KB);
   TcMaps maps{};
   const bool mapped = encode_page_maps(&maps.pages, m, a, kv);
-  TcParams p{a, kv, q, out, q_stride, out_stride, ws, TC_MIN_RUN, TileShape(a.q_heads, a.kv_heads, TC_R, TC_START, TC_DENSE, 128), mapped ? m.rows : 0, m.head_first, false, false};
+  TcParams p{a, kv, q, out, q_stride, out_stride, ws, TC_MIN_RUN, TileShape(a.q_heads, a.kv_heads, a.head_dim <= 128 ? TcShape<128>::R : TcShape<256>::R, TC_START, TC_DENSE, a.head_dim <= 128 ? 128 : 0xFFFFFFFFu), mapped ? m.rows : 0, m.head_first, false, false};
   p.q_mapped = p.ts.chunks == 1 && encode_row_map(&maps.q, q, a, kv.n_rows, q_stride, p.ts.heads, p.ts.tokens);
   p.out32 = a.head_dim % 16 == 0 && ((uintptr_t)out | out_stride * 2) % 32 == 0;
   return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);

@@ -138,7 +138,7 @@ def test_attention(backend, lens, q_heads, kv_heads, d, kind, page):
 
 @pytest.mark.parametrize("lens", ["decode", "draft", "prompts", "chunk", "long"])
 @pytest.mark.parametrize("window", [1, 2, 17, 128, 1000])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [64, 128, 256])
 def test_window_and_sinks(backend, lens, window, d):
     # tokens before every window are NaN, and so are the pages that hold only such tokens
     c = Cache(LENS[lens], 8, 2, d, "bf16", 16, heads_first=True, seed=window)
