@@ -422,10 +422,11 @@ int mer_moe_layer_forward_device(mer_backend *b, uint32_t layer, const float *d_
  *
  * Rows see nothing behind their own position, before their window, in pages that the table does not name or of other sequences, and
  * what no row of a tile sees is not read: it may hold anything.  A key or value that is not finite makes the rows that see it not finite
- * and may do so with other rows of its sequence in the same call.  A page number that is not below n_pages, a position beyond table_stride pages
+ * and may do so with other rows of its sequence in the same call.  A page number that is not below n_pages, a length beyond table_stride pages
  * or a sequence with more rows than tokens is latched as MER_DEVSTAT_BAD_CACHE and reported once, by mer_stream_check
- * (MER_ERR_VALIDATION_DISPATCH): a row without a place in its sequence is not appended and attends to nothing (zeros), a
- * token without a page is not appended and counts as zeros where it is seen.  No memory outside the given buffers is touched. ---- */
+ * (MER_ERR_VALIDATION_DISPATCH).  A token without a page is not appended and counts as zeros where it is seen; rows without a place in their
+ * sequence (the first ones of too many, all of one whose length is too large) are not appended and attend to nothing (zeros).  No memory outside
+ * the given buffers is touched. ---- */
 #define MER_VALUE_F32 0
 #define MER_VALUE_F16 1
 #define MER_VALUE_BF16 2
@@ -467,7 +468,7 @@ typedef struct mer_qkv_rows { /* device pointers; rows of heads side by side, e.
 } mer_qkv_rows;
 /* Norm and rotation in fp32 (angles in 64 bits), one rounding to the cache's type. */
 int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_qkv_rows *rows, void *stream);
-/* d_q and d_out: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8 below 2^26; 0 = no gaps).
+/* d_q and d_out, which do not overlap: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8 below 2^26; 0 = no gaps).
  * Scores, softmax and sums in fp32. */
 int mer_attention_forward_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const void *d_q, uint64_t q_stride,
                                  void *d_out, uint64_t out_stride, void *stream);

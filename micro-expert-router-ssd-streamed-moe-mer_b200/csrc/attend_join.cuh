@@ -21,7 +21,7 @@ struct RunWalk {
     at = run_first(r, blockIdx.x);
     left = r.total == 0 ? 0 : run_first(r, blockIdx.x + 1) - at;
   }
-  // The next tile of the run, or a part of one.  A block is the run's that its first unit lies in.
+  // The next tile of the run, or a part of one.
   __device__ bool next(TileWork *t) {
     do {
       if (left == 0) return false;
@@ -42,13 +42,8 @@ struct RunWalk {
         }
       }
       w.tile_blocks<KB>(tile, ts.tokens, window, &t->tile_lo, &t->tile_hi);
-      t->units = block_units(ts, w.n);
-      const uint32_t to = (uint32_t)min((uint64_t)(ts.start + (t->tile_hi - t->tile_lo) * t->units), from + left);
-      auto blocks_until = [&](uint32_t unit) { return unit <= ts.start ? 0u : t->units == 1 ? unit - ts.start : (unit - ts.start + t->units - 1) / t->units; };
-      t->at = at - from + ts.start;
-      t->lo = t->tile_lo + blocks_until(from), t->hi = t->tile_lo + blocks_until(to);
-      left -= to - from;
-      at += to - from;
+      const uint32_t taken = cut_tile(ts, w.n, at, from, left, t);
+      left -= taken, at += taken;
     } while (t->lo >= t->hi);  // no block of it
     t->seq = seq, t->row0 = w.row0, t->past = w.past;
     t->token0 = tile * ts.tokens;
@@ -82,9 +77,6 @@ __device__ void clear_rows_without_place(const AttnLayer &a, const KvBatchDev &k
 
 // Floats of a part: maximum and sum of R rows, and their outputs.
 __host__ __device__ constexpr uint32_t part_floats(uint32_t R, uint32_t DP) { return R * (DP + 2); }
-// Where a CTA leaves its part of a tile: a run has parts of two tiles at most, its first and its last.
-__device__ __forceinline__ uint32_t part_slot(const RunStart &r, const TileWork &t, uint32_t cta) { return 2 * cta + (run_first(r, cta) >= t.at ? 0 : 1); }
-
 // Four values from column c on of row r of a tile.
 template <typename T>
 __device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t, uint32_t r, uint32_t c, float top, float sum, const float4 &acc, T *out, uint64_t out_stride) {
@@ -96,14 +88,9 @@ __device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t,
   *reinterpret_cast<uint2 *>(out + (uint64_t)(t.row0 + t.token0 + tok) * out_stride + (uint64_t)head * a.head_dim + c) = v;
 }
 
-// The runs that have a part of a tile: c0, and n - 1 after it.
-__device__ __forceinline__ void runs_of_tile(const RunStart &run, const TileWork &t, uint32_t *c0, uint32_t *n) {
-  *c0 = run_of(run, t.at);
-  *n = run_of(run, t.at + (uint64_t)(t.tile_hi - t.tile_lo - 1) * t.units) - *c0 + 1;
-}
 // Part k of a tile in the workspace.
 __device__ __forceinline__ const float *part_of_tile(const RunStart &run, const TileWork &t, const float *parts, uint32_t c0, uint32_t k, uint32_t floats) {
-  return parts + (size_t)(k == 0 ? part_slot(run, t, c0) : 2 * (c0 + k)) * floats;
+  return parts + (size_t)slot_of_part(run, t, c0, k) * floats;
 }
 
 }  // namespace

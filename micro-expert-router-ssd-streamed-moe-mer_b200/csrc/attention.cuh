@@ -12,84 +12,20 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "attend_work.h"
 #include "attention.h"
 #include "../../include/mer_b200.h"
 #include "page_map.h"
 
 namespace {
 
-__device__ __forceinline__ uint32_t divided(uint32_t n, const FastDiv &f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
-// 64-bit division is 70 instructions; nearly always 32 bits will do.
-__device__ __forceinline__ uint64_t divided(uint64_t a, uint64_t b) { return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b; }
-
-// sum over 0 <= i < n of floor((a i + b) / m): the lattice points under a line, by Euclid's steps on (a, m).  a n + b below 2^32.
-__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  uint64_t sum = 0;
-  while (n) {
-    if (a >= m) sum += (uint64_t)(n - 1) * n / 2 * (a / m), a %= m;
-    if (b >= m) sum += (uint64_t)n * (b / m), b %= m;
-    const uint32_t y = a * n + b;
-    if (y < m) break;
-    n = y / m, b = y % m;
-    const uint32_t t = m;
-    m = a, a = t;
-  }
-  return sum;
-}
-
-// One sequence as a kernel with tiles of `tokens` tokens sees it.
-struct SeqWork {
-  uint32_t row0;    // the batch's row of its first token that has a place in the sequence
-  uint32_t n, past; // such tokens, and those of the cache before them
-  uint32_t tiles;   // per head
-
-  // Blocks of the first `j` tiles of a head.
-  template <uint32_t KB>
-  __device__ __forceinline__ uint64_t blocks_before(uint32_t j, uint32_t tokens, uint32_t window) const {
-    if (j == 0) return 0;
-    if (tiles == 1) {
-      uint32_t lo, hi;
-      tile_blocks<KB>(0, tokens, window, &lo, &hi);
-      return hi - lo;
-    }
-    const uint32_t full = j == tiles ? j - 1 : j;  // the last tile may be a short one
-    uint64_t hi = full == 0 ? 0 : floor_sum(full, KB, tokens, past + tokens + KB - 1);
-    if (full != j) hi += (past + n + KB - 1) / KB;
-    if (window == 0) return hi;
-    // a tile's first row sees nothing before past + j * tokens - window + 1
-    const uint32_t from = past + 1 >= window ? 0 : (window - 1 - past + tokens - 1) / tokens;
-    return from >= j ? hi : hi - floor_sum(j - from, KB, tokens, past + from * tokens + 1 - window);
-  }
-  template <uint32_t KB>
-  __device__ __forceinline__ void tile_blocks(uint32_t j, uint32_t tokens, uint32_t window, uint32_t *lo, uint32_t *hi) const {
-    const uint32_t first = j * tokens, last = min(n, first + tokens);
-    *hi = (past + last + KB - 1) / KB;
-    *lo = window && past + first + 1 > window ? (past + first + 1 - window) / KB : 0u;
-  }
-};
-
-// How heads and rows of a layer lie in tiles of R rows: heads of a group are taken `heads` at a time.
-struct TileShape {
-  uint32_t group, chunks, heads, tokens, v_heads, start, dense, sparse_rows;  // sparse_rows: a sequence with more has dense blocks
-  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R, uint32_t start_, uint32_t dense_, uint32_t sparse_rows_) : start(start_), dense(dense_), sparse_rows(sparse_rows_) {
-    group = q_heads / kv_heads;
-    chunks = (group + R - 1) / R;
-    heads = (group + chunks - 1) / chunks;
-    chunks = (group + heads - 1) / heads;
-    tokens = R / heads;
-    v_heads = kv_heads * chunks;
-  }
-};
-
-// Units of a block of a sequence.
-__device__ __forceinline__ uint32_t block_units(const TileShape &ts, uint32_t n) { return n * ts.heads > ts.sparse_rows ? ts.dense : 1; }
-
 // Rows of sequence s in the batch, cut to the batch: wrong tables read nothing outside it.
 __device__ __forceinline__ void seq_rows(const KvBatchDev &kv, uint32_t s, uint32_t *row, uint32_t *n, uint32_t *len) {
   const uint32_t a = __ldg(kv.row_start + s), e = min(__ldg(kv.row_start + s + 1), kv.n_rows);
   *row = a;
   *n = e > a ? e - a : 0;
-  *len = min(__ldg(kv.kv_len + s), 0x7FFFFFFFu);
+  const uint32_t l = __ldg(kv.kv_len + s);
+  *len = l <= kv.capacity ? l : 0;  // more than the table has pages for: no row of it has a place
 }
 // Rows that have no place (more rows than tokens) see nothing.
 __device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, uint32_t tokens) {
@@ -103,21 +39,12 @@ __device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, ui
   return w;
 }
 
-// The cut of a batch's blocks into runs, and where this CTA's starts.
-struct RunStart {
-  uint64_t total, each;  // units of the batch, units of a run: `more` runs have one more
-  uint32_t parts, more;  // CTAs that share the work
-  uint32_t seq;          // the sequence of the run's first unit
-  uint32_t v_head, tile, from;  // its head, its tile, and the tile's units before it
+// Where this CTA's run starts.
+struct RunStart : RunCut {
+  uint32_t seq;                // the sequence of the run's first unit
+  uint32_t v_head, tile, from; // its head, its tile, and the tile's units before it
   SeqWork w;
 };
-// First unit of a CTA's run.
-__device__ __forceinline__ uint64_t run_first(const RunStart &r, uint32_t cta) { return r.each * cta + min(cta, r.more); }
-// The CTA whose run holds unit x.
-__device__ __forceinline__ uint32_t run_of(const RunStart &r, uint64_t x) {
-  const uint64_t wide = (r.each + 1) * r.more;
-  return x < wide ? (uint32_t)divided(x, r.each + 1) : r.more + (uint32_t)divided(x - wide, r.each);
-}
 
 struct RunFound {
   uint64_t sums[16], more_sums[16];
@@ -164,10 +91,7 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
   }
   const uint64_t first = scan_threads<THREADS>(mine, found.sums, &total);
   RunStart r;
-  r.total = total;
-  r.parts = (uint32_t)max((uint64_t)1, min((uint64_t)ctas, min_units == 1 ? total : divided(total, min_units)));
-  r.each = divided(total, r.parts);
-  r.more = (uint32_t)(total - r.each * r.parts);
+  static_cast<RunCut &>(r) = cut_runs(total, ctas, min_units);
   const uint64_t x0 = run_first(r, min(cta, r.parts));
   if (x0 >= first && x0 < first + mine) {
     uint64_t at = first;
@@ -246,14 +170,11 @@ __device__ __forceinline__ void page_g2s(uint32_t dst, const CUtensorMap *map, u
 }
 
 // Which tile a CTA works on: its place in the batch and in the run.
-struct TileWork {
-  uint32_t row0, past;       // the sequence's first row and the tokens before it
-  uint32_t token0, tokens;   // of the sequence's rows
+struct TileWork : TileCut {
+  uint32_t row0, past;             // the sequence's first row and the tokens before it
+  uint32_t token0, tokens;         // of the sequence's rows
   uint32_t kv_head, head0, heads;  // query heads head0 .. head0 + heads
-  uint32_t seq, lo, hi;      // blocks of this run
-  uint32_t tile_lo, tile_hi; // blocks of the whole tile
-  uint64_t at;               // the unit of the tile's first block among all
-  uint32_t units;            // of a block
+  uint32_t seq;
 };
 
 // The first token that a row of the tile sees.

@@ -37,6 +37,7 @@ struct KvBatchDev {
   void *k_pages, *v_pages;
   uint64_t page_stride, token_stride, head_stride;  // in values; all places lie below KV_MAX_SPAN
   FastDiv page_tokens;
+  uint32_t capacity;  // tokens that a row of the table has pages for
   const uint32_t *page_table, *row_start, *kv_len;
   uint32_t n_pages, table_stride, n_seqs, n_rows;
 };

@@ -154,15 +154,22 @@ __global__ void __launch_bounds__(KV_WARPS * 32) k_kv_append(const KvParams p) {
   uint32_t pos = 0xFFFFFFFFu;
   uint64_t place = 0;
   {
+    uint32_t s0 = 0, s1 = p.kv.n_seqs;
+    while (s1 - s0 > 128) {  // many: the lanes look at 32 starts at a time
+      const uint32_t step = (s1 - s0 + 31) / 32, s = s0 + lane * step;
+      const uint32_t before = __popc(__ballot_sync(0xFFFFFFFFu, s < s1 && __ldg(p.kv.row_start + s) <= row));
+      if (before == 0) return;
+      s0 += (before - 1) * step, s1 = min(s1, s0 + step);
+    }
     uint32_t seq = 0, end = 0, len = 0;  // seq: its number + 1
-    for (uint32_t s = lane; s < p.kv.n_seqs; s += 32) {
+    for (uint32_t s = s0 + lane; s < s1; s += 32) {
       const uint32_t start = __ldg(p.kv.row_start + s), e = __ldg(p.kv.row_start + s + 1), n = __ldg(p.kv.kv_len + s);
-      if (start <= row) seq = s + 1, end = e, len = n;
+      if (start <= row) seq = s + 1, end = e, len = n <= p.kv.capacity ? n : 0;
     }
     const uint32_t last = __reduce_max_sync(0xFFFFFFFFu, seq);
     if (last == 0) return;
     const uint32_t from = __ffs(__ballot_sync(0xFFFFFFFFu, seq == last)) - 1;
-    end = min(__shfl_sync(0xFFFFFFFFu, end, from), p.kv.n_rows), len = min(__shfl_sync(0xFFFFFFFFu, len, from), 0x7FFFFFFFu);
+    end = min(__shfl_sync(0xFFFFFFFFu, end, from), p.kv.n_rows), len = __shfl_sync(0xFFFFFFFFu, len, from);
     if (row >= end) return;  // behind the last sequence
     const uint32_t behind = end - row;  // this row and those after it: 1 for the newest
     if (behind <= len) {

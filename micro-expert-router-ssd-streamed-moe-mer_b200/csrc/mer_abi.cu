@@ -2186,7 +2186,9 @@ MER_EXPORT int mer_stream_check(mer_backend *b, uint32_t layer, void *stream) {
     CU(MER_ERR_READBACK_MAP, "cudaMemcpyAsync(attention status)", cudaMemcpyAsync(b->h_attn_status, b->attn_ws.status, 4, cudaMemcpyDeviceToHost, s));
   CU(MER_ERR_READBACK_MAP, "cudaStreamSynchronize", cudaStreamSynchronize(s));
   if (b->h_attn_status && (attn = *b->h_attn_status) != 0) {  // kept until it is read here
-    CU(MER_ERR_READBACK_MAP, "cudaMemsetAsync(attention status)", cudaMemsetAsync(b->attn_ws.status, 0, 4, s));
+    // with the counts in front of it, which a call that gave up a wait may have left
+    const size_t counts = (attn & MER_DEVSTAT_TIMEOUT) ? attend_counts(b->sm_count) : 0;
+    CU(MER_ERR_READBACK_MAP, "cudaMemsetAsync(attention status)", cudaMemsetAsync(b->attn_ws.status - counts, 0, (counts + 1) * 4, s));
     CU(MER_ERR_READBACK_MAP, "cudaStreamSynchronize", cudaStreamSynchronize(s));
   }
   const int rc = check_device_status(b, b->h_u32[b->max_pairs] | attn, layer, expert);

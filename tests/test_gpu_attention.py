@@ -128,7 +128,8 @@ LENS = {
 
 @pytest.mark.parametrize("lens", LENS)
 @pytest.mark.parametrize("q_heads,kv_heads,d,kind,page", [(8, 1, 128, "bf16", 16), (32, 4, 128, "f16", 32), (6, 6, 64, "bf16", 1), (20, 4, 80, "f16", 24),
-                                                          (2, 1, 8, "bf16", 3), (40, 1, 64, "f16", 64), (4, 2, 256, "bf16", 16), (7, 1, 136, "f16", 5)])
+                                                          (2, 1, 8, "bf16", 3), (40, 1, 64, "f16", 64), (4, 2, 256, "bf16", 16), (7, 1, 136, "f16", 5),
+                                                          (2, 2, 8, "f16", 32), (3, 1, 24, "bf16", 16), (300, 1, 8, "f16", 16), (130, 1, 200, "bf16", 128), (1, 1, 256, "f16", 24)])
 def test_attention(backend, lens, q_heads, kv_heads, d, kind, page):
     c = Cache(LENS[lens], q_heads, kv_heads, d, kind, page, behind=3).fill().install(backend)
     c.forward(backend)
@@ -178,6 +179,41 @@ def test_query_and_output_strides(backend):
     assert (wide[:, 512:] == 3.0).all()
 
 
+@pytest.mark.parametrize("gap", [8, 64, 256])
+def test_query_rows_that_have_no_map(backend, gap):
+    # rows that are no whole number of heads apart are copied one by one
+    for d in (64, 256):
+        c = Cache(LENS["prompts"], 8, 2, d, "f16", 16, q_gap=gap, behind=2).fill().install(backend)
+        c.forward(backend)
+        c.check()
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (0, 2, 1), (2, 0, 1), (1, 0, 2), (2, 1, 0)])
+@pytest.mark.parametrize("lens", ["decode", "prompts"])
+def test_pages_tokens_and_heads_in_any_order(backend, order, lens):
+    # the pool's dimensions [page, token, head] outermost first, with a hole behind each token's head
+    c = Cache(LENS[lens], 8, 4, 64, "bf16", 16)
+    sizes = [(c.n_pages, 16, 4)[o] for o in order]
+    for name in ("k", "v"):
+        pool = torch.full((*sizes, 72), math.nan, dtype=c.kind, device="cuda")
+        setattr(c, name, pool.permute(*(order.index(i) for i in range(3)), 3)[..., :64])
+    c.fill().install(backend)
+    c.forward(backend)
+    c.check()
+    append_and_check(backend, c, "bf16", norm=True, rope_dims=64, pairs=False)
+
+
+def test_keys_and_values_of_one_pool(backend):
+    # [page][keys, values][token][head]
+    for lens in ("decode", "chunk"):
+        c = Cache(LENS[lens], 8, 4, 128, "f16", 32)
+        pool = torch.full((c.n_pages, 2, 32, 4, 128), math.nan, dtype=c.kind, device="cuda")
+        c.k, c.v = pool[:, 0], pool[:, 1]
+        c.fill().install(backend)
+        c.forward(backend)
+        c.check()
+
+
 def test_same_bits_every_time(backend):
     c = Cache([(1, 5000), (3, 900), (40, 2000), (1, 2)], 16, 2, 128, "bf16", 16).fill().install(backend)
     first = c.forward(backend).clone()
@@ -216,6 +252,31 @@ def test_page_that_is_not_there(backend, wrong):
         backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
     assert torch.equal(c.out[0], good[0]) and torch.equal(c.out[3], good[3])
     assert torch.isfinite(c.out.float()).all()
+
+
+def test_length_beyond_the_table(backend):
+    # lengths that were never written: nothing of such a sequence is run, the others are
+    for lens in ([(1, 100), (1, 30), (1, 60)], [(3, 100), (40, 50), (1, 60)]):
+        c = Cache(lens, 8, 2, 64).fill().install(backend)
+        good = c.forward(backend).clone()
+        for wrong in (0x7FFFFFFF, -1, c.table.shape[1] * 16 + 1):
+            c.kv_len[1] = wrong
+            c.out.fill_(7.0)
+            c.forward(backend)
+            with pytest.raises(mer_b200.GpuExpertDispatchError) as e:
+                backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
+            assert e.value.kind == DISPATCH
+            a, b = c.starts[1], c.starts[2]
+            assert torch.equal(c.out[:a], good[:a]) and torch.equal(c.out[b:], good[b:]) and (c.out[a:b] == 0).all()
+            before = c.k_pool.view(torch.int16).clone()
+            x = torch.randn((c.rows, 512), device="cuda", dtype=c.kind)
+            rows = mer_b200.QkvRows(k=x.data_ptr(), v=x.data_ptr(), k_stride=512, v_stride=512, value_type=c.value_type)
+            c.row_start.copy_(torch.tensor([0, 0, b - a, b - a], dtype=torch.int32))  # that sequence alone
+            backend.kv_append_device(0, c.batch(n_rows=b - a), rows, torch.cuda.current_stream().cuda_stream)
+            with pytest.raises(mer_b200.GpuExpertDispatchError):
+                backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
+            assert torch.equal(c.k_pool.view(torch.int16), before)
+            c.row_start.copy_(torch.tensor(c.starts, dtype=torch.int32))
 
 
 def test_values_that_are_not_finite_stay_in_their_sequence(backend):
@@ -324,6 +385,22 @@ def test_append_many_rows(backend):
     append_and_check(backend, c, "f32", norm=False, rope_dims=64, pairs=True)
 
 
+def test_append_thousands_of_sequences(backend):
+    rng = np.random.default_rng(6)
+    lens = [(int(n), int(n + k)) for n, k in zip(rng.integers(0, 3, 3000), rng.integers(0, 20, 3000))]
+    c = Cache(lens, 2, 1, 64, "f16", 8, behind=3)
+    x = torch.randn((c.rows, 256), device="cuda").to(c.kind)
+    c.install(backend)
+    rows = mer_b200.QkvRows(k=x.data_ptr() + 256, v=x.data_ptr() + 384, k_stride=256, v_stride=256, value_type=c.value_type)
+    backend.kv_append_device(0, c.batch(), rows, torch.cuda.current_stream().cuda_stream)
+    backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
+    seq = torch.tensor([i for i, (n, _) in enumerate(lens) for _ in range(n)], device="cuda")
+    pos = torch.tensor([k - n + j for n, k in lens for j in range(n)], device="cuda")
+    pages = c.table[seq, pos // 8].long()
+    assert torch.equal(c.k[pages, pos % 8, 0], x[:len(seq), 128:192]) and torch.equal(c.v[pages, pos % 8, 0], x[:len(seq), 192:])
+    assert int((~torch.isnan(c.k_pool)).sum()) == 64 * len(seq)
+
+
 def test_append_far_positions(backend):
     # positions of a million: an angle in 32 bits would be off by 0.06
     c = Cache([(2, 1 << 20), (1, 999999)], 2, 1, 64, "f16", 1 << 14)
@@ -409,6 +486,48 @@ def test_layers_step_by_step(backend):
     backend.stream_check(0, stream)
 
 
+def test_beside_the_expert_layers_of_one_backend():
+    """The calls of two decoder layers on one stream, nothing waited for between them: rows appended, attended to, and through the experts."""
+    synth = __import__("importlib").import_module("mer_b200.synth")
+    dtype, experts, d_model, d_ff, layers, n = mer_b200.DTYPE_Q8_0, 4, 256, 256, 2, 6
+    stride = (256 + mer_b200.expert_bytes(dtype, d_model, d_ff) + 4095) // 4096 * 4096
+    with mer_b200.Backend(dtype, d_model, d_ff, stride * experts * layers, experts * layers, max_tokens=64, max_top_k=2) as b:
+        for e in range(experts * layers):
+            b.admit(e, 1, synth.make_expert_blob(dtype, d_model, d_ff, 1, e // experts, e % experts))
+        for layer in range(layers):
+            mer_b200.LinearGate(synth.make_router(experts, d_model, layer), experts, d_model, 2).bind(b, layer)
+        stream = torch.cuda.current_stream().cuda_stream
+        for lens in ([(1, 40), (1, 700), (1, 3), (1, 90), (1, 16), (1, 17)], [(6, 300)]):
+            caches = [Cache(lens, 8, 2, 64, "bf16", 16, seed=l).fill() for l in range(layers)]
+            x = torch.randn((n, d_model), device="cuda")
+            qkv = torch.randn((n, 12 * 64), device="cuda")
+            rows = lambda c: mer_b200.QkvRows(q=qkv.data_ptr(), k=qkv.data_ptr() + 4 * 512, v=qkv.data_ptr() + 4 * 640, q_out=c.q.data_ptr(), q_stride=768,  # noqa: E731
+                                              k_stride=768, v_stride=768, value_type=mer_b200.VALUE_F32)
+            for layer, c in enumerate(caches):
+                c.install(b, layer, rope_freq=1e4 ** (-np.arange(32) / 32))
+            outs = [[], []]
+            for wait in (True, False):  # call by call, then all at once, several times
+                for _ in range(1 if wait else 8):
+                    y = [x.clone() for _ in range(layers + 1)]
+                    for layer, c in enumerate(caches):
+                        b.kv_append_device(layer, c.batch(), rows(c), stream)
+                        if wait:
+                            torch.cuda.synchronize()
+                        b.attention_forward_device(layer, c.batch(), c.q.data_ptr(), c.out.data_ptr(), stream)
+                        if wait:
+                            torch.cuda.synchronize()
+                        b.moe_layer_forward_device(layer, y[layer].data_ptr(), n, y[layer + 1].data_ptr(), stream)
+                        if wait:
+                            torch.cuda.synchronize()
+                    torch.cuda.synchronize()
+                    outs[not wait].append([y[-1].clone(), *(c.out.clone() for c in caches)])
+            for got in outs[1]:
+                assert all(torch.equal(a, w) for a, w in zip(got, outs[0][0]))
+            for c in caches:
+                c.check()
+        b.stream_check(0, stream)
+
+
 def test_captured_call_follows_its_tables(backend):
     """One graph for every step of a batch: lengths, tables and rows change between replays, sequences come and go."""
     hq, hk, d = 8, 2, 64
@@ -425,13 +544,37 @@ def test_captured_call_follows_its_tables(backend):
         s = torch.cuda.current_stream().cuda_stream
         backend.kv_append_device(0, batch, rows, s)
         backend.attention_forward_device(0, batch, c.q.data_ptr(), c.out.data_ptr(), s)
-    for step, lens in enumerate([[(1, 5), (1, 190), (1, 64), (1, 1)], [(1, 6), (0, 190), (2, 66), (1, 2)], [(0, 6), (0, 190), (0, 66), (4, 4)], [(0, 0)] * 4]):
+    check_steps = [[(1, 5), (1, 190), (1, 64), (1, 1)], [(1, 6), (0, 190), (2, 66), (1, 2)], [(0, 6), (0, 190), (0, 66), (4, 4)], [(0, 0)] * 4]
+    for step, lens in enumerate(check_steps):
         c.lens, c.starts = lens, np.concatenate([[0], np.cumsum([n for n, _ in lens])]).tolist()
         c.row_start.copy_(torch.tensor(c.starts, dtype=torch.int32))
         c.kv_len.copy_(torch.tensor([k for _, k in lens], dtype=torch.int32))
         x.copy_(torch.randn(x.shape, device="cuda").to(x.dtype))
         c.out.fill_(7.0)
         graph.replay()
+        torch.cuda.synchronize()
+        c.check()
+    backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
+
+
+def test_captured_chunks_follow_their_tables(backend):
+    # the same for the kernel of many rows: 96 rows at most, in any split, or none
+    c = Cache([(1, 400)] * 5, 8, 2, 128, "bf16", 16).fill()
+    c.install(backend, 0)
+    c.rows = 96
+    c.q_all = c.q = torch.randn((96, 1024), device="cuda").to(c.kind)
+    c.out = torch.empty_like(c.q)
+    batch, side, graph = c.batch(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        backend.attention_forward_device(0, batch, c.q.data_ptr(), c.out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    for lens in ([(1, 400), (90, 390), (0, 3), (4, 4), (1, 77)], [(0, 400)] * 5, [(96, 96), (0, 0), (0, 1), (0, 400), (0, 2)], [(1, 300)] * 5, [(0, 5)] * 4 + [(96, 400)]):
+        c.lens, c.starts = lens, np.concatenate([[0], np.cumsum([n for n, _ in lens])]).tolist()
+        c.row_start.copy_(torch.tensor(c.starts, dtype=torch.int32))
+        c.kv_len.copy_(torch.tensor([k for _, k in lens], dtype=torch.int32))
+        for _ in range(3):
+            c.out.fill_(7.0)
+            graph.replay()
         torch.cuda.synchronize()
         c.check()
     backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
