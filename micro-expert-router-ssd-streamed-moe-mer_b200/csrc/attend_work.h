@@ -63,8 +63,10 @@ struct SeqWork {
 
 // How heads and rows of a layer lie in tiles of R rows: heads of a group are taken `heads` at a time.
 struct TileShape {
-  uint32_t group, chunks, heads, tokens, v_heads, start, dense, sparse_rows;  // sparse_rows: a sequence with more has dense blocks
-  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R, uint32_t start_, uint32_t dense_, uint32_t sparse_rows_) : start(start_), dense(dense_), sparse_rows(sparse_rows_) {
+  uint32_t group, chunks, heads, tokens, v_heads;
+  uint32_t start, dense, sparse_rows, whole;  // sparse_rows: a sequence with more has dense blocks; whole: blocks of a tile that is not cut
+  TileShape(uint32_t q_heads, uint32_t kv_heads, uint32_t R, uint32_t start_, uint32_t dense_, uint32_t sparse_rows_, uint32_t whole_)
+      : start(start_), dense(dense_), sparse_rows(sparse_rows_), whole(whole_) {
     group = q_heads / kv_heads;
     chunks = (group + R - 1) / R;
     heads = (group + chunks - 1) / chunks;
@@ -107,13 +109,16 @@ struct TileCut {
   uint32_t tile_lo, tile_hi; // blocks of the whole tile
 };
 // The part of a tile from its unit `from` on, which is unit `at` of all, for a run with `left` units to go; the units it takes.  A block is the run's that its first
-// unit lies in.
+// unit lies in; a tile of few blocks is wholly the run's that its own first unit lies in: joining parts of it would take longer than its blocks.
 ATTEND_HD uint32_t cut_tile(const TileShape &ts, uint32_t n, uint64_t at, uint32_t from, uint64_t left, TileCut *t) {
   t->units = block_units(ts, n);
   const uint32_t all = ts.start + (t->tile_hi - t->tile_lo) * t->units, to = all < from + left ? all : (uint32_t)(from + left);
   const auto blocks_until = [&](uint32_t unit) { return unit <= ts.start ? 0u : t->units == 1 ? unit - ts.start : (unit - ts.start + t->units - 1) / t->units; };
   t->at = at - from + ts.start;
-  t->lo = t->tile_lo + blocks_until(from), t->hi = t->tile_lo + blocks_until(to);
+  if (t->tile_hi - t->tile_lo <= ts.whole)
+    t->lo = t->tile_lo, t->hi = from == 0 ? t->tile_hi : t->tile_lo;
+  else
+    t->lo = t->tile_lo + blocks_until(from), t->hi = t->tile_lo + blocks_until(to);
   return to - from;
 }
 // The runs that have a part of a tile: c0, and n - 1 after it.

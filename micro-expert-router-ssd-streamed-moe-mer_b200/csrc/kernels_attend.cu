@@ -19,6 +19,7 @@
 
 namespace {
 
+constexpr uint32_t WHOLE_BLOCKS = 4;  // of a tile that is not cut
 constexpr uint32_t START_UNITS = 3;  // what a tile costs beside its blocks, in blocks
 
 struct AttendParams {
@@ -399,7 +400,7 @@ cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *
   const PageMapShape m(a, kv, 16);
   PageMaps maps{};
   const bool mapped = encode_page_maps(&maps, m, a, kv);
-  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, 16, START_UNITS, 1, 0), mapped ? m.rows : 0, m.head_first};
+  const AttendParams p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, 16, START_UNITS, 1, 0, WHOLE_BLOCKS), mapped ? m.rows : 0, m.head_first};
   *launches += 1;
   return a.cache_type == MER_VALUE_F16 ? launch_stream<__half>(p, maps, sm_count, s) : launch_stream<__nv_bfloat16>(p, maps, sm_count, s);
 }

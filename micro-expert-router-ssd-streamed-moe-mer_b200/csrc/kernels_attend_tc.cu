@@ -62,7 +62,7 @@ constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
 // What a tile costs beside its blocks, and a block of two groups of rows, in blocks of one: 8000, 3500 and 1900 cycles (heads of 128; wide heads have tiles of
 // one group alone).
-constexpr uint32_t TC_START = 4, TC_DENSE = 2, TC_MIN_RUN = 4;
+constexpr uint32_t TC_START = 4, TC_DENSE = 2, TC_MIN_RUN = 4, TC_WHOLE = 10;
 static_assert(TC_MIN_RUN >= TC_DENSE, "every run inside a tile has a block of it");
 constexpr float LAG = 7.0f;        // with P_SHIFT the largest weight is 2^15 (scores of a standard deviation of 2: 157 us at 3, 146 so)
 constexpr uint32_t TC_CONTROL = 3072;  // barriers and words in front of the operands, which lie on whole atoms of 1024 bytes
@@ -650,7 +650,7 @@ cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const voi
   const PageMapShape m(a, kv, TC_KB);
   TcMaps maps{};
   const bool mapped = encode_page_maps(&maps.pages, m, a, kv);
-  TcParams p{a, kv, q, out, q_stride, out_stride, ws, TC_MIN_RUN, TileShape(a.q_heads, a.kv_heads, a.head_dim <= 128 ? TcShape<128>::R : TcShape<256>::R, TC_START, TC_DENSE, a.head_dim <= 128 ? 128 : 0xFFFFFFFFu), mapped ? m.rows : 0, m.head_first, false, false};
+  TcParams p{a, kv, q, out, q_stride, out_stride, ws, TC_MIN_RUN, TileShape(a.q_heads, a.kv_heads, a.head_dim <= 128 ? TcShape<128>::R : TcShape<256>::R, TC_START, TC_DENSE, a.head_dim <= 128 ? 128 : 0xFFFFFFFFu, TC_WHOLE), mapped ? m.rows : 0, m.head_first, false, false};
   p.q_mapped = p.ts.chunks == 1 && encode_row_map(&maps.q, q, a, kv.n_rows, q_stride, p.ts.heads, p.ts.tokens);
   p.out32 = a.head_dim % 16 == 0 && ((uintptr_t)out | out_stride * 2) % 32 == 0;
   return a.cache_type == MER_VALUE_F16 ? launch_tc<__half>(p, maps, sm_count, s) : launch_tc<__nv_bfloat16>(p, maps, sm_count, s);

@@ -19,7 +19,7 @@ SOURCE = r"""
 extern "C" {
 uint32_t div_by(uint32_t n, uint32_t d) { return divided(n, fast_div(d)); }
 void shape(uint32_t q_heads, uint32_t kv_heads, uint32_t rows, uint32_t *out) {
-  const TileShape t(q_heads, kv_heads, rows, 0, 1, 0);
+  const TileShape t(q_heads, kv_heads, rows, 0, 1, 0, 0);
   out[0] = t.group, out[1] = t.chunks, out[2] = t.heads, out[3] = t.tokens, out[4] = t.v_heads;
 }
 uint64_t before(uint32_t past, uint32_t n, uint32_t tokens, uint32_t j, uint32_t window) {
@@ -31,9 +31,9 @@ void blocks(uint32_t past, uint32_t n, uint32_t tokens, uint32_t j, uint32_t win
   w.tile_blocks<128>(j, tokens, window, lo, hi);
 }
 // tiles: [n][3] rows of the tile's sequence, its first block, the block behind its last.  cuts: [ctas][most][4] tile, first block, block behind the last, slot (~0: whole)
-uint32_t cut(const uint32_t *tiles, uint32_t n, uint32_t heads, uint32_t start, uint32_t dense, uint32_t sparse, uint32_t ctas, uint32_t min_units, uint32_t most, uint32_t *cuts,
+uint32_t cut(const uint32_t *tiles, uint32_t n, uint32_t heads, uint32_t start, uint32_t dense, uint32_t sparse, uint32_t whole, uint32_t ctas, uint32_t min_units, uint32_t most, uint32_t *cuts,
              uint32_t *owners) {
-  TileShape ts(heads, 1, 256, start, dense, sparse);
+  TileShape ts(heads, 1, 256, start, dense, sparse, whole);
   uint64_t total = 0;
   for (uint32_t i = 0; i < n; i++) total += start + (uint64_t)(tiles[3 * i + 2] - tiles[3 * i + 1]) * block_units(ts, tiles[3 * i]);
   const RunCut r = cut_runs(total, ctas, min_units);
@@ -54,8 +54,8 @@ uint32_t cut(const uint32_t *tiles, uint32_t n, uint32_t heads, uint32_t start, 
       if (k == most) return 0;
       uint32_t *o = cuts + ((size_t)c * most + k++) * 4;
       o[0] = i + 1, o[1] = t.lo, o[2] = t.hi, o[3] = t.lo == t.tile_lo && t.hi == t.tile_hi ? 0xFFFFFFFFu : part_slot(r, t, c);
-      uint32_t c0, parts;
-      runs_of_tile(r, t, &c0, &parts);
+      uint32_t c0 = c, parts = 1;
+      if (o[3] != 0xFFFFFFFFu) runs_of_tile(r, t, &c0, &parts);
       owners[2 * i] = c0, owners[2 * i + 1] = parts;
       if (o[3] != 0xFFFFFFFFu && slot_of_part(r, t, c0, c - c0) != o[3]) return 0;
     }
@@ -131,8 +131,8 @@ def test_blocks_of_tiles_are_summed_in_closed_form(rules):
     assert rules.before(2 ** 31 - 70000, 4096, 32, 128, 0) == sum(tile(2 ** 31 - 70000, 4096, j, 32, 0)[1] for j in range(128))
 
 
-@pytest.mark.parametrize("start,dense,sparse,min_units", [(3, 1, 0, 1), (4, 2, 128, 4), (0, 1, 0, 1), (1, 2, 64, 2)])
-def test_runs_have_every_block_once_and_the_parts_where_the_join_looks(rules, start, dense, sparse, min_units):
+@pytest.mark.parametrize("start,dense,sparse,whole,min_units", [(3, 1, 0, 4, 1), (4, 2, 128, 6, 4), (0, 1, 0, 0, 1), (1, 2, 64, 1, 2)])
+def test_runs_have_every_block_once_and_the_parts_where_the_join_looks(rules, start, dense, sparse, whole, min_units):
     rng = random.Random(start)
     for ctas in (1, 2, 7, 148):
         for _ in range(60):
@@ -142,7 +142,7 @@ def test_runs_have_every_block_once_and_the_parts_where_the_join_looks(rules, st
                 tiles.append((n, lo, lo + rng.randint(1, rng.choice([1, 4, 60, 400]))))
             flat, most = [v for t in tiles for v in t], len(tiles) + 2
             cuts, owners = (C.c_uint32 * (ctas * most * 4))(), (C.c_uint32 * (2 * len(tiles)))()
-            parts = rules.cut((C.c_uint32 * len(flat))(*flat), len(tiles), heads, start, dense, sparse, ctas, min_units, most, cuts, owners)
+            parts = rules.cut((C.c_uint32 * len(flat))(*flat), len(tiles), heads, start, dense, sparse, whole, ctas, min_units, most, cuts, owners)
             assert 1 <= parts <= ctas
             got, slots = {}, set()
             for c in range(parts):
@@ -155,6 +155,7 @@ def test_runs_have_every_block_once_and_the_parts_where_the_join_looks(rules, st
                             slots.add(slot)
             for i, (n, lo, hi) in enumerate(tiles):
                 assert got[i][0][1] == lo and got[i][-1][2] == hi and all(a[2] == b[1] for a, b in zip(got[i], got[i][1:]))
+                assert hi - lo > whole or len(got[i]) == 1
                 assert [c for c, _, _ in got[i]] == list(range(owners[2 * i], owners[2 * i] + owners[2 * i + 1]))
 
 
