@@ -4,12 +4,13 @@
 //   y = x / sqrt(mean(x^2) + eps) * w;   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * frequency_j
 //
 // A thread holds the two vectors that rotate into one another (halves: values j.. and j + rope_dims / 2..; neighbours: 2 V consecutive
-// values) and a group of lanes one head, so a head is read once and its mean of squares is a few shuffles.  A warp has a row, or some of its heads, and goes
-// through them a few at a time: cosines, sines and weights stay in its registers, and the heads to come are on their way.  Angles are made in
+// values) and a group of lanes one head, so a head is read once and its mean of squares is a few shuffles.  A CTA is a warp, which has a row, or some of its heads, and
+// goes through them a few at a time: cosines, sines and weights stay in its registers, and the heads to come are on their way.  Angles are made in
 // half turns reduced in 64 bits: positions of millions lose nothing, and the reduced angle goes to sincospif in 32.  Sums and rotations in fp32, two
 // values an instruction; one rounding at the end.
-// What bounds it: memory for thousands of rows, and before that the instructions: with a CTA for four rows, whose threads took any head and
-// read cosines and weights again for each, a step of 16 values a thread took a quarter more (13411 rows of 32 + 2 * 8 heads of 128: 69.5 us, 65.8 so).
+// What bounds it: memory for thousands of rows, with the instructions close behind (200 a step of 16 values a thread).  A warp to a CTA, because a CTA's place is free
+// only when its last warp has ended: 13411 rows of 32 + 2 * 8 heads of 128 in f16 60.3 us with CTAs of one warp, 64.1 of two, 67.8 of four, 78.1 of
+// eight (two steps ahead each; three: 57.0, 5.8 TB/s).  With a CTA for four rows, whose threads took any head and read cosines and weights again for each, 69.5.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -21,8 +22,7 @@
 
 namespace {
 
-constexpr uint32_t KV_WARPS = 4;  // of a CTA: each works for itself
-constexpr int AHEAD = 2;          // steps whose values a warp has asked for
+constexpr int AHEAD = 3;          // steps whose values a warp has asked for (2: 60.3 us, 4: 61.0, where registers cost warps)
 
 // V values as they lie in memory.
 template <typename T, int V>
@@ -77,19 +77,19 @@ __device__ __forceinline__ void times(float (&a)[V], const float (&b)[V]) {
 }
 // (a, b) -> (a c - b s, a s + b c)
 template <int V>
-__device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V], const float (&minus_s)[V]) {
+__device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
   if constexpr (V % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < V; i += 2) {
       const uint64_t a2 = pack2(a[i], a[i + 1]), b2 = pack2(b[i], b[i + 1]), c2 = pack2(c[i], c[i + 1]), s2 = pack2(s[i], s[i + 1]);
-      unpack2(fma2(b2, pack2(minus_s[i], minus_s[i + 1]), mul2(a2, c2)), a[i], a[i + 1]);
+      unpack2(fma2(pack2(-b[i], -b[i + 1]), s2, mul2(a2, c2)), a[i], a[i + 1]);
       unpack2(fma2(b2, c2, mul2(a2, s2)), b[i], b[i + 1]);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const float x = a[i], y = b[i];
-      a[i] = x * c[i] + y * minus_s[i], b[i] = x * s[i] + y * c[i];
+      a[i] = x * c[i] - y * s[i], b[i] = x * s[i] + y * c[i];
     }
   }
 }
@@ -107,13 +107,10 @@ struct KvParams {
 
 // IN: the rows' type, OUT: the cache's and q_out's, V: values of a vector.
 template <typename IN, typename OUT, int V>
-__global__ void __launch_bounds__(KV_WARPS * 32) k_kv_append(const KvParams p) {
-  extern __shared__ float2 s_turns[];  // [warp][rope_dims / 2] cosine and sine
+__global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
+  extern __shared__ float2 turns[];  // [rope_dims / 2] cosine and sine
   const AttnLayer &a = p.a;
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint64_t job = (uint64_t)blockIdx.x * KV_WARPS + warp;
-  const uint32_t row = (uint32_t)(job / p.chunks), chunk = (uint32_t)(job - (uint64_t)row * p.chunks);
-  if (row >= p.kv.n_rows) return;
+  const uint32_t lane = threadIdx.x, row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
   const uint32_t D = a.head_dim, half = a.rope_dims / 2, sub = lane & (p.group - 1), of = lane / p.group, heads = 32 / p.group;
   // Pair m of a head's vectors.  Behind the rotated values neighbours pair up, of which the last may have no second.
   constexpr int STEPS = V == 1 ? 4 : 1;  // V == 1: 32 lanes take up to 4 pairs each
@@ -185,7 +182,6 @@ __global__ void __launch_bounds__(KV_WARPS * 32) k_kv_append(const KvParams p) {
       return;
     }
   }
-  float2 *turns = s_turns + warp * half;
   for (uint32_t j = lane; j < half; j += 32) {
     const double x = (double)pos * __ldg(a.turns + j);
     float sin, cos;
@@ -195,7 +191,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32) k_kv_append(const KvParams p) {
   __syncwarp();
   // A thread's cosines and sines: of the pairs across its two vectors, or within each of them.
   constexpr int PAIRS = V == 1 ? 1 : V;
-  float c[STEPS][PAIRS], s[STEPS][PAIRS], minus_s[STEPS][PAIRS];
+  float c[STEPS][PAIRS], s[STEPS][PAIRS];
 #pragma unroll
   for (int k = 0; k < STEPS; k++) {
     const uint32_t m = sub + k * p.group;
@@ -203,7 +199,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32) k_kv_append(const KvParams p) {
     for (int i = 0; i < PAIRS; i++) {
       // halves: pair m V + i; neighbours: the V pairs of 2 V values; one value a vector: pair m
       const float2 t = m < rot ? turns[m * V + i] : make_float2(1.0f, 0.0f);
-      c[k][i] = t.x, s[k][i] = t.y, minus_s[k][i] = -t.y;
+      c[k][i] = t.x, s[k][i] = t.y;
     }
   }
   OUT *const q_dst = (OUT *)p.r.q_out + row * p.r.q_out_stride, *const k_dst = (OUT *)p.kv.k_pages + place, *const v_dst = (OUT *)p.kv.v_pages + place;
@@ -274,11 +270,11 @@ __global__ void __launch_bounds__(KV_WARPS * 32) k_kv_append(const KvParams p) {
           float e0[V], e1[V];
 #pragma unroll
           for (int v = 0; v < V; v++) e0[v] = x[k][2 * v / V][2 * v % V], e1[v] = x[k][(2 * v + 1) / V][(2 * v + 1) % V];
-          turn<V>(e0, e1, c[k], s[k], minus_s[k]);
+          turn<V>(e0, e1, c[k], s[k]);
 #pragma unroll
           for (int v = 0; v < V; v++) x[k][2 * v / V][2 * v % V] = e0[v], x[k][(2 * v + 1) / V][(2 * v + 1) % V] = e1[v];
         } else {
-          turn<V>(x[k][0], x[k][1], c[k], s[k], minus_s[k]);
+          turn<V>(x[k][0], x[k][1], c[k], s[k]);
         }
       }
     }
@@ -308,7 +304,7 @@ bool vec_ok(const void *p, uint64_t stride, uint32_t v, uint32_t size) {
 
 template <typename IN, typename OUT, int V>
 cudaError_t launch_kv(KvParams &p, dim3 grid, size_t smem, cudaStream_t s) {
-  return launch_overlapped(k_kv_append<IN, OUT, V>, grid, KV_WARPS * 32, smem, s, false, p);
+  return launch_overlapped(k_kv_append<IN, OUT, V>, grid, 32, smem, s, false, p);
 }
 template <typename IN, typename OUT>
 cudaError_t launch_kv(KvParams &p, uint32_t v, dim3 grid, size_t smem, cudaStream_t s) {
@@ -340,9 +336,8 @@ cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const Qkv
   p.chunks = (uint32_t)std::min<uint64_t>(steps, std::max<uint64_t>(1, (uint64_t)sm_count * 16 / kv.n_rows));
   p.each = (steps + p.chunks - 1) / p.chunks;
   p.chunks = (steps + p.each - 1) / p.each;
-  const uint64_t warps = (uint64_t)kv.n_rows * p.chunks;
-  const dim3 grid((uint32_t)((warps + KV_WARPS - 1) / KV_WARPS));
-  const size_t smem = (size_t)KV_WARPS * (a.rope_dims / 2) * sizeof(float2);
+  const dim3 grid(kv.n_rows * p.chunks);  // one row's warps only where rows are few: below 2^31
+  const size_t smem = (size_t)(a.rope_dims / 2) * sizeof(float2);
   return r.type == MER_VALUE_F32   ? launch_kv<float>(p, v, grid, smem, s)
          : r.type == MER_VALUE_F16 ? launch_kv<__half>(p, v, grid, smem, s)
                                    : launch_kv<__nv_bfloat16>(p, v, grid, smem, s);
