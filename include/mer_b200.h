@@ -421,8 +421,9 @@ int mer_moe_layer_forward_device(mer_backend *b, uint32_t layer, const float *d_
  * workspace of the backend: calls on different streams must not overlap.  Pointers are memory of the backend's device.
  *
  * Rows see nothing behind their own position, before their window, in pages that the table does not name or of other sequences, and
- * what no row of a tile sees is not read: it may hold anything.  A key or value that is not finite makes the rows that see it not finite
- * and may do so with other rows of its sequence in the same call.  A page number that is not below n_pages, a length beyond table_stride pages
+ * what no row of a tile sees is not read: it may hold anything.  A value or a score that is not finite makes the rows that see it not finite
+ * and may do so with other rows of its sequence in the same call; a score of -infinity is one without weight, and rows with no other ones
+ * attend to nothing.  A page number that is not below n_pages, a length beyond table_stride pages
  * or a sequence with more rows than tokens is latched as MER_DEVSTAT_BAD_CACHE and reported once, by mer_stream_check
  * (MER_ERR_VALIDATION_DISPATCH).  A token without a page is not appended and counts as zeros where it is seen; rows without a place in their
  * sequence (the first ones of too many, all of one whose length is too large) are not appended and attend to nothing (zeros).  No memory outside

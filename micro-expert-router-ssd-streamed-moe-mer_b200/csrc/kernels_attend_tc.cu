@@ -65,7 +65,7 @@ static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the oth
 constexpr uint32_t TC_START = 4, TC_DENSE = 2, TC_MIN_RUN = 4, TC_WHOLE = 10;
 static_assert(TC_MIN_RUN >= TC_DENSE, "every run inside a tile has a block of it");
 constexpr float LAG = 7.0f;        // with P_SHIFT the largest weight is 2^15 (scores of a standard deviation of 2: 157 us at 3, 146 so)
-constexpr uint32_t TC_CONTROL = 3072;  // barriers and words in front of the operands, which lie on whole atoms of 1024 bytes
+constexpr uint32_t TC_CONTROL = 3 * 1024;  // barriers and words in front of the operands, which lie on whole atoms of 1024 bytes
 
 template <int DP>
 struct TcShape {
@@ -392,7 +392,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     uint32_t tiles = 0, blocks0 = 0, blocks1 = 0, at = 0, turns = 0;  // phases of q_full and p_ready; places of the ring before the tile's: keys of its block j are at + 2 j, values the next
     auto place = [&](uint64_t *bars, uint32_t q) { return &bars[q % S::STAGES]; };
     auto landed = [&](uint32_t q) { return wait(place(ctl.full, q), (q / S::STAGES) & 1); };
-    // the low words of the descriptors; those of the pieces of an operand lie constants apart
+    // Descriptors of rows of 128 bytes in atoms of 8 rows (1024 bytes), 128-byte swizzle.  Bits: start >> 4 [0,14), leading offset >> 4 [16,30), stride offset >> 4
+    // [32,46), version 1 [46,48), swizzle 2 [61,64).  An operand whose rows run along K: 1024 between atoms, no leading offset; one whose rows run along N: 1024
+    // between groups of 8 of K, the leading offset between pieces of 64 values of a row.  The starts of an operand's pieces lie constants apart.
     constexpr uint64_t ALONG_K = (64ull << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16), ALONG_N = (64ull << 32) | (1ull << 46) | (2ull << 61) | ((uint64_t)(TC_KB * 128 >> 4) << 16);
     const uint32_t q_at = s_q >> 4, ring_at = s_ring >> 4;
     auto qk = [&](uint32_t x, uint32_t rows_of, uint32_t q) {  // the scores of a group for the keys at place q
@@ -622,6 +624,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (!ok) break;
     }
     copies_left<0>();
+    if (aborted())
+      for (uint32_t s = 0; s < S::STAGES; s++) mbar_drain(&ctl.full[s], 0, 10000000ull), mbar_drain(&ctl.full[s], 1, 10000000ull);
     if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
   }
   tm_fence_before();

@@ -86,11 +86,5 @@ __device__ __forceinline__ void tm_mma_ts(uint32_t leader, uint32_t d, uint32_t 
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-// Rows of 128 bytes in atoms of 8 rows (1024 bytes), 128-byte swizzle.  Bits: start >> 4 [0,14), leading offset >> 4 [16,30), stride offset >> 4
-// [32,46), version 1 [46,48), swizzle 2 [61,64).  An operand whose rows run along K: 1024 between atoms, no leading offset.  One whose
-// rows run along M or N: 1024 between groups of 8 of K, the leading offset between pieces of 64 values of a row.
-__device__ __forceinline__ uint64_t tm_desc(uint32_t addr, uint32_t leading) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
 
 }  // namespace

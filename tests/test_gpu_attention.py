@@ -294,6 +294,31 @@ def test_values_that_are_not_finite_stay_in_their_sequence(backend):
     assert torch.isnan(out[1:3, :4]).all() and torch.equal(out[0], good.view(-1, 8, 64)[0])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 40), (1, 3), (1, 2000)], [(40, 40), (300, 700), (2, 3), (3, 3)]])
+def test_scores_of_minus_infinity_have_no_weight(backend, lens, d):
+    c = Cache(lens, 8, 2, d, "bf16", 16).fill().install(backend)
+    c.q.view(-1, 8, d)[:, :, 0] = c.q.view(-1, 8, d)[:, :, 0].abs() + 0.5  # -infinity times it, plus what is finite
+    for i, (n, k) in enumerate(lens):
+        pages, slots = c.places(i, 0, 3)
+        c.k[pages, slots, 0, 0] = -math.inf  # the first three tokens, for the first key head
+    c.forward(backend)
+    backend.stream_check(0, torch.cuda.current_stream().cuda_stream)
+    u = torch.finfo(c.kind).eps / 2
+    for i, (n, k) in enumerate(lens):
+        keys, values = (x[c.places(i)].double().transpose(0, 1) for x in (c.k, c.v))
+        q = c.q[c.starts[i]:c.starts[i + 1]].double().view(n, 2, 4, d).permute(1, 2, 0, 3)
+        s = torch.einsum("hgnd,htd->hgnt", q, keys) * d ** -0.5
+        hidden = torch.arange(k, device="cuda") > torch.arange(k - n, k, device="cuda")[:, None]
+        s = s.masked_fill(hidden, -math.inf)
+        p = torch.nan_to_num(torch.softmax(s, 3), nan=0.0)
+        want, a = torch.einsum("hgnt,htd->hgnd", p, values), torch.einsum("hgnt,htd->hgnd", p, values.abs())
+        # |q| |k| scale is below d * 5 * 5 / sqrt(d) here
+        bound = u * (a + want.abs()) * 1.01 + (2 * 25 * d ** 0.5 * (d + 3) * 2.0 ** -24 + 2.0 ** -18) * a + 2.0 ** -24
+        got = c.out[c.starts[i]:c.starts[i + 1]].double().view(n, 2, 4, d).permute(1, 2, 0, 3)
+        assert ((got - want).abs() <= bound).all(), (i, n, k)
+
+
 # ------------------------------------------------------------------------------------------------ appending
 
 
@@ -657,7 +682,8 @@ def test_refused_rows(backend):
     x = torch.randn((2, 12 * 64), device="cuda", dtype=c.kind)
     good = dict(q=x.data_ptr(), k=x.data_ptr() + 1024, v=x.data_ptr() + 1280, q_out=c.out.data_ptr(), value_type=c.value_type)
     for change, kind in ((dict(k=None), INVALID), (dict(v=None), INVALID), (dict(q_out=None), INVALID), (dict(value_type=7), INVALID), (dict(q_stride=511), DISPATCH),
-                         (dict(k_stride=127), DISPATCH), (dict(v_stride=1), DISPATCH), (dict(q_out_stride=500), DISPATCH), (dict(k=x.data_ptr() + 1), DISPATCH)):
+                         (dict(k_stride=127), DISPATCH), (dict(v_stride=1), DISPATCH), (dict(q_out_stride=500), DISPATCH), (dict(k=x.data_ptr() + 1), DISPATCH),
+                         (dict(q_out=x.data_ptr(), q_stride=768), DISPATCH), (dict(q_out=x.data_ptr(), value_type=mer_b200.VALUE_F32), DISPATCH)):
         with pytest.raises(mer_b200.GpuExpertDispatchError) as e:
             backend.kv_append_device(0, c.batch(), mer_b200.QkvRows(**{**good, **change}))
         assert e.value.kind == kind, change
