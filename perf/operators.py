@@ -218,15 +218,29 @@ def prepare(case, seed):
     return s
 
 
+class _Program:
+    """What a program of this framework has for its whole life, whatever its inputs: one backend, and layers that are installed in it."""
+    backend, layers = None, 0
+
+    @classmethod
+    def new_layer(cls):
+        """The backend, and a layer of it that no state in use has: a layer's constants are a state's own, as its inputs are."""
+        import mer_b200
+        if cls.backend is None:
+            cls.backend = mer_b200.Backend(mer_b200.DTYPE_Q8_0, 64, 64, 1 << 20, 1, max_tokens=1, max_top_k=1)
+        cls.layers += 1
+        return cls.backend, cls.layers % 64
+
+
 def _bind(s):
     import mer_b200
     c, host = s.case, lambda t: None if t is None else t.cpu().numpy()
     types = {"f32": mer_b200.VALUE_F32, "f16": mer_b200.VALUE_F16, "bf16": mer_b200.VALUE_BF16}
-    s.backend = mer_b200.Backend(mer_b200.DTYPE_Q8_0, 64, 64, 1 << 20, 1, max_tokens=1, max_top_k=1)
+    s.backend, s.layer = _Program.new_layer()
     append = c["kind"] == "append"
     more = dict(q_norm=host(s.q_weight) if c["norm"] else None, k_norm=host(s.k_weight) if c["norm"] else None, norm_eps=EPS, rope_freq=host(s.freq),
                 rope_pairs=c["pairs"]) if append else dict(window=c["window"], sinks=host(s.sinks))
-    s.backend.install_attention(0, c["q_heads"], c["kv_heads"], c["head_dim"], types[c["cache"]], c["page"], **more)
+    s.backend.install_attention(s.layer, c["q_heads"], c["kv_heads"], c["head_dim"], types[c["cache"]], c["page"], **more)
     s.batch = mer_b200.KvBatch(k_pages=s.k_pages.data_ptr(), v_pages=s.v_pages.data_ptr(), n_pages=s.k_pages.shape[0], page_stride=s.k_pages.stride(0),
                                token_stride=s.k_pages.stride(1), head_stride=s.k_pages.stride(2), page_table=s.table.data_ptr(),
                                table_stride=s.table.shape[1], row_start=s.row_start.data_ptr(), kv_len=s.kv_len.data_ptr(), n_seqs=len(s.lens), n_rows=s.rows)
@@ -245,9 +259,9 @@ def run(state):
     if own:
         stream = torch.cuda.current_stream().cuda_stream
         if append:
-            s.backend.kv_append_device(0, s.batch, s.qkv_rows, stream)
+            s.backend.kv_append_device(s.layer, s.batch, s.qkv_rows, stream)
         else:
-            s.backend.attention_forward_device(0, s.batch, s.q.data_ptr(), s.out.data_ptr(), stream)
+            s.backend.attention_forward_device(s.layer, s.batch, s.q.data_ptr(), s.out.data_ptr(), stream)
     elif append:
         _append(s)
     else:
