@@ -30,6 +30,7 @@
 #include <algorithm>
 
 #include "attend_join.cuh"
+#include "attend_wait.cuh"
 #include "attention.cuh"
 #include "kernels.h"
 #include "pack2.cuh"
@@ -144,15 +145,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   tm_fence_after();
   const uint32_t tm = ctl.tmem;
   // columns: S (and P) of the two groups at 0 and 128, their O at 256 and 256 + DP
-  // For whole warps, which stay together whatever comes of it.
-  auto wait = [&](uint64_t *bar, uint32_t parity) {
-    const bool ok = mbar_wait(bar, parity, &ctl.abort);
-    if (!ok && !ctl.abort) {
-      ctl.abort = 1;
-      atomicOr(p.ws.status, MER_DEVSTAT_TIMEOUT);
-    }
-    return __all_sync(0xFFFFFFFFu, ok) != 0;
-  };
+  auto wait = [&](uint64_t *bar, uint32_t parity) { return wait_or_stop(bar, parity, &ctl.abort, p.ws.status); };
   auto aborted = [&] { return __any_sync(0xFFFFFFFFu, ctl.abort) != 0; };
   // The run's tiles, one after the other; done_with() when the warp no longer looks at one.
   uint32_t turn = 0;
@@ -626,13 +619,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (!ok) break;
     }
     copies_left<0>();
-    if (aborted())
-      for (uint32_t s = 0; s < S::STAGES; s++) mbar_drain(&ctl.full[s], 0, 10000000ull), mbar_drain(&ctl.full[s], 1, 10000000ull);
     if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
   }
   tm_fence_before();
   __syncthreads();
   if (warp == TC_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
+  // Tiled copies of keys, values and queries.  Only here is it certain that no warp gives up any more: the copying warps may have ended long before.
+  if (ctl.abort && tid <= S::STAGES) drain_copies(tid < S::STAGES ? &ctl.full[tid] : &ctl.q_full);
 }
 
 template <typename T, int DP>
