@@ -16,6 +16,7 @@
 
 #include "attention.cuh"
 #include "attend_join.cuh"
+#include "attend_wait.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
 
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   __shared__ uint64_t s_full[NW * ST];  // a chunk has landed: every lane of its warp arrives
   __shared__ RunFound s_found;
   __shared__ uint32_t s_flag;
+  __shared__ volatile uint32_t s_stop;  // a wait has run out
   __shared__ uint64_t s_join;
   uint8_t *s_ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // [NW][ST][k, v][DP / 64][16][64]
   uint8_t *s_q = s_ring + NW * ST * S::CHUNK;                                  // [DP / 64][R][64]
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   const uint32_t D = p.a.head_dim, page_tokens = p.a.page_tokens, window = p.a.window;
   const TileShape &ts = p.ts;
   for (uint32_t i = tid; i < NW * ST; i += THREADS) mbar_init(&s_full[i], 32);
-  if (tid == 0) mbar_init(&s_join, 1);
+  if (tid == 0) mbar_init(&s_join, 1), s_stop = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   if (tid == 0 && p.box) prefetch_map(&maps.k), prefetch_map(&maps.v);
   grid_dep_wait();
@@ -103,7 +105,8 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
   if (blockIdx.x >= run.parts) return;
   RunWalk<KB> walk(p.kv, ts, window, run);
   const float to_log2 = p.a.scale * LOG2E;
-  uint32_t fill = 0, stage = 0, stage_phase = 0, join_phase = 0, timed_out = 0;  // of the warp's ring: what is asked for next, what is taken next
+  uint32_t fill = 0, stage = 0, stage_phase = 0, join_phase = 0;  // of the warp's ring: what is asked for next, what is taken next
+  bool chunk_lost = false, join_lost = false;  // the warp has given up the wait for a chunk, or for parts
   const uint32_t ring = smem_u32(s_ring) + warp * (ST * S::CHUNK), q_addr = smem_u32(s_q);
 
   TileWork t;
@@ -189,7 +192,10 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
       }
       if (!wanted(blk)) continue;
       const uint32_t key0 = blk * KB + warp * 16, base = ring + stage * S::CHUNK;
-      timed_out |= !mbar_wait(&s_full[warp * ST + stage], stage_phase);
+      if (!wait_or_stop(&s_full[warp * ST + stage], stage_phase, &s_stop, p.ws.status)) {
+        chunk_lost = true;
+        break;
+      }
       stage = stage + 1 == ST ? 0 : stage + 1, stage_phase ^= stage == 0;
       float s[2][4];
       {
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
     // ---- the warps' results: [warp][row] maximum and sum, [warp][row][DP] output, where the rings were
     constexpr int OP = DP + 8;  // floats of a row of it: the rows of a fragment lie in different banks
     float *s_m = reinterpret_cast<float *>(s_ring), *s_l = s_m + NW * R, *s_o = s_l + NW * R;
-    __syncthreads();
+    if (__syncthreads_or(chunk_lost)) break;  // copies may still land in the rings
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       float sum = l[e];
@@ -318,11 +324,11 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         for (uint32_t k0 = 0; k0 < n; k0 += at_once) {
           const uint32_t some = min(at_once, n - k0);
           asm volatile("fence.proxy.async;" ::: "memory");
-          __syncthreads();
+          if (__syncthreads_or(join_lost)) break;
           if (tid == 0) mbar_expect_tx(&s_join, some * each * 4);
           for (uint32_t k = tid; k < some; k += THREADS)
             bulk_g2s(s_ring + (size_t)k * each * 4, part_of_tile(run, t, p.ws.parts, c0, k0 + k, part_floats(R, DP)), each * 4, &s_join);
-          timed_out |= !mbar_wait(&s_join, join_phase);
+          join_lost = !wait_or_stop(&s_join, join_phase, &s_stop, p.ws.status);
           join_phase ^= 1;
 #pragma unroll
           for (int u = 0; u < TURNS; u++) {
@@ -364,9 +370,14 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
     }
     // the rings are tiled copies' again
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
+    if (__syncthreads_or(join_lost)) break;
   }
-  if (timed_out) atomicOr(p.ws.status, MER_DEVSTAT_TIMEOUT);
+  // The way out after a wait that has run out: nothing more is asked for, and what is in flight lands before the CTA ends.
+  if (chunk_lost) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (lane < ST) drain_copies(&s_full[warp * ST + lane]);
+  }
+  if (join_lost) drain_copies(&s_join);
 }
 
 template <typename T, int DP>
