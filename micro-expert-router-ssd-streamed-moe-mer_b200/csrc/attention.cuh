@@ -19,12 +19,13 @@
 
 namespace {
 
-// Rows of sequence s in the batch, cut to the batch: wrong tables read nothing outside it.
+// Rows of sequence s in the batch, cut to the batch: wrong tables read nothing outside it.  Tables are read by ordinary loads: this kernel may have started
+// while the one in front of it still ran, which may have written them, and loads of what is constant for a kernel's whole life are not ordered behind that.
 __device__ __forceinline__ void seq_rows(const KvBatchDev &kv, uint32_t s, uint32_t *row, uint32_t *n, uint32_t *len) {
-  const uint32_t a = __ldg(kv.row_start + s), e = min(__ldg(kv.row_start + s + 1), kv.n_rows);
+  const uint32_t a = kv.row_start[s], e = min(kv.row_start[s + 1], kv.n_rows);
   *row = a;
   *n = e > a ? e - a : 0;
-  const uint32_t l = __ldg(kv.kv_len + s);
+  const uint32_t l = kv.kv_len[s];
   *len = l <= kv.capacity ? l : 0;  // more than the table has pages for: no row of it has a place
 }
 // Rows that have no place (more rows than tokens) see nothing.
@@ -149,7 +150,7 @@ struct PagePlaces {
   // The entry of the table for a token: to be asked for well before the place.
   __device__ __forceinline__ uint32_t entry(uint32_t key) const {
     const uint32_t slot = divided(key, div);
-    return slot < widest ? __ldg(pages + slot) : 0xFFFFFFFFu;
+    return slot < widest ? pages[slot] : 0xFFFFFFFFu;
   }
   __device__ __forceinline__ uint32_t in_page(uint32_t key) const { return key - divided(key, div) * page_tokens; }
   // The token's place in pieces of 16 bytes; ~0 and `bad` where the page is not there.

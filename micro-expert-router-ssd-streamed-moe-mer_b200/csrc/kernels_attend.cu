@@ -53,10 +53,10 @@ __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
 __device__ __forceinline__ void ldm4_trans(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
-// A load that stays where it stands among the copies.
+// A load that stays where it stands among the copies.  An ordinary one: the kernel in front, which writes the queries, may still run when this one starts.
 __device__ __forceinline__ uint4 load_now(const void *p) {
   uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 template <typename T>

@@ -156,13 +156,13 @@ __global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
     uint32_t s0 = 0, s1 = p.kv.n_seqs;
     while (s1 - s0 > 128) {  // many: the lanes look at 32 starts at a time
       const uint32_t step = (s1 - s0 + 31) / 32, s = s0 + lane * step;
-      const uint32_t before = __popc(__ballot_sync(0xFFFFFFFFu, s < s1 && __ldg(p.kv.row_start + s) <= row));
+      const uint32_t before = __popc(__ballot_sync(0xFFFFFFFFu, s < s1 && p.kv.row_start[s] <= row));
       if (before == 0) return;
       s0 += (before - 1) * step, s1 = min(s1, s0 + step);
     }
     uint32_t seq = 0, end = 0, len = 0;  // seq: its number + 1
     for (uint32_t s = s0 + lane; s < s1; s += 32) {
-      const uint32_t start = __ldg(p.kv.row_start + s), e = __ldg(p.kv.row_start + s + 1), n = __ldg(p.kv.kv_len + s);
+      const uint32_t start = p.kv.row_start[s], e = p.kv.row_start[s + 1], n = p.kv.kv_len[s];
       if (start <= row) seq = s + 1, end = e, len = n <= p.kv.capacity ? n : 0;
     }
     const uint32_t last = __reduce_max_sync(0xFFFFFFFFu, seq);
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
     const uint32_t behind = end - row;  // this row and those after it: 1 for the newest
     if (behind <= len) {
       const uint32_t slot = divided(len - behind, p.kv.page_tokens);
-      const uint32_t page = slot < p.kv.table_stride ? __ldg(p.kv.page_table + (uint64_t)(last - 1) * p.kv.table_stride + slot) : 0xFFFFFFFFu;
+      const uint32_t page = slot < p.kv.table_stride ? p.kv.page_table[(uint64_t)(last - 1) * p.kv.table_stride + slot] : 0xFFFFFFFFu;
       if (page < p.kv.n_pages) {
         pos = len - behind;
         place = page * p.kv.page_stride + (uint64_t)(pos - slot * a.page_tokens) * p.kv.token_stride;
