@@ -447,7 +447,7 @@ typedef struct mer_attention_cfg {
   uint32_t reserved;
   const float *q_norm, *k_norm;  /* host [head_dim] RMSNorm weights of each head, or NULL = no norm */
   const double *rope_freq;       /* host [rope_dims / 2] radians per position */
-  const float *sinks;            /* host [q_heads] a score without a value in each head's softmax, or NULL */
+  const float *sinks;            /* host [q_heads] a score without a value in each head's softmax (-infinity: the head has none), or NULL */
 } mer_attention_cfg;
 /* Copies the host arrays.  Installing a layer anew waits for the device; graphs captured with the old one must not be replayed. */
 int mer_attention_install(mer_backend *b, uint32_t layer, const mer_attention_cfg *cfg);

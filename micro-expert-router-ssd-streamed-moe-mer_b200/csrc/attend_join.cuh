@@ -82,7 +82,7 @@ template <typename T>
 __device__ __forceinline__ void store_row(const AttnLayer &a, const TileWork &t, uint32_t r, uint32_t c, float top, float sum, const float4 &acc, T *out, uint64_t out_stride) {
   if (c >= a.head_dim) return;
   const uint32_t tok = r / t.heads, head = t.head0 + r - tok * t.heads;
-  if (a.sinks) sum += exp2_approx(__ldg(a.sinks + head) * LOG2E - top + P_SHIFT);
+  if (a.sinks) sum += sink_weight(a.sinks, head, top);
   const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
   uint2 v = make_uint2(Num<T>::pack(acc.x * f, acc.y * f), Num<T>::pack(acc.z * f, acc.w * f));
   *reinterpret_cast<uint2 *>(out + (uint64_t)(t.row0 + t.token0 + tok) * out_stride + (uint64_t)head * a.head_dim + c) = v;

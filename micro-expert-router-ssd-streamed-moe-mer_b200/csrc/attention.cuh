@@ -220,5 +220,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // long row's many small ones sum to is not lost.  The shift is in the sums as well and cancels.
 constexpr float P_SHIFT = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
+// Weight of a head's sink beside scores whose reference is `top`; a sink of -infinity has none, also where all scores are -infinity.
+__device__ __forceinline__ float sink_weight(const float *sinks, uint32_t head, float top) {
+  const float sink = __ldg(sinks + head);
+  return sink == -INFINITY ? 0.0f : exp2_approx(sink * LOG2E - top + P_SHIFT);
+}
 
 }  // namespace

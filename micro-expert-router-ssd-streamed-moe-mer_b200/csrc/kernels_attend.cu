@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
           if (r >= rows) continue;
           const uint32_t tok = r / t.heads, head = t.head0 + r - tok * t.heads;
           float sum = total[u];
-          if (p.a.sinks) sum += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top[u] + P_SHIFT);
+          if (p.a.sinks) sum += sink_weight(p.a.sinks, head, top[u]);
           const float unit = sum == 0.0f ? 0.0f : 1.0f / sum;
           T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D + lane * V;
 #pragma unroll

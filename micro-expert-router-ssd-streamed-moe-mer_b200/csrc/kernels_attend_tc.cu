@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
           const float *from = part_of_tile(run, t, p.ws.parts, c0, k, part_floats(S::R, DP)) + row;
           total = k == 0 ? weight(__ldcg(from)) * __ldcg(from + S::R) : fmaf(weight(__ldcg(from)), __ldcg(from + S::R), total);
         }
-        if (p.a.sinks) total += exp2_approx(__ldg(p.a.sinks + head) * LOG2E - top + P_SHIFT);
+        if (p.a.sinks) total += sink_weight(p.a.sinks, head, top);
         const float f = total == 0.0f ? 0.0f : 1.0f / total;
         T *out = (T *)p.out + (uint64_t)(t.row0 + t.token0 + tok) * p.out_stride + (uint64_t)head * D;
 #pragma unroll 1

@@ -45,3 +45,43 @@ def test_append_in_place_and_attention_right_behind_it(backend, lens, d, offset,
             else:
                 assert torch.equal(out, want)
     backend.stream_check(0, current())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 40), (1, 3), (1, 9000)], [(40, 40), (300, 700), (2, 3), (5, 6000)]])
+def test_sinks_of_minus_infinity(backend, lens, d):  # noqa: F811
+    """A head whose sink is -infinity has none; beside scores that are all -infinity its rows attend to nothing."""
+    c = Cache(lens, 8, 2, d, "bf16", 16).fill()
+    sinks = np.array([-math.inf, 1.0, -math.inf, 0.0, -math.inf, -2.0, 3.0, -math.inf], np.float32)
+    c.install(backend, sinks=sinks)
+    c.forward(backend)
+    c.check()
+    c.q.view(-1, 8, d)[:, :, 0] = c.q.view(-1, 8, d)[:, :, 0].abs() + 0.5
+    for i, (n, k) in enumerate(lens):
+        c.k[(*c.places(i), 0, 0)] = -math.inf  # every token of the first key head: heads 0 .. 3
+    c.forward(backend)
+    out = c.out.view(-1, 8, d)
+    assert (out[:, :4] == 0).all()
+    # the other key head's queries have new first values: against its own formula
+    u = torch.finfo(c.kind).eps / 2
+    for i, (n, k) in enumerate(lens):
+        keys, values = (x[c.places(i)][:, 1].double() for x in (c.k, c.v))
+        q = c.q[c.starts[i]:c.starts[i + 1]].double().view(n, 8, d)[:, 4:].transpose(0, 1)
+        s = q @ keys.T * d ** -0.5
+        size = (q.abs() @ keys.abs().T * d ** -0.5).amax(2, keepdim=True)
+        hidden = torch.arange(k, device="cuda") > torch.arange(k - n, k, device="cuda")[:, None]
+        s = s.masked_fill(hidden, -math.inf)
+        total = torch.logaddexp(torch.logsumexp(s, 2, keepdim=True), torch.tensor(sinks[4:], dtype=torch.float64, device="cuda")[:, None, None])
+        p = (s - total).exp()
+        want, a = p @ values, p @ values.abs()
+        bound = u * (a + want.abs()) * 1.01 + (2 * size * (d + 3) * 2.0 ** -24 + 2.0 ** -18) * a + 2.0 ** -24
+        got = out[c.starts[i]:c.starts[i + 1], 4:].double().transpose(0, 1)
+        assert ((got - want).abs() <= bound).all()
+
+
+def test_a_sink_that_is_not_a_number_is_refused(backend):  # noqa: F811
+    sinks = np.zeros(8, np.float32)
+    sinks[5] = math.nan
+    with pytest.raises(mer_b200.GpuExpertDispatchError) as e:
+        backend.install_attention(9, 8, 2, 64, mer_b200.VALUE_F16, 16, sinks=sinks)
+    assert e.value.kind == INVALID
