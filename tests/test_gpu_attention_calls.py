@@ -85,3 +85,26 @@ def test_a_sink_that_is_not_a_number_is_refused(backend):  # noqa: F811
     with pytest.raises(mer_b200.GpuExpertDispatchError) as e:
         backend.install_attention(9, 8, 2, 64, mer_b200.VALUE_F16, 16, sinks=sinks)
     assert e.value.kind == INVALID
+
+
+def test_first_calls_on_a_stream_of_their_own(backend):  # noqa: F811
+    """A layer is ready when its installation returns, on streams too that do not wait for the one its constants were copied on."""
+    d, stream = 256, torch.cuda.Stream()
+    c = Cache([(1, 40), (1, 900)], 8, 2, d, "bf16", 16).fill()
+    x = torch.randn((2, 12 * d), device="cuda")
+    weights, freq, sinks = np.linspace(0.5, 1.5, d).astype(np.float32), 1e4 ** (-np.arange(d // 2) * 2 / d), np.linspace(-2, 2, 8).astype(np.float32)
+    outs = [torch.zeros((2, 8 * d), device="cuda", dtype=c.kind) for _ in range(31)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        # every installation is the first one of its layer, in memory that held other constants
+        with mer_b200.Backend(mer_b200.DTYPE_Q8_0, 64, 64, 1 << 20, 1, max_tokens=1, max_top_k=1) as b:
+            b.install_attention(1, 8, 2, d, c.value_type, 16, q_norm=-7 * weights, k_norm=weights + 3, rope_freq=freq[::-1], sinks=sinks + 5)
+            b.install_attention(2, 8, 2, d, c.value_type, 16, q_norm=weights, k_norm=weights, rope_freq=freq, sinks=sinks)
+            rows = mer_b200.QkvRows(q=x.data_ptr(), k=x.data_ptr() + 4 * 8 * d, v=x.data_ptr() + 4 * 10 * d, q_out=c.q.data_ptr(), q_stride=12 * d, k_stride=12 * d,
+                                    v_stride=12 * d, value_type=mer_b200.VALUE_F32)
+            b.kv_append_device(2, c.batch(), rows, stream.cuda_stream)
+            b.attention_forward_device(2, c.batch(), c.q.data_ptr(), out.data_ptr(), stream.cuda_stream)
+            torch.cuda.synchronize()
+            assert torch.equal(out, outs[0]), i
+    c.opts = dict(sinks=sinks)
+    c.check(torch.cat([outs[0], c.out[2:]]))
