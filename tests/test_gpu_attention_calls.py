@@ -108,3 +108,67 @@ def test_first_calls_on_a_stream_of_their_own(backend):  # noqa: F811
             assert torch.equal(out, outs[0]), i
     c.opts = dict(sinks=sinks)
     c.check(torch.cat([outs[0], c.out[2:]]))
+
+
+SINGLE, SEVERAL = [(1, 100), (1, 900), (1, 60)], [(1, 100), (6, 900), (70, 75)]  # one row a sequence: the streaming kernel; more: the other one
+
+
+@pytest.mark.parametrize("lens", [SINGLE, SEVERAL])
+@pytest.mark.parametrize("page", [16, 5])  # with tiled copies, and row by row
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (128, 300), (256, 0)])
+def test_tokens_without_a_page_count_as_zeros(backend, lens, page, d, window):  # noqa: F811
+    c = Cache(lens, 8, 2, d, "bf16", page).fill().install(backend, window=window)
+    stands = Cache(lens, 8, 2, d, "bf16", page)  # the same with zeros in those places
+    stands.k, stands.v, stands.q, stands.table, stands.opts = c.k.clone(), c.v.clone(), c.q, c.table.clone(), c.opts
+    held = -(-lens[1][1] // page)
+    for slot, number in ((2, c.n_pages), (held // 2, -1), (held - 3, 0x7FFFFFFF), (held - 2, c.n_pages + 1)):
+        first, last = slot * page, min(slot * page + page, lens[1][1])
+        for x in (stands.k, stands.v):
+            x[stands.places(1, first, last)] = 0.0
+        c.table[1, slot] = number
+    c.forward(backend)
+    with pytest.raises(mer_b200.GpuExpertDispatchError) as e:
+        backend.stream_check(0, current())
+    assert e.value.kind == DISPATCH
+    stands.check(c.out)
+
+
+@pytest.mark.parametrize("lens", [SINGLE, SEVERAL])
+@pytest.mark.parametrize("page,d", [(16, 64), (5, 64), (16, 128), (16, 256)])
+def test_values_that_are_not_finite_stay_in_their_sequence_and_head(backend, lens, page, d):  # noqa: F811
+    c = Cache(lens, 8, 2, d, "bf16", page).fill().install(backend)
+    good = c.forward(backend).clone().view(-1, 8, d)
+    pages, slots = c.places(1)
+    a, b = c.starts[1], c.starts[2]
+    c.v[pages[850], slots[850], 1, 5] = math.inf
+    c.forward(backend)
+    out = c.out.clone().view(-1, 8, d)
+    assert not torch.isfinite(out[a:b, 4:, 5]).any()  # the first value of its group's heads that every row sees
+    out[a:b, 4:, 5] = good[a:b, 4:, 5]
+    assert torch.equal(out, good)
+    c.k[pages[20], slots[20], 0, 3] = math.nan
+    c.forward(backend)
+    out = c.out.view(-1, 8, d)
+    assert torch.isnan(out[a:b, :4]).all()
+    assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])
+
+
+@pytest.mark.parametrize("lens", [[(1, 200), (1, 170), (1, 2000), (1, 129)], [(5, 200), (40, 170), (1, 2000), (3, 131)]])
+@pytest.mark.parametrize("page", [16, 5])
+def test_sequences_that_share_the_pages_of_their_beginning(backend, lens, page):  # noqa: F811
+    c = Cache(lens, 8, 2, 128, "f16", page)
+    shared = 100 // page
+    c.table[1:, :shared] = c.table[0, :shared]
+    c.fill().install(backend)
+    before = c.k.clone()
+    x = torch.randn((c.rows, 12 * 128), device="cuda", dtype=c.kind)
+    at = x.data_ptr()
+    rows = mer_b200.QkvRows(q=at, k=at + 2048, v=at + 2560, q_out=c.q.data_ptr(), q_stride=1536, k_stride=1536, v_stride=1536, value_type=c.value_type)
+    backend.kv_append_device(0, c.batch(), rows, current())  # no norms, no rotation: as they are
+    c.forward(backend)
+    backend.stream_check(0, current())
+    assert torch.equal(c.k[c.table[0, :shared].long()], before[c.table[0, :shared].long()])
+    for i, (n, k) in enumerate(lens):
+        assert torch.equal(c.k[c.places(i, k - n)].flatten(1), x[c.starts[i]:c.starts[i + 1], 1024:1280])
+    assert torch.equal(c.q, x[:, :1024])
+    c.check()
