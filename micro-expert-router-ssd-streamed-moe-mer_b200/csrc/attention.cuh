@@ -163,6 +163,11 @@ struct PagePlaces {
   }
 };
 
+// 16 bytes, of which those behind the first `bytes` are zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 // 64 values of a run of tokens of a page, swizzled; zeros where the page number is not one of the map's.
 __device__ __forceinline__ void page_g2s(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t token, uint32_t head, uint32_t page, bool head_first, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x),

@@ -44,9 +44,6 @@ struct StreamShape {
   static constexpr uint32_t KB = NW * 16, THREADS = NW * 32, CHUNK = 2 * 16 * DP * 2;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
@@ -149,8 +146,8 @@ __global__ void __launch_bounds__(StreamShape<DP>::THREADS, 1) k_attend_stream(c
         const uint32_t at = __shfl_sync(0xFFFFFFFFu, place, r);
         const bool in = at != 0xFFFFFFFFu && c * 8 < D;
         const uint64_t off = in ? ((uint64_t)at + c) * 16 : 0;
-        cp_async16(dst + piece<16>(r, c), (const char *)p.kv.k_pages + off, in ? 16 : 0);
-        cp_async16(dst + 16 * DP * 2 + piece<16>(r, c), (const char *)p.kv.v_pages + off, in ? 16 : 0);
+        copy16(dst + piece<16>(r, c), (const char *)p.kv.k_pages + off, in ? 16 : 0);
+        copy16(dst + 16 * DP * 2 + piece<16>(r, c), (const char *)p.kv.v_pages + off, in ? 16 : 0);
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     };

@@ -94,9 +94,6 @@ struct TcControl {
 };
 static_assert(sizeof(TcControl) <= TC_CONTROL && TC_CONTROL % 1024 == 0, "control block");
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 template <int N>
 __device__ __forceinline__ void copies_left() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
