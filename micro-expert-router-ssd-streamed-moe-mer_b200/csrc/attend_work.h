@@ -15,17 +15,18 @@ ATTEND_HD uint32_t divided(uint32_t n, const FastDiv &f) { return ((uint32_t)((u
 // 64-bit division is 70 instructions; nearly always 32 bits will do.
 ATTEND_HD uint64_t divided(uint64_t a, uint64_t b) { return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b; }
 
-// sum over 0 <= i < n of floor((a i + b) / m): the lattice points under a line, by Euclid's steps on (a, m).  a n + b below 2^32.
-ATTEND_HD uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+// Sum over 0 <= i < n of floor((a i + b) / m), a n + b below 2^32: points of the grid under a line, n columns of them.  Whole steps of slope and start
+// apart, the last column is `top` high and holds the most; of the n * top points up to there, row j + 1 has those of its columns above the line that start before the
+// line reaches it, ceil((m (j + 1) - b) / a): a sum of the same kind with a and m in each other's places, to be taken away.  As many turns as Euclid's algorithm has.
+ATTEND_HD uint64_t points_under(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   uint64_t sum = 0;
-  while (n) {
-    if (a >= m) sum += (uint64_t)(n - 1) * n / 2 * (a / m), a %= m;
-    if (b >= m) sum += (uint64_t)n * (b / m), b %= m;
-    const uint32_t y = a * n + b;
-    if (y < m) break;
-    n = y / m, b = y % m;
-    const uint32_t t = m;
-    m = a, a = t;
+  for (bool away = false; n; away = !away) {
+    uint64_t part = (uint64_t)n * (n - 1) / 2 * (a / m) + (uint64_t)n * (b / m);
+    a %= m, b %= m;
+    const uint32_t top = (a * (n - 1) + b) / m, slope = a;
+    part += (uint64_t)n * top;
+    sum = away ? sum - part : sum + part;
+    n = top, b = m - b + slope - 1, a = m, m = slope;
   }
   return sum;
 }
@@ -46,12 +47,12 @@ struct SeqWork {
       return hi - lo;
     }
     const uint32_t full = j == tiles ? j - 1 : j;  // the last tile may be a short one
-    uint64_t hi = full == 0 ? 0 : floor_sum(full, KB, tokens, past + tokens + KB - 1);
+    uint64_t hi = full == 0 ? 0 : points_under(full, KB, tokens, past + tokens + KB - 1);
     if (full != j) hi += (past + n + KB - 1) / KB;
     if (window == 0) return hi;
     // a tile's first row sees nothing before past + j * tokens - window + 1
     const uint32_t from = past + 1 >= window ? 0 : (window - 1 - past + tokens - 1) / tokens;
-    return from >= j ? hi : hi - floor_sum(j - from, KB, tokens, past + from * tokens + 1 - window);
+    return from >= j ? hi : hi - points_under(j - from, KB, tokens, past + from * tokens + 1 - window);
   }
   template <uint32_t KB>
   ATTEND_HD void tile_blocks(uint32_t j, uint32_t tokens, uint32_t window, uint32_t *lo, uint32_t *hi) const {

@@ -4,7 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-// Division of numbers below 2^31 by a constant of a launch.
+// Division of numbers below 2^31 by a constant of a launch: multiplier and shift of Granlund and Montgomery, "Division by invariant integers using
+// multiplication" (1994), section 4; below 2^31 its last sum has room in 32 bits.
 struct FastDiv {
   uint32_t mul, shift;
 };
