@@ -427,7 +427,8 @@ int mer_moe_layer_forward_device(mer_backend *b, uint32_t layer, const float *d_
  * or a sequence with more rows than tokens is latched as MER_DEVSTAT_BAD_CACHE and reported once, by mer_stream_check
  * (MER_ERR_VALIDATION_DISPATCH).  A token without a page is not appended and counts as zeros where it is seen; rows without a place in their
  * sequence (the first ones of too many, all of one whose length is too large) are not appended and attend to nothing (zeros).  No memory outside
- * the given buffers is touched. ---- */
+ * the given buffers is touched.  A wait inside the attention kernels that runs out (a copy that never lands) is latched as MER_DEVSTAT_TIMEOUT, and the outputs of
+ * that call and of those behind it are not to be used until mer_stream_check has reported it. ---- */
 #define MER_VALUE_F32 0
 #define MER_VALUE_F16 1
 #define MER_VALUE_BF16 2
@@ -470,7 +471,10 @@ typedef struct mer_qkv_rows { /* device pointers; rows of heads side by side, e.
 /* Norm and rotation in fp32 (angles in 64 bits), one rounding to the cache's type. */
 int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_qkv_rows *rows, void *stream);
 /* d_q and d_out, which do not overlap: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8 below 2^26; 0 = no gaps).
- * Scores, softmax and sums in fp32. */
+ * Scores, exponentials and sums in fp32; the weights are rounded to the cache's type before they multiply the values, as the matrix units take both (2^-9 of a
+ * weight at most in bf16, 2^-12 in f16), and the output once at the end.  The host sees no lengths, so n_rows <= n_seqs alone
+ * picks the kernel that is made for one row a sequence; any batch is right with it, but a long chunk among idle sequences is faster without these, or with n_rows above
+ * n_seqs (200 rows behind 30000, 32 and 4 heads of 128: 124 us alone, 784 with 255 idle sequences). */
 int mer_attention_forward_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const void *d_q, uint64_t q_stride,
                                  void *d_out, uint64_t out_stride, void *stream);
 

@@ -7,9 +7,10 @@
 // tokens of a page; row by row, 16 bytes a lane, where a sequence's end or a window cuts a chunk or pages have no such runs) into a ring that no other warp sees, multiplies the one that has landed (mma.sync on 16 x 16 tiles; at this rate of
 // operations the legacy tensor path is idle most of the time) and keeps maximum, sum and output of its own tokens in registers: no barrier
 // in the loop.  The warps' results are joined in shared memory at the end of a tile, those of several CTAs through the workspace (attention.cuh).
-// 64 tokens behind 800 to 8000 (32 and 4 heads of 128, bf16) 81 us, 5.8 TB/s; one behind 32000 22 us, of which 10 are reading and the rest the
-// dependent reads at the run's beginning and the join at its end.  Tiles of up to 4 blocks are not cut: 16 windows of 128 tokens 7.0 us, 8.9 cut.
+// 64 tokens behind 800 to 8000 (32 and 4 heads of 128, bf16) 81 to 87 us by the box, 5.4 to 5.8 TB/s; one behind 32000 22 us, of which 10 are reading and the rest the
+// dependent reads at the run's beginning and the join at its end.  Pages of one token, copied row by row: 84 us for the 64 tokens, 81 with pages of 16 on the same box.  Tiles of up to 4 blocks are not cut: 16 windows of 128 tokens 7.0 us, 8.9 cut.
 // The weights go to the second product in the cache's type, 2^-9 (bf16) or 2^-12 (f16) of each at most, like the values they multiply; sums are fp32.
+// Every wait is bounded; one that runs out is latched as MER_DEVSTAT_TIMEOUT and stops the CTA (attend_wait.cuh).
 #include <cuda_runtime.h>
 
 #include <algorithm>

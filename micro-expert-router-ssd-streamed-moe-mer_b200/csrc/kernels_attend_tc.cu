@@ -18,13 +18,15 @@
 //     barrier: the MMAs complete in order, so the S of block j being there says that the P V of block j - 1 has been added (with wide heads a barrier says so).
 //   * Keys and values come by tiled copies of runs of tokens of a page, 64 values wide; blocks that a sequence's end or a window cuts, and pages that
 //     have no such runs (of 1 or 5 tokens, say), row by row, 16 bytes a lane (cp.async), zeros where nothing is to be read.  Row by row alone a
-//     block took 4000 cycles.
+//     block took 4000 cycles in a loop of its own; a prompt of 2048 with pages of one token takes 57 us, 55 with pages of 16.
 //   * Rows of P that see nothing of a block hold zeros, and what no row sees is filled with zeros instead of being read.
+//   * P is in the cache's type, which the matrix unit wants of both operands: 2^-9 (bf16) or 2^-12 (f16) of each weight at most.  The sums that the output is divided
+//     by are of the weights before that, in fp32: their roundings are as often up as down.
 // What bounds it: exponentials and MMAs, 2048 cycles each for a block of both groups at 16 and 8192 a cycle; a block takes 3500, the softmax of a group being a
-// chain of 2000 between its two MMAs.  32 and 4 heads of 128 in bf16: 2048 rows behind 30700 tokens 975 us (1.08 PFLOP/s, under the power limit), a
+// chain of 2000 between its two MMAs.  32 and 4 heads of 128 in bf16: 2048 rows behind 30700 tokens 970 to 990 us (1.08 PFLOP/s, under the power limit), a
 // prompt of 2048 56 us.  Tiles of up to 10 blocks are not cut: prompts of 512, 1024 and 2048 18.6, 26.6 and 55.9 us; cut 24.2, 36.4 and 53.4.
-// Every wait is bounded; on expiry the CTA latches MER_DEVSTAT_TIMEOUT, stops issuing work, waits (bounded) for what is in flight,
-// frees its tensor memory and returns.
+// Every wait is bounded; on expiry the CTA latches MER_DEVSTAT_TIMEOUT, stops issuing work, frees its tensor memory, waits (bounded) for all copies that are in
+// flight and returns (attend_wait.cuh).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -9,7 +9,8 @@
 // their way.  Angles are made in half turns reduced in 64 bits: positions of millions lose nothing, and the reduced angle goes to sincospif in
 // 32.  Sums and rotations in fp32, two values an instruction; one rounding at the end.
 // What bounds it: memory for thousands of rows, with the instructions close behind (200 a step of 16 values a thread, 300 for a row's place and
-// cosines), which bound rows of few heads: 20781 of 2 + 2 heads of 128 28 us, where the bytes take 6.5.  A warp to a CTA, because a CTA's place is
+// cosines), which bound rows of few heads: 20781 of 2 + 2 heads of 128 28 us, where the bytes take 6.5; queries, keys and values take whole steps each, so that 2, 1 and 1 heads
+// are three steps which use half, a quarter and a quarter of the lanes.  A warp to a CTA, because a CTA's place is
 // free only when its last warp has ended: 13411 rows of 32 + 2 * 8 heads of 128 in f16 60.3 us with CTAs of one warp, 64.1 of two, 67.8 of four,
 // 78.1 of eight (two steps ahead each; three: 57.0, 5.8 TB/s).  With a CTA for four rows, whose threads took any head and read cosines and weights
 // again for each, 69.5; with two rows to a warp, whose state takes 122 registers instead of 106, 68.8.

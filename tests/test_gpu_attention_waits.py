@@ -56,6 +56,8 @@ def kernel(tmp_path_factory):
     src, lib = d / "waits.cu", d / "libwaits.so"
     src.write_text(SOURCE)
     nvcc = os.environ.get("NVCC") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no CUDA compiler here")
     subprocess.check_call([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-I", CSRC, str(src),
                            "-o", str(lib)])
     k = C.CDLL(str(lib))
