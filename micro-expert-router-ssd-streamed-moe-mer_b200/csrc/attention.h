@@ -16,7 +16,7 @@ inline FastDiv fast_div(uint32_t d) {
   return f;
 }
 
-// One installed layer (mer_attention_install); the pointers are device memory.
+// One installed layer (mer_attention_install); the pointers are device memory, parts of `constants`.
 struct AttnLayer {
   uint32_t q_heads, kv_heads, head_dim, page_tokens;
   uint32_t window;                // tokens that a row sees, itself among them; 0 = all before it
@@ -28,6 +28,7 @@ struct AttnLayer {
   const float *q_norm, *k_norm;   // [head_dim] or null
   const double *turns;            // [rope_dims / 2] half turns per position: frequency / pi
   const float *sinks;             // [q_heads] or null
+  void *constants;
 };
 
 // A token's place in the pages as a 32-bit number of 16-byte pieces.
