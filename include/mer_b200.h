@@ -450,7 +450,7 @@ typedef struct mer_attention_cfg {
   const double *rope_freq;       /* host [rope_dims / 2] radians per position */
   const float *sinks;            /* host [q_heads] a score without a value in each head's softmax (-infinity: the head has none), or NULL */
 } mer_attention_cfg;
-/* Copies the host arrays.  Installing a layer anew waits for the device; graphs captured with the old one must not be replayed. */
+/* Copies the host arrays and waits for the device; graphs captured with a layer that is installed anew must not be replayed. */
 int mer_attention_install(mer_backend *b, uint32_t layer, const mer_attention_cfg *cfg);
 
 typedef struct mer_kv_batch { /* device pointers; strides in values, multiples of 8; pages on 16 bytes, keys and values within 64 GB each */
