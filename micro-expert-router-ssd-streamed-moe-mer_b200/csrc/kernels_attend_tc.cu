@@ -25,8 +25,8 @@
 // What bounds it: exponentials and MMAs, 2048 cycles each for a block of both groups at 16 and 8192 a cycle; a block takes 3500, the softmax of a group being a
 // chain of 2000 between its two MMAs.  32 and 4 heads of 128 in bf16: 2048 rows behind 30700 tokens 970 to 990 us (1.08 PFLOP/s, under the power limit), a
 // prompt of 2048 56 us.  Tiles of up to 10 blocks are not cut: prompts of 512, 1024 and 2048 18.6, 26.6 and 55.9 us; cut 24.2, 36.4 and 53.4.
-// Every wait is bounded; on expiry the CTA latches MER_DEVSTAT_TIMEOUT, stops issuing work, frees its tensor memory, waits (bounded) for all copies that are in
-// flight and returns (attend_wait.cuh).
+// Every wait is bounded; on expiry the CTA latches MER_DEVSTAT_TIMEOUT, stops issuing work, waits (bounded) for all MMAs and copies that are in
+// flight, frees its tensor memory and returns (attend_wait.cuh).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -500,10 +500,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (!ok) break;
       at += 2 * n;
     }
-    if (aborted()) {
-      tm_commit(leader, &ctl.drain);
-      mbar_drain(&ctl.drain, 0, 1000000000ull);
-    }
     } else if (warp == TC_WALK) {
       // -------------------------------------------------------------- the way through the run
       RunWalk<TC_KB> walk(p.kv, ts, window, ctl.run);
@@ -622,9 +618,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   }
   tm_fence_before();
   __syncthreads();
-  if (warp == TC_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
-  // Tiled copies of keys, values and queries.  Only here is it certain that no warp gives up any more: the copying warps may have ended long before.
-  if (ctl.abort && tid <= S::STAGES) drain_copies(tid < S::STAGES ? &ctl.full[tid] : &ctl.q_full);
+  // After a wait that has run out: MMAs, and tiled copies of keys, values and queries.  Only here is it certain that no warp gives up any more: those that
+  // issued them may have ended long before.
+  const bool gave_up = ctl.abort != 0;
+  if (warp == TC_MMA) {
+    if (gave_up) {
+      tm_commit(tm_elect(), &ctl.drain);  // the lane that issued: the same one is elected every time
+      mbar_drain(&ctl.drain, 0, 1000000000ull);
+    }
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
+  }
+  if (gave_up && tid <= S::STAGES) drain_copies(tid < S::STAGES ? &ctl.full[tid] : &ctl.q_full);
 }
 
 template <typename T, int DP>
