@@ -434,18 +434,19 @@ int mer_moe_layer_forward_device(mer_backend *b, uint32_t layer, const float *d_
 #define MER_VALUE_BF16 2
 #define MER_ATTENTION_MAX_HEAD_DIM 256
 #define MER_ATTENTION_ROPE_PAIRS 0x1u /* neighbours (2j, 2j + 1) rotate into one another, not halves (j, j + rope_dims / 2) */
+#define MER_ATTENTION_CACHE_Q4 0x2u   /* keys and values are held in 4 bits: see below */
 typedef struct mer_attention_cfg {
   uint32_t q_heads, kv_heads;  /* kv_heads divides q_heads: query head h reads key head h / (q_heads / kv_heads) */
   uint32_t head_dim;           /* a multiple of 8 up to MER_ATTENTION_MAX_HEAD_DIM */
   uint32_t page_tokens;        /* any number */
-  int32_t cache_type;          /* MER_VALUE_F16 or MER_VALUE_BF16: keys, values, queries and outputs */
+  int32_t cache_type;          /* MER_VALUE_F16 or MER_VALUE_BF16: keys, values, queries and outputs (queries and outputs alone where the cache holds 4 bits) */
   uint32_t window;             /* a row sees itself and window - 1 tokens before; 0 = all */
   uint32_t rope_dims;          /* leading values of a head that are rotated; 0 = none */
   uint32_t flags;              /* MER_ATTENTION_* */
   float scale;                 /* of the scores; 0 = 1 / sqrt(head_dim) */
   float norm_eps;
   float rope_scale;            /* times cosine and sine (YaRN's attention factor); 0 = 1 */
-  uint32_t reserved;
+  uint32_t cache_group;          /* with MER_ATTENTION_CACHE_Q4: neighbouring values of a head that share a scale, 32 or 64; 0 = 32 */
   const float *q_norm, *k_norm;  /* host [head_dim] RMSNorm weights of each head, or NULL = no norm */
   const double *rope_freq;       /* host [rope_dims / 2] radians per position */
   const float *sinks;            /* host [q_heads] a score without a value in each head's softmax (-infinity: the head has none), or NULL */
@@ -453,7 +454,7 @@ typedef struct mer_attention_cfg {
 /* Copies the host arrays and waits for the device; graphs captured with a layer that is installed anew must not be replayed. */
 int mer_attention_install(mer_backend *b, uint32_t layer, const mer_attention_cfg *cfg);
 
-typedef struct mer_kv_batch { /* device pointers; strides in values, multiples of 8; pages on 16 bytes, keys and values within 64 GB each */
+typedef struct mer_kv_batch { /* device pointers; strides in values, multiples of 8; pages on 16 bytes, keys and values within 64 GB each (4 bits: below) */
   void *k_pages, *v_pages;    /* value d of head h of token t of page p lies at p * page_stride + t * token_stride + h * head_stride + d */
   uint64_t page_stride, token_stride, head_stride;
   const uint32_t *page_table; /* [n_seqs x table_stride] */
@@ -470,6 +471,31 @@ typedef struct mer_qkv_rows { /* device pointers; rows of heads side by side, e.
 } mer_qkv_rows;
 /* Norm and rotation in fp32 (angles in 64 bits), one rounding to the cache's type. */
 int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_qkv_rows *rows, void *stream);
+
+/* A cache of 4 bits (MER_ATTENTION_CACHE_Q4; same calls, same batches).  Groups of cache_group neighbouring values of a head share a scale and a minimum, both f16; a value
+ * x is held as a code of 4 bits and stands for scale * code + minimum:
+ *   minimum = f16(min x)   scale = f16(f32(max x - min x) * f32(1 / 15))   code = clamp(rint((x - minimum) * f32(1 / scale)), 0, 15), 0 where scale is 0
+ * (5 bits a value with groups of 32, 4.5 with 64; the error of a value is half a scale, plus what f16 cuts off the minimum where that is far larger than the group's
+ * range).  Keys are quantised behind norm and rotation; all of it in 64 bits, so the codes are the definition's.  A group with a value that is not finite, or
+ * of a magnitude above 60000, has the minimum NaN: its values read back as NaN, and rows that see them are not finite.
+ * Page p of key head h is a block of mer_kv4_block_bytes at k_pages (v_pages) + p * page_stride + h * head_stride, all in BYTES and multiples of 16; token_stride
+ * is 0.  A block has the codes of its tokens one behind the other, then their scales and minima.  A head's codes are stored for 64, 96, 128, 192 or 256 values, units = 2, 3, 4, 6 or 8
+ * of 32, 16 bytes each (append writes zeros behind the head's own values; a cache filled in another way has codes of any value there, and finite scales and minima):
+ *   keys    32-bit word j * units + u of a token (j < 4): values 32 u + 8 j + 2 p and + 2 p + 1 from bits 4 p and 16 + 4 p on (p < 4)
+ *   values  16-bit word r * units + u of a token (r < 8): values 32 u + 4 r + i from bit 4 i on (i < 4)
+ *   scales  token t, group g: scale and minimum, two f16, at (t * groups + g) * 4 behind the block's codes; groups = 32 * units / cache_group, rounded up
+ * Everything else is as with 16 bits: what rows see, tables, strides of rows, pages that are not there (their tokens count as zeros), windows, sinks. */
+uint64_t mer_kv4_block_bytes(uint32_t head_dim, uint32_t page_tokens, uint32_t group); /* 0: no such cache */
+
+/* Keys and values of the batch's rows, which the cache holds, as rows of numbers: a prefix to hand on, rows for another kernel.  Any cache; one rounding to value_type.  Rows
+ * behind the last sequence are left as they were; those without a place or a page are zeros, latched as MER_DEVSTAT_BAD_CACHE. */
+typedef struct mer_kv_rows { /* device pointers */
+  void *k, *v;                 /* [n_rows x kv_heads * head_dim] each; one of them may be NULL: not wanted */
+  uint64_t k_stride, v_stride; /* values between rows; 0 = rows without gaps */
+  int32_t value_type;          /* MER_VALUE_* */
+  uint32_t reserved;
+} mer_kv_rows;
+int mer_kv_read_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_kv_rows *rows, void *stream);
 /* d_q and d_out, which do not overlap: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8 below 2^26; 0 = no gaps).
  * Scores, exponentials and sums in fp32; the weights are rounded to the cache's type before they multiply the values, as the matrix units take both (2^-9 of a
  * weight at most in bf16, 2^-12 in f16), and the output once at the end.  The host sees no lengths, so n_rows <= n_seqs alone

@@ -48,6 +48,14 @@ def expert_bytes(dtype, d_model, d_ff):
     return int(capi.load_library().mer_expert_bytes(dtype, d_model, d_ff))
 
 
+def kv4_block_bytes(head_dim, page_tokens, group=32):
+    """Bytes of a page of one key head in a cache of 4 bits: what page and head strides are at least (multiples of 16)."""
+    n = int(capi.load_library().mer_kv4_block_bytes(head_dim, page_tokens, group))
+    if n == 0:
+        raise ValueError(f"no cache of 4 bits has heads of {head_dim} in pages of {page_tokens} tokens and groups of {group}")
+    return n
+
+
 def routed_expert_gpu_compatibility(dtype, d_model, d_ff):
     """routed_expert_gpu_compatibility (backend/mod.rs:4691-4720): True when the shape can run on the GPU."""
     return capi.load_library().mer_routed_expert_compatibility(dtype, d_model, d_ff) == 0
@@ -269,16 +277,21 @@ class Backend:
 
     # -- attention over a paged cache ---------------------------------------------------------
     def install_attention(self, layer, q_heads, kv_heads, head_dim, cache_type, page_tokens, window=0, scale=0.0, q_norm=None, k_norm=None,
-                          norm_eps=1e-6, rope_freq=None, rope_pairs=False, rope_scale=1.0, sinks=None):
+                          norm_eps=1e-6, rope_freq=None, rope_pairs=False, rope_scale=1.0, sinks=None, cache_bits=16, cache_group=32):
         """The attention side of `layer`: heads, cache (VALUE_F16 or VALUE_BF16, tokens of a page), window, per-head RMSNorm weights
-        [head_dim], rotation frequencies in radians per position (two values of a head each), sinks [q_heads]."""
+        [head_dim], rotation frequencies in radians per position (two values of a head each), sinks [q_heads].  With cache_bits=4 keys and
+        values are held in 4 bits, cache_group (32 or 64) neighbouring values sharing a scale and a minimum, and cache_type is that of
+        queries and outputs; pages are blocks of kv4_block_bytes and the batch's strides are in bytes."""
+        if cache_bits not in (4, 16):
+            raise ValueError("cache_bits must be 4 or 16")
         keep = [None if v is None else np.ascontiguousarray(v, dtype=t) for v, t in
                 ((q_norm, np.float32), (k_norm, np.float32), (rope_freq, np.float64), (sinks, np.float32))]
         for v, name, n in zip(keep, ("q_norm", "k_norm", "rope_freq", "sinks"), (head_dim, head_dim, None, q_heads)):
             if v is not None and (v.ndim != 1 or (n is not None and v.size != n)):
                 raise ValueError(f"{name} must have length {n}" if n is not None else f"{name} must have one axis")
         cfg = capi.MerAttentionCfg(q_heads, kv_heads, head_dim, page_tokens, cache_type, window, 0 if keep[2] is None else 2 * keep[2].size,
-                                   capi.ATTENTION_ROPE_PAIRS if rope_pairs else 0, scale, norm_eps, rope_scale, 0,
+                                   (capi.ATTENTION_ROPE_PAIRS if rope_pairs else 0) | (capi.ATTENTION_CACHE_Q4 if cache_bits == 4 else 0), scale, norm_eps, rope_scale,
+                                   cache_group if cache_bits == 4 else 0,
                                    *(None if v is None else v.ctypes.data for v in keep))
         self._check(self.lib.mer_attention_install(self.h, layer, C.byref(cfg)))
 
@@ -286,6 +299,12 @@ class Backend:
         """Rows of q|k|v (QkvRows) of a batch (KvBatch): norms, rotation, queries out, keys and values into the pages; asynchronous on
         `stream` (a cudaStream_t as int)."""
         rc = self.lib.mer_kv_append_device(self.h, layer, batch, rows, stream)
+        if rc != 0:
+            self._check(rc)
+
+    def kv_read_device(self, layer, batch, rows, stream=0):
+        """Keys and values of a batch's rows, out of the pages into rows of numbers (KvRows); asynchronous on `stream`."""
+        rc = self.lib.mer_kv_read_device(self.h, layer, batch, rows, stream)
         if rc != 0:
             self._check(rc)
 

@@ -11,7 +11,7 @@ EXPERT_NONE = 0xFFFFFFFF
 ADMIT_ANCHOR, ADMIT_ASYNC, ADMIT_NO_READER_WAIT = 1, 2, 4
 LAYER_RESIDUAL = 1
 VALUE_F32, VALUE_F16, VALUE_BF16 = 0, 1, 2
-ATTENTION_ROPE_PAIRS = 1
+ATTENTION_ROPE_PAIRS, ATTENTION_CACHE_Q4 = 1, 2
 
 
 class MerBackendCfg(C.Structure):
@@ -34,11 +34,11 @@ class MerLayerCfg(C.Structure):
 class MerAttentionCfg(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("q_heads", "kv_heads", "head_dim", "page_tokens")] + [("cache_type", C.c_int32)] + [
         (n, C.c_uint32) for n in ("window", "rope_dims", "flags")] + [(n, C.c_float) for n in ("scale", "norm_eps", "rope_scale")] + [
-        ("reserved", C.c_uint32)] + [(n, C.c_void_p) for n in ("q_norm", "k_norm", "rope_freq", "sinks")]
+        ("cache_group", C.c_uint32)] + [(n, C.c_void_p) for n in ("q_norm", "k_norm", "rope_freq", "sinks")]
 
 
 class KvBatch(C.Structure):
-    """mer_kv_batch: sequences and the paged cache they live in.  Device pointers (ints), strides in values."""
+    """mer_kv_batch: sequences and the paged cache they live in.  Device pointers (ints), strides in values (a cache of 4 bits: in bytes, no token_stride)."""
     _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p)] + [(n, C.c_uint64) for n in ("page_stride", "token_stride", "head_stride")] + [
         (n, C.c_void_p) for n in ("page_table", "row_start", "kv_len")] + [(n, C.c_uint32) for n in ("n_pages", "table_stride", "n_seqs", "n_rows")]
 
@@ -47,6 +47,11 @@ class QkvRows(C.Structure):
     """mer_qkv_rows: the rows to append.  Device pointers (ints), strides in values (0 = rows without gaps)."""
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + [
         ("value_type", C.c_int32), ("reserved", C.c_uint32)]
+
+
+class KvRows(C.Structure):
+    """mer_kv_rows: rows that keys and values are read back to.  Device pointers (ints, None: not wanted), strides in values (0 = rows without gaps)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64), ("value_type", C.c_int32), ("reserved", C.c_uint32)]
 
 
 class MerUthProjection(C.Structure):
@@ -187,6 +192,8 @@ ABI_SYMBOLS = {
     "mer_ep_layer_forward_a2a_device": (C.c_int, [_vp, _u32, _vp, _sz, _vp, _vp]),
     "mer_attention_install": (C.c_int, [_vp, _u32, C.POINTER(MerAttentionCfg)]),
     "mer_kv_append_device": (C.c_int, [_vp, _u32, C.POINTER(KvBatch), C.POINTER(QkvRows), _vp]),
+    "mer_kv4_block_bytes": (_u64, [_u32, _u32, _u32]),
+    "mer_kv_read_device": (C.c_int, [_vp, _u32, C.POINTER(KvBatch), C.POINTER(KvRows), _vp]),
     "mer_attention_forward_device": (C.c_int, [_vp, _u32, C.POINTER(KvBatch), _vp, _u64, _vp, _u64, _vp]),
     "mer_stream_check": (C.c_int, [_vp, _u32, _vp]),
     "mer_moe_layer_forward_submit": (C.c_int, [_vp, _u32, _vp, _sz, _vp, _u32]),

@@ -138,6 +138,42 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
   return r;
 }
 
+// Where a row of the batch stands, found by a whole warp.  The row's sequence is the last one that starts at the row or before it: the lanes read all starts and
+// lengths in one round trip.
+struct RowPlace {
+  uint32_t seq, pos;       // pos: ~0 where its sequence has no place for the row
+  uint32_t page, in_page;  // of a row that has one
+  uint32_t end;            // the batch's row behind the sequence's last one
+};
+// False: the row belongs to no sequence.
+__device__ __forceinline__ bool find_row(const KvBatchDev &kv, uint32_t page_tokens, uint32_t row, uint32_t lane, RowPlace *found) {
+  uint32_t s0 = 0, s1 = kv.n_seqs;
+  while (s1 - s0 > 128) {  // many: the lanes look at 32 starts at a time
+    const uint32_t step = (s1 - s0 + 31) / 32, s = s0 + lane * step;
+    const uint32_t before = __popc(__ballot_sync(0xFFFFFFFFu, s < s1 && kv.row_start[s] <= row));
+    if (before == 0) return false;
+    s0 += (before - 1) * step, s1 = min(s1, s0 + step);
+  }
+  uint32_t seq = 0, end = 0, len = 0;  // seq: its number + 1
+  for (uint32_t s = s0 + lane; s < s1; s += 32) {
+    const uint32_t start = kv.row_start[s], e = kv.row_start[s + 1], n = kv.kv_len[s];
+    if (start <= row) seq = s + 1, end = e, len = n <= kv.capacity ? n : 0;
+  }
+  const uint32_t last = __reduce_max_sync(0xFFFFFFFFu, seq);
+  if (last == 0) return false;
+  const uint32_t from = __ffs(__ballot_sync(0xFFFFFFFFu, seq == last)) - 1;
+  end = min(__shfl_sync(0xFFFFFFFFu, end, from), kv.n_rows), len = __shfl_sync(0xFFFFFFFFu, len, from);
+  if (row >= end) return false;  // behind the last sequence
+  found->seq = last - 1, found->end = end, found->pos = 0xFFFFFFFFu;
+  const uint32_t behind = end - row;  // this row and those after it: 1 for the newest
+  if (behind <= len) {
+    const uint32_t slot = divided(len - behind, kv.page_tokens);
+    const uint32_t page = slot < kv.table_stride ? kv.page_table[(uint64_t)(last - 1) * kv.table_stride + slot] : 0xFFFFFFFFu;
+    if (page < kv.n_pages) found->pos = len - behind, found->page = page, found->in_page = found->pos - slot * page_tokens;
+  }
+  return true;
+}
+
 // Where the tokens of a sequence lie, for one key head.
 struct PagePlaces {
   const uint32_t *pages;

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "kv4.h"
+
 // Division of numbers below 2^31 by a constant of a launch: multiplier and shift of Granlund and Montgomery, "Division by invariant integers using
 // multiplication" (1994), section 4; below 2^31 its last sum has room in 32 bits.
 struct FastDiv {
@@ -21,7 +23,9 @@ struct AttnLayer {
   uint32_t q_heads, kv_heads, head_dim, page_tokens;
   uint32_t window;                // tokens that a row sees, itself among them; 0 = all before it
   float scale;                    // of the scores
-  int cache_type;                 // MER_VALUE_F16 or MER_VALUE_BF16
+  int cache_type;                 // MER_VALUE_F16 or MER_VALUE_BF16: queries, outputs, and the cache where it does not hold 4 bits
+  bool q4;                        // keys and values in 4 bits, as kv4 says
+  Kv4Shape kv4;
   uint32_t rope_dims;             // leading values of a head that are rotated
   int rope_pairs;                 // neighbours instead of halves
   float rope_scale, norm_eps;
@@ -37,7 +41,7 @@ struct AttnLayer {
 // mer_kv_batch as the kernels take it.
 struct KvBatchDev {
   void *k_pages, *v_pages;
-  uint64_t page_stride, token_stride, head_stride;  // in values; all places lie below KV_MAX_SPAN
+  uint64_t page_stride, token_stride, head_stride;  // in values; all places lie below KV_MAX_SPAN.  In 4 bits: in bytes, and no token_stride
   FastDiv page_tokens;
   uint32_t capacity;  // tokens that a row of the table has pages for
   const uint32_t *page_table, *row_start, *kv_len;
@@ -53,6 +57,15 @@ struct QkvRowsDev {
 
 // kernels_kv.cu
 cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const QkvRowsDev &rows, uint32_t *status, int sm_count, cudaStream_t s);
+
+// Rows that keys and values are read back to; either may be null.
+struct KvRowsDev {
+  void *k, *v;
+  uint64_t k_stride, v_stride;  // in values
+  int type;
+};
+// kernels_kv_read.cu
+cudaError_t launch_kv_read(const AttnLayer &a, const KvBatchDev &kv, const KvRowsDev &rows, uint32_t *status, int sm_count, cudaStream_t s);
 
 // Workspace of the attention kernels: `parts` floats and `counts` zeroed words that every call leaves zero.
 struct AttnWorkspace {

@@ -106,14 +106,28 @@ struct KvParams {
   uint32_t q_steps, kv_steps; // steps of 32 / group heads
   uint32_t chunks, each;      // warps of a row, and steps of each
   float per_value;            // 1 / head_dim
+  // A cache of 4 bits: the warps above have the queries alone, keys and values are those of kv4_append.
+  uint32_t kv4_lanes;             // of a head, a power of two
+  uint32_t kv4_steps, kv4_each;   // steps of 32 / kv4_lanes heads for the keys, and as many for the values; of a warp
+  uint32_t kv4_chunks;            // warps of a row
+  bool kv4_vec;                   // rows by vectors of 8 values
 };
 
-// IN: the rows' type, OUT: the cache's and q_out's, V: values of a vector.
-template <typename IN, typename OUT, int V>
+#include "kv4_append.cuh"
+
+// IN: the rows' type, OUT: the cache's and q_out's, V: values of a vector, Q4: the cache holds 4 bits.
+template <typename IN, typename OUT, int V, bool Q4>
 __global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
-  extern __shared__ float2 turns[];  // [rope_dims / 2] cosine and sine
+  extern __shared__ __align__(16) float2 turns[];  // [rope_dims / 2] cosine and sine
   const AttnLayer &a = p.a;
-  const uint32_t lane = threadIdx.x, row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
+  const uint32_t warps = Q4 ? p.chunks + p.kv4_chunks : p.chunks;
+  const uint32_t lane = threadIdx.x, row = blockIdx.x / warps, chunk = blockIdx.x - row * warps;
+  if constexpr (Q4) {
+    if (chunk >= p.chunks) {
+      kv4_append<IN>(p, row, chunk - p.chunks, reinterpret_cast<double2 *>(turns));
+      return;
+    }
+  }
   const uint32_t D = a.head_dim, half = a.rope_dims / 2, sub = lane & (p.group - 1), of = lane / p.group, heads = 32 / p.group;
   // Pair m of a head's vectors.  Behind the rotated values neighbours pair up, of which the last may have no second.
   constexpr int STEPS = V == 1 ? 4 : 1;  // V == 1: 32 lanes take up to 4 pairs each
@@ -150,41 +164,14 @@ __global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
   grid_dep_launch();
 #pragma unroll
   for (int d = 0; d < AHEAD; d++) ask(first_step + d, ahead[d]);  // while position and place are looked up
-  // The row's sequence is the last one that starts at the row or before it: the lanes read all starts and lengths in one round trip.
-  uint32_t pos = 0xFFFFFFFFu;
-  uint64_t place = 0;
-  {
-    uint32_t s0 = 0, s1 = p.kv.n_seqs;
-    while (s1 - s0 > 128) {  // many: the lanes look at 32 starts at a time
-      const uint32_t step = (s1 - s0 + 31) / 32, s = s0 + lane * step;
-      const uint32_t before = __popc(__ballot_sync(0xFFFFFFFFu, s < s1 && p.kv.row_start[s] <= row));
-      if (before == 0) return;
-      s0 += (before - 1) * step, s1 = min(s1, s0 + step);
-    }
-    uint32_t seq = 0, end = 0, len = 0;  // seq: its number + 1
-    for (uint32_t s = s0 + lane; s < s1; s += 32) {
-      const uint32_t start = p.kv.row_start[s], e = p.kv.row_start[s + 1], n = p.kv.kv_len[s];
-      if (start <= row) seq = s + 1, end = e, len = n <= p.kv.capacity ? n : 0;
-    }
-    const uint32_t last = __reduce_max_sync(0xFFFFFFFFu, seq);
-    if (last == 0) return;
-    const uint32_t from = __ffs(__ballot_sync(0xFFFFFFFFu, seq == last)) - 1;
-    end = min(__shfl_sync(0xFFFFFFFFu, end, from), p.kv.n_rows), len = __shfl_sync(0xFFFFFFFFu, len, from);
-    if (row >= end) return;  // behind the last sequence
-    const uint32_t behind = end - row;  // this row and those after it: 1 for the newest
-    if (behind <= len) {
-      const uint32_t slot = divided(len - behind, p.kv.page_tokens);
-      const uint32_t page = slot < p.kv.table_stride ? p.kv.page_table[(uint64_t)(last - 1) * p.kv.table_stride + slot] : 0xFFFFFFFFu;
-      if (page < p.kv.n_pages) {
-        pos = len - behind;
-        place = page * p.kv.page_stride + (uint64_t)(pos - slot * a.page_tokens) * p.kv.token_stride;
-      }
-    }
-    if (pos == 0xFFFFFFFFu) {
-      if (lane == 0) atomicOr(p.status, MER_DEVSTAT_BAD_CACHE);
-      return;
-    }
+  RowPlace at_row;
+  if (!find_row(p.kv, a.page_tokens, row, lane, &at_row)) return;
+  const uint32_t pos = at_row.pos;
+  if (pos == 0xFFFFFFFFu) {
+    if (lane == 0) atomicOr(p.status, MER_DEVSTAT_BAD_CACHE);
+    return;
   }
+  const uint64_t place = at_row.page * p.kv.page_stride + (uint64_t)at_row.in_page * p.kv.token_stride;
   for (uint32_t j = lane; j < half; j += 32) {
     const double x = (double)pos * __ldg(a.turns + j);
     float sin, cos;
@@ -307,7 +294,8 @@ bool vec_ok(const void *p, uint64_t stride, uint32_t v, uint32_t size) {
 
 template <typename IN, typename OUT, int V>
 cudaError_t launch_kv(KvParams &p, dim3 grid, size_t smem, cudaStream_t s) {
-  return launch_overlapped(k_kv_append<IN, OUT, V>, grid, 32, smem, s, false, p);
+  return p.a.q4 ? launch_overlapped(k_kv_append<IN, OUT, V, true>, grid, 32, smem, s, false, p)
+                : launch_overlapped(k_kv_append<IN, OUT, V, false>, grid, 32, smem, s, false, p);
 }
 template <typename IN, typename OUT>
 cudaError_t launch_kv(KvParams &p, uint32_t v, dim3 grid, size_t smem, cudaStream_t s) {
@@ -323,7 +311,7 @@ cudaError_t launch_kv(KvParams &p, uint32_t v, dim3 grid, size_t smem, cudaStrea
 }  // namespace
 
 cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const QkvRowsDev &r, uint32_t *status, int sm_count, cudaStream_t s) {
-  KvParams p{a, kv, r, status, 1, 0, 0, 1, 0, 1.0f / (float)a.head_dim};
+  KvParams p{a, kv, r, status, 1, 0, 0, 1, 0, 1.0f / (float)a.head_dim, 1, 0, 0, 0, false};
   const uint32_t in = r.type == MER_VALUE_F32 ? 4 : 2;
   // The widest vector up to 16 bytes that neither a rotated pair nor an address cuts.  (Eight fp32 values a vector: 24652 rows of 8 + 2 heads of 128 61 us,
   // 50 so, with 72 registers instead of 121; four f16 values: 13411 rows of 32 + 2 * 8 heads 83 us, 57 with eight.)
@@ -337,13 +325,27 @@ cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const Qkv
   while (p.group < pairs && p.group < 32) p.group *= 2;
   const uint32_t heads = 32 / p.group;
   p.q_steps = (a.q_heads + heads - 1) / heads, p.kv_steps = (a.kv_heads + heads - 1) / heads;
+  if (a.q4) {
+    p.q_steps = r.q ? p.q_steps : 0, p.kv_steps = 0;
+    while (p.kv4_lanes < 4 * a.kv4.units) p.kv4_lanes *= 2;
+    p.kv4_steps = (a.kv_heads + 32 / p.kv4_lanes - 1) / (32 / p.kv4_lanes);
+    p.kv4_vec = vec_ok(r.k, r.k_stride, 8, in) && vec_ok(r.v, r.v_stride, 8, in) && (a.rope_pairs || a.rope_dims % 16 == 0);
+  }
   // A warp a row, and more of them while there are fewer than 16 an SM: fewer steps one after the other.
-  const uint32_t steps = p.q_steps + 2 * p.kv_steps;
-  p.chunks = (uint32_t)std::min<uint64_t>(steps, std::max<uint64_t>(1, (uint64_t)sm_count * 16 / kv.n_rows));
-  p.each = (steps + p.chunks - 1) / p.chunks;
-  p.chunks = (steps + p.each - 1) / p.each;
-  const dim3 grid(kv.n_rows * p.chunks);  // one row's warps only where rows are few: below 2^31
-  const size_t smem = (size_t)(a.rope_dims / 2) * sizeof(float2);
+  const auto split = [&](uint32_t steps, uint32_t *chunks, uint32_t *each) {
+    *chunks = (uint32_t)std::min<uint64_t>(steps, std::max<uint64_t>(1, (uint64_t)sm_count * 16 / kv.n_rows));
+    *each = *chunks ? (steps + *chunks - 1) / *chunks : 0;
+    *chunks = *each ? (steps + *each - 1) / *each : 0;
+  };
+  split(p.q_steps + 2 * p.kv_steps, &p.chunks, &p.each);
+  size_t smem = (size_t)(a.rope_dims / 2) * sizeof(float2);
+  if (a.q4) {
+    split(2 * p.kv4_steps, &p.kv4_chunks, &p.kv4_each);
+    smem = (size_t)(a.rope_dims / 2) * sizeof(double2);
+  }
+  // more than a warp or two a row only where rows are few; the grid's x goes up to 2^31 - 1
+  if ((uint64_t)kv.n_rows * (p.chunks + p.kv4_chunks) > 0x7FFFFFFFu) return cudaErrorInvalidValue;
+  const dim3 grid(kv.n_rows * (p.chunks + p.kv4_chunks));
   return r.type == MER_VALUE_F32   ? launch_kv<float>(p, v, grid, smem, s)
          : r.type == MER_VALUE_F16 ? launch_kv<__half>(p, v, grid, smem, s)
                                    : launch_kv<__nv_bfloat16>(p, v, grid, smem, s);
