@@ -402,6 +402,10 @@ size_t attend_counts(int sm_count) { return (size_t)sm_count; }
 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
+  if (a.q4) {
+    *launches += 1;
+    return launch_attend_tc4(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+  }
   // One row a sequence and no more heads of a key head than a tile has rows: the streaming kernel.  Any more rows: the tensor-core kernel, whose 128 rows a group cost
   // the same whatever they hold.
   if (kv.n_rows > kv.n_seqs || a.q_heads / a.kv_heads > 16) {
