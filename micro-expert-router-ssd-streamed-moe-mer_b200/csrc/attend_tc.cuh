@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "attend_join.cuh"
 #include "attend_wait.cuh"
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
           tm_fence_after();
           // the queries' units came with the queries; the tile after the next one's take this place
           if constexpr (U != 0)
-            if (blk == blk0) to_log2 = p.a.scale * LOG2E * ctl.unit[turn & 1][row];
+            if (blk == blk0) to_log2 = fmaxf(p.a.scale * LOG2E * ctl.unit[turn & 1][row], FLT_MIN);  // a hidden score times it is one still
           float s[4][32];
 #pragma unroll
           for (int h = 0; h < 4; h++) tm_load_begin(s_at + h * 32, s[h]);

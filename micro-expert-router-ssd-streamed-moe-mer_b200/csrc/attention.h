@@ -80,6 +80,10 @@ cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const voi
 // kernels_attend_tc4.cu
 cudaError_t launch_attend_tc4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                               int sm_count, cudaStream_t s);
+// kernels_attend4.cu
+size_t attend4_part_floats(int sm_count);
+cudaError_t launch_attend4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count,
+                           cudaStream_t s);
 // kernels_attend.cu
 size_t attend_counts(int sm_count);
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,

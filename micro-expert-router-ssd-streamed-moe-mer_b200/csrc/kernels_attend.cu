@@ -396,14 +396,15 @@ cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_co
 }  // namespace
 
 size_t attend_part_floats(int sm_count) {
-  return std::max((size_t)2 * sm_count * part_floats(16, 256), attend_tc_part_floats(sm_count));
+  return std::max((size_t)2 * sm_count * part_floats(16, 256), std::max(attend_tc_part_floats(sm_count), attend4_part_floats(sm_count)));
 }
-size_t attend_counts(int sm_count) { return (size_t)sm_count; }
+size_t attend_counts(int sm_count) { return (size_t)sm_count * 4; }  // a CTA's each: four an SM at most
 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
   if (a.q4) {
     *launches += 1;
+    if (kv.n_rows <= kv.n_seqs && a.q_heads / a.kv_heads <= 16) return launch_attend4(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
     return launch_attend_tc4(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
   }
   // One row a sequence and no more heads of a key head than a tile has rows: the streaming kernel.  Any more rows: the tensor-core kernel, whose 128 rows a group cost

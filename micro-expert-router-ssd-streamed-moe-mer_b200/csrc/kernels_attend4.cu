@@ -1,0 +1,39 @@
+// Attention of single new tokens over a paged cache of 4 bits: attend4.cuh.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <stdint.h>
+
+namespace {
+constexpr uint32_t ATTEND4_WHOLE = 6;    // blocks of a tile that is not cut
+constexpr uint32_t ATTEND4_START = 4;    // what a tile costs beside its blocks, in blocks
+constexpr uint32_t ATTEND4_MIN_RUN = 6;  // units of the shortest run
+}  // namespace
+
+#include "attend4.cuh"
+
+namespace {
+
+template <int GS, int NT>
+cudaError_t launch_stream4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count, cudaStream_t s) {
+  switch (a.kv4.units) {
+    case 2: return launch_stream4<2, GS, NT>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+    case 3: return launch_stream4<3, GS, NT>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+    case 4: return launch_stream4<4, GS, NT>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+    case 6: return launch_stream4<6, GS, NT>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+    default: return launch_stream4<8, GS, NT>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+  }
+}
+
+}  // namespace
+
+size_t attend4_part_floats(int sm_count) { return (size_t)2 * sm_count * std::max(4 * part_floats(8, 128), 2 * part_floats(16, 256)); }
+
+cudaError_t launch_attend4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count,
+                           cudaStream_t s) {
+  // Up to eight query heads of a key head: eight rows a tile, else sixteen.
+  const bool few = a.q_heads / a.kv_heads <= 8;
+  if (a.kv4.group == 32)
+    return few ? launch_stream4<0, 1>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s) : launch_stream4<0, 2>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+  return few ? launch_stream4<1, 1>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s) : launch_stream4<1, 2>(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+}
