@@ -10,9 +10,10 @@
 //   * Keys:  q . k = sum_g scale_g (q . code)_g + minimum_g (sum of q)_g.  The first product is exact in fp32 and takes its scale there; the second is one more
 //     matrix product, whose operand the words (scale, minimum) are as they lie in memory, against (0, sum of q) in two parts of f16.
 //   * Values:  o = sum_g (p scale_g) . code + p . minimum_g.  A weight times a scale is rounded to f16, the weights themselves once more; minima are an operand as above.
-//     The product has the head's values along M and the rows along N: the scores' registers are its B operand as they are, and eight rows cost half of sixteen.
-//   * Queries are f16 divided by a power of two of their row.  Weights are made as 2^(s - m + 15 - e), where 2^e, at least 1, holds every scale of a value so far: a weight
-//     and its product with a scale stay below 2^15, and small ones above the last bit of f16 for 2^-30 of the largest.
+//   * Both products have tokens or the head's values along M and the rows along N, so that eight rows cost half of sixteen; the weights are transposed between them (movmatrix).
+//   * Queries are f16 divided by a power of two of their row.  A row's reference m follows its maximum only when that has grown by more than 2^LAG4.  Weights are made as
+//     2^(s - m + 15 - LAG4 - e), where 2^e, at least 2, is above every scale of a value so far: a weight and its product with a scale stay below 2^15, and small ones
+//     above the last bit of f16 for 2^-34 of the largest.
 //
 // Copies are cp.async of 16 bytes a lane into a ring that no other warp sees, so nothing waits on a barrier; their places in it are such that no load has a bank conflict.
 #pragma once
@@ -25,10 +26,11 @@
 #include "attention.cuh"
 #include "kernels.h"
 #include "kv4_unpack.cuh"
-#include "pack2.cuh"
 #include "ptx.cuh"
 
 namespace {
+
+constexpr float LAG4 = 4.0f;
 
 struct Attend4Params {
   AttnLayer a;
@@ -39,6 +41,7 @@ struct Attend4Params {
   AttnWorkspace ws;
   TileShape ts;
   uint32_t min_units;
+  uint32_t page_units;  // 16 bytes between pages
   bool whole_pages;  // a chunk of 16 tokens lies in one page
 };
 
@@ -68,7 +71,7 @@ __device__ __forceinline__ constexpr uint32_t value_piece(uint32_t t, uint32_t c
   return U == 8 ? c ^ ((t & 3) << 1) : U == 4 ? c ^ (t & 2) : c;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) { copy16(dst, src, in ? 16 : 0); }
+__device__ __forceinline__ void copy16_all(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(in ? N : 0) : "memory");
@@ -98,19 +101,38 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
     for (int i = 0; i < N; i++) w[i] = lds32(a + i * 4);
   }
 }
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// A value that is computed where it stands: nothing that is made of it moves in front of a branch that is hardly ever taken.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t t;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 template <int U, int GS, int NT>
-__global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape<U, GS, NT>::CTAS) k_attend4(const Attend4Params p) {
+__global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape<U, GS, NT>::CTAS) k_attend4(const __grid_constant__ Attend4Params p) {
   using S = Stream4Shape<U, GS, NT>;
   constexpr int NW = S::NW, ST = S::ST, R = S::R, G = S::G;
   constexpr uint32_t KB = S::KB, THREADS = S::THREADS;
   extern __shared__ __align__(128) uint8_t smem[];  // [NW][ST] chunks
   __shared__ RunFound s_found;
+  __shared__ RunStart s_run;
+  __shared__ RunPlace s_walk;
+  __shared__ TileWork s_tile;  // here, not in registers: the loop over a tile's blocks needs all of these for itself.  tokens == 0: there is none left
   __shared__ uint32_t s_flag;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, eighth = lane >> 2;
   const uint32_t D = p.a.head_dim, page_tokens = p.a.page_tokens, window = p.a.window;
@@ -118,7 +140,12 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
   const TileShape &ts = p.ts;
   grid_dep_wait();
   grid_dep_launch();
-  const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, p.min_units, s_found);
+  {
+    const RunStart run = find_run<KB, THREADS>(p.kv, ts, window, blockIdx.x, gridDim.x, p.min_units, s_found);
+    if (tid == 0) s_run = run, s_walk = RunWalk<KB>(p.kv, ts, window, run);
+  }
+  __syncthreads();
+  const RunStart &run = s_run;
   if (blockIdx.x == 0) {
     if (f16)
       clear_rows_without_place<__half, THREADS>(p.a, p.kv, (__half *)p.out, p.out_stride, p.ws.status);
@@ -126,70 +153,107 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
       clear_rows_without_place<__nv_bfloat16, THREADS>(p.a, p.kv, (__nv_bfloat16 *)p.out, p.out_stride, p.ws.status);
   }
   if (blockIdx.x >= run.parts) return;
-  RunWalk<KB> walk(p.kv, ts, window, run);
   const uint32_t ring = smem_u32(smem) + warp * (ST * S::CHUNK);
   const float to_log2 = p.a.scale * LOG2E;
   uint32_t bad = 0;
+  // Where in a chunk the lane's pieces go: of codes, piece i * 32 + lane of the chunk's; of scales, lanes 0 .. 15 the keys', the others the values'.
+  uint32_t k_to[(U + 1) / 2], v_to[(U + 1) / 2], scale_to = S::CODES + (lane < 16 ? 0 : S::CODES + S::SCALES) + slot_of(lane & 15) * (4 * G);
+  const char *const scale_pages = (const char *)(lane < 16 ? p.kv.k_pages : p.kv.v_pages);
+#pragma unroll
+  for (int i = 0; i < (U + 1) / 2; i++) {
+    const uint32_t e = i * 32 + lane, tok = e / U % 16, c = e % U, slot = slot_of(tok);
+    k_to[i] = slot * (16 * U) + key_piece<U>(slot, c) * 16, v_to[i] = S::CODES + S::SCALES + tok * (16 * U) + value_piece<U>(tok, c) * 16;
+    if (U == 4 && i) k_to[i] = k_to[0] + 512, v_to[i] = v_to[0] + 512;  // eight tokens on
+    if (U == 4 ? i == 0 : true) asm volatile("" : "+r"(k_to[i]), "+r"(v_to[i]));  // kept, not made again for every chunk
+  }
+  asm volatile("" : "+r"(scale_to));
 
-  TileWork t;
-  while (walk.next(&t)) {
-    const uint32_t rows = t.tokens * t.heads;
+  const TileWork &t = s_tile;
+  for (;;) {
+    if (tid == 0) {
+      RunWalk<KB> walk(p.kv, ts, window, s_walk);
+      TileWork next;
+      if (!walk.next(&next)) next.tokens = 0;
+      s_tile = next, s_walk = walk;
+    }
+    __syncthreads();
+    if (t.tokens == 0) break;
+    const uint32_t tile_rows = t.tokens * t.heads;
     const uint32_t end = t.past + t.token0 + t.tokens;  // behind the last token that a row of the tile sees
     const uint32_t start = first_seen(t, window);
-    // ---- the ring: chunk i of the warp's lies in stage i % ST.  A lane knows the page of one token of a chunk, ST chunks ahead.
+    // ---- the ring: the warp's blocks are b_lo .. b_hi, block b_lo + i lies in stage i % ST.  A lane knows the page of one token of a chunk, ST chunks ahead.
+    const uint32_t w16 = warp * 16;
+    const uint32_t b_lo = max(t.lo, start < w16 + 16 ? 0u : (start - w16 - 16) / KB + 1), b_hi = end <= w16 ? t.lo : min(t.hi, (end - w16 + KB - 1) / KB);
+    // Blocks f_lo .. f_lo + f_n: whole chunks of one page each.
+    const uint32_t f_lo = start <= w16 ? 0u : (start - w16 + KB - 1) / KB, f_hi = end < w16 + 16 || !p.whole_pages ? 0u : (end - w16 - 16) / KB + 1, f_n = min(f_hi, b_hi) > f_lo ? min(f_hi, b_hi) - f_lo : 0;
     const uint32_t *const table = p.kv.page_table + (uint64_t)t.seq * p.kv.table_stride;
-    auto wanted = [&](uint32_t blk) { return blk < t.hi && blk * KB + warp * 16 < end && blk * KB + warp * 16 + 16 > start; };
-    auto entry = [&](uint32_t blk) {
-      const uint32_t key = blk * KB + warp * 16 + (lane & 15), slot = divided(key, p.kv.page_tokens);
-      return blk < t.hi && (p.whole_pages || (key >= start && key < end)) && slot < p.kv.table_stride ? table[slot] : 0xFFFFFFFFu;
+    struct Place {
+      uint32_t number, in;  // page, and the token in it (whole_pages: the chunk's first)
     };
-    auto issue = [&](uint32_t blk, uint32_t number, uint32_t stage) {
-      if (wanted(blk)) {
-        const uint32_t key0 = blk * KB + warp * 16, key = key0 + (lane & 15);
-        const bool seen = key >= start && key < end, there = seen && number < p.kv.n_pages;
-        if (seen && !there) bad = 1;
-        const uint32_t in = key - divided(key, p.kv.page_tokens) * page_tokens;  // of the lane's token
-        const uint64_t block = number < p.kv.n_pages ? number * p.kv.page_stride + t.kv_head * p.kv.head_stride : 0;
-        const uint32_t dst = ring + stage * S::CHUNK;
-        const uint32_t valid = __ballot_sync(0xFFFFFFFFu, there);  // tokens of the chunk, twice
-        const uint64_t first = block + (uint64_t)(in - (lane & 15)) * (16 * U);  // of the chunk's codes, where it lies in one page
+    auto entry = [&](uint32_t blk) {
+      const uint32_t key = blk * KB + w16 + (p.whole_pages ? 0 : lane & 15), slot = divided(key, p.kv.page_tokens);
+      Place at;
+      at.in = key - slot * page_tokens;
+      at.number = blk < b_hi && (p.whole_pages || (key >= first_seen(t, window) && key < t.past + t.token0 + t.tokens)) && slot < p.kv.table_stride ? table[slot] : 0xFFFFFFFFu;
+      return at;
+    };
+    const uint64_t head_at = t.kv_head * p.kv.head_stride;
+    // in 16 bytes; scales in 4
+    const uint64_t codes_at = head_at / 16 + lane, scales_at = (head_at + p.a.kv4.codes) / 4 + (lane & 15) * G;
+    auto issue = [&](uint32_t blk, const Place &at, uint32_t stage) {
+      constexpr int N = G % 4 == 0 ? 16 : G % 2 == 0 ? 8 : 4;
+      const uint32_t dst = ring + stage * S::CHUNK;
+      if (blk - f_lo < f_n && at.number < p.kv.n_pages) {
+        const uint64_t page = (uint64_t)at.number * p.page_units;
+        const uint64_t first = page + codes_at + at.in * U;
 #pragma unroll
         for (int i = 0; i < (U + 1) / 2; i++) {
-          const uint32_t e = i * 32 + lane, tok = e / U, c = e - tok * U;
-          if (U % 2 && e >= 16 * U) continue;
-          const bool ok = valid >> tok & 1;
-          uint64_t off;
-          if (p.whole_pages) {
-            off = first + e * 16;
-          } else {
-            off = __shfl_sync(U % 2 && i == U / 2 ? 0xFFFFu : 0xFFFFFFFFu, block, tok) + (uint64_t)__shfl_sync(U % 2 && i == U / 2 ? 0xFFFFu : 0xFFFFFFFFu, in, tok) * (16 * U) + c * 16;
-          }
-          off = ok ? off : 0;
-          const uint32_t slot = slot_of(tok);
-          cp_async16(dst + slot * (16 * U) + key_piece<U>(slot, c) * 16, (const char *)p.kv.k_pages + off, ok);
-          cp_async16(dst + S::CODES + S::SCALES + tok * (16 * U) + value_piece<U>(tok, c) * 16, (const char *)p.kv.v_pages + off, ok);
+          if (U % 2 && i * 32 + lane >= 16 * U) continue;
+          copy16_all(dst + k_to[i], (const char *)p.kv.k_pages + (first * 16 + i * 512));
+          copy16_all(dst + v_to[i], (const char *)p.kv.v_pages + (first * 16 + i * 512));
         }
-        // scales: lanes 0 .. 15 of the keys, the others of the values
-        const char *src = (const char *)(lane < 16 ? p.kv.k_pages : p.kv.v_pages) + (there ? block + p.a.kv4.codes + (uint64_t)in * (4 * G) : 0);
-        const uint32_t to = dst + S::CODES + (lane < 16 ? 0 : S::CODES + S::SCALES) + slot_of(lane & 15) * (4 * G);
-        constexpr int N = G % 4 == 0 ? 16 : G % 2 == 0 ? 8 : 4;
+        const char *const src = scale_pages + (page * 16 + (scales_at + at.in * G) * 4);
 #pragma unroll
         for (int i = 0; i < 4 * G / N; i++) {
           if constexpr (N == 16)
-            cp_async16(to + i * N, src + (there ? i * N : 0), there);
+            copy16_all(dst + scale_to + i * N, src + i * N);
           else
-            cp_async_small<N>(to + i * N, src + (there ? i * N : 0), there);
+            cp_async_small<N>(dst + scale_to + i * N, src + i * N, true);
+        }
+      } else if (blk < b_hi) {  // token by token; what it needs of the tile is read again
+        const uint32_t end = t.past + t.token0 + t.tokens, start = first_seen(t, window);
+        const uint32_t key = here(blk) * KB + w16 + (lane & 15), in = p.whole_pages ? here(at.in) + (lane & 15) : at.in;
+        const bool seen = key >= start && key < end, there = seen && at.number < p.kv.n_pages;
+        if (seen && !there) bad = 1;
+        const uint64_t block = there ? at.number * p.kv.page_stride + t.kv_head * p.kv.head_stride : 0;
+        const uint32_t valid = __ballot_sync(0xFFFFFFFFu, there);  // tokens of the chunk, twice
+#pragma unroll
+        for (int i = 0; i < (U + 1) / 2; i++) {
+          const uint32_t e = i * 32 + here(lane), tok = e / U % 16, c = e % U;
+          const uint64_t off = __shfl_sync(0xFFFFFFFFu, block, tok) + (uint64_t)__shfl_sync(0xFFFFFFFFu, in, tok) * (16 * U) + c * 16;
+          if (U % 2 && e >= 16 * U) continue;
+          const bool ok = valid >> tok & 1;
+          copy16(dst + k_to[i], (const char *)p.kv.k_pages + (ok ? off : 0), ok ? 16 : 0);
+          copy16(dst + v_to[i], (const char *)p.kv.v_pages + (ok ? off : 0), ok ? 16 : 0);
+        }
+        const char *const src = scale_pages + (there ? block + p.a.kv4.codes + (uint64_t)in * (4 * G) : 0);
+#pragma unroll
+        for (int i = 0; i < 4 * G / N; i++) {
+          if constexpr (N == 16)
+            copy16(dst + scale_to + i * N, src + (there ? i * N : 0), there ? 16 : 0);
+          else
+            cp_async_small<N>(dst + scale_to + i * N, src + (there ? i * N : 0), there);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    uint32_t ahead[ST];
+    Place ahead[ST];
 #pragma unroll
-    for (int i = 0; i < ST; i++) ahead[i] = entry(t.lo + i);
+    for (int i = 0; i < ST; i++) ahead[i] = entry(b_lo + i);
     // ---- queries, before the copies: behind these they would wait for a full ring of every SM.  Lane (eighth, quad) has values 32 u + 8 quad .. of rows eighth and eighth + 8, as the
-    // product's A operand wants them: pair p of the eight meets the codes from bits 4 p and 16 + 4 p on, which stand for themselves times 2^-24 where p is even, 2^-20 where it is odd.
+    // product's B operand wants them: pair p of the eight meets the codes from bits 4 p and 16 + 4 p on, which stand for themselves times 2^-24 where p is even, 2^-20 where it is odd.
     uint32_t qf[NT][U][4], qs[NT][(G + 3) / 4][2];  // qs: sums of a group's queries in two parts, each behind a zero
-    float factor[NT];
+    float row_factor[NT];  // of row x * 8 + eighth
 #pragma unroll
     for (int x = 0; x < NT; x++) {
       const uint32_t r = x * 8 + eighth, tok = r / t.heads, h = r - tok * t.heads;
@@ -197,7 +261,7 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
 #pragma unroll
       for (int u = 0; u < U; u++) {
         raw[u] = make_uint4(0, 0, 0, 0);
-        if (r < rows && u * 32 + quad * 8 < D)
+        if (r < tile_rows && u * 32 + quad * 8 < D)
           raw[u] = *reinterpret_cast<const uint4 *>((const char *)p.q + ((uint64_t)(t.row0 + t.token0 + tok) * p.q_stride + (uint64_t)(t.head0 + h) * D + u * 32 + quad * 8) * 2);
       }
       float top = 0.0f;
@@ -213,7 +277,7 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       const uint32_t power = min(max(__float_as_uint(top) >> 23, 1u), 253u);
       const float per = __uint_as_float((254 - power) << 23);
-      factor[x] = fmaxf(to_log2 * __uint_as_float(power << 23), FLT_MIN);  // a hidden score times it is one still
+      row_factor[x] = fmaxf(to_log2 * __uint_as_float(power << 23), FLT_MIN);  // a hidden score times it is one still
       float sums[G];
 #pragma unroll
       for (int g = 0; g < G; g++) sums[g] = 0.0f;
@@ -244,17 +308,19 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
       }
     }
 #pragma unroll
-    for (int i = 0; i < ST - 1; i++) issue(t.lo + i, ahead[i], i);
-    uint32_t next_entry = ahead[ST - 1], stage = 0;
-    // the last token that the lane's rows see
-    uint32_t last[NT];
-#pragma unroll
-    for (int x = 0; x < NT; x++) last[x] = t.past + t.token0 + min(x * 8 + eighth, rows - 1) / t.heads;
-    const uint32_t all_see = t.past + t.token0, all_from = window && end > window ? end - window : 0;  // every row sees the tokens all_from .. all_see
-    float o[NT][S::TILES][4], least[NT][4], m[NT], l[NT];  // least: sums of weights times minima
+    for (int i = 0; i < ST - 1; i++) issue(b_lo + i, ahead[i], i);
+    Place next_place = ahead[ST - 1];
+    uint32_t stage = 0;
+    // Every row sees the tokens all_from .. all_see; of the warp's chunks, those of blocks n_lo .. n_lo + n_n have no others.
+    const uint32_t all_see = t.past + t.token0, all_from = window && end > window ? end - window : 0;
+    const uint32_t n_lo = all_from <= w16 ? 0u : (all_from - w16 + KB - 1) / KB, n_hi = all_see < w16 + 15 ? 0u : (all_see - w16 - 15) / KB + 1, n_n = n_hi > n_lo ? n_hi - n_lo : 0;
+    // The lane has rows x * 8 + quad * 2 + e of scores and outputs.  least: sums of weights times minima
+    // A weight is 2^(s * factor - less) with less = m - shift; limit: the score from which on m has to follow, -infinity while there is no m.
+    float o[NT][S::TILES][4], least[NT][4], less[NT][2], limit[NT][2], l[NT][2], factor[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; x++) {
-      m[x] = -INFINITY, l[x] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 2; e++) less[x][e] = 0.0f, limit[x][e] = -INFINITY, l[x][e] = 0.0f, factor[x][e] = __shfl_sync(0xFFFFFFFFu, row_factor[x], quad * 8 + e * 4);
 #pragma unroll
       for (int e = 0; e < 4; e++) least[x][e] = 0.0f;
 #pragma unroll
@@ -262,137 +328,145 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
 #pragma unroll
         for (int e = 0; e < 4; e++) o[x][i][e] = 0.0f;
     }
-    uint32_t room = 0x3C003C00u;  // 2^e that holds the values' scales so far, f16, twice
-    float shift = 15.0f;          // 15 - e
-    for (uint32_t blk = t.lo; blk < t.hi; blk++) {
+    uint32_t room = 16;  // the exponent field of 2^e as an f16 has it
+    for (uint32_t blk = b_lo; blk < b_hi; blk++) {
       {
-        const uint32_t number = next_entry;
-        next_entry = entry(blk + ST);
+        const Place at = next_place;
+        next_place = entry(blk + ST);
         __syncwarp();  // the chunk that lay in this stage has been read
-        issue(blk + ST - 1, number, stage == 0 ? ST - 1 : stage - 1);
+        issue(blk + ST - 1, at, stage == 0 ? ST - 1 : stage - 1);
       }
       const uint32_t base = ring + stage * S::CHUNK;
       stage = stage + 1 == ST ? 0 : stage + 1;
-      if (!wanted(blk)) continue;
       asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
       __syncwarp();
-      // ---- scores: s[x][T][e] of row x * 8 + eighth and token T * 8 + quad + 4 e
-      const uint32_t key0 = blk * KB + warp * 16, kscales = base + S::CODES, values = base + S::CODES + S::SCALES, vscales = values + S::CODES;
+      // ---- scores: s[x][T][e] of row x * 8 + quad * 2 + e and the token of slot T * 8 + eighth
+      const uint32_t kscales = base + S::CODES, values = base + S::CODES + S::SCALES, vscales = values + S::CODES;
       float s[NT][2][2];
       {
-        uint64_t part[NT][2];
+        uint32_t words[2][U], sc[2][G];
 #pragma unroll
         for (int T = 0; T < 2; T++) {
-          uint32_t words[U];
           const uint32_t row = base + (T * 8 + eighth) * (16 * U);
           if constexpr (U == 8) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
               const uint4 v = lds128(row + key_piece<U>(eighth, quad * 2 + i) * 16);
-              words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
+              words[T][4 * i] = v.x, words[T][4 * i + 1] = v.y, words[T][4 * i + 2] = v.z, words[T][4 * i + 3] = v.w;
             }
           } else {
-            lds_words<U>(row + quad * (4 * U), words);
+            lds_words<U>(row + quad * (4 * U), words[T]);
           }
-          uint32_t sc[2][G];  // scales and minima of the lane's two tokens
-          lds_words<G>(kscales + (T * 8 + quad * 2) * (4 * G), sc[0]);
-          lds_words<G>(kscales + (T * 8 + quad * 2 + 1) * (4 * G), sc[1]);
-          float mins[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          lds_words<G>(kscales + (T * 8 + eighth) * (4 * G), sc[T]);
+        }
+        float mins[NT][4];
 #pragma unroll
-          for (int b = 0; b < (G + 3) / 4; b++) {
-            const uint32_t w = b * 4 + quad < G ? lds32(kscales + (T * 8 + eighth) * (4 * G) + (b * 4 + quad) * 4) : 0u;
-            mma_f16(mins, qs[0][b][0], NT == 2 ? qs[NT - 1][b][0] : 0u, qs[0][b][1], NT == 2 ? qs[NT - 1][b][1] : 0u, w, w);
-          }
+        for (int b = 0; b < (G + 3) / 4; b++) {
+          uint32_t w[2];
 #pragma unroll
-          for (int g = 0; g < G; g++) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int u = g << GS; u < ((g + 1) << GS) && u < U; u++) {
-              const uint32_t w = words[u], v = w >> 8;
-              mma_f16(c, qf[0][u][0], NT == 2 ? qf[NT - 1][u][0] : 0u, qf[0][u][1], NT == 2 ? qf[NT - 1][u][1] : 0u, w & 0x000F000Fu, w & 0x00F000F0u);
-              mma_f16(c, qf[0][u][2], NT == 2 ? qf[NT - 1][u][2] : 0u, qf[0][u][3], NT == 2 ? qf[NT - 1][u][3] : 0u, v & 0x000F000Fu, v & 0x00F000F0u);
-            }
-            const uint64_t scale = pack2(__low2float(as_half2(sc[0][g])), __low2float(as_half2(sc[1][g])));
-#pragma unroll
-            for (int x = 0; x < NT; x++) {
-              const uint64_t v = pack2(c[2 * x], c[2 * x + 1]);
-              part[x][T] = g == 0 ? mul2(v, scale) : fma2(v, scale, part[x][T]);
-            }
-          }
+          for (int T = 0; T < 2; T++) w[T] = b * 4 + quad < G ? lds32(kscales + (T * 8 + eighth) * (4 * G) + (b * 4 + quad) * 4) : 0u;
 #pragma unroll
           for (int x = 0; x < NT; x++) {
-            const uint64_t million = pack2(1048576.0f, 1048576.0f);
-            unpack2(fma2(part[x][T], million, pack2(mins[2 * x], mins[2 * x + 1])), s[x][T][0], s[x][T][1]);
+            if (b == 0)
+              mma_f16_first(mins[x], w[0], w[1], w[0], w[1], qs[x][b][0], qs[x][b][1]);
+            else
+              mma_f16(mins[x], w[0], w[1], w[0], w[1], qs[x][b][0], qs[x][b][1]);
           }
         }
-      }
-      if (key0 + 15 > all_see || key0 < all_from) {
+        float part[NT][4];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          float c[NT][4];
+#pragma unroll
+          for (int u = g << GS; u < ((g + 1) << GS) && u < U; u++) {
+            const uint32_t w0 = words[0][u], w1 = words[1][u], v0 = w0 >> 8, v1 = w1 >> 8;
+#pragma unroll
+            for (int x = 0; x < NT; x++) {
+              if (u == g << GS)
+                mma_f16_first(c[x], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[x][u][0], qf[x][u][1]);
+              else
+                mma_f16(c[x], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[x][u][0], qf[x][u][1]);
+              mma_f16(c[x], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u, qf[x][u][2], qf[x][u][3]);
+            }
+          }
+          const float s0 = __low2float(as_half2(sc[0][g])), s1 = __low2float(as_half2(sc[1][g]));
+#pragma unroll
+          for (int x = 0; x < NT; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) part[x][e] = g == 0 ? c[x][e] * (e < 2 ? s0 : s1) : fmaf(c[x][e], e < 2 ? s0 : s1, part[x][e]);
+        }
 #pragma unroll
         for (int x = 0; x < NT; x++)
 #pragma unroll
-          for (int T = 0; T < 2; T++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const uint32_t at = key0 + T * 8 + quad + 4 * e;
-              if (!(at <= last[x] && (window == 0 || at + window > last[x]))) s[x][T][e] = -INFINITY;
-            }
+          for (int e = 0; e < 4; e++) s[x][e / 2][e % 2] = fmaf(part[x][e], 1048576.0f, mins[x][e]);
       }
-      // ---- values' scales of the lane's tokens, by pairs
-      uint32_t vs[2][G];
-      uint32_t most = 0;
+      if (blk - n_lo >= n_n) {
+        const uint32_t at = here(blk) * KB + w16 + (eighth >> 1) + (eighth & 1) * 4;
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint32_t last = t.past + t.token0 + min(x * 8 + quad * 2 + e, t.tokens * t.heads - 1) / t.heads;  // that the row sees
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+              if (!(at + T * 8 <= last && (window == 0 || at + T * 8 + window > last))) s[x][T][e] = -INFINITY;
+          }
+      }
+      // ---- values' scales of the lane's tokens of slots T * 8 + quad * 2 and the next, by pairs
+      uint32_t vs[2][G], any = 0;
 #pragma unroll
       for (int T = 0; T < 2; T++) {
         uint32_t sc[2][G];
         lds_words<G>(vscales + (T * 8 + quad * 2) * (4 * G), sc[0]);
         lds_words<G>(vscales + (T * 8 + quad * 2 + 1) * (4 * G), sc[1]);
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-          vs[T][g] = __byte_perm(sc[0][g], sc[1][g], 0x5410);
-          most = T == 0 && g == 0 ? vs[T][g] : as_u32(__hmax2(as_half2(most), as_half2(vs[T][g])));
-        }
+        for (int g = 0; g < G; g++) vs[T][g] = __byte_perm(sc[0][g], sc[1][g], 0x5410), any |= vs[T][g];
       }
       // ---- weights
-      float top[NT];
-      bool grows = __hgt2_mask(as_half2(most), as_half2(room)) != 0;
+      bool grows = (any & 0x40004000u) != 0;  // a scale of 2 or more
 #pragma unroll
-      for (int x = 0; x < NT; x++) {
-        top[x] = fmaxf(fmaxf(s[x][0][0], s[x][0][1]), fmaxf(s[x][1][0], s[x][1][1]));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xFFFFFFFFu, top[x], 1));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xFFFFFFFFu, top[x], 2));
-        top[x] = fmaxf(top[x] * factor[x], m[x]);
-        grows |= top[x] != m[x];
-      }
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) grows |= fmaxf(s[x][0][e], s[x][1][e]) > limit[x][e];
       if (__any_sync(0xFFFFFFFFu, grows)) {
-        // numbers that are not negative have the order of their bits
-        const uint32_t lane_most = max(most & 0x7FFFu, most >> 16 & 0x7FFFu), all_most = __reduce_max_sync(0xFFFFFFFFu, lane_most);
-        float wider = 1.0f;
-        if (all_most > (room & 0xFFFFu)) {
-          const uint32_t power = (all_most + 0x3FFu) & 0x7C00u;  // the next power of two
-          wider = __uint_as_float((127u + (room >> 10 & 31u) - (power >> 10)) << 23);
-          shift = 30.0f - (float)(power >> 10);
-          room = power | power << 16;
-        }
+        uint32_t most = 0;
 #pragma unroll
-        for (int x = 0; x < NT; x++) {
-          const float f = m[x] == -INFINITY ? 0.0f : exp2_approx(m[x] - top[x]) * wider;
-          l[x] *= f;
-          m[x] = top[x];
-          // the output's rows are others than the scores'
-          const float f0 = __shfl_sync(0xFFFFFFFFu, f, quad * 8), f1 = __shfl_sync(0xFFFFFFFFu, f, quad * 8 + 4);
+        for (int T = 0; T < 2; T++)
 #pragma unroll
-          for (int i = 0; i < S::TILES; i++) o[x][i][0] *= f0, o[x][i][1] *= f1, o[x][i][2] *= f0, o[x][i][3] *= f1;
-          least[x][0] *= f0, least[x][1] *= f1, least[x][2] *= f0, least[x][3] *= f1;
-        }
+          for (int g = 0; g < G; g++) most = max(most, max(here(vs[T][g]) & 0x7FFFu, here(vs[T][g]) >> 16 & 0x7FFFu));  // numbers that are not negative have the order of their bits
+        most = max((__reduce_max_sync(0xFFFFFFFFu, most) >> 10) + 1, room);  // the exponent of a power of two above them all
+        const float was = 30.0f - LAG4 - (float)room, shift = 30.0f - LAG4 - (float)most, wider = __uint_as_float((127u + room - most) << 23);
+        room = most;
+#pragma unroll
+        for (int x = 0; x < NT; x++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float top = fmaxf(s[x][0][e], s[x][1][e]);
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            top *= factor[x][e];
+            const bool first = limit[x][e] == -INFINITY;
+            const float m = less[x][e] + was, now = first ? top : fmaxf(top, m), f = first ? 0.0f : exp2_approx(m - now) * wider;
+            less[x][e] = now == -INFINITY ? 0.0f : now - shift;
+            limit[x][e] = now == -INFINITY ? now : (now + LAG4) / factor[x][e];
+            l[x][e] *= f;
+#pragma unroll
+            for (int i = 0; i < S::TILES; i++) o[x][i][e] *= f, o[x][i][2 + e] *= f;
+            least[x][e] *= f, least[x][2 + e] *= f;
+          }
       }
       uint32_t pf[NT][2];
 #pragma unroll
       for (int x = 0; x < NT; x++) {
-        const float less = m[x] == -INFINITY ? 0.0f : m[x] - shift;
-        float w[4];
+        float w[2][2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = exp2_approx(fmaf(s[x][i / 2][i % 2], factor[x], -less));
-        l[x] += (w[0] + w[1]) + (w[2] + w[3]);
-        pf[x][0] = Num<__half>::pack(w[0], w[1]), pf[x][1] = Num<__half>::pack(w[2], w[3]);
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+          for (int T = 0; T < 2; T++) w[T][e] = exp2_approx(fmaf(s[x][T][e], factor[x][e], -less[x][e]));
+          l[x][e] += w[0][e] + w[1][e];
+        }
+#pragma unroll
+        for (int T = 0; T < 2; T++) pf[x][T] = transposed(Num<__half>::pack(w[T][0], w[T][1]));
       }
       // ---- minima: row 2 g + 1 of the product (row g where a token's words are no whole 16 bytes) has group g's
       {
@@ -448,14 +522,18 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
     // ---- the warps' results: [warp][row] reference and sum, [warp][row][OP] output, where the rings were
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
+    const uint32_t rows = t.tokens * t.heads;
     float *const s_m = reinterpret_cast<float *>(smem), *const s_l = s_m + NW * R, *const s_o = s_l + NW * R;
 #pragma unroll
     for (int x = 0; x < NT; x++) {
-      float sum = l[x];
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-      const uint32_t r = x * 8 + eighth;
-      if (quad == 0 && r < rows) s_m[warp * R + r] = m[x] + P_SHIFT - shift, s_l[warp * R + r] = sum;  // the reference that the joins count with
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float sum = l[x][e];
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        const uint32_t r = x * 8 + quad * 2 + e;
+        if (eighth == 0 && r < rows) s_m[warp * R + r] = limit[x][e] == -INFINITY ? limit[x][e] : less[x][e] + P_SHIFT, s_l[warp * R + r] = sum;  // the reference that the joins count with
+      }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int g = u >> GS, at = G % 4 == 0 && g >= 4 ? 2 : 0, src = G % 4 == 0 ? (g % 4 * 2 + 1) * 4 : g * 4;
@@ -539,7 +617,7 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
 template <int U, int GS, int NT>
 cudaError_t launch_stream4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count, cudaStream_t s) {
   using S = Stream4Shape<U, GS, NT>;
-  const Attend4Params p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, S::R, ATTEND4_START, 1, 0, ATTEND4_WHOLE), ATTEND4_MIN_RUN, a.page_tokens % 16 == 0};
+  const Attend4Params p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, S::R, ATTEND4_START, 1, 0, ATTEND4_WHOLE), ATTEND4_MIN_RUN, (uint32_t)(kv.page_stride / 16), a.page_tokens % 16 == 0};
   const cudaError_t e = allow_smem<k_attend4<U, GS, NT>>(S::SMEM);
   if (e != cudaSuccess) return e;
   return launch_overlapped(k_attend4<U, GS, NT>, dim3(sm_count * S::CTAS), S::THREADS, S::SMEM, s, false, p);

@@ -6,21 +6,26 @@
 
 namespace {
 
-template <uint32_t KB>
-struct RunWalk {
-  const KvBatchDev &kv;
-  const TileShape &ts;
-  uint32_t window;
+// How far it has come.
+struct RunPlace {
   uint64_t left, at;  // units of the run that are left, and the next one's number
   SeqWork w;
   uint32_t seq, v_head, tile, from;  // from: what of the tile is not this run's (its first tile alone)
-  bool fresh = true;
+  bool fresh;
+};
 
-  __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, const RunStart &r)
-      : kv(kv_), ts(ts_), window(window_), w(r.w), seq(r.seq), v_head(r.v_head), tile(r.tile), from(r.from) {
+template <uint32_t KB>
+struct RunWalk : RunPlace {
+  const KvBatchDev &kv;
+  const TileShape &ts;
+  uint32_t window;
+
+  __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, const RunStart &r) : kv(kv_), ts(ts_), window(window_) {
+    w = r.w, seq = r.seq, v_head = r.v_head, tile = r.tile, from = r.from, fresh = true;
     at = run_first(r, blockIdx.x);
     left = r.total == 0 ? 0 : run_first(r, blockIdx.x + 1) - at;
   }
+  __device__ RunWalk(const KvBatchDev &kv_, const TileShape &ts_, uint32_t window_, const RunPlace &r) : RunPlace(r), kv(kv_), ts(ts_), window(window_) {}
   // The next tile of the run, or a part of one.
   __device__ bool next(TileWork *t) {
     do {

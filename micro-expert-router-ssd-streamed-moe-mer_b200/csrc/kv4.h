@@ -40,6 +40,7 @@ inline const char *kv4_pages_fault(const Kv4Shape &s, uint32_t page_tokens, uint
   if ((page_stride | head_stride) % 16) return "page and head strides must be multiples of 16 bytes";
   const uint64_t block = kv4_block_bytes(s, page_tokens), most = 1ull << 47;
   if ((kv_heads > 1 && head_stride < block) || (n_pages > 1 && page_stride < block)) return "a stride is smaller than a head's block";
+  if (page_stride >> 36 || head_stride >> 36) return "pages or heads lie 64 GB or more apart";
   if ((n_pages > 1 && page_stride > most / (n_pages - 1)) || (kv_heads > 1 && head_stride > most / (kv_heads - 1))) return "keys or values reach over more than 2^47 bytes";
   return nullptr;
 }

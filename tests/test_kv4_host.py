@@ -70,5 +70,8 @@ def test_pages_that_are_refused(rules):
         assert b"multiples" in ask(**kw)
     for kw in (dict(page_stride=block - 16), dict(head_stride=block - 16), dict(head_stride=0)):
         assert b"smaller" in ask(**kw)
-    for kw in (dict(page_stride=1 << 45), dict(head_stride=1 << 46), dict(page_stride=(1 << 64) - 16), dict(head_stride=(1 << 64) - 16), dict(n=0xFFFFFFFF, page_stride=1 << 20)):
+    for kw in (dict(page_stride=1 << 36), dict(head_stride=1 << 46), dict(page_stride=(1 << 64) - 16), dict(head_stride=(1 << 64) - 16)):
+        assert b"64 GB" in ask(**kw)
+    assert ask(n=3, page_stride=(1 << 36) - 16) is None
+    for kw in (dict(n=0xFFFFFFFF, page_stride=1 << 20), dict(n=4000, page_stride=(1 << 36) - 16), dict(heads=4000, head_stride=(1 << 36) - 16)):
         assert b"2^47" in ask(**kw)
