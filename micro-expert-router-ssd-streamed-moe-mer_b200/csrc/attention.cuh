@@ -141,7 +141,8 @@ __device__ RunStart find_run(const KvBatchDev &kv, const TileShape &ts, uint32_t
 // Where a row of the batch stands, found by a whole warp.  The row's sequence is the last one that starts at the row or before it: the lanes read all starts and
 // lengths in one round trip.
 struct RowPlace {
-  uint32_t seq, pos;       // pos: ~0 where its sequence has no place for the row
+  uint32_t seq, first;     // first: the token that the row is, ~0 where its sequence has not so many
+  uint32_t pos;            // the same, ~0 also where the token's page is not there
   uint32_t page, in_page;  // of a row that has one
   uint32_t end;            // the batch's row behind the sequence's last one
 };
@@ -164,9 +165,10 @@ __device__ __forceinline__ bool find_row(const KvBatchDev &kv, uint32_t page_tok
   const uint32_t from = __ffs(__ballot_sync(0xFFFFFFFFu, seq == last)) - 1;
   end = min(__shfl_sync(0xFFFFFFFFu, end, from), kv.n_rows), len = __shfl_sync(0xFFFFFFFFu, len, from);
   if (row >= end) return false;  // behind the last sequence
-  found->seq = last - 1, found->end = end, found->pos = 0xFFFFFFFFu;
+  found->seq = last - 1, found->end = end, found->first = found->pos = 0xFFFFFFFFu;
   const uint32_t behind = end - row;  // this row and those after it: 1 for the newest
   if (behind <= len) {
+    found->first = len - behind;
     const uint32_t slot = divided(len - behind, kv.page_tokens);
     const uint32_t page = slot < kv.table_stride ? kv.page_table[(uint64_t)(last - 1) * kv.table_stride + slot] : 0xFFFFFFFFu;
     if (page < kv.n_pages) found->pos = len - behind, found->page = page, found->in_page = found->pos - slot * page_tokens;

@@ -2,31 +2,32 @@
 //
 //   16-bit cache: the value itself;  4 bits: scale * code + minimum, one fma in fp32 (the product has 15 bits);  one rounding to the rows' type.
 //
-// What bounds it: memory.  A lane has eight neighbouring values of a head (a word of codes and its group's scale and minimum in, one or two 16-byte vectors out); a
-// warp takes some rows one behind the other, which mostly follow one another in a sequence, so that their place is looked up once and their pages' numbers are one load.
+// What bounds it: memory.  A lane has a part of a token's head that is one piece of its bytes: four units' words of a key or a value (32 values of a head of 128; its scales are
+// one vector more), or eight 16-bit values.  A warp takes some rows one behind the other, which mostly follow one another in a sequence, so that their place is
+// looked up once and their pages' numbers are one load; the lanes share out the rows' parts, and the loads of two parts are in flight before the first is stored.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "kernels.h"
+#include "kv4_unpack.cuh"
 #include "ptx.cuh"
 
 namespace {
 
-constexpr uint32_t READ_THREADS = 128;
-constexpr int READ_AT_ONCE = 4;  // items of a lane in flight
+constexpr uint32_t READ_THREADS = 128, READ_ROWS = 8;
 
 struct ReadParams {
   AttnLayer a;
   KvBatchDev kv;
   KvRowsDev r;
   uint32_t *status;
-  uint32_t rows;      // of a warp, at most 32
-  uint32_t pieces;    // eights of a head
-  FastDiv by_pieces;
-  uint32_t items;     // of a row: keys, then values
-  bool vec;           // rows are whole vectors of 16 bytes
+  uint32_t rows;   // of a warp, at most 32
+  uint32_t parts;  // of a head
+  FastDiv by_parts;
+  bool vec;        // rows are whole vectors of 16 bytes
 };
 
 template <typename OUT>
@@ -45,110 +46,178 @@ __device__ __forceinline__ void store_eight(OUT *p, const float (&x)[8], bool ve
   for (int i = 0; i < 8; i++) p[i] = Num<OUT>::one(x[i]);
 }
 
-// CACHE: the pages' type, or uint8_t where they hold 4 bits.
-template <typename CACHE, typename OUT>
-__global__ void __launch_bounds__(READ_THREADS) k_kv_read(const ReadParams p) {
-  constexpr bool Q4 = sizeof(CACHE) == 1;
-  const AttnLayer &a = p.a;
-  const Kv4Shape &f = a.kv4;
-  const uint32_t lane = threadIdx.x & 31, warp = blockIdx.x * (READ_THREADS / 32) + threadIdx.x / 32;
-  grid_dep_wait();
-  grid_dep_launch();
-  const uint64_t row0 = (uint64_t)warp * p.rows;
-  if (row0 >= p.kv.n_rows) return;
-  const uint32_t behind = (uint32_t)min((uint64_t)p.kv.n_rows, row0 + p.rows), per_part = a.kv_heads * p.pieces;
-  RowPlace at;
-  at.end = 0;
-  uint32_t numbers = 0, first = 0;  // the lanes have the page numbers of the rows from `first` on
-  for (uint32_t row = (uint32_t)row0; row < behind; row++) {
-    bool placed = row < at.end;  // the same sequence as the row before
-    if (!placed) {
-      if (!find_row(p.kv, a.page_tokens, row, lane, &at)) continue;
-      first = row;
-      if (at.pos != 0xFFFFFFFFu) {
-        const uint32_t slot = divided(at.pos + lane, p.kv.page_tokens);
-        numbers = row + lane < min(at.end, behind) && slot < p.kv.table_stride ? p.kv.page_table[(uint64_t)at.seq * p.kv.table_stride + slot] : 0xFFFFFFFFu;
-      } else {
-        at.end = row + 1;  // the next row is looked up again: it may have a place
-      }
-    }
-    uint32_t page = 0xFFFFFFFFu, in_page = 0;
-    if (at.pos != 0xFFFFFFFFu) {
-      const uint32_t pos = at.pos + (row - first);
-      page = __shfl_sync(0xFFFFFFFFu, numbers, row - first);
-      in_page = pos - divided(pos, p.kv.page_tokens) * a.page_tokens;
-    }
-    const bool held = page < p.kv.n_pages;
-    if (!held && lane == 0) atomicOr(p.status, MER_DEVSTAT_BAD_CACHE);
-    for (uint32_t i0 = lane; i0 < p.items; i0 += 32 * READ_AT_ONCE) {
-      float x[READ_AT_ONCE][8];
-      OUT *dst[READ_AT_ONCE];
-      uint4 raw[READ_AT_ONCE];
-      uint32_t scale_min[READ_AT_ONCE];
-      bool key[READ_AT_ONCE];
+// Eight codes: of a word of a key, pair i from bits 4 i and 16 + 4 i on; of two words of a value, the same bits of the first half and of the second are values i and i + 4.
+__device__ __forceinline__ void eight_codes(uint32_t w, __half2 (&n)[4]) {
+  const __half2 whole = as_half2(0x64006400u), sixteenth = as_half2(0x2C002C00u), back = as_half2(0xD400D400u);  // 1024, 1 / 16, -64
+  const uint32_t v = w >> 8;
+  n[0] = __hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), whole), n[1] = __hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), sixteenth, back);
+  n[2] = __hsub2(as_half2((v & 0x000F000Fu) | 0x64006400u), whole), n[3] = __hfma2(as_half2((v & 0x00F000F0u) | 0x64006400u), sixteenth, back);
+}
+
+// N words from an address on a multiple of 4 N (at most 16) bytes.
+template <int N>
+__device__ __forceinline__ void load_words(const char *p, uint32_t (&w)[N]) {
 #pragma unroll
-      for (int n = 0; n < READ_AT_ONCE; n++) {
-        const uint32_t i = i0 + n * 32;
-        key[n] = i < per_part;
-        const uint32_t e = key[n] ? i : i - per_part, head = divided(e, p.by_pieces), piece = e - head * p.pieces;
-        OUT *rows = (OUT *)(key[n] ? p.r.k : p.r.v);
-        dst[n] = i < p.items && rows ? rows + row * (key[n] ? p.r.k_stride : p.r.v_stride) + head * a.head_dim + piece * 8 : nullptr;
-        raw[n] = make_uint4(0, 0, 0, 0), scale_min[n] = 0;
-        if (!dst[n] || !held) continue;
-        const char *pages = (const char *)(key[n] ? p.kv.k_pages : p.kv.v_pages);
-        if constexpr (Q4) {
-          const char *block = pages + page * p.kv.page_stride + head * p.kv.head_stride;
-          const char *codes = block + (uint64_t)in_page * f.token_bytes();
-          const uint32_t u = piece / 4, j = piece % 4;
-          if (key[n]) {
-            raw[n].x = *reinterpret_cast<const uint32_t *>(codes + (j * f.units + u) * 4);
-          } else {
-            raw[n].x = *reinterpret_cast<const uint16_t *>(codes + (2 * j * f.units + u) * 2);
-            raw[n].y = *reinterpret_cast<const uint16_t *>(codes + ((2 * j + 1) * f.units + u) * 2);
-          }
-          scale_min[n] = *reinterpret_cast<const uint32_t *>(block + f.codes + (uint64_t)in_page * f.scale_bytes() + piece * 8 / f.group * 4);
-        } else {
-          raw[n] = *reinterpret_cast<const uint4 *>((const CACHE *)pages + page * p.kv.page_stride + (uint64_t)in_page * p.kv.token_stride + head * p.kv.head_stride + piece * 8);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < READ_AT_ONCE; n++) {
-        if constexpr (Q4) {
-          const __half2 h = *reinterpret_cast<const __half2 *>(&scale_min[n]);
-          const float scale = __low2float(h), least = __high2float(h);
-#pragma unroll
-          for (int v = 0; v < 8; v++) {
-            const uint32_t code = key[n] ? raw[n].x >> (v / 2 * 4 + v % 2 * 16) & 15 : (v < 4 ? raw[n].x : raw[n].y) >> (v % 4 * 4) & 15;
-            x[n][v] = fmaf(scale, (float)code, least);
-          }
-        } else {
-          const CACHE *t = reinterpret_cast<const CACHE *>(&raw[n]);
-#pragma unroll
-          for (int v = 0; v < 8; v++) x[n][v] = Num<CACHE>::f(t[v]);
-        }
-        if (dst[n]) store_eight<OUT>(dst[n], x[n], p.vec);
-      }
+  for (int i = 0; i < N; i += N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1) {
+    if constexpr (N % 4 == 0) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(p + i * 4);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    } else if constexpr (N % 2 == 0) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(p + i * 4);
+      w[i] = v.x, w[i + 1] = v.y;
+    } else {
+      w[i] = *reinterpret_cast<const uint32_t *>(p + i * 4);
     }
   }
 }
 
-template <typename CACHE>
+// A part of a token's head on its way: U units' words of a cache of 4 bits, or (U == 0) eight 16-bit values.
+template <typename CACHE, int U>
+struct Part {
+  uint32_t words[U ? U : 4], scales[U ? U : 1];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t &w : words) w = 0;
+#pragma unroll
+    for (uint32_t &w : scales) w = 0;
+  }
+  // `token`: the first of the head's bytes of the token; part `j`
+  __device__ __forceinline__ void load(const char *token, const char *token_scales, uint32_t j, bool wide) {
+    if constexpr (U == 0) {
+      load_words<4>(token + j * 16, words);
+    } else {
+      load_words<U>(token + j * (4 * U), words);
+      if (wide) {
+        uint32_t g[(U + 1) / 2];
+        load_words<(U + 1) / 2>(token_scales, g);
+#pragma unroll
+        for (int u = 0; u < U; u++) scales[u] = g[u / 2];
+      } else {
+        load_words<U>(token_scales, scales);
+      }
+    }
+  }
+  template <typename OUT>
+  __device__ __forceinline__ void store(OUT *head, uint32_t j, uint32_t head_dim, bool key, bool vec) const {
+    float x[8];
+    if constexpr (U == 0) {
+      const CACHE *const t = reinterpret_cast<const CACHE *>(words);
+#pragma unroll
+      for (int v = 0; v < 8; v++) x[v] = Num<CACHE>::f(t[v]);
+      store_eight<OUT>(head + j * 8, x, vec);
+    } else {
+      // words u of 16 bits of a value's rows 2 j and 2 j + 1 are the halves u and U + u of the part
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (u * 32 + j * 8 >= head_dim) break;
+        const float scale = __low2float(as_half2(scales[u])), least = __high2float(as_half2(scales[u]));
+        const uint32_t w = key ? words[u] : __byte_perm(words[u / 2], words[(U + u) / 2], (u % 2 ? 0x32u : 0x10u) | ((U + u) % 2 ? 0x7600u : 0x5400u));
+        __half2 code[4];
+        eight_codes(w, code);
+        float y[4][2];
+#pragma unroll
+        for (int v = 0; v < 4; v++) y[v][0] = fmaf(scale, __low2float(code[v]), least), y[v][1] = fmaf(scale, __high2float(code[v]), least);
+#pragma unroll
+        for (int v = 0; v < 8; v++) x[v] = key ? y[v / 2][v % 2] : y[v % 4][v / 4];
+        store_eight<OUT>(head + u * 32 + j * 8, x, vec);
+      }
+    }
+  }
+};
+
+// CACHE: the pages' type where they hold 16 bits (U == 0).
+template <typename CACHE, int U, typename OUT>
+__global__ void __launch_bounds__(READ_THREADS) k_kv_read(const __grid_constant__ ReadParams p) {
+  const Kv4Shape &f = p.a.kv4;
+  const uint32_t lane = threadIdx.x & 31, warp = blockIdx.x * (READ_THREADS / 32) + threadIdx.x / 32;
+  grid_dep_wait();
+  grid_dep_launch();
+  const uint64_t first = (uint64_t)warp * p.rows;
+  if (first >= p.kv.n_rows) return;
+  const uint32_t row0 = (uint32_t)first, n_rows = min(p.rows, p.kv.n_rows - row0);
+  // Lane r has row r's page and the token in it; ~0: none, zeros, ~1: the row belongs to no sequence.
+  uint32_t page = 0xFFFFFFFFu, in_page = 0;
+  for (uint32_t r = 0; r < n_rows;) {
+    RowPlace at;
+    if (!find_row(p.kv, p.a.page_tokens, row0 + r, lane, &at)) {
+      if (lane == r++) page = 0xFFFFFFFEu;
+      continue;
+    }
+    // Rows r .. last of its sequence have a place if the first one has; one without is looked up alone.
+    const uint32_t last = at.first == 0xFFFFFFFFu ? r + 1 : min(n_rows, at.end - row0);
+    if (at.first != 0xFFFFFFFFu && lane >= r && lane < last) {
+      const uint32_t pos = at.first + (lane - r), slot = divided(pos, p.kv.page_tokens);
+      const uint32_t number = slot < p.kv.table_stride ? p.kv.page_table[(uint64_t)at.seq * p.kv.table_stride + slot] : 0xFFFFFFFFu;
+      page = number < p.kv.n_pages ? number : 0xFFFFFFFFu;
+      in_page = pos - slot * p.a.page_tokens;
+    }
+    r = last;
+  }
+  if (lane < n_rows && page == 0xFFFFFFFFu) atomicOr(p.status, MER_DEVSTAT_BAD_CACHE);
+  // Item e of the warp's: part e % parts of head (e / parts) % kv_heads of the keys, then of the values, of the rows one behind the other.
+  const uint32_t per_row = 2 * p.a.kv_heads * p.parts, items = n_rows * per_row;
+  uint32_t key_or_value, head, j, row = 0, e = lane;  // of the item; rows are counted, not divided
+  const auto locate = [&](uint32_t in_row) {
+    const uint32_t h = divided(in_row, p.by_parts);
+    j = in_row - h * p.parts;
+    key_or_value = h >= p.a.kv_heads, head = key_or_value ? h - p.a.kv_heads : h;
+  };
+  uint32_t in_row = lane;
+  for (; e - lane < items; e += 64) {
+    Part<CACHE, U> part[2];
+    OUT *dst[2];
+    uint32_t js[2];
+    bool keys[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      while (in_row >= per_row) in_row -= per_row, row++;
+      const uint32_t number = __shfl_sync(0xFFFFFFFFu, page, row & 31), in = __shfl_sync(0xFFFFFFFFu, in_page, row & 31);
+      locate(in_row);
+      js[b] = j, keys[b] = !key_or_value;
+      OUT *const rows = (OUT *)(key_or_value ? p.r.v : p.r.k);
+      dst[b] = row < n_rows && number != 0xFFFFFFFEu && rows ? rows + (uint64_t)(row0 + row) * (key_or_value ? p.r.v_stride : p.r.k_stride) + head * p.a.head_dim : nullptr;
+      part[b].clear();
+      if (dst[b] && number != 0xFFFFFFFFu) {
+        const char *const pages = (const char *)(key_or_value ? p.kv.v_pages : p.kv.k_pages);
+        if constexpr (U != 0) {
+          const char *const block = pages + number * p.kv.page_stride + head * p.kv.head_stride;
+          part[b].load(block + in * (16 * U), block + f.codes + in * f.scale_bytes(), j, f.group == 64);
+        } else {
+          part[b].load(pages + (number * p.kv.page_stride + in * p.kv.token_stride + head * p.kv.head_stride) * sizeof(CACHE), nullptr, j, false);
+        }
+      }
+      in_row += 32;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+      if (dst[b]) part[b].store(dst[b], js[b], p.a.head_dim, keys[b], p.vec);
+  }
+}
+
+template <typename CACHE, int U>
 cudaError_t launch_read(const ReadParams &p, uint32_t grid, cudaStream_t s) {
-  return p.r.type == MER_VALUE_F32   ? launch_overlapped(k_kv_read<CACHE, float>, dim3(grid), READ_THREADS, 0, s, false, p)
-         : p.r.type == MER_VALUE_F16 ? launch_overlapped(k_kv_read<CACHE, __half>, dim3(grid), READ_THREADS, 0, s, false, p)
-                                     : launch_overlapped(k_kv_read<CACHE, __nv_bfloat16>, dim3(grid), READ_THREADS, 0, s, false, p);
+  return p.r.type == MER_VALUE_F32   ? launch_overlapped(k_kv_read<CACHE, U, float>, dim3(grid), READ_THREADS, 0, s, false, p)
+         : p.r.type == MER_VALUE_F16 ? launch_overlapped(k_kv_read<CACHE, U, __half>, dim3(grid), READ_THREADS, 0, s, false, p)
+                                     : launch_overlapped(k_kv_read<CACHE, U, __nv_bfloat16>, dim3(grid), READ_THREADS, 0, s, false, p);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_read(const AttnLayer &a, const KvBatchDev &kv, const KvRowsDev &r, uint32_t *status, int sm_count, cudaStream_t s) {
   ReadParams p{a, kv, r, status};
-  p.pieces = a.head_dim / 8, p.by_pieces = fast_div(p.pieces), p.items = 2 * a.kv_heads * p.pieces;
+  p.parts = a.q4 ? 4 : a.head_dim / 8, p.by_parts = fast_div(p.parts);
   const uint32_t size = r.type == MER_VALUE_F32 ? 4 : 2;
   p.vec = ((uintptr_t)r.k | (uintptr_t)r.v | (r.k ? r.k_stride * size : 0) | (r.v ? r.v_stride * size : 0)) % 16 == 0;
   // Rows of a warp: several where there are more than fill the machine.
-  p.rows = (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, kv.n_rows / ((uint64_t)sm_count * 32)));
-  const uint64_t warps = ((uint64_t)kv.n_rows + p.rows - 1) / p.rows, ctas = (warps + READ_THREADS / 32 - 1) / (READ_THREADS / 32);
-  const uint32_t grid = (uint32_t)ctas;  // below 2^31: n_rows is
-  return a.cache_type == MER_VALUE_F16 && !a.q4 ? launch_read<__half>(p, grid, s) : !a.q4 ? launch_read<__nv_bfloat16>(p, grid, s) : launch_read<uint8_t>(p, grid, s);
+  p.rows = (uint32_t)std::min<uint64_t>(READ_ROWS, std::max<uint64_t>(1, kv.n_rows / ((uint64_t)sm_count * 32)));
+  const uint64_t warps = ((uint64_t)kv.n_rows + p.rows - 1) / p.rows;
+  const uint32_t grid = (uint32_t)((warps + READ_THREADS / 32 - 1) / (READ_THREADS / 32));  // below 2^31: n_rows is
+  if (!a.q4) return a.cache_type == MER_VALUE_F16 ? launch_read<__half, 0>(p, grid, s) : launch_read<__nv_bfloat16, 0>(p, grid, s);
+  switch (a.kv4.units) {
+    case 2: return launch_read<uint8_t, 2>(p, grid, s);
+    case 3: return launch_read<uint8_t, 3>(p, grid, s);
+    case 4: return launch_read<uint8_t, 4>(p, grid, s);
+    case 6: return launch_read<uint8_t, 6>(p, grid, s);
+    default: return launch_read<uint8_t, 8>(p, grid, s);
+  }
 }
