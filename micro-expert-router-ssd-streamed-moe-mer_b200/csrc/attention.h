@@ -58,6 +58,9 @@ struct QkvRowsDev {
 // kernels_kv.cu
 cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const QkvRowsDev &rows, uint32_t *status, int sm_count, cudaStream_t s);
 
+// kernels_kv4.cu: the same for a cache of 4 bits
+cudaError_t launch_kv4_append(const AttnLayer &a, const KvBatchDev &kv, const QkvRowsDev &rows, uint32_t *status, int sm_count, cudaStream_t s);
+
 // Rows that keys and values are read back to; either may be null.
 struct KvRowsDev {
   void *k, *v;

@@ -20,6 +20,7 @@
 
 #include "attention.cuh"
 #include "kernels.h"
+#include "kv_rows.cuh"
 #include "pack2.cuh"
 #include "ptx.cuh"
 
@@ -27,46 +28,6 @@ namespace {
 
 constexpr int AHEAD = 3;          // steps whose values a warp has asked for (2: 60.3 us, 4: 61.0, where registers cost warps)
 
-// V values as they lie in memory.
-template <typename T, int V>
-struct Raw {
-  static constexpr int BYTES = sizeof(T) * V;
-  __align__(16) T t[V];
-  __device__ __forceinline__ void load(const T *p) {
-    if constexpr (BYTES % 16 == 0) {
-#pragma unroll
-      for (int i = 0; i < BYTES / 16; i++) reinterpret_cast<uint4 *>(t)[i] = *(reinterpret_cast<const uint4 *>(p) + i);
-    } else if constexpr (BYTES == 8) {
-      reinterpret_cast<uint2 *>(t)[0] = *reinterpret_cast<const uint2 *>(p);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i++) t[i] = p[i];
-    }
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < BYTES / 2; i++) reinterpret_cast<uint16_t *>(t)[i] = 0;
-  }
-  __device__ __forceinline__ void get(float (&x)[V]) const {
-#pragma unroll
-    for (int i = 0; i < V; i++) x[i] = Num<T>::f(t[i]);
-  }
-};
-template <typename T, int V>
-__device__ __forceinline__ void store_vec(T *p, const float (&x)[V]) {
-  if constexpr (V % 2 == 0) {
-    uint32_t t[V / 2];
-#pragma unroll
-    for (int i = 0; i < V / 2; i++) t[i] = Num<T>::pack(x[2 * i], x[2 * i + 1]);
-    if constexpr (V == 8)
-      *reinterpret_cast<uint4 *>(p) = make_uint4(t[0], t[1], t[2], t[3]);
-    else
-      *reinterpret_cast<uint2 *>(p) = make_uint2(t[0], t[1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) p[i] = Num<T>::one(x[i]);
-  }
-}
 // a[i] * b[i], two at a time.
 template <int V>
 __device__ __forceinline__ void times(float (&a)[V], const float (&b)[V]) {
@@ -106,28 +67,14 @@ struct KvParams {
   uint32_t q_steps, kv_steps; // steps of 32 / group heads
   uint32_t chunks, each;      // warps of a row, and steps of each
   float per_value;            // 1 / head_dim
-  // A cache of 4 bits: the warps above have the queries alone, keys and values are those of kv4_append.
-  uint32_t kv4_lanes;             // of a head, a power of two
-  uint32_t kv4_steps, kv4_each;   // steps of 32 / kv4_lanes heads for the keys, and as many for the values; of a warp
-  uint32_t kv4_chunks;            // warps of a row
-  bool kv4_vec;                   // rows by vectors of 8 values
 };
 
-#include "kv4_append.cuh"
-
-// IN: the rows' type, OUT: the cache's and q_out's, V: values of a vector, Q4: the cache holds 4 bits.
-template <typename IN, typename OUT, int V, bool Q4>
+// IN: the rows' type, OUT: the cache's and q_out's, V: values of a vector.
+template <typename IN, typename OUT, int V>
 __global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
-  extern __shared__ __align__(16) float2 turns[];  // [rope_dims / 2] cosine and sine
+  extern __shared__ float2 turns[];  // [rope_dims / 2] cosine and sine
   const AttnLayer &a = p.a;
-  const uint32_t warps = Q4 ? p.chunks + p.kv4_chunks : p.chunks;
-  const uint32_t lane = threadIdx.x, row = blockIdx.x / warps, chunk = blockIdx.x - row * warps;
-  if constexpr (Q4) {
-    if (chunk >= p.chunks) {
-      kv4_append<IN>(p, row, chunk - p.chunks, reinterpret_cast<double2 *>(turns));
-      return;
-    }
-  }
+  const uint32_t lane = threadIdx.x, row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
   const uint32_t D = a.head_dim, half = a.rope_dims / 2, sub = lane & (p.group - 1), of = lane / p.group, heads = 32 / p.group;
   // Pair m of a head's vectors.  Behind the rotated values neighbours pair up, of which the last may have no second.
   constexpr int STEPS = V == 1 ? 4 : 1;  // V == 1: 32 lanes take up to 4 pairs each
@@ -286,16 +233,9 @@ __global__ void __launch_bounds__(32) k_kv_append(const KvParams p) {
   }
 }
 
-// Whether `v` values of `size` bytes from `p`, `stride` apart, can be moved as one vector.
-bool vec_ok(const void *p, uint64_t stride, uint32_t v, uint32_t size) {
-  const uint32_t bytes = v * size < 16 ? v * size : 16;
-  return p == nullptr || ((uintptr_t)p % bytes == 0 && stride * size % bytes == 0);
-}
-
 template <typename IN, typename OUT, int V>
 cudaError_t launch_kv(KvParams &p, dim3 grid, size_t smem, cudaStream_t s) {
-  return p.a.q4 ? launch_overlapped(k_kv_append<IN, OUT, V, true>, grid, 32, smem, s, false, p)
-                : launch_overlapped(k_kv_append<IN, OUT, V, false>, grid, 32, smem, s, false, p);
+  return launch_overlapped(k_kv_append<IN, OUT, V>, grid, 32, smem, s, false, p);
 }
 template <typename IN, typename OUT>
 cudaError_t launch_kv(KvParams &p, uint32_t v, dim3 grid, size_t smem, cudaStream_t s) {
@@ -311,7 +251,8 @@ cudaError_t launch_kv(KvParams &p, uint32_t v, dim3 grid, size_t smem, cudaStrea
 }  // namespace
 
 cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const QkvRowsDev &r, uint32_t *status, int sm_count, cudaStream_t s) {
-  KvParams p{a, kv, r, status, 1, 0, 0, 1, 0, 1.0f / (float)a.head_dim, 1, 0, 0, 0, false};
+  if (a.q4) return launch_kv4_append(a, kv, r, status, sm_count, s);
+  KvParams p{a, kv, r, status, 1, 0, 0, 1, 0, 1.0f / (float)a.head_dim};
   const uint32_t in = r.type == MER_VALUE_F32 ? 4 : 2;
   // The widest vector up to 16 bytes that neither a rotated pair nor an address cuts.  (Eight fp32 values a vector: 24652 rows of 8 + 2 heads of 128 61 us,
   // 50 so, with 72 registers instead of 121; four f16 values: 13411 rows of 32 + 2 * 8 heads 83 us, 57 with eight.)
@@ -325,27 +266,13 @@ cudaError_t launch_kv_append(const AttnLayer &a, const KvBatchDev &kv, const Qkv
   while (p.group < pairs && p.group < 32) p.group *= 2;
   const uint32_t heads = 32 / p.group;
   p.q_steps = (a.q_heads + heads - 1) / heads, p.kv_steps = (a.kv_heads + heads - 1) / heads;
-  if (a.q4) {
-    p.q_steps = r.q ? p.q_steps : 0, p.kv_steps = 0;
-    while (p.kv4_lanes < 4 * a.kv4.units) p.kv4_lanes *= 2;
-    p.kv4_steps = (a.kv_heads + 32 / p.kv4_lanes - 1) / (32 / p.kv4_lanes);
-    p.kv4_vec = vec_ok(r.k, r.k_stride, 8, in) && vec_ok(r.v, r.v_stride, 8, in) && (a.rope_pairs || a.rope_dims % 16 == 0);
-  }
   // A warp a row, and more of them while there are fewer than 16 an SM: fewer steps one after the other.
-  const auto split = [&](uint32_t steps, uint32_t *chunks, uint32_t *each) {
-    *chunks = (uint32_t)std::min<uint64_t>(steps, std::max<uint64_t>(1, (uint64_t)sm_count * 16 / kv.n_rows));
-    *each = *chunks ? (steps + *chunks - 1) / *chunks : 0;
-    *chunks = *each ? (steps + *each - 1) / *each : 0;
-  };
-  split(p.q_steps + 2 * p.kv_steps, &p.chunks, &p.each);
-  size_t smem = (size_t)(a.rope_dims / 2) * sizeof(float2);
-  if (a.q4) {
-    split(2 * p.kv4_steps, &p.kv4_chunks, &p.kv4_each);
-    smem = (size_t)(a.rope_dims / 2) * sizeof(double2);
-  }
-  // more than a warp or two a row only where rows are few; the grid's x goes up to 2^31 - 1
-  if ((uint64_t)kv.n_rows * (p.chunks + p.kv4_chunks) > 0x7FFFFFFFu) return cudaErrorInvalidValue;
-  const dim3 grid(kv.n_rows * (p.chunks + p.kv4_chunks));
+  const uint32_t steps = p.q_steps + 2 * p.kv_steps;
+  p.chunks = (uint32_t)std::min<uint64_t>(steps, std::max<uint64_t>(1, (uint64_t)sm_count * 16 / kv.n_rows));
+  p.each = (steps + p.chunks - 1) / p.chunks;
+  p.chunks = (steps + p.each - 1) / p.each;
+  const dim3 grid(kv.n_rows * p.chunks);  // one row's warps only where rows are few: below 2^31
+  const size_t smem = (size_t)(a.rope_dims / 2) * sizeof(float2);
   return r.type == MER_VALUE_F32   ? launch_kv<float>(p, v, grid, smem, s)
          : r.type == MER_VALUE_F16 ? launch_kv<__half>(p, v, grid, smem, s)
                                    : launch_kv<__nv_bfloat16>(p, v, grid, smem, s);
