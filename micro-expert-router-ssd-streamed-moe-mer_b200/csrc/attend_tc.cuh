@@ -7,7 +7,7 @@
 //   O[128 x d] += P[128 x 128] V[128 x d]       P from tensor memory, where it takes the place of S; V's rows run along N
 //
 //   * Warps 0..3 and 4..7 are the softmax of one group of rows each, warps 8..11 copy, warp 12 issues the MMAs, warp 13 goes ahead through the run and leaves
-//     the next tile's place in shared memory (14 and 15 fill the group).  While one group's
+//     the next tile's place in shared memory (14 and 15 fill the group, or unpack with the copying warps where the cache holds 4 bits).  While one group's
 //     softmax runs the tensor core multiplies for the other: [P V of block j, Q K of block j + 1] of one, then of the other.
 //   * A tile of up to 128 rows (single tokens, drafts) has one group of rows; the two take its blocks in turn and their results are joined at its end, so that it is
 //     read as fast as two groups of rows would be multiplied.
@@ -65,7 +65,7 @@ struct TcMaps {
 };
 
 constexpr uint32_t TC_KB = 128, TC_WARPS = 16, TC_THREADS = TC_WARPS * 32, SOFT_THREADS = 256;
-constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12, TC_WALK = 13, TILE_USERS = 13;  // the warps that work on a tile
+constexpr uint32_t TC_LOAD = 8, TC_LOADERS = 4, TC_MMA = 12, TC_WALK = 13;
 // Registers of a thread: the launch's 128 times 512 threads, as 192 for the two softmax groups of four warps and 64 for the two others.
 constexpr uint32_t SOFT_REGS = 192, OTHER_REGS = 64;
 static_assert(2 * SOFT_REGS + 2 * OTHER_REGS == 4 * 128, "what one takes the others give");
@@ -84,15 +84,17 @@ struct TcShape {
   static constexpr uint32_t STAGE = SUBS * TC_KB * 128;    // keys or values of a block
   static constexpr bool WIDE = DP == 256;                  // one group of rows, whose outputs take as much tensor memory as two groups' of 128 values
   static constexpr uint32_t R = WIDE ? 128 : 256;          // rows of a tile
-  static constexpr uint32_t STAGES = DP == 256 ? 2 : DP == 128 ? (U ? 3 : 5) : U ? 8 : 10;
+  static constexpr uint32_t STAGES = DP == 256 ? 2 : DP == 128 ? (U ? 4 : 5) : U ? 8 : 10;
   static constexpr uint32_t QSUB = R * 128;              // 64 values of all queries of a tile
   // What has been asked for of a cache of 4 bits, by each of the copying warps for itself: RAW steps of RAW_ROWS tokens, each its codes and its scales in
   // RAW_STRIDE bytes, an odd number of 16, so that eight lanes' rows lie in different banks.
   static constexpr uint32_t HALVES = U > 4 ? 2 : 1, RAW_ROWS = 32 / HALVES;  // lanes of a token
   static constexpr uint32_t RAW_STRIDE = ((U + (U + 3) / 4) | 1) * 16, RAW_STEP = RAW_ROWS * RAW_STRIDE;
-  static constexpr uint32_t RAW = U == 0 ? 0 : DP == 256 ? 2 : DP == 128 ? 6 : 8;
+  static constexpr uint32_t UNPACKERS = U == 0 ? 0 : U == 8 ? 5 : 6;  // warps that unpack: as many as shared memory has room for
+  static constexpr uint32_t RAW = U == 0 ? 0 : DP == 256 ? 2 : DP == 128 ? 2 : 6;
+  static constexpr uint32_t TILE_USERS = 9 + (U ? UNPACKERS : TC_LOADERS);  // the warps that work on a tile
   static constexpr uint32_t CONTROL = U ? TC_CONTROL4 : TC_CONTROL;
-  static constexpr size_t SMEM = CONTROL + SUBS * QSUB + STAGES * STAGE + TC_LOADERS * RAW * RAW_STEP;
+  static constexpr size_t SMEM = CONTROL + SUBS * QSUB + STAGES * STAGE + UNPACKERS * RAW * RAW_STEP;
   static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -141,11 +143,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
   const uint32_t D = p.a.head_dim, window = p.a.window;
   const TileShape &ts = p.ts;
   if (tid == 0) {
-    for (uint32_t i = 0; i < S::STAGES; i++) mbar_init(&ctl.full[i], TC_LOADERS * 32), mbar_init(&ctl.empty[i], 1);
+    for (uint32_t i = 0; i < S::STAGES; i++) mbar_init(&ctl.full[i], TC_LOADERS * 32 * S::HALVES), mbar_init(&ctl.empty[i], 1);
     mbar_init(&ctl.q_full, TC_LOADERS * 32), mbar_init(&ctl.q_empty, 1);
     for (int x = 0; x < 2; x++) mbar_init(&ctl.s_full[x], U ? 2 : 1), mbar_init(&ctl.p_half[x], 4), mbar_init(&ctl.p_ready[x], 4), mbar_init(&ctl.o_full[x], 1);
     mbar_init(&ctl.added, 1), mbar_init(&ctl.soft, SOFT_THREADS / 32), mbar_init(&ctl.drain, 1);
-    for (int i = 0; i < 2; i++) mbar_init(&ctl.tile_full[i], 1), mbar_init(&ctl.tile_empty[i], TILE_USERS);
+    for (int i = 0; i < 2; i++) mbar_init(&ctl.tile_full[i], 1), mbar_init(&ctl.tile_empty[i], S::TILE_USERS);
     ctl.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       if (one) sync();  // both outputs have been read
       done_with();
     }
-  } else if (warp >= TC_MMA) {
+  } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
     if (warp == TC_MMA) {
     // ---------------------------------------------------------------- MMA issue
@@ -444,11 +446,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       // Blocks below `by_rows` and from `by_rows_again` on are filled row by row: not by the proxy that the tensor core reads through.
       const uint32_t by_rows = p.box ? (first_seen(t, window) + TC_KB - 1) / TC_KB : 0xFFFFFFFFu, by_rows_again = (t.past + t.token0 + t.tokens) / TC_KB;
       auto visible = [&](uint32_t j) {
-        if (U == 0 && (lo + j < by_rows || lo + j >= by_rows_again)) proxy_fence();
+        if (U != 0 || lo + j < by_rows || lo + j >= by_rows_again) proxy_fence();
       };
       done_with();
       if (!wait(&ctl.q_full, tiles++ & 1)) break;
-      if (U == 0 && !p.q_mapped) proxy_fence();
+      if (!p.q_mapped) proxy_fence();
       bool ok = true;
       if (S::WIDE) {  // the places for scores take the blocks in turn
         for (uint32_t j = 0; j <= n && ok; j++) {
@@ -541,15 +543,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
         }
         if (!more) break;
       }
-    }
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    } else {
     // ---------------------------------------------------------------- copies: warp w has the rows w * 32 .. of a block, and a quarter of the queries
-    const uint32_t w = warp - TC_LOAD;
+    const uint32_t w = warp < TC_MMA ? warp - TC_LOAD : warp - TC_WALK - 1 + TC_LOADERS;
     uint32_t stage = 0, phase = 0, tiles = 0, bad = 0;
     if constexpr (U != 0) {
-      tc4_copies<IO, DP, U>(p, ctl, w, lane, s_q, s_ring, s_ring + S::STAGES * S::STAGE, turn, &bad, next_tile, done_with, wait);
-    } else {
+      if (w < S::UNPACKERS) tc4_copies<IO, DP, U>(p, ctl, w, lane, s_q, s_ring, s_ring + S::STAGES * S::STAGE, turn, &bad, next_tile, done_with, wait);
+    } else if (w < TC_LOADERS) {
     // The barrier counts a lane's copies when they have landed; the MMA warp makes them visible to the tensor core.  (A proxy fence
     // here would wait for the copies behind them as well: 4900 cycles a block, 2 stages in flight instead of 5.)
     auto submit = [&](uint64_t *bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
@@ -646,6 +646,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
     }
     copies_left<0>();
     if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
+    }
   }
   tm_fence_before();
   __syncthreads();

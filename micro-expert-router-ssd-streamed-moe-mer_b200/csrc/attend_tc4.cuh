@@ -1,7 +1,9 @@
 // The copying warps of attend_tc.cuh over a cache of 4 bits: queries as f16 rows, keys and values unpacked into f16 rows.  Included by it.
 //
-// Codes and scales are asked for some steps ahead (cp.async, into a part of shared memory that one warp alone uses: no barrier but the warp's own), then a lane takes
-// a token of the step, or half of one, and stores its numbers as the tiled copies of a 16-bit cache would have them.
+// The keys or the values of a block are some parts of 32 tokens (16 of wide heads), which the unpacking warps take in turn: the four that copy otherwise and the two beside the MMA
+// warp, which a 16-bit cache leaves idle (four alone: 2000 cycles for the keys of a block and as many for its values, more than the softmax takes; 2048 rows behind 8200 407 us).
+// Codes and scales are asked for some parts ahead (cp.async, into shared memory that one warp alone uses: no barrier but the warp's own), then a lane takes
+// a token of the part, or half of one, and stores its numbers as the tiled copies of a 16-bit cache would have them.
 
 // 4, 8 or 16 bytes, or zeros.
 template <int N>
@@ -10,6 +12,14 @@ __device__ __forceinline__ void copy_some(uint32_t dst, const void *src, bool in
     copy16(dst, src, in ? 16 : 0);
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(in ? N : 0) : "memory");
+}
+// WORDS words of a token, shared out to its HALVES lanes, in vectors as wide as their addresses allow.
+template <int WORDS, int HALVES>
+__device__ __forceinline__ void copy_scales(uint32_t dst, const char *src, uint32_t half, bool in) {
+  constexpr int N = WORDS % 4 == 0 ? 16 : WORDS % 2 == 0 ? 8 : 4;
+#pragma unroll
+  for (int b = 0; b < WORDS * 4; b += N)
+    if (HALVES == 1 || b / N % 2 == (int)half) copy_some<N>(dst + b, in ? src + b : src, in);
 }
 __device__ __forceinline__ void sts128(uint32_t a, const uint4 &v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -41,7 +51,8 @@ __device__ __forceinline__ void tc4_queries(const TcParams &p, const TileWork &t
   }
 }
 
-// The numbers of a lane's words of codes into a row of keys or values.  raw: the token's bytes; dst: its row of the stage.
+// The numbers of a lane's words of codes into a row of keys or values.  raw: the token's bytes; dst: its row of the stage, on 128 bytes
+// (its place in the swizzle is the row's low bits, exclusive-or that of the piece).
 template <int DP, int U, bool KEYS>
 __device__ __forceinline__ void tc4_unpack(uint32_t raw, uint32_t half, uint32_t dst, uint32_t row, uint32_t wide) {
   using S = TcShape<DP, U>;
@@ -58,6 +69,9 @@ __device__ __forceinline__ void tc4_unpack(uint32_t raw, uint32_t half, uint32_t
     const uint4 v = lds128(raw + 16 * U + i * 16);
     scales[4 * i] = v.x, scales[4 * i + 1] = v.y, scales[4 * i + 2] = v.z, scales[4 * i + 3] = v.w;
   }
+  uint32_t at[2][PER];
+#pragma unroll
+  for (uint32_t i = 0; i < 2 * PER; i++) at[i / PER][i % PER] = (dst | ((row & 7) << 4)) ^ ((4 * (i / PER) + i % PER) << 4) ^ (half * (PER << 4));
 #pragma unroll
   for (uint32_t u = 0; u < U; u++) {
     const __half2 h = as_half2(wide ? scales[u / 2] : scales[u]);
@@ -71,8 +85,7 @@ __device__ __forceinline__ void tc4_unpack(uint32_t raw, uint32_t half, uint32_t
         const uint32_t a = 2 * i * U + u, b = a + U;  // two words of 16 bits
         word = __byte_perm(words[a / 2], words[b / 2], (a % 2 ? 0x32u : 0x10u) | (b % 2 ? 0x7600u : 0x5400u));
       }
-      const uint32_t col = 4 * (u & 1) + half * PER + i;
-      sts128(dst + (u / 2) * (TC_KB * 128) + ((col ^ (row & 7)) << 4), kv4_numbers(word, scale, least));
+      sts128(at[u & 1][i] + (u / 2) * (TC_KB * 128), kv4_numbers(word, scale, least));
     }
   }
 }
@@ -81,93 +94,97 @@ template <typename IO, int DP, int U, typename Next, typename Done, typename Wai
 __device__ __forceinline__ void tc4_copies(const TcParams &p, TcControl4 &ctl, uint32_t w, uint32_t lane, uint32_t s_q, uint32_t s_ring, uint32_t s_raw, const uint32_t &turn, uint32_t *bad,
                                            const Next &next_tile, const Done &done_with, const Wait &wait) {
   using S = TcShape<DP, U>;
-  constexpr uint32_t HALVES = S::HALVES, ROWS = S::RAW_ROWS, RAW = S::RAW;
+  constexpr uint32_t HALVES = S::HALVES, ROWS = S::RAW_ROWS, RAW = S::RAW, PARTS = TC_KB / ROWS;  // parts of a block's keys, and of its values
   const Kv4Shape &f = p.a.kv4;
-  const uint32_t window = p.a.window, raw = s_raw + w * (RAW * S::RAW_STEP), wide = f.group == 64;
-  uint32_t stage = 0, phase = 0, tiles = 0;
+  const uint32_t window = p.a.window, raw = s_raw + w * (RAW * S::RAW_STEP), wide = f.group == 64, own = lane % ROWS;
+  const bool whole = p.a.page_tokens % 16 == 0;  // 16 tokens lie side by side
+  uint32_t tiles = 0, halves = 0;                // halves of blocks before the tile's: half h is in stage h % STAGES
   // columns that no unit has are zeros for good: queries are zero there, but a product with what shared memory held may not be
   if constexpr (U * 32 < DP) {
-    for (uint32_t i = 0; i < S::STAGES; i++)
-      for (uint32_t c = 4 * U; c < DP / 8; c++)
-        sts128(s_ring + i * S::STAGE + (c / 8) * (TC_KB * 128) + (w * 32 + lane) * 128 + (((c ^ lane) & 7) << 4), make_uint4(0, 0, 0, 0));
+    if (w < TC_LOADERS) {
+      for (uint32_t i = 0; i < S::STAGES; i++)
+        for (uint32_t c = 4 * U; c < DP / 8; c++)
+          sts128(s_ring + i * S::STAGE + (c / 8) * (TC_KB * 128) + (w * 32 + lane) * 128 + (((c ^ lane) & 7) << 4), make_uint4(0, 0, 0, 0));
+    }
   }
   while (next_tile()) {
     const TileWork t = ctl.tile[turn & 1];
     done_with();
-    if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
-    tc4_queries<IO, DP, U>(p, t, ctl.unit[tiles & 1], w, lane, s_q);
-    proxy_fence();
-    mbar_arrive(&ctl.q_full);
+    if (w < TC_LOADERS) {
+      if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
+      tc4_queries<IO, DP, U>(p, t, ctl.unit[tiles & 1], w, lane, s_q);
+      mbar_arrive(&ctl.q_full);
+    }
     tiles++;
     const uint32_t end = t.past + t.token0 + t.tokens, start = first_seen(t, window);
     const uint32_t *const table = p.kv.page_table + (uint64_t)t.seq * p.kv.table_stride;
-    auto entry = [&](uint32_t blk) {
-      const uint32_t key = blk * TC_KB + w * 32 + lane, slot = divided(key, p.kv.page_tokens);
-      return blk < t.hi && key >= start && key < end && slot < p.kv.table_stride ? table[slot] : 0xFFFFFFFFu;
+    const uint64_t head_at = t.kv_head * p.kv.head_stride;
+    // The warp's parts are n = w, w + UNPACKERS, ..: part n % PARTS of the keys or the values (n / PARTS even or odd) of block lo + n / (2 PARTS).
+    const uint32_t parts = (t.hi - t.lo) * 2 * PARTS;
+    auto token_of = [&](uint32_t n) { return (t.lo + n / (2 * PARTS)) * TC_KB + n % PARTS * ROWS + own; };
+    auto entry = [&](uint32_t n) {
+      const uint32_t key = token_of(n), at = divided(key, p.kv.page_tokens);
+      return n < parts && key >= start && key < end && at < p.kv.table_stride ? table[at] : 0xFFFFFFFFu;
     };
-    // Step n is of block lo + n / (2 HALVES): keys, then values, each in HALVES parts of the warp's tokens.
-    const uint32_t steps = (t.hi - t.lo) * 2 * HALVES;
-    uint32_t number = entry(t.lo), in_page = 0, slot = 0;  // slot: of the next step that is asked for
-    uint64_t block = 0;                                    // where the lane's token's page begins
+    uint32_t number = entry(w), slot = 0;  // of the next part that is asked for
     auto ask = [&](uint32_t n) {
-      if (n < steps) {
-        if (n % (2 * HALVES) == 0) {
-          const uint32_t blk = t.lo + n / (2 * HALVES), key = blk * TC_KB + w * 32 + lane;
-          const bool seen = key >= start && key < end, there = seen && number < p.kv.n_pages;
-          if (seen && !there) *bad = 1;
-          in_page = there ? key - divided(key, p.kv.page_tokens) * p.a.page_tokens : 0xFFFFFFFFu;
-          block = there ? number * p.kv.page_stride + t.kv_head * p.kv.head_stride : 0;
-          number = entry(blk + 1);
-        }
-        const char *const base = (const char *)(n / HALVES % 2 ? p.kv.v_pages : p.kv.k_pages);
-        const uint32_t first = n % HALVES * ROWS, dst = raw + slot * S::RAW_STEP;
+      if (n < parts) {
+        const uint32_t key = token_of(n);
+        const bool seen = key >= start && key < end, there = seen && number < p.kv.n_pages;
+        if (seen && !there) *bad = 1;
+        const uint32_t in_page = key - divided(key, p.kv.page_tokens) * p.a.page_tokens;
+        const uint64_t block = there ? number * p.kv.page_stride + head_at : 0;
+        const uint64_t codes = block + in_page * (16 * U);
+        number = entry(n + S::UNPACKERS);
+        const char *const base = (const char *)(n / PARTS % 2 ? p.kv.v_pages : p.kv.k_pages);
+        const uint32_t dst = raw + slot * S::RAW_STEP;
+        const uint32_t all = __ballot_sync(0xFFFFFFFFu, there);
+        if (whole && all == 0xFFFFFFFFu) {
+          const uint64_t run0 = __shfl_sync(0xFFFFFFFFu, codes, 0), run1 = HALVES == 1 ? __shfl_sync(0xFFFFFFFFu, codes, 16) : run0;
 #pragma unroll
-        for (uint32_t i = 0; i < U * ROWS / 32; i++) {
-          const uint32_t e = i * 32 + lane, r = e / U, c = e - r * U;
-          const uint64_t at = __shfl_sync(0xFFFFFFFFu, block, first + r);
-          const uint32_t in = __shfl_sync(0xFFFFFFFFu, in_page, first + r);
-          const bool there = in != 0xFFFFFFFFu;
-          copy_some<16>(dst + r * S::RAW_STRIDE + c * 16, there ? base + at + (uint64_t)in * (16 * U) + c * 16 : base, there);
-        }
-        const uint32_t r = lane % ROWS, c = lane / ROWS;
-        const uint64_t at = __shfl_sync(0xFFFFFFFFu, block, first + r);
-        const uint32_t in = __shfl_sync(0xFFFFFFFFu, in_page, first + r), bytes = f.scale_bytes();
-        const bool there = in != 0xFFFFFFFFu;
-        const char *const from = there ? base + at + f.codes + (uint64_t)in * bytes : base;
-        const uint32_t to = dst + r * S::RAW_STRIDE + 16 * U;
-        if (bytes % 16 == 0) {
-          for (uint32_t b = c * 16; b < bytes; b += HALVES * 16) copy_some<16>(to + b, there ? from + b : base, there);
-        } else if (bytes % 8 == 0) {
-          for (uint32_t b = c * 8; b < bytes; b += HALVES * 8) copy_some<8>(to + b, there ? from + b : base, there);
+          for (uint32_t i = 0; i < U * ROWS / 32; i++) {
+            const uint32_t e = i * 32 + lane, r = e / U, c = e - r * U;
+            copy16(dst + r * S::RAW_STRIDE + c * 16, base + (HALVES == 1 && (U % 2 ? e >= 16 * U : i >= U / 2) ? run1 + (e - 16 * U) * 16 : run0 + e * 16), 16);
+          }
         } else {
-          for (uint32_t b = c * 4; b < bytes; b += HALVES * 4) copy_some<4>(to + b, there ? from + b : base, there);
+#pragma unroll
+          for (uint32_t i = 0; i < U * ROWS / 32; i++) {
+            const uint32_t e = i * 32 + lane, r = e / U, c = e - r * U;
+            const uint64_t at = __shfl_sync(0xFFFFFFFFu, codes, r);
+            const bool in = all >> r & 1;
+            copy16(dst + r * S::RAW_STRIDE + c * 16, in ? base + at + c * 16 : base, in ? 16 : 0);
+          }
         }
+        const char *const from = there ? base + block + f.codes + in_page * f.scale_bytes() : base;
+        const uint32_t to = dst + own * S::RAW_STRIDE + 16 * U;
+        if (wide)
+          copy_scales<(U + 1) / 2, HALVES>(to, from, lane / ROWS, there);
+        else
+          copy_scales<U, HALVES>(to, from, lane / ROWS, there);
       }
       slot = slot + 1 == RAW ? 0 : slot + 1;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (uint32_t n = 0; n < RAW - 1; n++) ask(n);
+    for (uint32_t i = 0; i < RAW - 1; i++) ask(w + i * S::UNPACKERS);
     uint32_t taken = 0;
     bool ok = true;
-    for (uint32_t n = 0; n < steps; n++) {
-      ask(n + RAW - 1);
+    for (uint32_t n = w; n < parts; n += S::UNPACKERS) {
+      ask(n + (RAW - 1) * S::UNPACKERS);
       copies_left<RAW - 1>();
       __syncwarp();
-      if (n % HALVES == 0 && !(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
-      const uint32_t r = lane % ROWS, half = lane / ROWS, row = w * 32 + n % HALVES * ROWS + r;
-      const uint32_t from = raw + taken * S::RAW_STEP + r * S::RAW_STRIDE, dst = s_ring + stage * S::STAGE + row * 128;
-      if (n / HALVES % 2)
-        tc4_unpack<DP, U, false>(from, half, dst, row, wide);
+      const uint32_t h = halves + n / PARTS, stage = h % S::STAGES, row = n % PARTS * ROWS + own;
+      if (!(ok = wait(&ctl.empty[stage], (h / S::STAGES & 1) ^ 1))) break;
+      const uint32_t from = raw + taken * S::RAW_STEP + own * S::RAW_STRIDE, dst = s_ring + stage * S::STAGE + row * 128;
+      if (n / PARTS % 2)
+        tc4_unpack<DP, U, false>(from, lane / ROWS, dst, row, wide);
       else
-        tc4_unpack<DP, U, true>(from, half, dst, row, wide);
+        tc4_unpack<DP, U, true>(from, lane / ROWS, dst, row, wide);
       taken = taken + 1 == RAW ? 0 : taken + 1;
-      if (n % HALVES == HALVES - 1) {
-        proxy_fence();
-        mbar_arrive(&ctl.full[stage]);
-        stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
-      }
-      __syncwarp();  // the step's place may be asked for again
+      // The MMA warp makes the stage visible to the tensor core.
+      mbar_arrive(&ctl.full[stage]);
+      __syncwarp();  // the part's place may be asked for again
     }
     if (!ok) break;
+    halves += (t.hi - t.lo) * 2;
   }
 }

@@ -33,9 +33,10 @@ __device__ __forceinline__ SeqWork seq_work(const KvBatchDev &kv, uint32_t s, ui
   uint32_t row, n, len;
   seq_rows(kv, s, &row, &n, &len);
   const uint32_t skip = n > len ? n - len : 0;
+  const bool ours = n >= kv.least_rows && n <= kv.most_rows;
   SeqWork w;
-  w.row0 = row + skip, w.n = n - skip, w.past = len - w.n;
-  if (n == 0) w.past = 0;
+  w.row0 = row + skip, w.n = ours ? n - skip : 0, w.past = len - w.n;
+  if (n == 0 || !ours) w.past = 0;
   w.tiles = (w.n + tokens - 1) / tokens;
   return w;
 }

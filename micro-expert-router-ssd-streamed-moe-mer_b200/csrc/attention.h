@@ -46,6 +46,7 @@ struct KvBatchDev {
   uint32_t capacity;  // tokens that a row of the table has pages for
   const uint32_t *page_table, *row_start, *kv_len;
   uint32_t n_pages, table_stride, n_seqs, n_rows;
+  uint32_t least_rows = 0, most_rows = 0xFFFFFFFFu;  // the sequences that an attention kernel sees to bring so many rows
 };
 
 struct QkvRowsDev {

@@ -403,9 +403,19 @@ size_t attend_counts(int sm_count) { return (size_t)sm_count * 4; }  // a CTA's 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
   if (a.q4) {
+    // The streaming kernel where a sequence's rows are a few of its tiles (up to 32: 8 drafts of 5 tokens and 4 heads 44 us, 55 on the tensor cores), the tensor-core kernel where they are
+    // more; a batch of several sequences may hold both kinds, which only the device knows, so both are launched and take their own.
+    const uint32_t group = a.q_heads / a.kv_heads, few = group <= 16 ? 32 / group : 0;
+    KvBatchDev small = kv, large = kv;
+    if (kv.n_rows > kv.n_seqs && kv.n_seqs > 1) small.most_rows = few, large.least_rows = few + 1;
+    const bool streams = few && (kv.n_rows <= kv.n_seqs || kv.n_seqs > 1 || kv.n_rows <= few), tiles = !few || (kv.n_rows > kv.n_seqs && kv.n_rows > few);
+    if (streams) {
+      *launches += 1;
+      const cudaError_t e = launch_attend4(a, small, q, q_stride, out, out_stride, ws, sm_count, s);
+      if (e != cudaSuccess || !tiles) return e;
+    }
     *launches += 1;
-    if (kv.n_rows <= kv.n_seqs && a.q_heads / a.kv_heads <= 16) return launch_attend4(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
-    return launch_attend_tc4(a, kv, q, q_stride, out, out_stride, ws, sm_count, s);
+    return launch_attend_tc4(a, large, q, q_stride, out, out_stride, ws, sm_count, s);
   }
   // One row a sequence and no more heads of a key head than a tile has rows: the streaming kernel.  Any more rows: the tensor-core kernel, whose 128 rows a group cost
   // the same whatever they hold.
