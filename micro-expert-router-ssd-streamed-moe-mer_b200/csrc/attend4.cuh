@@ -434,15 +434,30 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
           __syncwarp();
         }
       }
-      // ---- values' scales of the lane's tokens, by pairs
-      uint32_t vs[2][G];
+      // ---- values' scales of the lane's tokens, by pairs, and the minima as an operand: row 2 g + 1 of it (row g where a token's words are no whole 16 bytes) has group g's
+      uint32_t vs[2][G], least_of[4] = {0, 0, 0, 0};
+      if constexpr (G % 4 == 0) {
+        const uint32_t at = vscales + (token_of(lane & 7) + (lane & 8)) * (4 * G) + (G == 8 ? (lane >> 4) * 16 : 0);
+        if constexpr (G == 8)
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(least_of[0]), "=r"(least_of[2]), "=r"(least_of[1]), "=r"(least_of[3]) : "r"(at) : "memory");
+        else
+          asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(least_of[0]), "=r"(least_of[2]) : "r"(at) : "memory");
+        // its row 2 g has the scales of group g, and a lane those of its tokens
 #pragma unroll
-      for (int T = 0; T < 2; T++) {
-        uint32_t sc[2][G];
-        lds_words<G>(vscales + (T * 8 + even_token) * (4 * G), sc[0]);
-        lds_words<G>(vscales + (T * 8 + odd_token) * (4 * G), sc[1]);
+        for (int T = 0; T < 2; T++)
 #pragma unroll
-        for (int g = 0; g < G; g++) vs[T][g] = __byte_perm(sc[0][g], sc[1][g], 0x5410);
+          for (int g = 0; g < G; g++) vs[T][g] = __shfl_sync(0xFFFFFFFFu, least_of[2 * T + g / 4], g % 4 * 8 + quad);
+      } else {
+#pragma unroll
+        for (int T = 0; T < 2; T++) {
+          uint32_t sc[2][G];
+          lds_words<G>(vscales + (T * 8 + even_token) * (4 * G), sc[0]);
+          lds_words<G>(vscales + (T * 8 + odd_token) * (4 * G), sc[1]);
+#pragma unroll
+          for (int g = 0; g < G; g++) vs[T][g] = __byte_perm(sc[0][g], sc[1][g], 0x5410);
+          const uint32_t even = vscales + (T * 8 + even_token) * (4 * G) + (eighth % G) * 4, odd = vscales + (T * 8 + odd_token) * (4 * G) + (eighth % G) * 4;
+          least_of[2 * T] = __byte_perm(lds32(even), lds32(odd), 0x7632);
+        }
       }
       // ---- weights
       bool grows = false;
@@ -482,23 +497,8 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
 #pragma unroll
         for (int T = 0; T < 2; T++) pf[x][T] = transposed(Num<__half>::pack(w[T][0], w[T][1]));
       }
-      // ---- minima: row 2 g + 1 of the product (row g where a token's words are no whole 16 bytes) has group g's
-      {
-        uint32_t a0, a1 = 0, a2, a3 = 0;
-        if constexpr (G % 4 == 0) {
-          const uint32_t at = vscales + (token_of(lane & 7) + (lane & 8)) * (4 * G) + (G == 8 ? (lane >> 4) * 16 : 0);
-          if constexpr (G == 8)
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a0), "=r"(a2), "=r"(a1), "=r"(a3) : "r"(at) : "memory");
-          else
-            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a0), "=r"(a2) : "r"(at) : "memory");
-        } else {
-          const uint32_t even = vscales + even_token * (4 * G) + (eighth % G) * 4, odd = vscales + odd_token * (4 * G) + (eighth % G) * 4;
-          a0 = __byte_perm(lds32(even), lds32(odd), 0x7632);
-          a2 = __byte_perm(lds32(even + 8 * 4 * G), lds32(odd + 8 * 4 * G), 0x7632);
-        }
 #pragma unroll
-        for (int x = 0; x < NT; x++) mma_f16(least[x], a0, a1, a2, a3, pf[x][0], pf[x][1]);
-      }
+      for (int x = 0; x < NT; x++) mma_f16(least[x], least_of[0], least_of[1], least_of[2], least_of[3], pf[x][0], pf[x][1]);
       // ---- values: a lane has words eighth * U .. of its four tokens
       {
         uint32_t w[2][U];  // word u of the lane's two tokens, of 16 bits each
@@ -518,12 +518,13 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          const uint32_t v0 = w[0][u] >> 8, v1 = w[1][u] >> 8;
+          // rows of a tile: a code, and that code with sixteen times the next one, which the end takes apart again: four instructions a word where the codes alone are five
+          const uint32_t l0 = w[0][u] & 0x00FF00FFu, l1 = w[1][u] & 0x00FF00FFu, h0 = __byte_perm(w[0][u], 0, 0x4341), h1 = __byte_perm(w[1][u], 0, 0x4341);
 #pragma unroll
           for (int x = 0; x < NT; x++) {
             const uint32_t b0 = as_u32(__hmul2(as_half2(pf[x][0]), as_half2(vs[0][u >> GS]))), b1 = as_u32(__hmul2(as_half2(pf[x][1]), as_half2(vs[1][u >> GS])));
-            mma_f16(o[x][2 * u], w[0][u] & 0x000F000Fu, w[0][u] & 0x00F000F0u, w[1][u] & 0x000F000Fu, w[1][u] & 0x00F000F0u, b0, b1);
-            mma_f16(o[x][2 * u + 1], v0 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x000F000Fu, v1 & 0x00F000F0u, b0, b1);
+            mma_f16(o[x][2 * u], l0 & 0x000F000Fu, l0, l1 & 0x000F000Fu, l1, b0, b1);
+            mma_f16(o[x][2 * u + 1], h0 & 0x000F000Fu, h0, h1 & 0x000F000Fu, h1, b0, b1);
           }
         }
       }
@@ -562,14 +563,15 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
       for (int u = 0; u < U; u++) {
         const int g = u >> GS, at = G % 4 == 0 && g >= 4 ? 2 : 0, src = G % 4 == 0 ? (g % 4 * 2 + 1) * 4 : g * 4;
         const float l0 = __shfl_sync(0xFFFFFFFFu, least[x][at], src + quad), l1 = __shfl_sync(0xFFFFFFFFu, least[x][at + 1], src + quad);
-        constexpr float LOW = 16777216.0f, HIGH = 1048576.0f;  // 2^24 and 2^20
+        constexpr float CODE = 16777216.0f, NEXT = 1048576.0f;  // 2^24, and 2^20: sixteen times the code
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const uint32_t row = x * 8 + quad * 2 + e;
-          const float least_of = e ? l1 : l0;
+          const float of_group = e ? l1 : l0;
           if (row < rows)
             *reinterpret_cast<float4 *>(s_o + ((size_t)warp * R + row) * S::OP + u * 32 + eighth * 4) =
-                make_float4(fmaf(o[x][2 * u][e], LOW, least_of), fmaf(o[x][2 * u][2 + e], HIGH, least_of), fmaf(o[x][2 * u + 1][e], LOW, least_of), fmaf(o[x][2 * u + 1][2 + e], HIGH, least_of));
+                make_float4(fmaf(o[x][2 * u][e], CODE, of_group), fmaf(o[x][2 * u][2 + e] - o[x][2 * u][e], NEXT, of_group), fmaf(o[x][2 * u + 1][e], CODE, of_group),
+                            fmaf(o[x][2 * u + 1][2 + e] - o[x][2 * u + 1][e], NEXT, of_group));
         }
       }
     }
