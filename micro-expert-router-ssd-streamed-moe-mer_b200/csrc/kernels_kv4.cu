@@ -247,8 +247,9 @@ __global__ void __launch_bounds__(32, 16) k_kv4_append(const __grid_constant__ K
       if (norm && there) cw[i] *= (F)__ldg(norm + v), sw[i] *= (F)__ldg(norm + mate(v));
     }
   };
-  // Norm and rotation of eight values in 32 bits.
-  auto turned = [&](const float(&x)[8], const float(&o)[8], const float(&cw)[8], const float(&sw)[8], bool norm, float(&z)[8]) {
+  // Norm and rotation of eight values in 32 bits.  Returned: what the norm multiplies by.
+  auto turned = [&](const float(&x)[8], const float(&o)[8], const float(&cw)[8], const float(&sw)[8], bool norm, float(&z)[8]) -> float {
+    float unit = 1.0f;
     uint64_t y[4], sq = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -264,12 +265,13 @@ __global__ void __launch_bounds__(32, 16) k_kv4_append(const __grid_constant__ K
       for (uint32_t d = 1; d < 8; d *= 2) lo += __shfl_xor_sync(0xFFFFFFFFu, lo, d);
       if (p.lanes > 8) lo += __shfl_xor_sync(0xFFFFFFFFu, lo, 8);
       if (p.lanes > 16) lo += __shfl_xor_sync(0xFFFFFFFFu, lo, 16);
-      const float unit = rsqrtf(fmaf(lo, p.per_value, a.norm_eps));
+      unit = rsqrtf(fmaf(lo, p.per_value, a.norm_eps));
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = mul2(y[e], pack2(unit, unit));
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) unpack2(y[e], z[2 * e], z[2 * e + 1]);
+    return unit;
   };
   // ---- queries
   if (step < min(end, k_first)) {
@@ -325,17 +327,19 @@ __global__ void __launch_bounds__(32, 16) k_kv4_append(const __grid_constant__ K
       {
         float x[8], o[8], z[8];
         mine.get(x), theirs.get(o);
-        turned(x, o, cw, sw, a.k_norm != nullptr, z);
+        const float unit = turned(x, o, cw, sw, a.k_norm != nullptr, z);
         // What is rotated into one another has together at most twice the largest rotated value, so with cosines and sines off by 2^-22.6 (sincospif: 1 ulp, an angle's
         // rounding, two products), three roundings of what they multiply, and a norm whose sum has nine roundings and its root two units, a value is off by at most 2^-20.1 of the
-        // head's largest.
+        // head's largest.  No square is infinite, and none that counts has lost bits, while their mean lies between 2^-96
+        // and 2^120.
         float most = fmaxf(fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3]))), fmaxf(fmaxf(fabsf(z[4]), fabsf(z[5])), fmaxf(fabsf(z[6]), fabsf(z[7]))));
         const float sum = ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));  // what is no number stays none
 #pragma unroll
         for (uint32_t d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
         if (p.lanes > 8) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 8));
         if (p.lanes > 16) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
-        sure = kv4_key_codes_fast(z, most * 0x1p-20f + FLT_MIN, there, lanes, code, &scale_min) && most < 0.98f * KV4_MOST && sum - sum == 0.0f;
+        sure = kv4_key_codes_fast(z, most * 0x1p-20f + FLT_MIN, there, lanes, code, &scale_min) && most < 0.98f * KV4_MOST && sum - sum == 0.0f &&
+               unit > 0x1p-60f && unit < 0x1p48f;
       }
       if (!__all_sync(0xFFFFFFFFu, sure)) {
         if (!have64) {

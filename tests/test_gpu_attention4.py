@@ -147,6 +147,20 @@ def test_values_of_any_size(backend, size):  # noqa: F811
         check(c)
 
 
+@pytest.mark.parametrize("page,d,group", [(5, 128, 32), (16, 80, 32), (24, 64, 64), (48, 256, 32)])
+def test_large_values_in_tiles_behind_one_another(backend, page, d, group):  # noqa: F811
+    # weights times scales that f16 has no room for, in some of the sequences that a CTA has one after the other, and not in others
+    for lens in ([(1, 90 + i % 7) for i in range(900)], [(1 + i % 3, 400 + 50 * (i % 9)) for i in range(300)]):
+        c = Cache4(lens, 8, 2, d, "bf16", page, group)
+        for i, (n, k) in enumerate(lens):
+            for keys in (True, False):
+                size = 8000.0 if not keys and i % 5 == 2 else 1.0
+                c.put(keys, c.places(i), *quantised(torch.randn((k, 2, d), device="cuda", generator=c.gen).double() * size, group))
+        c.install(backend)
+        forward(backend, c)
+        check(c)
+
+
 def test_queries_of_any_size(backend):  # noqa: F811
     for kind, sizes in (("bf16", (1e-30, 1e-5, 1e5)), ("f16", (1e-4, 300.0))):
         for lens in ([(1, 300), (1, 77)], [(30, 300), (3, 77)]):

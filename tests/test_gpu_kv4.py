@@ -166,7 +166,7 @@ def exact_rows(c, x, qw, kw, freq, pairs, eps, rope_scale=1.0):
     return exact
 
 
-def append(b, c, source="bf16", *, norm=True, rope_dims=0, pairs=False, theta=1e4, rope_scale=1.0, gap=0, offset=0, with_q=True, x=None):
+def append(b, c, source="bf16", *, norm=True, rope_dims=0, pairs=False, theta=1e4, rope_scale=1.0, gap=0, offset=0, with_q=True, x=None, eps=1e-5):
     """Appends rows; the rows in 64 bits as they come out of norm and rotation."""
     dtype, value_type = TYPES[source]
     width = (c.hq + 2 * c.hk) * c.d
@@ -177,7 +177,7 @@ def append(b, c, source="bf16", *, norm=True, rope_dims=0, pairs=False, theta=1e
     rng = np.random.default_rng(9)
     qw, kw = ((1 + 0.3 * rng.standard_normal(c.d)).astype(np.float32) for _ in range(2)) if norm else (None, None)
     freq = theta ** (-np.arange(rope_dims // 2) / max(1, rope_dims // 2))
-    eps = float(np.float32(1e-5))
+    eps = float(np.float32(eps))
     c.install(b, q_norm=qw, k_norm=kw, norm_eps=eps, rope_freq=freq if rope_dims else None, rope_pairs=pairs, rope_scale=rope_scale)
     at = rows.data_ptr()
     size = dtype.itemsize
@@ -251,6 +251,39 @@ def test_groups_of_every_kind(backend):
     for group in (32, 64):
         c = Cache4([(8, 20)], 1, 1, 128, "bf16", 16, group)
         check_append(backend, c, "f32", norm=False, x=x)
+
+
+@pytest.mark.parametrize("size,eps", [(1e18, 1e-5), (1e25, 1e-5), (1e37, 0.0), (1e-14, 0.0), (1e-17, 0.0), (1e-21, 0.0), (1e-30, 0.0), (1e-21, 1e-40)])
+def test_norms_of_rows_far_from_one(backend, size, eps):
+    # the sum of squares leaves 32 bits' range; the codes are those of 64 all the same
+    c = Cache4([(5, 9), (1, 30)], 2, 2, 128, "bf16", 16)
+    x = torch.randn((6, 6 * 128), device="cuda", generator=c.gen)
+    x[:, 256:512] *= size
+    exact = check_append(backend, c, "f32", rope_dims=64, with_q=False, x=x, eps=eps)
+    assert exact[:, 2:4].isfinite().all() and exact[:, 2:4].abs().max() > 0.1  # the oracle's own: 1e-21 a value over the root of 1e-40 + 1e-42 is 0.1
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("q_heads,kv_heads,d,lens,gap,offset", [(32, 4, 128, [(1, 100)], 0, 0), (20, 2, 80, [(3, 3), (0, 9), (1, 17)], 8, 0), (5, 5, 64, [(40, 77)], 3, 1), (64, 8, 256, [(2, 2)], 0, 0),
+                                                              (4, 2, 24, [(3000, 3000)], 0, 8)])
+def test_queries_in_place(backend, q_heads, kv_heads, d, lens, gap, offset, pairs):
+    # one warp a row, and several of them that each have some of its heads
+    got = {}
+    for place in ("own", "same"):
+        c = Cache4(lens, q_heads, kv_heads, d, "bf16", 16)
+        width, rope = (q_heads + 2 * kv_heads) * d + gap, d // 4 * 2
+        rows = torch.randn(c.rows * width + offset, device="cuda", generator=c.gen).to(torch.bfloat16)[offset:].view(c.rows, width)
+        kept = rows.clone()
+        q_out = rows if place == "same" else torch.zeros_like(rows)
+        norm = (1 + 0.3 * np.random.default_rng(3).standard_normal(d)).astype(np.float32)
+        c.install(backend, q_norm=norm, k_norm=norm, norm_eps=1e-5, rope_freq=1e4 ** (-np.arange(rope // 2) / (rope // 2)), rope_pairs=pairs)
+        at = rows.data_ptr()
+        backend.kv_append_device(0, c.batch(), mer_b200.QkvRows(q=at, k=at + q_heads * d * 2, v=at + (q_heads + kv_heads) * d * 2, q_out=q_out.data_ptr(), q_stride=width, k_stride=width,
+                                                                v_stride=width, q_out_stride=width, value_type=mer_b200.VALUE_BF16), stream())
+        backend.stream_check(0, stream())
+        assert torch.equal(rows[:, q_heads * d:], kept[:, q_heads * d:]) and (place == "same" or torch.equal(rows, kept))
+        got[place] = [q_out[:, :q_heads * d].clone(), *(p.clone() for p in c.pools)]
+    assert all(torch.equal(a, b) for a, b in zip(got["own"], got["same"]))
 
 
 @pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf, 60001.0, -1e30])
