@@ -480,11 +480,16 @@ int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *bat
  * of a magnitude above 60000, has the minimum NaN: its values read back as NaN, and rows that see them are not finite.
  * Page p of key head h is a block of mer_kv4_block_bytes at k_pages (v_pages) + p * page_stride + h * head_stride, all in BYTES and multiples of 16; token_stride
  * is 0.  A block has the codes of its tokens one behind the other, then their scales and minima.  A head's codes are stored for 64, 96, 128, 192 or 256 values, units = 2, 3, 4, 6 or 8
- * of 32, 16 bytes each (append writes zeros behind the head's own values; a cache filled in another way has codes of any value there, and finite scales and minima):
+ * of 32, 16 bytes each (append writes zeros behind the head's own values; a cache filled in another way has codes of any value there, finite scales and minima, and everywhere groups
+ * whose sixteen values lie within f16's range):
  *   keys    32-bit word j * units + u of a token (j < 4): values 32 u + 8 j + 2 p and + 2 p + 1 from bits 4 p and 16 + 4 p on (p < 4)
  *   values  16-bit word r * units + u of a token (r < 8): values 32 u + 4 r + i from bit 4 i on (i < 4)
  *   scales  token t, group g: scale and minimum, two f16, at (t * groups + g) * 4 behind the block's codes; groups = 32 * units / cache_group, rounded up
- * Everything else is as with 16 bits: what rows see, tables, strides of rows, pages that are not there (their tokens count as zeros), windows, sinks. */
+ * Everything else is as with 16 bits: what rows see, tables, strides of rows, pages that are not there (their tokens count as zeros), windows, sinks; but of a page with tokens that a
+ * row sees the other ones' bytes may be read, too (they may hold anything).
+ * Attention rounds operands to f16 whatever cache_type is: queries beside their row's power of two, weights, and either weights times scales (few rows) or the keys' and values'
+ * numbers (many); scores, sums and outputs are fp32.  A sequence with up to 32 rows times query heads of a key head is taken by a kernel that streams (at most 16 query heads to a key head, or one
+ * row a sequence), others by the tensor cores; with n_rows above n_seqs and several sequences both are launched, and each takes its own on the device. */
 uint64_t mer_kv4_block_bytes(uint32_t head_dim, uint32_t page_tokens, uint32_t group); /* 0: no such cache */
 
 /* Keys and values of the batch's rows, which the cache holds, as rows of numbers: a prefix to hand on, rows for another kernel.  Any cache; one rounding to value_type.  Rows

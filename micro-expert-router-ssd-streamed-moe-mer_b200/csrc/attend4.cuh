@@ -1,22 +1,29 @@
-// Attention of single new tokens over a paged cache of 4 bits.  Head sizes up to 256 in steps of 8.
+// Attention of a few new tokens a sequence over a paged cache of 4 bits.  Head sizes up to 256 in steps of 8.
 //
 //   o = sum_j p_j v_j / (sum_j p_j [+ sink]),  p_j = 2^(s_j - m),  s_j = q . k_j * scale * log2 e,  m = max_j s_j
 //
 // in one pass, as in kernels_attend.cu: a warp is a stream of its own, chunks of 16 tokens, maximum, sum and output of its own tokens in registers.  Reading a token's
-// codes takes a quarter of a 16-bit cache's time, so the instructions that unpack are what counts, and codes are multiplied as they are:
+// codes takes a third of a 16-bit cache's time, so the instructions that unpack are what counts, and codes are multiplied as they are:
 //
 //   * A code's four bits, masked in place, are an f16 number: a subnormal one, code * 2^-24 or code * 2^-20 as they stand in the lower or the upper half of a byte, which the matrix
-//     units multiply exactly.  One AND makes two operands' values, and every second word a shift before that.
-//   * Keys:  q . k = sum_g scale_g (q . code)_g + minimum_g (sum of q)_g.  The first product is exact in fp32 and takes its scale there; the second is one more
-//     matrix product, whose operand the words (scale, minimum) are as they lie in memory, against (0, sum of q) in two parts of f16.
-//   * Values:  o = sum_g (p scale_g) . code + p . minimum_g.  A weight times a scale is rounded to f16, the weights themselves once more; minima are an operand as above.
+//     units multiply exactly.
+//   * Keys:  q . k = sum_g scale_g (q . code)_g + minimum_g (sum of q)_g.  One AND makes two operands' values, and every second word a shift before that.  The first product is exact
+//     in fp32 and takes its scale there; the second is one more matrix product, whose operand the words (scale, minimum) are as they lie in memory, against (0, sum of q) in two
+//     parts of f16.
+//   * Values:  o = sum_g (p scale_g) . code + p . minimum_g.  Operands are a code and that code with sixteen times the next one (a byte as it is: 2^-24 (code + 16 next)), which the
+//     end takes apart again: four instructions a word, where the codes alone are five.  A weight times a scale is rounded to f16, the weights themselves once more; minima are an operand as above.
 //   * Both products have tokens or the head's values along M and the rows along N, so that eight rows cost half of sixteen; the weights are transposed between them (movmatrix).
 //   * Queries are f16 divided by a power of two of their row.  A row's reference m follows its maximum only when that has grown by more than 2^LAG4.  Weights are made as
 //     2^(s - m + 10): a weight is below 2^14, its product with a scale below 4 fits f16, and small ones lie above its last bit for 2^-34 of the largest.  Where a product did not fit
-//     (an output that is not finite says so), the warp takes its blocks of the tile once more with weights 2^13 times smaller, which fit with any scale.
+//     (an output that is not finite says so), the warp takes its blocks of the tile once more with weights 2^13 times smaller, which fit with the scales of any values that f16 holds.
 //
 // A warp's ring of chunks is seen by no other warp.  Where pages are whole chunks (multiples of 16 tokens) a lane makes a chunk's four bulk copies: the addresses of several chunks are
-// one instruction stream, so that a chunk costs a dozen instructions for its copies instead of sixty (copies of 16 bytes by every lane: 54 us for 64 tokens behind 800 to 8000, 49 so).  Other pages: cp.async of 16 bytes a lane, token by token.
+// one instruction stream, so that a chunk costs a dozen instructions for its copies instead of sixty (copies of 16 bytes by every lane: 54 us for 64 tokens behind 800 to 8000, 49
+// so, before values' codes were multiplied by pairs).  Other pages: cp.async of 16 bytes a lane, token by token.
+//
+// 32 and 4 heads of 128 in bf16, groups of 32, pages of 16: 64 tokens behind 800 to 8000 47.3 us = 3.1 TB/s (16 bits: 84.5 us), one behind 32000 22.6 us.  What bounds it: issuing.  A chunk is
+// 335 instructions, half of them on the ALU (2.4 cycles each for a quarter of an SM; an mma 5.8), and takes 296 ns a quarter of an SM, whatever the number of warps: 5.1 TB/s if it went on
+// all the time.  The rest is 6 us until the first chunk has landed, 2 us of switching for every tile that a CTA goes through, and CTAs that end before others.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -1,7 +1,9 @@
 // The copying warps of attend_tc.cuh over a cache of 4 bits: queries as f16 rows, keys and values unpacked into f16 rows.  Included by it.
 //
 // The keys or the values of a block are some parts of 32 tokens (16 of wide heads), which the unpacking warps take in turn: the four that copy otherwise and the two beside the MMA
-// warp, which a 16-bit cache leaves idle (four alone: 2000 cycles for the keys of a block and as many for its values, more than the softmax takes; 2048 rows behind 8200 407 us).
+// warp, which a 16-bit cache leaves idle (four alone: 2000 cycles for the keys of a block and as many for its values, more than the softmax takes; 2048 rows behind 8200 407 us,
+// 393 with six).  What bounds it: issuing, 44 % of all slots with two warps of softmax and up to two that unpack on a quarter of an SM; a block takes 5000 cycles, 3500 from 16 bits.
+// Three stages of numbers and four of codes, instead of four and two: 400.
 // Codes and scales are asked for some parts ahead (cp.async, into shared memory that one warp alone uses: no barrier but the warp's own), then a lane takes
 // a token of the part, or half of one, and stores its numbers as the tiled copies of a 16-bit cache would have them.
 

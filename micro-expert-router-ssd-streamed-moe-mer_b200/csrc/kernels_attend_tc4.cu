@@ -1,4 +1,4 @@
-// Attention of many new rows over a paged cache of 4 bits: attend_tc.cuh, whose copying warps unpack (attend_tc4.inc).
+// Attention of many new rows over a paged cache of 4 bits: attend_tc.cuh, whose copying warps unpack (attend_tc4.cuh).
 #include "attend_tc.cuh"
 
 namespace {
