@@ -27,6 +27,24 @@ __device__ __forceinline__ void sts128(uint32_t a, const uint4 &v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// N 32-bit words from an address on a multiple of 4 N (at most 16) bytes.
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
+  constexpr int V = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
+#pragma unroll
+  for (int i = 0; i < N; i += V) {
+    if constexpr (V == 4) {
+      const uint4 v = lds128(a + i * 4);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    } else if constexpr (V == 2) {
+      const uint2 v = lds64(a + i * 4);
+      w[i] = v.x, w[i + 1] = v.y;
+    } else {
+      w[i] = lds32(a + i * 4);
+    }
+  }
+}
+
 // Queries of a tile as f16: a row is divided by a power of two that brings its largest value between 1 and 2, which f16 holds as exactly as its own type did down to 2^-14
 // of that; the power goes to the scores' factor.
 template <typename IO, int DP, int U>
@@ -54,41 +72,53 @@ __device__ __forceinline__ void tc4_queries(const TcParams &p, const TileWork &t
 }
 
 // The numbers of a lane's words of codes into a row of keys or values.  raw: the token's bytes; dst: its row of the stage, on 128 bytes
-// (its place in the swizzle is the row's low bits, exclusive-or that of the piece).
-template <int DP, int U, bool KEYS>
-__device__ __forceinline__ void tc4_unpack(uint32_t raw, uint32_t half, uint32_t dst, uint32_t row, uint32_t wide) {
+// (its place in the swizzle is the row's low bits, exclusive-or that of the piece).  A lane has PER pieces of U words (one j of a key, a pair of r of a value).  For heads of up to 128 values a
+// loop, and one for keys and values: the softmax beside it needs the instruction cache (2048 rows behind 8200: 359 us unrolled and one for each; 327 as one, 322 so, 326 not
+// unrolled at all).  With wider heads the softmax waits for the unpacking, which is faster unrolled (1000 rows of 256 values behind 4000: 198, 203 to 207 so).
+template <int DP, int U>
+__device__ __forceinline__ void tc4_unpack(uint32_t raw, uint32_t half, uint32_t dst, uint32_t row, uint32_t wide, bool keys) {
   using S = TcShape<DP, U>;
-  constexpr uint32_t PER = 4 / S::HALVES;  // fours of words (j, or pairs of r) of a lane
-  static_assert(PER * U % 4 == 0, "a lane's words are whole vectors");
-  uint32_t words[PER * U], scales[(U + 3) / 4 * 4];
+  constexpr uint32_t PER = 4 / S::HALVES;
+  uint32_t scales[(U + 3) / 4 * 4];
+  auto load_scales = [&] {
 #pragma unroll
-  for (uint32_t i = 0; i < PER * U / 4; i++) {
-    const uint4 v = lds128(raw + half * (8 * U) + i * 16);
-    words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < (U + 3) / 4; i++) {
-    const uint4 v = lds128(raw + 16 * U + i * 16);
-    scales[4 * i] = v.x, scales[4 * i + 1] = v.y, scales[4 * i + 2] = v.z, scales[4 * i + 3] = v.w;
-  }
-  uint32_t at[2][PER];
-#pragma unroll
-  for (uint32_t i = 0; i < 2 * PER; i++) at[i / PER][i % PER] = (dst | ((row & 7) << 4)) ^ ((4 * (i / PER) + i % PER) << 4) ^ (half * (PER << 4));
-#pragma unroll
-  for (uint32_t u = 0; u < U; u++) {
-    const __half2 h = as_half2(wide ? scales[u / 2] : scales[u]);
-    const __half2 scale = __low2half2(h), least = __high2half2(h);
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) {
-      uint32_t word;
-      if constexpr (KEYS) {
-        word = words[i * U + u];
-      } else {
-        const uint32_t a = 2 * i * U + u, b = a + U;  // two words of 16 bits
-        word = __byte_perm(words[a / 2], words[b / 2], (a % 2 ? 0x32u : 0x10u) | (b % 2 ? 0x7600u : 0x5400u));
-      }
-      sts128(at[u & 1][i] + (u / 2) * (TC_KB * 128), kv4_numbers(word, scale, least));
+    for (uint32_t i = 0; i < (U + 3) / 4; i++) {
+      const uint4 v = lds128(raw + 16 * U + i * 16);
+      scales[4 * i] = v.x, scales[4 * i + 1] = v.y, scales[4 * i + 2] = v.z, scales[4 * i + 3] = v.w;
     }
+  };
+  // Word u of a value from those of its piece: two words of 16 bits.
+  auto of_value = [](const uint32_t(&w)[U], uint32_t u) { return __byte_perm(w[u / 2], w[(U + u) / 2], (u % 2 ? 0x32u : 0x10u) | ((U + u) % 2 ? 0x7600u : 0x5400u)); };
+  const uint32_t to = (dst | ((row & 7) << 4)) ^ (half * (PER << 4));
+  auto store = [&](uint32_t i, uint32_t u, uint32_t word) {
+    const __half2 h = as_half2(wide ? scales[u / 2] : scales[u]);
+    sts128((to ^ ((4 * (u & 1)) << 4) ^ (i << 4)) + (u / 2) * (TC_KB * 128), kv4_numbers(word, __low2half2(h), __high2half2(h)));
+  };
+  const uint32_t own = raw + half * (8 * U);
+  if constexpr (S::HALVES == 1) {
+    load_scales();
+#pragma unroll 2
+    for (uint32_t i = 0; i < PER; i++) {
+      uint32_t w[U], words[U];
+      lds_words<U>(own + i * (4 * U), w);
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) words[u] = w[u];
+      if (!keys) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) words[u] = of_value(w, u);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) store(i, u, words[u]);
+    }
+  } else {
+    uint32_t w[PER][U];
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) lds_words<U>(own + i * (4 * U), w[i]);
+    load_scales();
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+      for (uint32_t i = 0; i < PER; i++) store(i, u, keys ? w[i][u] : of_value(w[i], u));
   }
 }
 
@@ -177,10 +207,13 @@ __device__ __forceinline__ void tc4_copies(const TcParams &p, TcControl4 &ctl, u
       const uint32_t h = halves + n / PARTS, stage = h % S::STAGES, row = n % PARTS * ROWS + own;
       if (!(ok = wait(&ctl.empty[stage], (h / S::STAGES & 1) ^ 1))) break;
       const uint32_t from = raw + taken * S::RAW_STEP + own * S::RAW_STRIDE, dst = s_ring + stage * S::STAGE + row * 128;
-      if (n / PARTS % 2)
-        tc4_unpack<DP, U, false>(from, lane / ROWS, dst, row, wide);
+      const bool keys = n / PARTS % 2 == 0;
+      if constexpr (HALVES == 1)
+        tc4_unpack<DP, U>(from, lane / ROWS, dst, row, wide, keys);
+      else if (keys)
+        tc4_unpack<DP, U>(from, lane / ROWS, dst, row, wide, true);
       else
-        tc4_unpack<DP, U, true>(from, lane / ROWS, dst, row, wide);
+        tc4_unpack<DP, U>(from, lane / ROWS, dst, row, wide, false);
       taken = taken + 1 == RAW ? 0 : taken + 1;
       // The MMA warp makes the stage visible to the tensor core.
       mbar_arrive(&ctl.full[stage]);
