@@ -1,9 +1,9 @@
 // The copying warps of attend_tc.cuh over a cache of 4 bits: queries as f16 rows, keys and values unpacked into f16 rows.  Included by it.
 //
 // The keys or the values of a block are some parts of 32 tokens (16 of wide heads), which the unpacking warps take in turn: the four that copy otherwise and the two beside the MMA
-// warp, which a 16-bit cache leaves idle (four alone: 2000 cycles for the keys of a block and as many for its values, more than the softmax takes; 2048 rows behind 8200 407 us,
-// 393 with six).  What bounds it: issuing, 44 % of all slots with two warps of softmax and up to two that unpack on a quarter of an SM; a block takes 5000 cycles, 3500 from 16 bits.
-// Three stages of numbers and four of codes, instead of four and two: 400.
+// warp, which a 16-bit cache leaves idle.  What bounds it: their unpacking, a latency of its own for every part.  2048 rows behind 8200, 32 and 4 heads of 128, captured: with four, five
+// and six warps 370, 348 and 322 us; three stages of numbers instead of four 379, with one part of codes more in front 380.  A block takes 4400 cycles, 3500 from 16 bits; there are no
+// registers for more warps beside the softmax's.
 // Codes and scales are asked for some parts ahead (cp.async, into shared memory that one warp alone uses: no barrier but the warp's own), then a lane takes
 // a token of the part, or half of one, and stores its numbers as the tiled copies of a 16-bit cache would have them.
 
