@@ -403,8 +403,9 @@ size_t attend_counts(int sm_count) { return (size_t)sm_count * 4; }  // a CTA's 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {
   if (a.q4) {
-    // The streaming kernel where a sequence's rows are a few of its tiles (up to 32: 8 drafts of 5 tokens and 4 heads 44 us, 55 on the tensor cores), the tensor-core kernel where they are
-    // more; a batch of several sequences may hold both kinds, which only the device knows, so both are launched and take their own.
+    // The streaming kernel where a sequence's rows are a few of its tiles, the tensor-core kernel where they are more; a batch of several sequences may hold both kinds, which only the
+    // device knows, so both are launched and take their own.  Captured, 8 key heads of 128, us, streaming and tensor cores: 8 drafts of 20 rows a key head 42.9 and 49.6; 32 of 12 to 16 rows
+    // 79 and 114 to 119, of 32 rows 136 and 135; 4 of 32 rows 35.6 and 39.6.  A chunk of 777 tokens among 47 single ones: 155 by both, 190 by the tensor cores alone.
     const uint32_t group = a.q_heads / a.kv_heads, few = group <= 16 ? 32 / group : 0;
     KvBatchDev small = kv, large = kv;
     if (kv.n_rows > kv.n_seqs && kv.n_seqs > 1) small.most_rows = few, large.least_rows = few + 1;
