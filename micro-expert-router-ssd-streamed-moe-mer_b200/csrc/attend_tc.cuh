@@ -404,248 +404,256 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, c
       done_with();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-    if (warp == TC_MMA) {
-    // ---------------------------------------------------------------- MMA issue
-    const uint32_t leader = tm_elect();
-    constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t BASE = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((128u >> 4) << 24);
-    constexpr uint32_t QK = BASE | ((TC_KB >> 3) << 17), PV = BASE | (1u << 16) | ((DP >> 3) << 17);
-    uint32_t tiles = 0, blocks0 = 0, blocks1 = 0, at = 0, turns = 0;  // phases of q_full and p_ready; places of the ring before the tile's: keys of its block j are at + 2 j, values the next
-    auto place = [&](uint64_t *bars, uint32_t q) { return &bars[q % S::STAGES]; };
-    auto landed = [&](uint32_t q) { return wait(place(ctl.full, q), (q / S::STAGES) & 1); };
-    // Descriptors of rows of 128 bytes in atoms of 8 rows (1024 bytes), 128-byte swizzle.  Bits: start >> 4 [0,14), leading offset >> 4 [16,30), stride offset >> 4
-    // [32,46), version 1 [46,48), swizzle 2 [61,64).  An operand whose rows run along K: 1024 between atoms, no leading offset; one whose rows run along N: 1024
-    // between groups of 8 of K, the leading offset between pieces of 64 values of a row.  The starts of an operand's pieces lie constants apart.
-    constexpr uint64_t ALONG_K = (64ull << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16), ALONG_N = (64ull << 32) | (1ull << 46) | (2ull << 61) | ((uint64_t)(TC_KB * 128 >> 4) << 16);
-    const uint32_t q_at = s_q >> 4, ring_at = s_ring >> 4;
-    auto qk = [&](uint32_t x, uint32_t rows_of, uint32_t q) {  // the scores of a group for the keys at place q
-      const uint32_t a = q_at + rows_of * (16384 >> 4), b = ring_at + q % S::STAGES * (S::STAGE >> 4);
+    // One instruction for a group of four warps.  With 16 bits the last group stands apart as a whole, copying warps have no test of their own, and each side gives its registers
+    // away behind that branch: in front of it, as 4 bits need it, whose last group has warps on either side, heads of 256 spill 44 and 76 bytes (stores, loads; none so) and of 128 52 and 52
+    // (12 and 4): a prompt of 2048 with 16 and 4 heads of 256 83 us instead of 74, 49 sequences mixed, heads of 128, 127 instead of 122.4.
+    auto fewer_registers = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS)); };
+    if (U != 0) fewer_registers();
+    if (warp >= TC_MMA && (U == 0 || warp <= TC_WALK)) {
+      if (U == 0) fewer_registers();
+      if (warp == TC_MMA) {
+        // ---------------------------------------------------------------- MMA issue
+        const uint32_t leader = tm_elect();
+        constexpr uint32_t TYPE = std::is_same<T, __half>::value ? 0u : 1u;
+        constexpr uint32_t BASE = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((128u >> 4) << 24);
+        constexpr uint32_t QK = BASE | ((TC_KB >> 3) << 17), PV = BASE | (1u << 16) | ((DP >> 3) << 17);
+        uint32_t tiles = 0, blocks0 = 0, blocks1 = 0, at = 0, turns = 0;  // phases of q_full and p_ready; places of the ring before the tile's: keys of its block j are at + 2 j, values the next
+        auto place = [&](uint64_t *bars, uint32_t q) { return &bars[q % S::STAGES]; };
+        auto landed = [&](uint32_t q) { return wait(place(ctl.full, q), (q / S::STAGES) & 1); };
+        // Descriptors of rows of 128 bytes in atoms of 8 rows (1024 bytes), 128-byte swizzle.  Bits: start >> 4 [0,14), leading offset >> 4 [16,30), stride offset >> 4
+        // [32,46), version 1 [46,48), swizzle 2 [61,64).  An operand whose rows run along K: 1024 between atoms, no leading offset; one whose rows run along N: 1024
+        // between groups of 8 of K, the leading offset between pieces of 64 values of a row.  The starts of an operand's pieces lie constants apart.
+        constexpr uint64_t ALONG_K = (64ull << 32) | (1ull << 46) | (2ull << 61) | (1ull << 16), ALONG_N = (64ull << 32) | (1ull << 46) | (2ull << 61) | ((uint64_t)(TC_KB * 128 >> 4) << 16);
+        const uint32_t q_at = s_q >> 4, ring_at = s_ring >> 4;
+        auto qk = [&](uint32_t x, uint32_t rows_of, uint32_t q) {  // the scores of a group for the keys at place q
+          const uint32_t a = q_at + rows_of * (16384 >> 4), b = ring_at + q % S::STAGES * (S::STAGE >> 4);
 #pragma unroll
-      for (int k = 0; k < DP / 16; k++)
-        tm_mma_ss(leader, tm + x * 128, ALONG_K | (a + (k / 4) * (S::QSUB >> 4) + (k & 3) * 2), ALONG_K | (b + (k / 4) * (TC_KB * 128 >> 4) + (k & 3) * 2), QK, k != 0);
-      tm_commit(leader, &ctl.s_full[x]);
-      if (U != 0 && leader) mbar_arrive(&ctl.s_full[x]);  // ordinary memory that came with the queries
-    };
-    auto pv = [&](uint32_t x, uint32_t q, bool first) {  // its weights (of place x) times the values at place q
-      const uint32_t b = ring_at + q % S::STAGES * (S::STAGE >> 4);
+          for (int k = 0; k < DP / 16; k++)
+            tm_mma_ss(leader, tm + x * 128, ALONG_K | (a + (k / 4) * (S::QSUB >> 4) + (k & 3) * 2), ALONG_K | (b + (k / 4) * (TC_KB * 128 >> 4) + (k & 3) * 2), QK, k != 0);
+          tm_commit(leader, &ctl.s_full[x]);
+          if (U != 0 && leader) mbar_arrive(&ctl.s_full[x]);  // ordinary memory that came with the queries
+        };
+        auto pv = [&](uint32_t x, uint32_t q, bool first) {  // its weights (of place x) times the values at place q
+          const uint32_t b = ring_at + q % S::STAGES * (S::STAGE >> 4);
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (!wait(h ? &ctl.p_ready[x] : &ctl.p_half[x], (x ? blocks1 : blocks0) & 1)) return false;
-        tm_fence_after();
-#pragma unroll
-        for (int k = 4 * h; k < 4 * h + 4; k++) tm_mma_ts(leader, tm + 256 + (S::WIDE ? 0 : x * DP), tm + x * 128 + k * 8, ALONG_N | (b + k * 128), PV, k != 0 || !first);
-      }
-      blocks0 += x == 0, blocks1 += x == 1;
-      return true;
-    };
-    auto free_place = [&](uint32_t q) { tm_commit(leader, place(ctl.empty, q)); };
-    while (next_tile()) {
-      const TileWork &t = ctl.tile[turn & 1];
-      const uint32_t rows = t.tokens * t.heads, lo = t.lo, n = t.hi - t.lo;
-      // Blocks below `by_rows` and from `by_rows_again` on are filled row by row: not by the proxy that the tensor core reads through.
-      const uint32_t by_rows = p.box ? (first_seen(t, window) + TC_KB - 1) / TC_KB : 0xFFFFFFFFu, by_rows_again = (t.past + t.token0 + t.tokens) / TC_KB;
-      auto visible = [&](uint32_t j) {
-        if (U != 0 || lo + j < by_rows || lo + j >= by_rows_again) proxy_fence();
-      };
-      done_with();
-      if (!wait(&ctl.q_full, tiles++ & 1)) break;
-      if (!p.q_mapped) proxy_fence();
-      bool ok = true;
-      if (S::WIDE) {  // the places for scores take the blocks in turn
-        for (uint32_t j = 0; j <= n && ok; j++) {
-          if (j < n) {
-            if (!(ok = landed(at + 2 * j))) break;
-            visible(j);
+          for (int h = 0; h < 2; h++) {
+            if (!wait(h ? &ctl.p_ready[x] : &ctl.p_half[x], (x ? blocks1 : blocks0) & 1)) return false;
             tm_fence_after();
-            qk((turns + j) & 1, 0, at + 2 * j);
-            free_place(at + 2 * j);
-            if (j + 1 == n) tm_commit(leader, &ctl.q_empty);
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; k++) tm_mma_ts(leader, tm + 256 + (S::WIDE ? 0 : x * DP), tm + x * 128 + k * 8, ALONG_N | (b + k * 128), PV, k != 0 || !first);
           }
-          if (j == 0) continue;
-          const uint32_t v = at + 2 * j - 1;
-          if (!(ok = landed(v))) break;
-          visible(j - 1);
-          if (!(ok = pv((turns + j - 1) & 1, v, j == 1))) break;
-          free_place(v);
-          tm_commit(leader, &ctl.added);
-          if (j == n) tm_commit(leader, &ctl.o_full[0]);
-        }
-        turns += n;
-      } else if (rows <= 128) {  // the groups take the blocks in turn
-        for (uint32_t j = 0; j < 2 && j < n && ok; j++) {
-          if (!(ok = landed(at + 2 * j))) break;
-          visible(j);
-          tm_fence_after();
-          qk(j, 0, at + 2 * j);
-          free_place(at + 2 * j);
-          if (j + 1 == n) tm_commit(leader, &ctl.q_empty);
-        }
-        for (uint32_t j = 0; j < n && ok; j++) {
-          const uint32_t x = j & 1, v = at + 2 * j + 1, k = at + 2 * (j + 2);
-          if (!(ok = landed(v))) break;
-          visible(j);
-          if (!(ok = pv(x, v, j < 2))) break;
-          free_place(v);
-          if (j + 2 < n) {
-            if (!(ok = landed(k))) break;
-            visible(j + 2);
-            qk(x, 0, k);
-            free_place(k);
-            if (j + 3 == n) tm_commit(leader, &ctl.q_empty);
+          blocks0 += x == 0, blocks1 += x == 1;
+          return true;
+        };
+        auto free_place = [&](uint32_t q) { tm_commit(leader, place(ctl.empty, q)); };
+        while (next_tile()) {
+          const TileWork &t = ctl.tile[turn & 1];
+          const uint32_t rows = t.tokens * t.heads, lo = t.lo, n = t.hi - t.lo;
+          // Blocks below `by_rows` and from `by_rows_again` on are filled row by row: not by the proxy that the tensor core reads through.
+          const uint32_t by_rows = p.box ? (first_seen(t, window) + TC_KB - 1) / TC_KB : 0xFFFFFFFFu, by_rows_again = (t.past + t.token0 + t.tokens) / TC_KB;
+          auto visible = [&](uint32_t j) {
+            if (U != 0 || lo + j < by_rows || lo + j >= by_rows_again) proxy_fence();
+          };
+          done_with();
+          if (!wait(&ctl.q_full, tiles++ & 1)) break;
+          if (!p.q_mapped) proxy_fence();
+          bool ok = true;
+          if (S::WIDE) {  // the places for scores take the blocks in turn
+            for (uint32_t j = 0; j <= n && ok; j++) {
+              if (j < n) {
+                if (!(ok = landed(at + 2 * j))) break;
+                visible(j);
+                tm_fence_after();
+                qk((turns + j) & 1, 0, at + 2 * j);
+                free_place(at + 2 * j);
+                if (j + 1 == n) tm_commit(leader, &ctl.q_empty);
+              }
+              if (j == 0) continue;
+              const uint32_t v = at + 2 * j - 1;
+              if (!(ok = landed(v))) break;
+              visible(j - 1);
+              if (!(ok = pv((turns + j - 1) & 1, v, j == 1))) break;
+              free_place(v);
+              tm_commit(leader, &ctl.added);
+              if (j == n) tm_commit(leader, &ctl.o_full[0]);
+            }
+            turns += n;
+          } else if (rows <= 128) {  // the groups take the blocks in turn
+            for (uint32_t j = 0; j < 2 && j < n && ok; j++) {
+              if (!(ok = landed(at + 2 * j))) break;
+              visible(j);
+              tm_fence_after();
+              qk(j, 0, at + 2 * j);
+              free_place(at + 2 * j);
+              if (j + 1 == n) tm_commit(leader, &ctl.q_empty);
+            }
+            for (uint32_t j = 0; j < n && ok; j++) {
+              const uint32_t x = j & 1, v = at + 2 * j + 1, k = at + 2 * (j + 2);
+              if (!(ok = landed(v))) break;
+              visible(j);
+              if (!(ok = pv(x, v, j < 2))) break;
+              free_place(v);
+              if (j + 2 < n) {
+                if (!(ok = landed(k))) break;
+                visible(j + 2);
+                qk(x, 0, k);
+                free_place(k);
+                if (j + 3 == n) tm_commit(leader, &ctl.q_empty);
+              } else {
+                tm_commit(leader, &ctl.o_full[x]);
+              }
+            }
           } else {
-            tm_commit(leader, &ctl.o_full[x]);
-          }
-        }
-      } else {
-        if (!landed(at)) break;
-        visible(0);
-        tm_fence_after();
-        for (uint32_t x = 0; x < 2; x++) qk(x, x, at);
-        free_place(at);
-        if (n == 1) tm_commit(leader, &ctl.q_empty);
-        for (uint32_t j = 0; j < n && ok; j++) {
-          const uint32_t v = at + 2 * j + 1, k = v + 1;
-          const bool more = j + 1 < n;
-          if (!(ok = landed(v))) break;
-          if (more && !(ok = landed(k))) break;
-          visible(j);
-          if (more) visible(j + 1);
-          for (uint32_t x = 0; x < 2; x++) {
-            if (!(ok = pv(x, v, j == 0))) break;
-            if (more)
-              qk(x, x, k);
-            else
-              tm_commit(leader, &ctl.o_full[x]);
+            if (!landed(at)) break;
+            visible(0);
+            tm_fence_after();
+            for (uint32_t x = 0; x < 2; x++) qk(x, x, at);
+            free_place(at);
+            if (n == 1) tm_commit(leader, &ctl.q_empty);
+            for (uint32_t j = 0; j < n && ok; j++) {
+              const uint32_t v = at + 2 * j + 1, k = v + 1;
+              const bool more = j + 1 < n;
+              if (!(ok = landed(v))) break;
+              if (more && !(ok = landed(k))) break;
+              visible(j);
+              if (more) visible(j + 1);
+              for (uint32_t x = 0; x < 2; x++) {
+                if (!(ok = pv(x, v, j == 0))) break;
+                if (more)
+                  qk(x, x, k);
+                else
+                  tm_commit(leader, &ctl.o_full[x]);
+              }
+              if (!ok) break;
+              free_place(v);
+              if (more) {
+                free_place(k);
+                if (j + 2 == n) tm_commit(leader, &ctl.q_empty);
+              }
+            }
           }
           if (!ok) break;
-          free_place(v);
-          if (more) {
-            free_place(k);
-            if (j + 2 == n) tm_commit(leader, &ctl.q_empty);
+          at += 2 * n;
+        }
+      } else if (warp == TC_WALK) {
+        // -------------------------------------------------------------- the way through the run
+        RunWalk<TC_KB> walk(p.kv, ts, window, ctl.run);
+        TileWork t;
+        for (uint32_t i = 0;; i++) {
+          const bool more = walk.next(&t);
+          if (!more) t.tokens = 0;
+          if (!wait(&ctl.tile_empty[i & 1], ((i >> 1) & 1) ^ 1)) break;
+          if (lane == 0) {
+            ctl.tile[i & 1] = t;
+            mbar_arrive(&ctl.tile_full[i & 1]);
           }
+          if (!more) break;
         }
-      }
-      if (!ok) break;
-      at += 2 * n;
-    }
-    } else if (warp == TC_WALK) {
-      // -------------------------------------------------------------- the way through the run
-      RunWalk<TC_KB> walk(p.kv, ts, window, ctl.run);
-      TileWork t;
-      for (uint32_t i = 0;; i++) {
-        const bool more = walk.next(&t);
-        if (!more) t.tokens = 0;
-        if (!wait(&ctl.tile_empty[i & 1], ((i >> 1) & 1) ^ 1)) break;
-        if (lane == 0) {
-          ctl.tile[i & 1] = t;
-          mbar_arrive(&ctl.tile_full[i & 1]);
-        }
-        if (!more) break;
       }
     } else {
-    // ---------------------------------------------------------------- copies: warp w has the rows w * 32 .. of a block, and a quarter of the queries
-    const uint32_t w = warp < TC_MMA ? warp - TC_LOAD : warp - TC_WALK - 1 + TC_LOADERS;
-    uint32_t stage = 0, phase = 0, tiles = 0, bad = 0;
-    if constexpr (U != 0) {
-      if (w < S::UNPACKERS) tc4_copies<IO, DP, U>(p, ctl, w, lane, s_q, s_ring, s_ring + S::STAGES * S::STAGE, turn, &bad, next_tile, done_with, wait);
-    } else if (w < TC_LOADERS) {
-    // The barrier counts a lane's copies when they have landed; the MMA warp makes them visible to the tensor core.  (A proxy fence
-    // here would wait for the copies behind them as well: 4900 cycles a block, 2 stages in flight instead of 5.)
-    auto submit = [&](uint64_t *bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
-    // 32 rows from shared-memory address `dst` on; a lane has the place of one of them in pieces of 16 bytes, ~0: zeros.  Lane i copies piece
-    // i % PIECES of every row that it has a part in, whose place in the swizzle repeats after 8 rows.
-    constexpr uint32_t PIECES = DP / 8, AT_ONCE = 32 / PIECES;  // pieces of a row, rows of one instruction
-    const uint32_t c = lane % PIECES, r0 = lane / PIECES;
-    const uint32_t col = c & 7;
-    const bool in_head = c * 8 < D;
-    auto copy_rows = [&](uint32_t dst, uint32_t sub, const void *base, uint32_t place) {
-      const char *from = (const char *)base + c * 16;
-      dst += (c / 8) * sub + r0 * 128;
-#pragma unroll
-      for (uint32_t i = 0; i < 32 / AT_ONCE; i++) {
-        const uint32_t r = i * AT_ONCE + r0, at = __shfl_sync(0xFFFFFFFFu, place, r);
-        const bool in = at != 0xFFFFFFFFu && in_head;
-        copy16(dst + i * (AT_ONCE * 128) + ((col ^ (r & 7)) << 4), in ? from + (uint64_t)at * 16 : (const char *)base, in ? 16 : 0);
-      }
-    };
-    while (next_tile()) {
-      const TileWork t = ctl.tile[turn & 1];
-      done_with();
-      const uint32_t rows = t.tokens * t.heads;
-      if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
-      if (p.q_mapped) {
-        // 64 values of ts.heads heads of ts.tokens rows; those behind the sequence's end are other rows or zeros, which nobody stores
-        if (lane == 0 && w < S::SUBS) {
-          const uint32_t bar = smem_u32(&ctl.q_full);
-          mbar_expect_tx(&ctl.q_full, ts.tokens * ts.heads * 128);
-          asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(s_q + w * S::QSUB),
-                       "l"(&maps.q), "r"(w * 64), "r"(t.head0), "r"(t.row0 + t.token0), "r"(bar)
-                       : "memory");
-        } else {
-          mbar_arrive(&ctl.q_full);
-        }
+      if (U == 0) fewer_registers();
+      // ---------------------------------------------------------------- copies: warp w has the rows w * 32 .. of a block, and a quarter of the queries
+      const uint32_t w = U == 0 || warp < TC_MMA ? warp - TC_LOAD : warp - TC_WALK - 1 + TC_LOADERS;
+      uint32_t stage = 0, phase = 0, tiles = 0, bad = 0;
+      if constexpr (U != 0) {
+        if (w < S::UNPACKERS) tc4_copies<IO, DP, U>(p, ctl, w, lane, s_q, s_ring, s_ring + S::STAGES * S::STAGE, turn, &bad, next_tile, done_with, wait);
       } else {
-#pragma unroll 1
-        for (uint32_t i = 0; i < S::R / (TC_LOADERS * 32); i++) {
-          const uint32_t r = w * (S::R / TC_LOADERS) + i * 32 + lane, tok = r / t.heads;
-          // the tile's rows lie within 2^32 pieces of its first one
-          const uint32_t place = r < rows ? tok * (uint32_t)(p.q_stride / 8) + (r - tok * t.heads) * (D / 8) : 0xFFFFFFFFu;
-          copy_rows(s_q + (w * (S::R / TC_LOADERS) + i * 32) * 128, S::QSUB, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
-        }
-        submit(&ctl.q_full);
-      }
-      tiles++;
-      const uint32_t end = t.past + t.token0 + t.tokens;
-      const uint32_t start = first_seen(t, window);
-      const PagePlaces pages(p.kv, p.a.page_tokens, t.seq, t.kv_head);
-      // a lane's token of a block: the first of its tiled copy, or a row
-      constexpr uint32_t SUBS = S::SUBS;
-      const uint32_t copy = lane * TC_LOADERS + w, copy_row = copy / SUBS * p.box, copies = p.box ? TC_KB / p.box * SUBS : 0;
-      auto tiled = [&](uint32_t blk) { return p.box && blk * TC_KB >= start && blk * TC_KB + TC_KB <= end; };
-      auto entry = [&](uint32_t blk) {
-        const bool whole = tiled(blk);
-        const uint32_t key = blk * TC_KB + (whole ? copy_row : w * 32 + lane);
-        return blk < t.hi && (whole ? copy < copies : key >= start && key < end) ? pages.entry(key) : 0u;
-      };
-      uint32_t ahead[2] = {entry(t.lo), entry(t.lo + 1)};
-      bool ok = true;
-      for (uint32_t blk = t.lo; blk < t.hi && ok; blk++) {
-        const uint32_t number = ahead[0];
-        ahead[0] = ahead[1];
-        ahead[1] = entry(blk + 2);
-        if (tiled(blk)) {
-          const uint32_t token = pages.in_page(blk * TC_KB + copy_row);
-          if (copy < copies && number >= p.kv.n_pages) bad = 1;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; kv++) {
-            if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
-            if (copy < copies) {
-              mbar_expect_tx(&ctl.full[stage], p.box * 128);
-              page_g2s(s_ring + stage * S::STAGE + (copy % SUBS) * (TC_KB * 128) + copy_row * 128, kv ? &maps.pages.v : &maps.pages.k, (copy % SUBS) * 64, token, t.kv_head,
-                       min(number, p.kv.n_pages), p.head_first, smem_u32(&ctl.full[stage]));
+        // The barrier counts a lane's copies when they have landed; the MMA warp makes them visible to the tensor core.  (A proxy fence
+        // here would wait for the copies behind them as well: 4900 cycles a block, 2 stages in flight instead of 5.)
+        auto submit = [&](uint64_t *bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
+        // 32 rows from shared-memory address `dst` on; a lane has the place of one of them in pieces of 16 bytes, ~0: zeros.  Lane i copies piece
+        // i % PIECES of every row that it has a part in, whose place in the swizzle repeats after 8 rows.
+        constexpr uint32_t PIECES = DP / 8, AT_ONCE = 32 / PIECES;  // pieces of a row, rows of one instruction
+        const uint32_t c = lane % PIECES, r0 = lane / PIECES;
+        const uint32_t col = c & 7;
+        const bool in_head = c * 8 < D;
+        auto copy_rows = [&](uint32_t dst, uint32_t sub, const void *base, uint32_t place) {
+          const char *from = (const char *)base + c * 16;
+          dst += (c / 8) * sub + r0 * 128;
+#pragma unroll
+          for (uint32_t i = 0; i < 32 / AT_ONCE; i++) {
+            const uint32_t r = i * AT_ONCE + r0, at = __shfl_sync(0xFFFFFFFFu, place, r);
+            const bool in = at != 0xFFFFFFFFu && in_head;
+            copy16(dst + i * (AT_ONCE * 128) + ((col ^ (r & 7)) << 4), in ? from + (uint64_t)at * 16 : (const char *)base, in ? 16 : 0);
+          }
+        };
+        while (next_tile()) {
+          const TileWork t = ctl.tile[turn & 1];
+          done_with();
+          const uint32_t rows = t.tokens * t.heads;
+          if (!wait(&ctl.q_empty, (tiles & 1) ^ 1)) break;
+          if (p.q_mapped) {
+            // 64 values of ts.heads heads of ts.tokens rows; those behind the sequence's end are other rows or zeros, which nobody stores
+            if (lane == 0 && w < S::SUBS) {
+              const uint32_t bar = smem_u32(&ctl.q_full);
+              mbar_expect_tx(&ctl.q_full, ts.tokens * ts.heads * 128);
+              asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(s_q + w * S::QSUB),
+                           "l"(&maps.q), "r"(w * 64), "r"(t.head0), "r"(t.row0 + t.token0), "r"(bar)
+                           : "memory");
             } else {
-              mbar_arrive(&ctl.full[stage]);
+              mbar_arrive(&ctl.q_full);
             }
-            stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
-          }
-        } else {
-          const uint32_t key = blk * TC_KB + w * 32 + lane;
-          const uint32_t place = key >= start && key < end ? pages.place(key, number, &bad) : 0xFFFFFFFFu;
+          } else {
 #pragma unroll 1
-          for (int kv = 0; kv < 2; kv++) {
-            if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
-            copy_rows(s_ring + stage * S::STAGE + w * (32 * 128), TC_KB * 128, kv ? p.kv.v_pages : p.kv.k_pages, place);
-            submit(&ctl.full[stage]);
-            stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
+            for (uint32_t i = 0; i < S::R / (TC_LOADERS * 32); i++) {
+              const uint32_t r = w * (S::R / TC_LOADERS) + i * 32 + lane, tok = r / t.heads;
+              // the tile's rows lie within 2^32 pieces of its first one
+              const uint32_t place = r < rows ? tok * (uint32_t)(p.q_stride / 8) + (r - tok * t.heads) * (D / 8) : 0xFFFFFFFFu;
+              copy_rows(s_q + (w * (S::R / TC_LOADERS) + i * 32) * 128, S::QSUB, (const T *)p.q + (uint64_t)(t.row0 + t.token0) * p.q_stride + t.head0 * D, place);
+            }
+            submit(&ctl.q_full);
           }
+          tiles++;
+          const uint32_t end = t.past + t.token0 + t.tokens;
+          const uint32_t start = first_seen(t, window);
+          const PagePlaces pages(p.kv, p.a.page_tokens, t.seq, t.kv_head);
+          // a lane's token of a block: the first of its tiled copy, or a row
+          constexpr uint32_t SUBS = S::SUBS;
+          const uint32_t copy = lane * TC_LOADERS + w, copy_row = copy / SUBS * p.box, copies = p.box ? TC_KB / p.box * SUBS : 0;
+          auto tiled = [&](uint32_t blk) { return p.box && blk * TC_KB >= start && blk * TC_KB + TC_KB <= end; };
+          auto entry = [&](uint32_t blk) {
+            const bool whole = tiled(blk);
+            const uint32_t key = blk * TC_KB + (whole ? copy_row : w * 32 + lane);
+            return blk < t.hi && (whole ? copy < copies : key >= start && key < end) ? pages.entry(key) : 0u;
+          };
+          uint32_t ahead[2] = {entry(t.lo), entry(t.lo + 1)};
+          bool ok = true;
+          for (uint32_t blk = t.lo; blk < t.hi && ok; blk++) {
+            const uint32_t number = ahead[0];
+            ahead[0] = ahead[1];
+            ahead[1] = entry(blk + 2);
+            if (tiled(blk)) {
+              const uint32_t token = pages.in_page(blk * TC_KB + copy_row);
+              if (copy < copies && number >= p.kv.n_pages) bad = 1;
+#pragma unroll 1
+              for (int kv = 0; kv < 2; kv++) {
+                if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
+                if (copy < copies) {
+                  mbar_expect_tx(&ctl.full[stage], p.box * 128);
+                  page_g2s(s_ring + stage * S::STAGE + (copy % SUBS) * (TC_KB * 128) + copy_row * 128, kv ? &maps.pages.v : &maps.pages.k, (copy % SUBS) * 64, token, t.kv_head,
+                           min(number, p.kv.n_pages), p.head_first, smem_u32(&ctl.full[stage]));
+                } else {
+                  mbar_arrive(&ctl.full[stage]);
+                }
+                stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
+              }
+            } else {
+              const uint32_t key = blk * TC_KB + w * 32 + lane;
+              const uint32_t place = key >= start && key < end ? pages.place(key, number, &bad) : 0xFFFFFFFFu;
+#pragma unroll 1
+              for (int kv = 0; kv < 2; kv++) {
+                if (!(ok = wait(&ctl.empty[stage], phase ^ 1))) break;
+                copy_rows(s_ring + stage * S::STAGE + w * (32 * 128), TC_KB * 128, kv ? p.kv.v_pages : p.kv.k_pages, place);
+                submit(&ctl.full[stage]);
+                stage = stage + 1 == S::STAGES ? 0 : stage + 1, phase ^= stage == 0;
+              }
+            }
+          }
+          if (!ok) break;
         }
       }
-      if (!ok) break;
-    }
-    }
-    copies_left<0>();
-    if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
+      copies_left<0>();
+      if (bad) atomicOr(p.ws.status, MER_DEVSTAT_BAD_CACHE);
     }
   }
   tm_fence_before();
