@@ -19,7 +19,9 @@
 //   * Both products have tokens or the head's values along M and the rows along N, so that eight rows cost half of sixteen; the weights are transposed between them (movmatrix).
 //   * Queries are f16 divided by a power of two of their row.  A row's reference m follows its maximum only when that has grown by more than 2^LAG4.  Weights are made as
 //     2^(s - m + 10): a weight is below 2^14, its product with a scale below 4 fits f16, and small ones lie above its last bit for 2^-34 of the largest.  Where a product did not fit
-//     (an output that is not finite says so), the warp takes its blocks of the tile once more with weights 2^13 times smaller, which fit with the scales of any values that f16 holds.
+//     (an output that is not finite says so), the warp takes its blocks of the tile three times more, weights and reference as they were: each time the scales of one class, below 4, below
+//     256 and the others, times 1, 2^-6 and 2^-12, all of which fit and none of which loses a bit.  (Weights 2^13 times smaller in one more pass lost those below 2^-22 of the largest:
+//     the sum had them, the output did not.)
 //
 // A warp's ring of chunks is seen by no other warp.  Where pages are whole chunks (multiples of 16 tokens) a lane makes a chunk's four bulk copies: the addresses of several chunks are
 // one instruction stream, so that a chunk costs a dozen instructions for its copies instead of sixty (copies of 16 bytes by every lane: 54 us for 64 tokens behind 800 to 8000, 49
@@ -44,7 +46,7 @@
 
 namespace {
 
-constexpr float LAG4 = 4.0f;
+constexpr float LAG4 = 4.0f, SHIFT4 = 14.0f - LAG4;
 
 struct Attend4Params {
   AttnLayer a;
@@ -108,6 +110,13 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
     for (int i = 0; i < N; i++) w[i] = lds32(a + i * 4);
   }
 }
+// A scale and its minimum in a pass over one class of scales: what is below 4 (pass 1), below 256 times 2^-6 (2), the others times 2^-12 (3), and zero for what is in another class.
+// Minima are the first class's.
+__device__ __forceinline__ void scales_of_pass(uint32_t at, uint32_t pass) {
+  const uint32_t word = lds32(at), size = word & 0x7FFFu, of = size < 0x4400u ? 1u : size < 0x5C00u ? 2u : 3u;
+  const __half scale = __hmul(__ushort_as_half((uint16_t)word), __ushort_as_half(pass == 1 ? 0x3C00 : pass == 2 ? 0x2400 : 0x0C00));
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"((of == pass ? (uint32_t)__half_as_ushort(scale) : 0u) | (pass == 1 ? word & 0xFFFF0000u : 0u)) : "memory");
+}
 // The same from zero.
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -143,6 +152,7 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
   __shared__ TileWork s_tile;  // here, not in registers: the loop over a tile's blocks needs all of these for itself.  tokens == 0: there is none left
   __shared__ uint32_t s_flag;
   __shared__ uint64_t s_full[NW * ST];  // a chunk has landed
+  __shared__ uint32_t s_pass[NW];
   __shared__ volatile uint32_t s_stop;  // a wait has run out
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, eighth = lane >> 2;
   const uint32_t D = p.a.head_dim, page_tokens = p.a.page_tokens, window = p.a.window;
@@ -328,22 +338,30 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
         qs[x][b][1] = (uint32_t)__half_as_ushort(__float2half_rn(mine - __half2float(hi))) << 16;
       }
     }
-    // Every row sees the tokens all_from .. all_see; of the warp's chunks, those of blocks n_lo .. n_lo + n_n have no others.
+    // Every row sees the tokens all_from .. all_see; of the warp's chunks, those of blocks n_lo .. n_lo + n_all have no others.
     const uint32_t all_see = t.past + t.token0, all_from = window && end > window ? end - window : 0;
-    const uint32_t n_lo = all_from <= w16 ? 0u : (all_from - w16 + KB - 1) / KB, n_hi = all_see < w16 + 15 ? 0u : (all_see - w16 - 15) / KB + 1, n_n = n_hi > n_lo ? n_hi - n_lo : 0;
+    const uint32_t n_lo = all_from <= w16 ? 0u : (all_from - w16 + KB - 1) / KB, n_hi = all_see < w16 + 15 ? 0u : (all_see - w16 - 15) / KB + 1, n_all = n_hi > n_lo ? n_hi - n_lo : 0;
     // The lane has rows x * 8 + quad * 2 + e of scores and outputs.  least: sums of weights times minima
-    // A weight is 2^(s * factor - less) with less = m - shift; limit: the score from which on m has to follow, -infinity while there is no m.
+    // A weight is 2^(s * factor - less) with less = m - SHIFT4; limit: the score from which on m has to follow, -infinity while there is no m.
     float o[NT][S::TILES][4], least[NT][4], less[NT][2], limit[NT][2], l[NT][2], factor[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; x++)
 #pragma unroll
       for (int e = 0; e < 2; e++) factor[x][e] = __shfl_sync(0xFFFFFFFFu, row_factor[x], quad * 8 + e * 4);
-    float shift = 14.0f - LAG4;
+#pragma unroll
+    for (int x = 0; x < NT; x++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) less[x][e] = 0.0f, limit[x][e] = -INFINITY;
+    // s_pass 1 to 3: over one class of scales.  The references are the first pass's last ones and stay: no score is above what they allow.  What such a pass has beside the first one lies in
+    // memory and behind the branch of blocks that need a mask, so that the loop has the registers it had (sums kept in registers: 64 tokens behind 800 to 8000 48.1 us, 45.7 so).
+    if (lane == 0) s_pass[warp] = 0;
+    float kept[NT * (S::TILES + 1) * 4];  // the passes' sums
+    uint32_t n_n = n_all;
   again:
 #pragma unroll
     for (int x = 0; x < NT; x++) {
 #pragma unroll
-      for (int e = 0; e < 2; e++) less[x][e] = 0.0f, limit[x][e] = -INFINITY, l[x][e] = 0.0f;
+      for (int e = 0; e < 2; e++) l[x][e] = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; e++) least[x][e] = 0.0f;
 #pragma unroll
@@ -426,7 +444,7 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
 #pragma unroll
           for (int e = 0; e < 4; e++) s[x][e / 2][e % 2] = fmaf(part[x][e], 1048576.0f, mins[x][e]);
       }
-      if (blk - n_lo >= n_n) {
+      if (blk - n_lo >= n_n) {  // in the passes over classes of scales all blocks
         const uint32_t at = here(blk) * KB + w16 + key_token;
 #pragma unroll
         for (int x = 0; x < NT; x++)
@@ -442,6 +460,12 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
           if (lane < 16 && (key < first_seen(t, window) || key >= t.past + t.token0 + t.tokens))
             for (uint32_t i = 0; i < 4 * G; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(vscales + lane * (4 * G) + i), "r"(0u) : "memory");
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // later copies go where these zeros are
+          __syncwarp();
+        }
+        if (const uint32_t pass = s_pass[warp]) {
+#pragma unroll 1
+          for (uint32_t i = here(lane); i < 16 * G; i += 32) scales_of_pass(vscales + i * 4, pass);
+          if constexpr (WHOLE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
       }
@@ -488,8 +512,8 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
             for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
             top *= factor[x][e];
             const bool first = limit[x][e] == -INFINITY;
-            const float m = less[x][e] + shift, now = first ? top : fmaxf(top, m), f = first ? 0.0f : exp2_approx(m - now);
-            less[x][e] = now == -INFINITY ? 0.0f : now - shift;
+            const float m = less[x][e] + SHIFT4, now = first ? top : fmaxf(top, m), f = first ? 0.0f : exp2_approx(m - now);
+            less[x][e] = now == -INFINITY ? 0.0f : now - SHIFT4;
             limit[x][e] = now == -INFINITY ? now : (now + LAG4) / factor[x][e];
             l[x][e] *= f;
 #pragma unroll
@@ -551,16 +575,36 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
       }
     }
     if constexpr (!WHOLE) asm volatile("cp.async.wait_all;" ::: "memory");
-    if (shift > 0.0f && !lost) {
-      bool odd = false;
+    __syncwarp();
+    if (!lost) {
+      const uint32_t pass = s_pass[warp];
+      bool odd = pass == 1 || pass == 2;
+      if (pass == 0) {
 #pragma unroll
-      for (int x = 0; x < NT; x++)
+        for (int x = 0; x < NT; x++)
 #pragma unroll
-        for (int i = 0; i < S::TILES; i++)
+          for (int i = 0; i < S::TILES; i++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) odd |= !(fabsf(o[x][i][e]) <= FLT_MAX);
-      if (__any_sync(0xFFFFFFFFu, odd)) {  // a weight times a scale that f16 has no room for, or values that are not finite
-        shift -= 13.0f;
+            for (int e = 0; e < 4; e++) odd |= !(fabsf(o[x][i][e]) <= FLT_MAX);
+      } else {
+        asm volatile("" ::"l"(kept) : "memory");
+        const float unit = pass == 1 ? 1.0f : pass == 2 ? 0x1p6f : 0x1p12f;
+        auto keep = [&](float &v, int i) { kept[i] = v = pass == 1 ? v : fmaf(v, unit, kept[i]); };
+#pragma unroll
+        for (int x = 0; x < NT; x++) {
+#pragma unroll
+          for (int i = 0; i < S::TILES; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) keep(o[x][i][e], (x * (S::TILES + 1) + i) * 4 + e);
+#pragma unroll
+          for (int e = 0; e < 4; e++) keep(least[x][e], (x * (S::TILES + 1) + S::TILES) * 4 + e);
+        }
+        asm volatile("" ::"l"(kept) : "memory");
+      }
+      if (__any_sync(0xFFFFFFFFu, odd)) {  // a weight times a scale that f16 has no room for, or scores that are no numbers
+        n_n = 0;
+        __syncwarp();
+        if (lane == 0) s_pass[warp] = pass + 1;
         __syncwarp();
         start_ring();
         goto again;
