@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(32, 16) k_kv4_append(const __grid_constant__ K
         sure = kv4_key_codes_fast(z, most * 0x1p-20f + FLT_MIN, there, lanes, code, &scale_min) && most < 0.98f * KV4_MOST && sum - sum == 0.0f &&
                unit > 0x1p-60f && unit < 0x1p48f;
       }
-      if (!__all_sync(0xFFFFFFFFu, sure)) {
+      // A head that does not exist is zeros, whose least value may have either sign: nothing of it is stored, so it asks for nothing.  (An existing head of zeros does; its minimum has 64 bits' sign.)
+      if (!__all_sync(0xFFFFFFFFu, sure || head >= a.kv_heads)) {
         if (!have64) {
           for (uint32_t i = lane; i < half; i += 32) {
             double2 t;
