@@ -476,7 +476,7 @@ int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *bat
  * x is held as a code of 4 bits and stands for scale * code + minimum:
  *   minimum = f16(min x)   scale = f16(f32(max x - min x) * f32(1 / 15))   code = clamp(rint((x - minimum) * f32(1 / scale)), 0, 15), 0 where scale is 0
  * (5 bits a value with groups of 32, 4.5 with 64; the error of a value is half a scale, plus what f16 cuts off the minimum where that is far larger than the group's
- * range).  Keys are quantised behind norm and rotation; all of it in 64 bits, so the codes are the definition's.  A group with a value that is not finite, or
+ * range).  Keys are quantised behind norm and rotation, with the codes of 64-bit arithmetic: what 32 bits leave open is made again in 64.  A group with a value that is not finite, or
  * of a magnitude above 60000, has the minimum NaN: its values read back as NaN, and rows that see them are not finite.
  * Page p of key head h is a block of mer_kv4_block_bytes at k_pages (v_pages) + p * page_stride + h * head_stride, all in BYTES and multiples of 16; token_stride
  * is 0.  A block has the codes of its tokens one behind the other, then their scales and minima.  A head's codes are stored for 64, 96, 128, 192 or 256 values, units = 2, 3, 4, 6 or 8

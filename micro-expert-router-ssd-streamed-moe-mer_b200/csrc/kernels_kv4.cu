@@ -9,7 +9,7 @@
 // weight in one, stays in registers through a row's heads.
 // Codes, scales and minima are those of 64-bit arithmetic: 32 bits would give a value next to the border between two codes the other one about once in a million values, and a minimum next to
 // one between two f16 would take its whole group's codes with it.  So a step of keys or values is made in 32 bits with a bound on its error; where anything of it lies within that bound
-// of a border (about one step of keys in twenty), it is made again in 64.  A group with a value that is not finite, or beyond KV4_MOST, which f16 has no room for, has the minimum NaN: all of it reads back as NaN.
+// of a border (one step of keys in nine with two heads of 128 a step, one in seventeen with one), it is made again in 64.  A group with a value that is not finite, or beyond KV4_MOST, which f16 has no room for, has the minimum NaN: all of it reads back as NaN.
 // Queries: angles in half turns reduced in 64 bits, the rest in 32, one rounding at the end.
 //
 // What bounds it: issuing.  A step of queries is 111 instructions, one of keys and one of values 598 together, a warp 950 beside its steps.  Captured calls, us: prompt of 2048 rows of
@@ -100,7 +100,7 @@ __device__ __forceinline__ bool kv4_key_codes_fast(const float (&y)[8], float er
     if (d >= lanes) break;
     lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d)), hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
   }
-  const float range = hi - lo, more = 2.25f * error;  // its own rounding and that of the product among it: range is at most twice 2^20 errors
+  const float range = hi - lo, more = 2.25f * error;  // range, at most twice the head's largest value, is rounded by a twelfth of error at most; the other roundings keep the order
   const __half least = __float2half_rn(lo - error), scale = __float2half_rn((range - more) * (1.0f / 15.0f));
   bool sure = __half_as_ushort(least) == __half_as_ushort(__float2half_rn(lo + error)) && __half_as_ushort(scale) == __half_as_ushort(__float2half_rn((range + more) * (1.0f / 15.0f)));
   *scale_min = (uint32_t)__half_as_ushort(scale) | (uint32_t)__half_as_ushort(least) << 16;
@@ -332,17 +332,15 @@ __global__ void __launch_bounds__(32, 16) k_kv4_append(const __grid_constant__ K
         float x[8], o[8], z[8];
         mine.get(x), theirs.get(o);
         const float unit = turned(x, o, cw, sw, a.k_norm != nullptr, z);
-        // What is rotated into one another has together at most twice the largest rotated value, so with cosines and sines off by 2^-22.6 (sincospif: 1 ulp, an angle's
-        // rounding, two products), three roundings of what they multiply, and a norm whose sum has nine roundings and its root two units, a value is off by at most 2^-20.1 of the
-        // head's largest.  No square is infinite, and none that counts has lost bits, while their mean lies between 2^-96
-        // and 2^120.
+        // off by KV4_KEY_ERROR of the head's largest value at most.  No square is infinite, and none that counts has lost bits, while their mean lies between 2^-96 and 2^120; what
+        // other numbers lose below 2^-126 is times `unit` at most.
         float most = fmaxf(fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3]))), fmaxf(fmaxf(fabsf(z[4]), fabsf(z[5])), fmaxf(fabsf(z[6]), fabsf(z[7]))));
         const float sum = ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));  // what is no number stays none
 #pragma unroll
         for (uint32_t d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
         if (p.lanes > 8) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 8));
         if (p.lanes > 16) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
-        sure = kv4_key_codes_fast(z, most * 0x1p-20f + FLT_MIN, there, lanes, code, &scale_min) && most < 0.98f * KV4_MOST && sum - sum == 0.0f &&
+        sure = kv4_key_codes_fast(z, fmaf(most, KV4_KEY_ERROR, FLT_MIN * fmaxf(unit, 1.0f)), there, lanes, code, &scale_min) && most < 0.98f * KV4_MOST && sum - sum == 0.0f &&
                unit > 0x1p-60f && unit < 0x1p48f;
       }
       // A head that does not exist is zeros, whose least value may have either sign: nothing of it is stored, so it asks for nothing.  (An existing head of zeros does; its minimum has 64 bits' sign.)

@@ -18,6 +18,19 @@
 #define KV4_HD inline
 #endif
 
+// What a key's value is off by at most when norm and rotation are made in 32 bits, as a share of the largest value M of its head.  In units of 2^-24, with r the size of a pair (a, b)
+// that is turned, times norm's weights, r <= sqrt(2) M, and |a| + |b| <= sqrt(2) r <= 2 M:
+//   an angle of at most a half-turn rounded, 2^-25 of it: pi / 2 r              2.23
+//   cosine and sine, 1 unit in the last place below 1 as CUDA states: |a| + |b|   2
+//   they times rope_scale and times a weight: r each                            2.83
+//   the first of the two products: at most r                                    1.42
+//   their sum: M                                                                1
+//   the norm: a lane's four sums of squares, its halves, five exchanges (heads above 128 values), f32(1 / head_dim), the sum with eps: 12, of which the root takes half    6
+//   rsqrtf, 2 units in the last place as CUDA states, each up to 2^-23 of the value    4
+//   the product with it                                                         1
+// together 20.5, held as 24: a cosine of two units in the last place has room, too.
+constexpr float KV4_KEY_ERROR = 0x1.8p-20f;
+
 struct Kv4Shape {
   uint32_t group, units, groups;  // values that share a scale (32 or 64), stored units of 32 values, stored groups
   uint32_t codes;                 // bytes of a block's codes
