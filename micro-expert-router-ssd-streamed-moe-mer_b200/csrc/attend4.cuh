@@ -72,7 +72,9 @@ struct Stream4Shape {
   static constexpr uint32_t JOIN = NW * R * (OP + 2) * 4;  // the warps' maxima, sums and outputs
   static constexpr uint32_t MAX_PARTS = RING / 4 / R - 2;  // of a tile: their weights lie in the ring, and the rows' sums
   static constexpr size_t SMEM = RING > JOIN ? RING : JOIN;
+  static constexpr size_t SM_FLOATS = (size_t)2 * CTAS * part_floats(R, 32 * U);  // of parts that an SM's CTAs may leave
 };
+constexpr size_t ATTEND4_SM_FLOATS = Stream4Shape<8, 0, 2>::SM_FLOATS;  // the most of all shapes
 
 // The chunk's token that has place `slot` of eight among the products' rows: neighbours are one even and one odd token, whose codes lie in different banks.
 __device__ __forceinline__ constexpr uint32_t token_of(uint32_t slot) { return slot ^ ((slot >> 1) & 1); }
@@ -735,6 +737,7 @@ __global__ void __launch_bounds__(Stream4Shape<U, GS, NT>::THREADS, Stream4Shape
 template <int U, int GS, int NT>
 cudaError_t launch_stream4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count, cudaStream_t s) {
   using S = Stream4Shape<U, GS, NT>;
+  static_assert(S::CTAS <= ATTEND_CTAS && S::SM_FLOATS <= ATTEND4_SM_FLOATS, "the workspace has room for every CTA's count and parts");
   const Attend4Params p{a, kv, q, out, q_stride, out_stride, ws, TileShape(a.q_heads, a.kv_heads, S::R, ATTEND4_START, 1, 0, ATTEND4_WHOLE), ATTEND4_MIN_RUN};
   const auto launch = [&](auto whole, auto f16) {
     constexpr bool WHOLE = decltype(whole)::value, F16 = decltype(f16)::value;

@@ -85,6 +85,7 @@ cudaError_t launch_attend_tc(const AttnLayer &a, const KvBatchDev &kv, const voi
 cudaError_t launch_attend_tc4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                               int sm_count, cudaStream_t s);
 // kernels_attend4.cu
+constexpr uint32_t ATTEND_CTAS = 2;  // an SM's at most, of any attention kernel: a count each, and two parts
 size_t attend4_part_floats(int sm_count);
 cudaError_t launch_attend4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count,
                            cudaStream_t s);

@@ -398,7 +398,7 @@ cudaError_t launch_stream(const AttendParams &p, const PageMaps &maps, int sm_co
 size_t attend_part_floats(int sm_count) {
   return std::max((size_t)2 * sm_count * part_floats(16, 256), std::max(attend_tc_part_floats(sm_count), attend4_part_floats(sm_count)));
 }
-size_t attend_counts(int sm_count) { return (size_t)sm_count * 4; }  // a CTA's each: four an SM at most
+size_t attend_counts(int sm_count) { return (size_t)sm_count * ATTEND_CTAS; }  // a CTA's each
 
 cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws,
                           int sm_count, cudaStream_t s, int *launches) {

@@ -29,7 +29,7 @@ cudaError_t launch_stream4(const AttnLayer &a, const KvBatchDev &kv, const void 
 
 }  // namespace
 
-size_t attend4_part_floats(int sm_count) { return (size_t)2 * sm_count * std::max(4 * part_floats(8, 128), 2 * part_floats(16, 256)); }
+size_t attend4_part_floats(int sm_count) { return sm_count * ATTEND4_SM_FLOATS; }
 
 cudaError_t launch_attend4(const AttnLayer &a, const KvBatchDev &kv, const void *q, uint64_t q_stride, void *out, uint64_t out_stride, const AttnWorkspace &ws, int sm_count,
                            cudaStream_t s) {
