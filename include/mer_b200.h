@@ -488,8 +488,9 @@ int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *bat
  * Everything else is as with 16 bits: what rows see, tables, strides of rows, pages that are not there (their tokens count as zeros), windows, sinks; but of a page with tokens that a
  * row sees the other ones' bytes may be read, too (they may hold anything).
  * Attention rounds operands to f16 whatever cache_type is: queries beside their row's power of two, weights, and either weights times scales (few rows) or the keys' and values'
- * numbers (many); scores, sums and outputs are fp32.  A sequence with up to 32 rows times query heads of a key head is taken by a kernel that streams (at most 16 query heads to a key head, or one
- * row a sequence), others by the tensor cores; with n_rows above n_seqs and several sequences both are launched, and each takes its own on the device. */
+ * numbers (many); scores, sums and outputs are fp32.  A sequence is taken by a kernel that streams where n_rows <= n_seqs, whatever it brings, or
+ * where it brings few tokens: up to 32 of one query head to a key head, 16 of 2, 8 of 3 or 4, 4 of 6 to 8, 3 of 5 or 16, 2 of 9 to 15; else, and with more than 16 query heads to a key head always,
+ * by the tensor cores.  With n_rows above n_seqs, above these tokens and several sequences both are launched, and each takes its own on the device. */
 uint64_t mer_kv4_block_bytes(uint32_t head_dim, uint32_t page_tokens, uint32_t group); /* 0: no such cache */
 
 /* Keys and values of the batch's rows, which the cache holds, as rows of numbers: a prefix to hand on, rows for another kernel.  Any cache; one rounding to value_type.  Rows
