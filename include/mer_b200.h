@@ -489,7 +489,7 @@ int mer_kv_append_device(mer_backend *b, uint32_t layer, const mer_kv_batch *bat
  * row sees the other ones' bytes may be read, too (they may hold anything).
  * Attention rounds operands to f16 whatever cache_type is: queries beside their row's power of two, weights, and either weights times scales (few rows) or the keys' and values'
  * numbers (many); scores, sums and outputs are fp32.  A sequence is taken by a kernel that streams where n_rows <= n_seqs, whatever it brings, or
- * where it brings few tokens: up to 32 of one query head to a key head, 16 of 2, 8 of 3 or 4, 4 of 6 to 8, 3 of 5 or 16, 2 of 9 to 15; else, and with more than 16 query heads to a key head always,
+ * where it brings few tokens: up to 32 of one query head to a key head, 16 of 2, 6 of 3, 8 of 4, 3 of 5, 6 or 16, 4 of 7 or 8, 2 of 9 to 15; else, and with more than 16 query heads to a key head always,
  * by the tensor cores.  With n_rows above n_seqs, above these tokens and several sequences both are launched, and each takes its own on the device. */
 uint64_t mer_kv4_block_bytes(uint32_t head_dim, uint32_t page_tokens, uint32_t group); /* 0: no such cache */
 
@@ -503,8 +503,8 @@ typedef struct mer_kv_rows { /* device pointers */
 } mer_kv_rows;
 int mer_kv_read_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const mer_kv_rows *rows, void *stream);
 /* d_q and d_out, which do not overlap: [n_rows x q_heads * head_dim] of the cache's type, on 16 bytes, row strides in values (multiples of 8 below 2^26; 0 = no gaps).
- * Scores, exponentials and sums in fp32; the weights are rounded to the cache's type before they multiply the values, as the matrix units take both (2^-9 of a
- * weight at most in bf16, 2^-12 in f16), and the output once at the end.  The host sees no lengths, so n_rows <= n_seqs alone
+ * Scores, exponentials and sums in fp32; the weights are rounded to the cache's type before they multiply the values, as the matrix units take both (2^-8 of a
+ * weight at most in bf16, 2^-11 in f16), and the output once at the end.  The host sees no lengths, so n_rows <= n_seqs alone
  * picks the kernel that is made for one row a sequence; any batch is right with it, but a long chunk among idle sequences is faster without these, or with n_rows above
  * n_seqs (200 rows behind 30000, 32 and 4 heads of 128: 124 us alone, 784 with 255 idle sequences). */
 int mer_attention_forward_device(mer_backend *b, uint32_t layer, const mer_kv_batch *batch, const void *d_q, uint64_t q_stride,

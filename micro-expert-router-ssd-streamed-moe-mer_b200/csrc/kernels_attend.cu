@@ -9,7 +9,7 @@
 // in the loop.  The warps' results are joined in shared memory at the end of a tile, those of several CTAs through the workspace (attention.cuh).
 // 64 tokens behind 800 to 8000 (32 and 4 heads of 128, bf16) 81 to 87 us by the box, 5.4 to 5.8 TB/s; one behind 32000 22 us, of which 10 are reading and the rest the
 // dependent reads at the run's beginning and the join at its end.  Pages of one token, copied row by row: 84 us for the 64 tokens, 81 with pages of 16 on the same box.  Tiles of up to 4 blocks are not cut: 16 windows of 128 tokens 7.0 us, 8.9 cut.
-// The weights go to the second product in the cache's type, 2^-9 (bf16) or 2^-12 (f16) of each at most, like the values they multiply; sums are fp32.
+// The weights go to the second product in the cache's type, 2^-8 (bf16) or 2^-11 (f16) of each at most, like the values they multiply; sums are fp32.
 // Every wait is bounded; one that runs out is latched as MER_DEVSTAT_TIMEOUT and stops the CTA (attend_wait.cuh).
 #include <cuda_runtime.h>
 
@@ -405,21 +405,22 @@ cudaError_t launch_attend(const AttnLayer &a, const KvBatchDev &kv, const void *
   if (a.q4) {
     // The streaming kernel where a sequence's rows are a few of its tiles, the tensor-core kernel where they are more; a batch of several sequences may hold both kinds, which only the
     // device knows, so both are launched (5 to 9 us for an empty one, whichever it is) and take their own.  Streaming goes by tiles, each of which unpacks anew: 8 / group whole tokens, or one
-    // of 9 to 16 heads.  So: four tiles up to 8 heads, but three of 5, which leave three rows of a tile empty (32 drafts of four tokens behind 3000 to 4550: 157 us, 138 by the tensor cores);
-    // two of 9 to 15, three of 16.  Captured, drafts behind 1000 to 6000, 8 key heads of 128, us, streaming and tensor cores, each alone:
+    // of 9 to 16 heads.  So: four tiles with at most one empty row, three of 3, 5 and 6 heads, two of 9 to 15, three of 16.  Captured, drafts behind 1000 to 6000, 8 key heads of 128, us,
+    // streaming and tensor cores, each alone:
     //                                      8 drafts       32 drafts                                      8 drafts       32 drafts
-    //   four tiles: 32 tokens, 1 head    44.9  54.2    124.7  137.5     five tiles: 10 tokens, 3 heads  53.5  52.0    153.1  135.2
-    //               8 tokens, 3 heads    45.3  50.6    125.3  128.7                 5 tokens, 5 heads   53.4  51.1    152.7  129.4
-    //               8 tokens, 4 heads    44.8  52.5    124.1  135.8                 5 tokens, 6 heads   53.5  52.0    153.1  135.0
-    //               4 tokens, 5 heads    45.3  49.7    124.9  124.1                 5 tokens, 8 heads   52.7  54.4    151.4  142.9
-    //               4 tokens, 6 heads    45.4  50.5    125.3  127.7     six: 6 tokens, 5 heads          61.2  52.1    180.8  134.4
-    //               4 tokens, 8 heads    44.8  52.5    124.0  134.7
+    //   four tiles: 32 tokens, 1 head    44.9  54.2    124.7  137.5     five tiles: 5 tokens, 8 heads   52.7  54.4    151.4  142.9
+    //               8 tokens, 4 heads    44.8  52.5    124.1  135.8                 10 tokens, 3 heads  53.5  52.0    153.1  135.2
+    //               4 tokens, 7 heads    45.0  51.5    124.7  131.4     four:       8 tokens, 3 heads   45.3  50.6    125.3  128.7
+    //               4 tokens, 8 heads    44.8  52.5    124.0  134.7                 4 tokens, 5 heads   45.3  49.7    124.9  124.1
+    //   three:      6 tokens, 3 heads    37.2  49.4     97.7  121.9                 4 tokens, 6 heads   45.4  50.5    125.3  127.7
+    //               3 tokens, 5 heads    37.1  48.8     97.4  119.3
     //   two tiles:  2 tokens, 9 heads    40.1  49.6    101.7  121.2     three:      3 tokens, 9 heads   52.1  51.6    143.5  132.4
     //               2 tokens, 12 heads   40.8  50.7    101.9  126.6                 3 tokens, 12 heads  52.5  53.5    144.7  139.0
     //               2 tokens, 14 heads   42.9  51.7    105.9  130.8                 3 tokens, 14 heads  54.9  54.9    149.0  145.6
     //   three:      3 tokens, 16 heads   53.5  56.3    145.7  151.7     four:       4 tokens, 16 heads  66.0  59.9    187.8  167.1
+    // The more a batch has to read the earlier the tensor cores are ahead: 32 drafts of 24 rows in four tiles behind 3000 to 4550 take 158 us, of 27 on the tensor cores 145, the empty launch in both.
     // A chunk of 777 tokens among 47 single ones: 155 by both, 190 by the tensor cores alone.  More than 16 heads: the tensor cores for any rows.
-    const uint32_t group = a.q_heads / a.kv_heads, few = group > 16 ? 0 : group == 16 ? 3 : group > 8 ? 2 : group == 5 ? 3 : 4 * (8 / group);
+    const uint32_t group = a.q_heads / a.kv_heads, few = group > 16 ? 0 : group == 16 ? 3 : group > 8 ? 2 : 8 / group * (8 / group * group < 7 ? 3 : 4);
     KvBatchDev small = kv, large = kv;
     if (kv.n_rows > kv.n_seqs && kv.n_seqs > 1) small.most_rows = few, large.least_rows = few + 1;
     const bool streams = few && (kv.n_rows <= kv.n_seqs || kv.n_seqs > 1 || kv.n_rows <= few), tiles = !few || (kv.n_rows > kv.n_seqs && kv.n_rows > few);
