@@ -21,13 +21,14 @@
 //     2^(s - m + 10): a weight is below 2^14, its product with a scale below 4 fits f16, and small ones lie above its last bit for 2^-34 of the largest.  Where a product did not fit
 //     (an output that is not finite says so), the warp takes its blocks of the tile three times more, weights and reference as they were: each time the scales of one class, below 4, below
 //     256 and the others, times 1, 2^-6 and 2^-12, all of which fit and none of which loses a bit.  (Weights 2^13 times smaller in one more pass lost those below 2^-22 of the largest:
-//     the sum had them, the output did not.)
+//     the sum had them, the output did not.)  A product lies above f16's last bit for weights down to 2^-34 of the largest divided by its scale; what equal ones below that sum to is lost to
+//     bf16 outputs, where values are as small as 1e-4 and thousands of tokens share the rest of a row.
 //
 // A warp's ring of chunks is seen by no other warp.  Where pages are whole chunks (multiples of 16 tokens) a lane makes a chunk's four bulk copies: the addresses of several chunks are
 // one instruction stream, so that a chunk costs a dozen instructions for its copies instead of sixty (copies of 16 bytes by every lane: 54 us for 64 tokens behind 800 to 8000, 49
 // so, before values' codes were multiplied by pairs).  Other pages: cp.async of 16 bytes a lane, token by token.
 //
-// 32 and 4 heads of 128 in bf16, groups of 32, pages of 16: 64 tokens behind 800 to 8000 47.3 us = 3.1 TB/s (16 bits: 84.5 us), one behind 32000 22.6 us.  What bounds it: issuing.  A chunk is
+// 32 and 4 heads of 128 in bf16, groups of 32, pages of 16: captured: 64 tokens behind 800 to 8000 45.7 us = 3.3 TB/s (16 bits: 81.9 us), one behind 32000 22.5 us (18.4).  What bounds it: issuing.  A chunk is
 // 335 instructions, half of them on the ALU (2.4 cycles each for a quarter of an SM; an mma 5.8), and takes 296 ns a quarter of an SM, whatever the number of warps: 5.1 TB/s if it went on
 // all the time.  The rest is 6 us until the first chunk has landed, 2 us of switching for every tile that a CTA goes through, and CTAs that end before others.
 #pragma once

@@ -20,7 +20,7 @@
 //     have no such runs (of 1 or 5 tokens, say), row by row, 16 bytes a lane (cp.async), zeros where nothing is to be read.  Row by row alone a
 //     block took 4000 cycles in a loop of its own; a prompt of 2048 with pages of one token takes 57 us, 55 with pages of 16.
 //   * Rows of P that see nothing of a block hold zeros, and what no row sees is filled with zeros instead of being read.
-//   * P is in the cache's type, which the matrix unit wants of both operands: 2^-9 (bf16) or 2^-12 (f16) of each weight at most.  The sums that the output is divided
+//   * P is in the cache's type, which the matrix unit wants of both operands: 2^-8 (bf16) or 2^-11 (f16) of each weight at most.  The sums that the output is divided
 //     by are of the weights before that, in fp32: their roundings are as often up as down.
 // What bounds it: exponentials and MMAs, 2048 cycles each for a block of both groups at 16 and 8192 a cycle; a block takes 3500, the softmax of a group being a
 // chain of 2000 between its two MMAs.  32 and 4 heads of 128 in bf16: 2048 rows behind 30700 tokens 970 to 990 us (1.08 PFLOP/s, under the power limit), a
@@ -129,7 +129,7 @@ __device__ __forceinline__ void store32(void *p, const uint4 &a, const uint4 &b)
 
 #include "attend_tc4.cuh"
 
-// IO: the type of queries and outputs, which is the operands' too where the cache holds 16 bits; of 4 bits they are f16, which holds any of its values to 2^-12.
+// IO: the type of queries and outputs, which is the operands' too where the cache holds 16 bits; of 4 bits they are f16, which holds any of its values to 2^-11.
 template <typename IO, int DP, int U>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attend_tc(const TcParams p, const __grid_constant__ TcMaps maps) {
   using S = TcShape<DP, U>;

@@ -13,7 +13,7 @@
 // Queries: angles in half turns reduced in 64 bits, the rest in 32, one rounding at the end.
 //
 // What bounds it: issuing.  A step of queries is 111 instructions, one of keys and one of values 598 together, a warp 950 beside its steps.  Captured calls, us: prompt of 2048 rows of
-// 32 + 2 x 4 heads of 128, bf16, 16.9 (16-bit cache: 14.6); 13411 rows of 32 + 2 x 8 heads of 80 in f16 85 at 57 % of the issue slots; one token 4.2.  With their rows read back
+// 32 + 2 x 4 heads of 128, bf16, 17.0 (16-bit cache: 10.0); 13411 rows of 32 + 2 x 8 heads of 80 in f16 85 at 58 % of the issue slots; one token 4.2.  With their rows read back
 // the 13411 rows took 244 us with keys and values wholly in 64 bits, 125 with values in 32, 112 so.  No faster: CTAs of four warps, four an SM; two warps to every row.
 #include <cuda_runtime.h>
 
